@@ -280,6 +280,16 @@ class RoutedExpertWeights:
             sp = C.c_void_p(0 if s is None else s.ctypes.data)
         _check(lib().dsx_expert_store_load(self._h, slot, which, layout, qp, sp, 1 if on_dev else 0, _stream()))
 
+    def load_float(self, which: int, w: torch.Tensor, slot: int = -1):
+        """Quantise matrix `which` of `slot` (w [rows, K] f32 / bf16 / f16 on the GPU; -1: all slots, w [n_slots, rows, K])
+        to MXFP4 and load it (one term of :class:`deepstrix_b200.head.Mxfp4Quantize`; values must be finite)."""
+        from .head import Mxfp4Quantize
+        assert self.fmt == FMT_MXFP4, "load_float quantises to MXFP4 stores"
+        shape = (self.hidden, self.ffn) if which == MAT_DOWN else (self.ffn, self.hidden)
+        assert tuple(w.shape) == (shape if slot >= 0 else (self.n_slots,) + shape)
+        q = Mxfp4Quantize.launch(w if slot >= 0 else w.reshape(-1, shape[1]))
+        self.load(which, SRC_MXFP4_HF, q.codes, q.scales, slot)
+
     def unpack(self, slot: int, which: int):
         """Inverse repack -> (q, s) CUDA uint8 tensors in HF (MXFP4) / split (Q8_0) layout."""
         rows, k = (self.hidden, self.ffn) if which == MAT_DOWN else (self.ffn, self.hidden)

@@ -505,6 +505,45 @@ DSX_API int dsx_ep_counts(dsx_ep_comm* comm, const int32_t** counts);
  * Returns DSX_ERR_DEVICE when the word is non-zero, like dsx_moe_layer_check. */
 DSX_API int dsx_ep_check(dsx_ep_comm* comm, dsx_stream_t stream, uint32_t* error_word);
 
+/* ------------------------------------------------------------------------
+ * 4. The quantised head: MXFP4 rows, their product, token log probabilities
+ *
+ * For the dense products either side of the routed layer (the output head above all) and for what is read off
+ * the logits.  In the reference: the FP4 fake-quantiser of its CPU model (scripts/v41_oracle/kernel.py:129-147), its
+ * dense GEMVs (kernels/q8_0_matvec.hip, here in MXFP4) and the teacher-forced fidelity gate (tests/v41_golden_gate.rs).
+ * None of these calls allocates memory or keeps anything between calls; all may be captured into a graph.
+ * ---------------------------------------------------------------------- */
+enum dsx_dtype { DSX_F32 = 0, DSX_BF16 = 1, DSX_F16 = 2 };
+
+/* MXFP4 rows of K columns (K a multiple of 32), HF layout: codes [n_terms, rows, K/2] (element 2i in the low nibble; 16-byte
+ * aligned) and scales [n_terms, rows, K/32] (E8M0: 2^(e-127), 255 = NaN).  A row is the SUM of its terms.
+ *
+ * quantize: term 0 holds x, each further term what the earlier ones leave over, per block of 32 with the scale
+ * 2^ceil(log2(max|.| / 6)) (byte kept in 1..253) and codes rounded to nearest, ties to even.  Relative error of a row of normal
+ * values about 0.11 / 0.013 / 0.0016 for 1 / 2 / 3 terms.  A block holding a NaN or an infinity gets scale byte 255.
+ * x: rows of `dtype`, row_stride elements apart; any stride of at least k. */
+DSX_API int dsx_mxfp4_quantize(const void* x, int dtype, int64_t rows, int64_t k, int64_t row_stride, int n_terms, void* codes,
+                               void* scales, dsx_stream_t stream);
+/* The values the rows stand for: terms added in f32 in order, rounded once to `dtype`. */
+DSX_API int dsx_mxfp4_dequantize(const void* codes, const void* scales, int64_t rows, int64_t k, int n_terms, void* out, int dtype,
+                                 int64_t row_stride, dsx_stream_t stream);
+/* out[m, n] = sum over a's terms and k of a[m, k] * w[n, k]; a: n_terms x [m, k], w: one term [n, k]; f32 accumulation, one
+ * rounding to `dtype`; rows of out row_stride elements apart (columns past n are left as they are).  m < 2^22. */
+DSX_API int dsx_mxfp4_matmul(const void* a_codes, const void* a_scales, int n_terms, int64_t m, const void* w_codes,
+                             const void* w_scales, int64_t n, int64_t k, void* out, int dtype, int64_t row_stride,
+                             dsx_stream_t stream);
+/* Per row of v logits, with z = logit * inv_temperature:
+ *   logprobs     f32 [t, n_given]  z[token] - logsumexp(z) of the given tokens; a token outside [0, v) gives -inf
+ *   entropy      f32 [t]           of the row's distribution, in nats; may be NULL
+ *   alts         i32 [t, n_alt]    the n_alt largest logits' ids in descending order, equal logits -> lower id
+ *   alt_logprobs f32 [t, n_alt]    their log probabilities
+ * A logit of -inf is masked: no weight, never an alternative (ids run out as -1 with -inf).  A row that is masked as a whole:
+ * logprobs -inf, entropy 0, ids -1.  A row that holds a NaN or +inf: every number NaN (tokens outside [0, v): -inf), ids -1.
+ * n_given <= 1024, n_alt <= 32. */
+DSX_API int dsx_token_logprobs(const void* logits, int dtype, int64_t t, int64_t v, int64_t row_stride, float inv_temperature,
+                               const int32_t* tokens, int n_given, float* logprobs, float* entropy, int n_alt, int32_t* alts,
+                               float* alt_logprobs, dsx_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif
