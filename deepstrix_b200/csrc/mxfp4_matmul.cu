@@ -1,55 +1,497 @@
-// out[m, n] = sum over terms and k of A_term[m, k] * W[n, k], both operands MXFP4 rows, f32 accumulation, one rounding.
+// out[m, n] = sum over terms and k of A_term[m, k] * W[n, k]: both operands MXFP4 rows as stored, on the block-scaled FP4 tensor
+// cores (tcgen05.mma.kind::mxf4.block_scale), f32 accumulation in tensor memory, one rounding.
+//
+// Reference counterparts (paths relative to the deepstrix repository): the dense GEMV / GEMM of its projections and head
+// (crates/v4flash-kernels/kernels/q8_0_matvec.hip:64-150, f16_gemm_wmma.hip) and the FP4 product of its CPU model
+// (scripts/v41_oracle/kernel.py:161-167).
+//
+// Tile.  128 rows of W are the MMA's M side (a tensor-memory lane each), up to 208 rows of A its N side, so that one token and a
+// few hundred run on the same kernel: a decode batch is an N of 16 under a stream of weights.  The terms of A are further MMAs into
+// the same accumulator: W is read once for all of them.  A pipeline stage is 256 columns: 128-byte rows (128-byte swizzle) of W and of every
+// term, each one TMA box, zero-filled past the operand's edges; and their scale bytes.
+// Scales are read as stored (row-major bytes; nothing is laid out beforehand): two loader warps bring the stage's 8 bytes of
+// every row into shared memory as 4-byte asynchronous copies (single bytes where rows of scales are not 4-byte aligned), in the form of
+// scale-factor chunks -- 128 rows x 4 blocks as 32 lanes x 16 bytes -- and four scale warps, one per lane quarter, move a landed
+// stage's chunks to tensor memory (ld.shared + tcgen05.st; the tensor core's own copy would queue behind its MMAs).
+// Warp roles (12 warps): TMA producer, MMA issue, 2 scale loaders, 4 scale warps, 4 epilogue warps; two accumulators, so that a
+// tile is read out under the next one's MMAs.
+// Few tiles: the columns are split over the CTAs of a cluster; each leaves its partial tile in shared memory and the cluster adds
+// them in rank order through distributed shared memory, so results do not depend on timing and need no workspace.
+// Every wait is bounded; on a timeout the block drains, frees its tensor memory and sets bit 1 of the error word.
+#include <cuda.h>
+
+#include <algorithm>
+#include <atomic>
+
 #include "head.cuh"
+#include "prefill.cuh"
 
 namespace dsx {
 namespace {
 
-constexpr int kTile = 64;
+__device__ uint32_t g_head_error = 0;
 
-// 64 x 64 outputs a block, 4 x 4 a thread; 32 columns (one scale block) of both operands expanded to f32 in shared memory a step.
-template <int DT>
-__global__ void __launch_bounds__(256)
-mxfp4_matmul_kernel(const uint32_t* __restrict__ a_codes, const uint8_t* __restrict__ a_scales, int terms, int64_t M, const uint32_t* __restrict__ w_codes,
-                    const uint8_t* __restrict__ w_scales, int64_t N, int64_t K, void* __restrict__ out_, int64_t row_stride) {
-    using T = typename Elem<DT>::T;
-    __shared__ float sa[32][kTile + 1], sw[32][kTile + 1];
-    const int64_t n0 = (int64_t)blockIdx.x * kTile, m0 = (int64_t)blockIdx.y * kTile;
-    const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4;
-    const int64_t words = K / 8, blocks = K / 32;
-    float acc[4][4] = {};
-    for (int64_t b = 0; b < blocks; b++) {
-        {   // thread = (row tid / 4, eight columns (tid % 4))
-            const int r = tid >> 2, c = tid & 3;
-            float v[8] = {};
-            if (m0 + r < M)
-                for (int t = 0; t < terms; t++) {
-                    const int64_t row = (int64_t)t * M + m0 + r;
-                    const uint32_t w = a_codes[row * words + b * 4 + c];
-                    const float s = e8m0_value(a_scales[row * blocks + b]);
-                    for (int j = 0; j < 8; j++) v[j] += e2m1_to_f32(w >> (4 * j)) * s;
-                }
-            for (int j = 0; j < 8; j++) sa[c * 8 + j][r] = v[j];
-            float u[8] = {};
-            if (n0 + r < N) {
-                const uint32_t w = w_codes[(n0 + r) * words + b * 4 + c];
-                const float s = e8m0_value(w_scales[(n0 + r) * blocks + b]);
-                for (int j = 0; j < 8; j++) u[j] = e2m1_to_f32(w >> (4 * j)) * s;
-            }
-            for (int j = 0; j < 8; j++) sw[c * 8 + j][r] = u[j];
-        }
-        __syncthreads();
-        for (int k = 0; k < 32; k++)
-#pragma unroll
-            for (int i = 0; i < 4; i++)
-#pragma unroll
-                for (int j = 0; j < 4; j++) acc[i][j] = __fmaf_rn(sa[k][ty * 4 + i], sw[k][tx + 16 * j], acc[i][j]);
-        __syncthreads();
+constexpr int kThreads = 384;
+constexpr int kLoaders = 64;
+constexpr int kWRows = 128;          // W rows of a tile
+constexpr int kStageK = 256;         // columns of a stage
+constexpr int kRowBytes = kStageK / 2;
+constexpr int kWBytes = kWRows * kRowBytes;
+constexpr int kChunk = 512;          // scale bytes of 128 rows x 4 blocks
+constexpr int kMaxStages = 8;
+constexpr int kMaxTokens = 208;      // A rows of a tile: two accumulators and four scale slots fill tensor memory
+constexpr uint32_t kSpinLimit = 1u << 22;
+
+__device__ __forceinline__ uint32_t smem_u32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
+__device__ __forceinline__ void mbar_init(uint32_t bar, uint32_t count) {
+    asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count) : "memory");
+}
+__device__ __forceinline__ void mbar_expect_tx(uint32_t bar, uint32_t bytes) {
+    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void mbar_arrive(uint32_t bar) { asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory"); }
+__device__ __forceinline__ bool mbar_try(uint32_t bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(bar), "r"(parity)
+        : "memory");
+    return ok != 0;
+}
+// Bounded wait that also gives up when another role of the block has.
+__device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatile uint32_t* abort_flag) {
+    for (uint32_t i = 0; i < kSpinLimit; i++) {
+        if (mbar_try(bar, parity)) return true;
+        if ((i & 255u) == 255u && *abort_flag) return false;
     }
-    for (int i = 0; i < 4; i++)
-        for (int j = 0; j < 4; j++) {
-            const int64_t m = m0 + ty * 4 + i, n = n0 + tx + 16 * j;
-            if (m < M && n < N) reinterpret_cast<T*>(out_)[m * row_stride + n] = from_f32<T>(acc[i][j]);
+    *abort_flag = 1u;
+    return false;
+}
+__device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap* map, int c0, int c1, uint32_t bar) {
+    asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(dst), "l"(map),
+                 "r"(c0), "r"(c1), "r"(bar)
+                 : "memory");
+}
+__device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map, int c0, int c1, int c2, uint32_t bar) {
+    asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst),
+                 "l"(map), "r"(c0), "r"(c1), "r"(c2), "r"(bar)
+                 : "memory");
+}
+__device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tc_commit(uint32_t bar) {
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+}
+// D[128 x N] (+)= A[128 x 64] . B[N x 64]^T, E2M1 operands, one E8M0 scale per 32 columns of either operand.
+__device__ __forceinline__ void tc_mma_mxf4(uint32_t d, uint32_t a_lo, uint32_t b_lo, uint32_t hi, uint32_t idesc, uint32_t sfa, uint32_t sfb,
+                                            uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t.reg .b64 da, db;\n\t"
+        "setp.ne.b32 p, %7, 0;\n\t"
+        "mov.b64 da, {%1, %3};\n\t"
+        "mov.b64 db, {%2, %3};\n\t"
+        "tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], da, db, %4, [%5], [%6], p;\n\t}"
+        ::"r"(d), "r"(a_lo), "r"(b_lo), "r"(hi), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate)
+        : "memory");
+}
+__device__ __forceinline__ void tc_ld16(uint32_t taddr, uint32_t (&r)[16]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+        "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
+          "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(taddr));
+}
+__device__ __forceinline__ void tc_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tc_st8(uint32_t taddr, const uint4& a, const uint4& b) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(taddr), "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w),
+                 "r"(b.x), "r"(b.y), "r"(b.z), "r"(b.w)
+                 : "memory");
+}
+__device__ __forceinline__ uint32_t cluster_ctarank() {
+    uint32_t r;
+    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+    return r;
+}
+__device__ __forceinline__ uint32_t map_to_cta(uint32_t saddr, uint32_t cta) {
+    uint32_t r;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(saddr), "r"(cta));
+    return r;
+}
+__device__ __forceinline__ float ld_cluster_f32(uint32_t addr) {
+    float v;
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+    return v;
+}
+__device__ __forceinline__ void cluster_sync_all() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// K-major operand tile of 128-byte rows, 128-byte swizzle: 8-row groups of 1024 bytes.
+__device__ __forceinline__ uint64_t operand_desc(uint32_t saddr) {
+    uint64_t d = 0;
+    d |= (uint64_t)((saddr & 0x3FFFFu) >> 4);       // start address
+    d |= (uint64_t)(1024u >> 4) << 32;              // stride between 8-row groups
+    d |= (uint64_t)1 << 46;                         // descriptor version (sm_100)
+    d |= (uint64_t)2 << 61;                         // 128-byte swizzle
+    return d;
+}
+// kind::mxf4: E2M1 x E2M1 -> f32, E8M0 scales, K-major operands, M = 128, K = 64; sf = byte (0 or 2) of the 4-byte scale words
+// that holds this k step's first block.
+__device__ __forceinline__ uint32_t mxf4_idesc(int n, uint32_t sf) {
+    return (1u << 7) | (1u << 10) | ((uint32_t)(n >> 3) << 17) | (1u << 23) | ((128u >> 4) << 24) | (sf << 4) | (sf << 29);
+}
+
+struct MatmulArgs {
+    const uint8_t* w_scales;
+    const uint8_t* a_scales;
+    void* out;
+    int64_t row_stride;
+    int64_t M, N;
+    int K, terms;
+    int tokens;              // A rows of a tile (multiple of 16)
+    int stages, stage_bytes; // ring
+    int chunks;              // scale chunks of a stage and 128-column half: 1 (W) + terms * ceil(tokens / 128)
+    int tmem_cols;
+    int splits;              // CTAs of a cluster that share a tile's columns
+    int tiles_w, tiles;      // tile t: W tile t % tiles_w, token tile t / tiles_w
+    int words;               // rows of scales are 4-byte aligned
+};
+
+template <int DT>
+__global__ void __launch_bounds__(kThreads, 2)
+mxfp4_matmul_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CUtensorMap tmap_a, const MatmulArgs g) {
+    using T = typename Elem<DT>::T;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+    __shared__ __align__(8) uint64_t s_bars[3 * kMaxStages + 4];
+    __shared__ uint32_t s_misc[2];
+    const uint32_t sbase = smem_u32(smem), bar0 = smem_u32(s_bars);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    // FULL[s]: codes (TMA bytes) and scales (loaders) of the stage have landed; SC_FULL[s]: its scales are in tensor memory;
+    // EMPTY[s]: the MMAs that read it have completed; ACC_FULL / ACC_EMPTY[b]: accumulator b is complete / read out.
+    constexpr int FULL = 0, SC_FULL = kMaxStages, EMPTY = 2 * kMaxStages, ACC_FULL = 3 * kMaxStages, ACC_EMPTY = ACC_FULL + 2;
+    auto bar = [&](int i) { return bar0 + 8u * (uint32_t)i; };
+    volatile uint32_t* abort_flag = s_misc + 1;
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < kMaxStages; i++) {
+            mbar_init(bar(FULL + i), 1 + kLoaders);
+            mbar_init(bar(SC_FULL + i), 4);
+            mbar_init(bar(EMPTY + i), 1);
         }
+        for (int b = 0; b < 2; b++) {
+            mbar_init(bar(ACC_FULL + b), 1);
+            mbar_init(bar(ACC_EMPTY + b), 4);
+        }
+        *abort_flag = 0u;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        asm volatile("prefetch.tensormap [%0];" ::"l"(&tmap_w) : "memory");
+        asm volatile("prefetch.tensormap [%0];" ::"l"(&tmap_a) : "memory");
+    }
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(s_misc)), "r"(g.tmem_cols) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *(volatile uint32_t*)s_misc;
+    pdl_wait();   // the operands may come from the kernel before this one
+
+    const int rank = g.splits > 1 ? (int)cluster_ctarank() : 0;
+    const int n_kc = (g.K + kStageK - 1) / kStageK;
+    const int kc0 = (int)((int64_t)n_kc * rank / g.splits), kc1 = (int)((int64_t)n_kc * (rank + 1) / g.splits);
+    const int tile0 = (int)blockIdx.x / g.splits, tile_step = (int)gridDim.x / g.splits;
+    const int BN = g.tokens;
+    const uint32_t b_bytes = (uint32_t)(g.terms * BN * kRowBytes);
+    const uint32_t sc_off = kWBytes + b_bytes;                  // the stage's scale chunks: [128-column half][W, term 0, ...][512]
+    const uint32_t slot0 = tmem + 2u * (uint32_t)BN, slot_cols = 8u * (uint32_t)g.chunks;
+    const int nb = (BN + 127) >> 7;
+
+    if (warp == 0) {
+        // -------------------------------------------------------------- producer
+        if (lane == 0) {
+            uint32_t s = 0, ph = 0;
+            bool ok = true;
+            for (int tile = tile0; tile < g.tiles && ok; tile += tile_step) {
+                const int w0 = (tile % g.tiles_w) * kWRows, a0 = (tile / g.tiles_w) * BN;
+                for (int kc = kc0; kc < kc1; kc++) {
+                    ok = mbar_wait(bar(EMPTY) + 8u * s, ph ^ 1u, abort_flag);
+                    if (!ok) break;
+                    const uint32_t dst = sbase + s * (uint32_t)g.stage_bytes, full = bar(FULL) + 8u * s;
+                    mbar_expect_tx(full, kWBytes + b_bytes);
+                    tma_load_2d(dst, &tmap_w, kc * kRowBytes, w0, full);
+                    tma_load_3d(dst + kWBytes, &tmap_a, kc * kRowBytes, a0, 0, full);
+                    if (++s == (uint32_t)g.stages) { s = 0; ph ^= 1u; }
+                }
+            }
+            if (!ok)   // gave up: let the copies in flight land before the block goes away
+                for (uint32_t i = 0; i < (uint32_t)g.stages; i++)
+                    for (uint32_t n = 0; n < kSpinLimit / 64 && !mbar_try(bar(FULL) + 8u * i, i < s ? ph : ph ^ 1u); n++) {}
+        }
+    } else if (warp == 1) {
+        // ------------------------------------------------------------- MMA issue
+        if (lane == 0) {
+            uint32_t s = 0, ph = 0, t = 0;
+            bool ok = true;
+            const uint64_t d0 = operand_desc(sbase);
+            const uint32_t hi = (uint32_t)(d0 >> 32), lo0 = (uint32_t)d0;
+            const uint32_t term_step = (uint32_t)(BN * kRowBytes) >> 4;
+            const uint32_t idesc0 = mxf4_idesc(BN, 0u), idesc2 = mxf4_idesc(BN, 2u);
+            for (int tile = tile0; tile < g.tiles && ok; tile += tile_step, t++) {
+                const uint32_t b = t & 1u, acc = tmem + b * (uint32_t)BN;
+                ok = mbar_wait(bar(ACC_EMPTY) + 8u * b, ((t >> 1) & 1u) ^ 1u, abort_flag);
+                if (!ok) break;
+                tc_fence_after();
+                for (int kc = kc0; kc < kc1; kc++) {
+                    ok = mbar_wait(bar(SC_FULL) + 8u * s, ph, abort_flag) && mbar_wait(bar(FULL) + 8u * s, ph, abort_flag);
+                    if (!ok) break;
+                    tc_fence_after();
+                    const uint32_t a_lo = lo0 + s * ((uint32_t)g.stage_bytes >> 4), b_lo = a_lo + (kWBytes >> 4), sc = slot0 + s * slot_cols;
+                    const int steps = min(4, (g.K - kc * kStageK + 63) >> 6);
+                    for (int ks = 0; ks < steps; ks++) {
+                        const uint32_t sfw = sc + (uint32_t)(ks >> 1) * 4u * (uint32_t)g.chunks;
+                        for (int q = 0; q < g.terms; q++)
+                            tc_mma_mxf4(acc, a_lo + 2u * ks, b_lo + (uint32_t)q * term_step + 2u * ks, hi, (ks & 1) ? idesc2 : idesc0, sfw,
+                                        sfw + 4u + (uint32_t)(q * nb) * 4u, (kc > kc0 || ks > 0 || q > 0) ? 1u : 0u);
+                    }
+                    tc_commit(bar(EMPTY) + 8u * s);
+                    if (++s == (uint32_t)g.stages) { s = 0; ph ^= 1u; }
+                }
+                if (ok) tc_commit(bar(ACC_FULL) + 8u * b);
+            }
+        }
+    } else if (warp < 4) {
+        // --------------------------------------------------------- scale loaders
+        // Thread i brings the rows i and i + 64 of every 128-row group: two words (the stage's two 128-column halves) a row.
+        const int i = threadIdx.x - 64;
+        const int nblk = g.K >> 5;
+        uint32_t s = 0, ph = 0;
+        bool ok = true;
+        for (int tile = tile0; tile < g.tiles && ok; tile += tile_step) {
+            const int64_t w0 = (int64_t)(tile % g.tiles_w) * kWRows, a0 = (int64_t)(tile / g.tiles_w) * BN;
+            for (int kc = kc0; kc < kc1; kc++) {
+                ok = mbar_wait(bar(EMPTY) + 8u * s, ph ^ 1u, abort_flag);
+                if (!ok) break;
+                const uint32_t sc = sbase + s * (uint32_t)g.stage_bytes + sc_off;
+                const int blk = kc * 8;
+                // row r of a chunk: 4 bytes at (r % 32) * 16 + (r / 32) * 4
+                auto bring = [&](const uint8_t* base, int64_t row, int64_t rows_end, int chunk, int r) {
+                    const bool live = row < rows_end;
+                    const uint8_t* src = base + (live ? row : 0) * nblk + blk;
+                    const uint32_t dst = sc + (uint32_t)chunk * kChunk + (uint32_t)((r & 31) * 16 + (r >> 5) * 4);
+#pragma unroll
+                    for (int h = 0; h < 2; h++) {
+                        const int n = live ? min(4, max(0, nblk - blk - 4 * h)) : 0;
+                        const uint32_t d = dst + (uint32_t)(h * g.chunks) * kChunk;
+                        if (g.words) {   // a word lies inside the row or past its end; zero-filled there
+                            asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(d), "l"(n ? src + 4 * h : base), "r"(n) : "memory");
+                        } else {
+                            uint32_t v = 0;
+                            for (int j = 0; j < n; j++) v |= (uint32_t)__ldg(src + 4 * h + j) << (8 * j);
+                            asm volatile("st.shared.b32 [%0], %1;" ::"r"(d), "r"(v) : "memory");
+                        }
+                    }
+                };
+#pragma unroll
+                for (int p = 0; p < 2; p++) {
+                    const int r = i + 64 * p;
+                    bring(g.w_scales, w0 + r, g.N, 0, r);
+                    for (int q = 0; q < g.terms; q++)
+                        for (int c = 0; c < nb; c++) {
+                            const int ra = c * 128 + r;
+                            if (ra < BN) bring(g.a_scales + (int64_t)q * g.M * nblk, a0 + ra, g.M, 1 + q * nb + c, r);
+                        }
+                }
+                const uint32_t full = bar(FULL) + 8u * s;
+                if (g.words) asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(full) : "memory");
+                else mbar_arrive(full);
+                if (++s == (uint32_t)g.stages) { s = 0; ph ^= 1u; }
+            }
+        }
+        asm volatile("cp.async.wait_all;" ::: "memory");
+    } else if (warp < 8) {
+        // ----------------------------------------------------------- scale warps
+        const uint32_t q = (uint32_t)(warp & 3);
+        uint32_t s = 0, ph = 0;
+        bool ok = true;
+        for (int tile = tile0; tile < g.tiles && ok; tile += tile_step)
+            for (int kc = kc0; kc < kc1; kc++) {
+                ok = mbar_wait(bar(FULL) + 8u * s, ph, abort_flag);
+                if (!ok) break;
+                const uint8_t* src = smem + (size_t)s * g.stage_bytes + sc_off + lane * 16;
+                const uint32_t dst = slot0 + s * slot_cols + ((q * 32u) << 16);
+                for (int c = 0; c < g.chunks; c++) {   // 2 * chunks of them, stored two at a time
+                    const uint4 v0 = *reinterpret_cast<const uint4*>(src + (2 * c) * kChunk), v1 = *reinterpret_cast<const uint4*>(src + (2 * c + 1) * kChunk);
+                    tc_st8(dst + 8u * (uint32_t)c, v0, v1);
+                }
+                asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(bar(SC_FULL) + 8u * s);
+                if (++s == (uint32_t)g.stages) { s = 0; ph ^= 1u; }
+            }
+    } else {
+        // -------------------------------------------------------------- epilogue
+        const uint32_t q = (uint32_t)(warp & 3);
+        uint32_t t = 0;
+        bool ok = true;
+        for (int tile = tile0; tile < g.tiles && ok; tile += tile_step, t++) {
+            const int64_t n = (int64_t)(tile % g.tiles_w) * kWRows + q * 32 + lane, m0 = (int64_t)(tile / g.tiles_w) * BN;
+            const uint32_t b = t & 1u, acc = tmem + b * (uint32_t)BN + ((q * 32u) << 16);
+            ok = mbar_wait(bar(ACC_FULL) + 8u * b, (t >> 1) & 1u, abort_flag);
+            if (!ok) break;
+            tc_fence_after();
+            for (int c0 = 0; c0 < BN; c0 += 16) {
+                uint32_t v[16];
+                tc_ld16(acc + (uint32_t)c0, v);
+                tc_wait_ld();
+                if (g.splits > 1) {   // the partial tile, token-major, in the ring's memory (every stage has been consumed)
+                    float* p = reinterpret_cast<float*>(smem) + (size_t)c0 * kWRows + q * 32 + lane;
+#pragma unroll
+                    for (int j = 0; j < 16; j++) p[j * kWRows] = __uint_as_float(v[j]);
+                } else if (n < g.N) {
+                    T* o = reinterpret_cast<T*>(g.out) + (m0 + c0) * g.row_stride + n;
+#pragma unroll
+                    for (int j = 0; j < 16; j++)
+                        if (m0 + c0 + j < g.M) o[j * g.row_stride] = from_f32<T>(__uint_as_float(v[j]));
+                }
+            }
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(bar(ACC_EMPTY) + 8u * b);
+        }
+    }
+
+    tc_fence_before();
+    __syncthreads();
+    if (threadIdx.x == 0 && *abort_flag) atomicOr(&g_head_error, 1u);
+    if (g.splits > 1) {
+        cluster_sync_all();
+        // CTA `rank` adds the tokens rank, rank + splits, ... of all partial tiles, in rank order
+        const int64_t w0 = (int64_t)(tile0 % g.tiles_w) * kWRows, m0 = (int64_t)(tile0 / g.tiles_w) * BN;
+        const int r = threadIdx.x & 127;
+        for (int c = rank + g.splits * (int)(threadIdx.x >> 7); c < BN; c += g.splits * (kThreads / 128)) {
+            if (m0 + c >= g.M || w0 + r >= g.N) continue;
+            const uint32_t at = sbase + (uint32_t)(c * kWRows + r) * 4u;
+            float sum = 0.0f;
+            for (int p = 0; p < g.splits; p++) sum += ld_cluster_f32(map_to_cta(at, (uint32_t)p));
+            reinterpret_cast<T*>(g.out)[(m0 + c) * g.row_stride + w0 + r] = from_f32<T>(sum);
+        }
+        cluster_sync_all();   // nobody's shared memory goes away while another CTA reads it
+    }
+    if (warp == 1) {
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(g.tmem_cols) : "memory");
+    }
+}
+
+// Two sizes of block, so that tensor memory is never over-committed by blocks of this kernel that share an SM (a cluster whose
+// blocks wait for tensor memory held by another such cluster could wait for ever): at most 112 KB of shared memory and 256
+// columns (two blocks an SM, a third does not fit beside 77 KB or more), or at least 160 KB (alone on its SM).
+constexpr int kSmallMin = 77 * 1024, kSmallMax = 112 * 1024, kLargeMin = 160 * 1024, kLargeMax = 225 * 1024;
+
+struct Plan {
+    int tokens, stages, stage_bytes, chunks, tmem_cols, smem, per_sm, splits, tiles_w, tiles_m;
+};
+
+bool plan_block(int terms, int tokens, Plan* p) {
+    const int nb = (tokens + 127) / 128, chunks = 1 + terms * nb;
+    p->tokens = tokens;
+    p->chunks = chunks;
+    p->stage_bytes = kWBytes + terms * tokens * kRowBytes + 2 * chunks * kChunk;
+    auto cols = [&](int stages) { return 2 * tokens + stages * 8 * chunks; };
+    auto pow2 = [](int c) { int r = 32; while (r < c) r *= 2; return r; };
+    int st = std::min(kMaxStages, (kSmallMax - 1024) / p->stage_bytes);
+    while (st > 3 && cols(st) > 256) st--;
+    if (st >= 3 && cols(st) <= 256) {
+        p->stages = st;
+        p->smem = std::max(kSmallMin, st * p->stage_bytes + 1024);
+        p->per_sm = 2;
+    } else {
+        st = std::min(kMaxStages, (kLargeMax - 1024) / p->stage_bytes);
+        while (st > 2 && cols(st) > 512) st--;
+        if (st < 2 || cols(st) > 512) return false;
+        p->stages = st;
+        p->smem = std::max(kLargeMin, st * p->stage_bytes + 1024);
+        p->per_sm = 1;
+    }
+    p->tmem_cols = pow2(cols(p->stages));
+    return p->stages * p->stage_bytes >= tokens * kWRows * 4;   // a partial tile fits into the ring
+}
+
+// Tokens a tile and splits of the columns, from a model of the time in clocks: a stage costs an SM its MMAs (tokens / 2 clocks per 64
+// columns and term) or its copies (about 40 bytes a clock and SM from L2), whichever is longer; a block about 3000 clocks before and
+// after its stages, a joined tile another 1500; and the operands come from HBM at about 23 bytes a clock and SM.
+bool make_plan(int64_t M, int64_t N, int K, int terms, int sms, Plan* best) {
+    const int n_kc = (K + kStageK - 1) / kStageK;
+    const int tiles_w = (int)((N + kWRows - 1) / kWRows);
+    double best_t = 1e300;
+    const int most = terms == 1 ? kMaxTokens : 128;
+    for (int tokens = 16; tokens <= most && tokens < M + 16; tokens += 16) {
+        Plan p;
+        if (!plan_block(terms, tokens, &p)) continue;
+        p.tiles_w = tiles_w;
+        p.tiles_m = (int)((M + tokens - 1) / tokens);
+        for (int s = 1; s <= 8 && s <= n_kc; s *= 2) {
+            const int64_t units = (int64_t)p.tiles_w * p.tiles_m * s;
+            if (s > 1 && units > (int64_t)sms * p.per_sm) break;
+            const double stage = std::max(4.0 * terms * tokens / 2, p.stage_bytes / 40.0);
+            const double busiest = (double)((units + sms - 1) / sms);
+            const double hbm = ((double)N + (double)terms * M) * K * 17 / 32 / (23.0 * sms);
+            const double t = std::max(busiest * ((n_kc + s - 1) / s) * stage, hbm) + 3000.0 * ((units + (int64_t)sms * p.per_sm - 1) / ((int64_t)sms * p.per_sm)) +
+                             (s > 1 ? 1500.0 + 20.0 * tokens : 0.0) + 30.0 * tokens;
+            if (t < best_t) {
+                best_t = t;
+                p.splits = s;
+                *best = p;
+            }
+        }
+    }
+    return best_t < 1e300;
+}
+
+template <int DT>
+int launch(const Plan& p, const CUtensorMap& w, const CUtensorMap& a, MatmulArgs g, int sms, cudaStream_t stream) {
+    cudaLaunchConfig_t cfg = {};
+    const int64_t units = (int64_t)p.tiles_w * p.tiles_m * p.splits;
+    cfg.gridDim = dim3((unsigned)(p.splits > 1 ? units : std::min<int64_t>(units, (int64_t)sms * p.per_sm)));
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = (size_t)p.smem;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = (unsigned)p.splits;
+    attr[1].val.clusterDim.y = 1;
+    attr[1].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = p.splits > 1 ? 2 : 1;
+    DSX_CUDA(cudaLaunchKernelEx(&cfg, mxfp4_matmul_kernel<DT>, w, a, g));
+    DSX_LAUNCHED();
+    return DSX_OK;
+}
+
+// SM count of the current device; the opt-in to large shared memory is made once per device.
+int configure(int* sms) {
+    constexpr int kMaxDevices = 64;
+    static std::atomic<int> sm_counts[kMaxDevices];
+    int dev = 0;
+    DSX_CUDA(cudaGetDevice(&dev));
+    DSX_REQUIRE(dev >= 0 && dev < kMaxDevices, "mxfp4_matmul: device index %d out of range", dev);
+    int n = sm_counts[dev].load(std::memory_order_acquire);
+    if (n == 0) {
+        DSX_CUDA(cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev));
+        DSX_CUDA(cudaFuncSetAttribute(mxfp4_matmul_kernel<DSX_F32>, cudaFuncAttributeMaxDynamicSharedMemorySize, kLargeMax));
+        DSX_CUDA(cudaFuncSetAttribute(mxfp4_matmul_kernel<DSX_BF16>, cudaFuncAttributeMaxDynamicSharedMemorySize, kLargeMax));
+        DSX_CUDA(cudaFuncSetAttribute(mxfp4_matmul_kernel<DSX_F16>, cudaFuncAttributeMaxDynamicSharedMemorySize, kLargeMax));
+        sm_counts[dev].store(n, std::memory_order_release);
+    }
+    *sms = n;
+    return DSX_OK;
 }
 
 }  // namespace
@@ -57,8 +499,10 @@ mxfp4_matmul_kernel(const uint32_t* __restrict__ a_codes, const uint8_t* __restr
 
 using namespace dsx;
 
-extern "C" int dsx_mxfp4_matmul(const void* a_codes, const void* a_scales, int n_terms, int64_t m, const void* w_codes, const void* w_scales, int64_t n,
-                                int64_t k, void* out, int dtype, int64_t row_stride, dsx_stream_t stream) {
+extern "C" {
+
+int dsx_mxfp4_matmul(const void* a_codes, const void* a_scales, int n_terms, int64_t m, const void* w_codes, const void* w_scales, int64_t n,
+                     int64_t k, void* out, int dtype, int64_t row_stride, dsx_stream_t stream) {
     DSX_REQUIRE(dtype_ok(dtype), "mxfp4_matmul: unknown element type %d", dtype);
     DSX_REQUIRE(m >= 0 && n >= 0 && k >= 32 && k % 32 == 0 && m < ((int64_t)1 << 22) && n < ((int64_t)1 << 31) && k <= ((int64_t)1 << 30),
                 "mxfp4_matmul: %lld x %lld x %lld (k a multiple of 32)", (long long)m, (long long)n, (long long)k);
@@ -68,15 +512,52 @@ extern "C" int dsx_mxfp4_matmul(const void* a_codes, const void* a_scales, int n
     DSX_REQUIRE(row_stride >= n || m == 1, "mxfp4_matmul: row stride %lld below the %lld columns of a row", (long long)row_stride, (long long)n);
     DSX_REQUIRE((((uintptr_t)a_codes | (uintptr_t)w_codes) & 15) == 0 && ((uintptr_t)out & (dtype_size(dtype) - 1)) == 0,
                 "mxfp4_matmul: codes must be 16-byte aligned, out aligned to its elements");
-    const dim3 grid((unsigned)((n + kTile - 1) / kTile), (unsigned)((m + kTile - 1) / kTile));
+    int sms = 0;
+    if (int rc = configure(&sms)) return rc;
+    Plan p;
+    if (!make_plan(m, n, (int)k, n_terms, sms, &p)) return set_error(DSX_ERR_UNSUPPORTED, "mxfp4_matmul: no tile for %d terms", n_terms);
+    DSX_REQUIRE((int64_t)p.tiles_w * p.tiles_m < ((int64_t)1 << 30), "mxfp4_matmul: too many tiles");
+    CUtensorMap tw, ta;
+    {
+        const cuuint64_t dims[2] = {(cuuint64_t)(k / 2), (cuuint64_t)n};
+        const cuuint64_t strides[1] = {(cuuint64_t)(k / 2)};
+        const cuuint32_t box[2] = {(cuuint32_t)kRowBytes, (cuuint32_t)kWRows};
+        if (int rc = tmap_encode(&tw, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, w_codes, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B)) return rc;
+    }
+    {
+        const cuuint64_t dims[3] = {(cuuint64_t)(k / 2), (cuuint64_t)m, (cuuint64_t)n_terms};
+        const cuuint64_t strides[2] = {(cuuint64_t)(k / 2), (cuuint64_t)(m * (k / 2))};
+        const cuuint32_t box[3] = {(cuuint32_t)kRowBytes, (cuuint32_t)p.tokens, (cuuint32_t)n_terms};
+        if (int rc = tmap_encode(&ta, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, a_codes, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B)) return rc;
+    }
+    MatmulArgs g{};
+    g.w_scales = (const uint8_t*)w_scales;
+    g.a_scales = (const uint8_t*)a_scales;
+    g.out = out;
+    g.row_stride = row_stride;
+    g.M = m; g.N = n; g.K = (int)k; g.terms = n_terms;
+    g.tokens = p.tokens; g.stages = p.stages; g.stage_bytes = p.stage_bytes; g.chunks = p.chunks; g.tmem_cols = p.tmem_cols; g.splits = p.splits;
+    g.tiles_w = p.tiles_w; g.tiles = p.tiles_w * p.tiles_m;
+    g.words = k % 128 == 0 && (((uintptr_t)a_scales | (uintptr_t)w_scales) & 3) == 0;
     const cudaStream_t s = (cudaStream_t)stream;
-#define DSX_GO(DT)                                                                                                                              \
-    mxfp4_matmul_kernel<DT><<<grid, 256, 0, s>>>((const uint32_t*)a_codes, (const uint8_t*)a_scales, n_terms, m, (const uint32_t*)w_codes,       \
-                                                 (const uint8_t*)w_scales, n, k, out, row_stride)
-    if (dtype == DSX_F32) DSX_GO(DSX_F32);
-    else if (dtype == DSX_BF16) DSX_GO(DSX_BF16);
-    else DSX_GO(DSX_F16);
-#undef DSX_GO
-    DSX_LAUNCHED();
+    if (dtype == DSX_F32) return launch<DSX_F32>(p, tw, ta, g, sms, s);
+    if (dtype == DSX_BF16) return launch<DSX_BF16>(p, tw, ta, g, sms, s);
+    return launch<DSX_F16>(p, tw, ta, g, sms, s);
+}
+
+int dsx_head_check(dsx_stream_t stream_, uint32_t* error_word) {
+    cudaStream_t stream = (cudaStream_t)stream_;
+    uint32_t w = 0;
+    DSX_CUDA(cudaMemcpyFromSymbolAsync(&w, g_head_error, 4, 0, cudaMemcpyDeviceToHost, stream));
+    DSX_CUDA(cudaStreamSynchronize(stream));
+    if (w) {
+        const uint32_t zero = 0;
+        DSX_CUDA(cudaMemcpyToSymbolAsync(g_head_error, &zero, 4, 0, cudaMemcpyHostToDevice, stream));
+        DSX_CUDA(cudaStreamSynchronize(stream));
+    }
+    if (error_word) *error_word = w;
+    if (w) return set_error(DSX_ERR_DEVICE, "the MXFP4 product reported error word 0x%x (a bounded wait ran out)", w);
     return DSX_OK;
 }
+
+}  // extern "C"

@@ -112,6 +112,15 @@ class Mxfp4Matmul:
         return out
 
 
+def check() -> int:
+    """The product's device-side error word on the current device (0 = clean).  Clears it; synchronises the stream."""
+    w = C.c_uint32()
+    rc = lib().dsx_head_check(_stream(), C.byref(w))
+    if rc != -3:   # DSX_ERR_DEVICE only says that the word is non-zero
+        _check(rc)
+    return w.value
+
+
 class TokenLogprobs:
     """Log probabilities of given tokens, entropy and the most likely alternatives of rows of logits, in one pass over them."""
 

@@ -532,6 +532,9 @@ DSX_API int dsx_mxfp4_dequantize(const void* codes, const void* scales, int64_t 
 DSX_API int dsx_mxfp4_matmul(const void* a_codes, const void* a_scales, int n_terms, int64_t m, const void* w_codes,
                              const void* w_scales, int64_t n, int64_t k, void* out, int dtype, int64_t row_stride,
                              dsx_stream_t stream);
+/* Reads (and clears) the device-side error word of the product on the current device; synchronises the stream.  Non-zero (bit 1: a
+ * bounded wait inside dsx_mxfp4_matmul ran out, results of that call are missing) returns DSX_ERR_DEVICE. */
+DSX_API int dsx_head_check(dsx_stream_t stream, uint32_t* error_word);
 /* Per row of v logits, with z = logit * inv_temperature:
  *   logprobs     f32 [t, n_given]  z[token] - logsumexp(z) of the given tokens; a token outside [0, v) gives -inf
  *   entropy      f32 [t]           of the row's distribution, in nats; may be NULL

@@ -431,6 +431,13 @@ def test_captured_head_replays_on_new_inputs(torch_cuda, moe, T):
                 assert torch.equal(got, want)
 
 
+@pytest.fixture(autouse=True)
+def _no_wait_ran_out(torch_cuda, moe):
+    yield
+    from deepstrix_b200 import head
+    assert head.check() == 0
+
+
 def test_same_bits_on_every_call_and_stream(torch_cuda, moe):
     """No sum depends on the order in which blocks finish: repeated calls, on two streams at once, give the same bits."""
     torch = torch_cuda
