@@ -6,17 +6,17 @@
 // (crates/v4flash-kernels/kernels/softmax_sample.hip) and the teacher-forced scoring of tests/v41_golden_gate.rs.
 //
 // One pass.  A thread keeps its own running maximum and its s and u relative to it; it takes 32 bytes of logits at a time and rescales
-// only when their maximum is new, so an element costs about one conversion, one subtraction, one exponential and three
-// multiply-adds.  The alternatives ride on the same maximum: a chunk is looked at again only when its largest logit reaches the
-// block's threshold, a value that at least n_alt logits of the row are known to reach.  What reaches it goes to the warp's candidate list
-// in shared memory; 32 candidates at a time are sorted in registers and merged into the warp's best 32 (one key per lane), whose
-// n_alt-th becomes the new threshold.  A sorted row that beats the threshold at every element is slow, but right.
+// only when their maximum is new.  Pairs of f32 go through the packed add, multiply and fused multiply-add of sm_100: an element costs
+// about five and a half issue slots, one of them the exponential.
+// The alternatives cost the loop nothing: afterwards the n_alt-th largest of the threads' maxima (of pairs of threads) is a value that
+// at least n_alt logits reach, and hardly more do, so only the threads whose maximum reaches it have their chunks read again (from L2) for
+// the few logits that do; those are ranked by counting.  Where more than the list holds reach it -- a row of equal logits, say, or one masked with the
+// lowest value -- a second pass keeps the best 32 of every warp in registers, sorting candidates 32 at a time.
 // A row belongs to one block, or, when there are few rows, to the blocks of a cluster that join their sums and lists through
 // distributed shared memory: one launch, no workspace, and the order of every addition is fixed.
 //
-// Bound: HBM for f32 and for short lists; bf16 and f16 rows at full HBM rate are 11.6 elements a clock and SM, of which the exponentials
-// take 16 lanes a clock -- so the instruction count above is what matters there.
-#include <algorithm>
+// Bound: HBM; bf16 and f16 rows at the full rate are 11.6 elements a clock and SM, of which the exponentials can take 16.
+#include <atomic>
 
 #include "head.cuh"
 
@@ -77,238 +77,424 @@ __device__ __forceinline__ uint64_t merge32(uint64_t a, uint64_t b, int lane) {
     return k;
 }
 
-// s and u relative to m: sums of 2^t and t 2^t with t = (x - m) * c.
+// Two f32 in one register pair.
+__device__ __forceinline__ uint64_t pair(float a, float b) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ void unpair(uint64_t p, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(p)); }
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+
+// 32 bytes of logits: 8 floats or 16 halves, as they were loaded.
+template <typename T> struct Chunk;
+template <> struct Chunk<float> {
+    static constexpr int n = 8;
+    __device__ static void two(const uint32_t (&w)[8], int j, float& a, float& b) { a = __uint_as_float(w[2 * j]); b = __uint_as_float(w[2 * j + 1]); }
+    __device__ static float top(const uint32_t (&w)[8]) {
+        float t = __uint_as_float(w[0]);
+#pragma unroll
+        for (int j = 1; j < 8; j++) t = fmaxf(t, __uint_as_float(w[j]));
+        return t;
+    }
+};
+template <typename T> struct HalfChunk {
+    static constexpr int n = 16;
+    __device__ static void two(const uint32_t (&w)[8], int j, float& a, float& b) { const float2 f = unpack2<T>(w[j]); a = f.x; b = f.y; }
+};
+template <> struct Chunk<__nv_bfloat16> : HalfChunk<__nv_bfloat16> {
+    __device__ static float top(const uint32_t (&w)[8]) {
+        __nv_bfloat162 t = *reinterpret_cast<const __nv_bfloat162*>(&w[0]);
+#pragma unroll
+        for (int j = 1; j < 8; j++) t = __hmax2(t, *reinterpret_cast<const __nv_bfloat162*>(&w[j]));
+        return fmaxf(__low2float(t), __high2float(t));
+    }
+};
+template <> struct Chunk<__half> : HalfChunk<__half> {
+    __device__ static float top(const uint32_t (&w)[8]) {
+        __half2 t = *reinterpret_cast<const __half2*>(&w[0]);
+#pragma unroll
+        for (int j = 1; j < 8; j++) t = __hmax2(t, *reinterpret_cast<const __half2*>(&w[j]));
+        return fmaxf(__low2float(t), __high2float(t));
+    }
+};
+template <typename T>
+__device__ __forceinline__ void load_chunk(const T* p, uint32_t (&w)[8]) {
+    const uint4 w0 = __ldg(reinterpret_cast<const uint4*>(p)), w1 = __ldg(reinterpret_cast<const uint4*>(p) + 1);
+    w[0] = w0.x; w[1] = w0.y; w[2] = w0.z; w[3] = w0.w; w[4] = w1.x; w[5] = w1.y; w[6] = w1.z; w[7] = w1.w;
+}
+
+// A thread's sums relative to its maximum: of 2^t and of t 2^t with t = (x - m) * c.  s = 0 exactly where nothing has been seen.
 struct Sums {
     float m, s, u;
-    // to a larger maximum; s = 0 (nothing yet) stays 0 whatever the difference
+    // to a maximum at least as large; s = 0 stays 0 whatever the difference
     __device__ __forceinline__ void raise(float to, float c) {
         const float t = fmaxf((m - to) * c, -200.0f), e = exp2_fast(t);
         u = (u + s * t) * e;
         s *= e;
         m = to;
     }
-    __device__ __forceinline__ void add(Sums o, float c) {
-        const float to = fmaxf(m, o.m);
-        raise(to, c);
-        o.raise(to, c);
-        s += o.s;
-        u += o.u;
-    }
 };
 
-template <typename T> struct Chunk;   // 32 bytes: 8 floats or 16 halves
-template <> struct Chunk<float> { static constexpr int n = 8; };
-template <> struct Chunk<__nv_bfloat16> { static constexpr int n = 16; };
-template <> struct Chunk<__half> { static constexpr int n = 16; };
+constexpr int kList = 512;   // candidates the block ranks by counting
 
 struct Shared {
-    uint32_t threshold;                     // order of a value that n_alt logits of the row reach (kFloor: any)
-    int pending[kWarps];                    // candidates on the warps' lists
-    Sums sums[kWarps];
-    uint64_t best[kWarps][32];
-    Sums block_sums;
+    float warp_m[kWarps], warp_s[kWarps], warp_u[kWarps];
+    uint32_t group_top[kThreads / 2];       // order of the maxima of pairs of threads, 0 where they saw nothing
+    uint32_t threshold;                     // order of a value that n_alt logits of the row's part reach (kFloor: any)
+    int count;                              // candidates that reach it
+    int pending[kWarps];                    // second pass: candidates on the warps' lists
+    uint64_t list[kList];
+    uint64_t best[kMaxAlt];                 // the part's best, descending, 0 = nothing
+    float block_sums[3];
     float stats[2];                         // the row's m and ln s
 };
 
+// best[0 .. n_alt) = the n_alt largest of the n distinct keys of `list`, descending: a key's place is the number of larger ones.
+__device__ __forceinline__ void rank_list(const uint64_t* list, int n, int n_alt, uint64_t* best) {
+    for (int i = threadIdx.x; i < n; i += kThreads) {
+        const uint64_t k = list[i];
+        int r = 0;
+        for (int j = 0; j < n; j++) r += list[j] > k ? 1 : 0;
+        if (r < n_alt) best[r] = k;
+    }
+}
+
 template <int DT>
 __global__ void __launch_bounds__(kThreads)
-token_logprobs_kernel(const void* __restrict__ logits, int64_t T_rows, int64_t V, int64_t row_stride, float scale, const int32_t* __restrict__ tokens,
-                      int n_given, float* __restrict__ logprobs, float* __restrict__ entropy, int n_alt, int32_t* __restrict__ alts,
-                      float* __restrict__ alt_logprobs, int splits) {
+token_logprobs_kernel(const void* __restrict__ logits, int64_t V, int64_t row_stride, float scale, const int32_t* __restrict__ tokens, int n_given,
+                      float* __restrict__ logprobs, float* __restrict__ entropy, int n_alt, int32_t* __restrict__ alts, float* __restrict__ alt_logprobs,
+                      int splits) {
     using T = typename Elem<DT>::T;
-    constexpr int kChunk = Chunk<T>::n;
-    constexpr int kList = 64 + 32 * kChunk;     // candidates of a warp: fewer than 32 left over, a chunk of every lane, the elements at the edges
-    extern __shared__ uint64_t s_list[];        // [warps][kList]
-    __shared__ Shared sh;
+    using Ch = Chunk<T>;
+    constexpr int kChunk = Ch::n;
+    constexpr int kWarpList = 64 + 32 * kChunk;  // second pass, candidates of a warp: fewer than 32 left over, a chunk of every lane, the edges
+    extern __shared__ uint64_t s_warp_list[];    // [warps][kWarpList]
+    __shared__ __align__(16) Shared sh;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const uint32_t rank = splits > 1 ? blockIdx.x % splits : 0;
+    const int rank = splits > 1 ? (int)(blockIdx.x % (unsigned)splits) : 0;
+    const int64_t row = blockIdx.x / (unsigned)splits;
     const float c = scale * kLog2e;
-    uint64_t* list = s_list + (size_t)warp * kList;
+    const T* __restrict__ x = reinterpret_cast<const T*>(logits) + row * row_stride;
+    // whole 16-byte words from the row's first aligned element on; the few elements before and after them one by one
+    const int head = (int)min((int64_t)(((16u - (uint32_t)((uintptr_t)x & 15u)) & 15u) / sizeof(T)), V);
+    const int64_t n_chunks = (V - head) / kChunk;
+    const int64_t body = head + n_chunks * kChunk;
+    const int extra = rank == 0 ? head + (int)(V - body) : 0;          // fewer than 8 + kChunk, one a lane of the first block's first warp
+    const int64_t extra_at = lane < head ? lane : body + (lane - head);
+    const bool has_extra = warp == 0 && lane < extra;
+    // chunk i of this thread is first + i * step
+    const int64_t step = (int64_t)kThreads * splits, first = (int64_t)rank * kThreads + threadIdx.x;
+    const T* chunks = x + head;
 
-    for (int64_t row = blockIdx.x / splits; row < T_rows; row += gridDim.x / splits) {
-        const T* __restrict__ x = reinterpret_cast<const T*>(logits) + row * row_stride;
-        if (threadIdx.x == 0) sh.threshold = kFloor;
-        if (threadIdx.x < kWarps) sh.pending[threadIdx.x] = 0;
-        __syncthreads();
-        // whole 16-byte words from the row's first aligned element on; the few elements before and after them one by one
-        const int head = (int)min((int64_t)(((16u - (uint32_t)((uintptr_t)x & 15u)) & 15u) / sizeof(T)), V);
-        const int64_t n_chunks = (V - head) / kChunk;
-        const int64_t body = head + n_chunks * kChunk;
-        Sums a{kLowest, 0.0f, 0.0f};
-        uint64_t mine = 0ull;                   // the warp's best, descending over its lanes
-        uint32_t own = kFloor;                  // lowest order that may still enter that list, for elements behind those in it
-        auto flush = [&](bool all) {            // merge candidates 32 at a time; the rest stays (or goes too, padded with nothing)
-            int pending = *(volatile int*)&sh.pending[warp];
-            if (!all && pending < 32) return;
-            while (pending >= 32 || (all && pending > 0)) {
-                const int n = min(pending, 32);
-                const uint64_t k = lane < n ? list[pending - n + lane] : 0ull;
-                pending -= n;
-                mine = merge32(mine, sort32(k, lane), lane);
-            }
-            __syncwarp();
-            const uint32_t kth = (uint32_t)(__shfl_sync(0xFFFFFFFFu, mine, n_alt - 1) >> 32);
-            if (lane == 0) {
-                sh.pending[warp] = pending;
-                if (kth != 0u) atomicMax(&sh.threshold, kth);
-            }
-            if (kth != 0u) own = kth + 1u;      // what comes later has a higher index: an equal logit loses
-            __syncwarp();
-        };
-        auto load = [&](int64_t ch, uint32_t (&w)[8]) {
-            const uint4* p = reinterpret_cast<const uint4*>(x + head + ch * kChunk);
-            const uint4 w0 = __ldg(p), w1 = __ldg(p + 1);
-            w[0] = w0.x; w[1] = w0.y; w[2] = w0.z; w[3] = w0.w; w[4] = w1.x; w[5] = w1.y; w[6] = w1.z; w[7] = w1.w;
-        };
-        // every warp takes whole rounds, so that its votes are complete; the next round's logits are requested before this one's work
-        const int64_t per_round = (int64_t)kThreads * splits;
-        const int64_t ch0 = (int64_t)rank * kThreads + threadIdx.x;
+    // ------------------------------------------------------------------ sums
+    Sums a{kLowest, 0.0f, 0.0f};
+    if (has_extra) {
+        const float v = to_f32(x[extra_at]);
+        if (v > a.m) a.m = v;
+        const float t = max_nan((v - a.m) * c, -200.0f);
+        a.s = exp2_fast(t);
+        a.u = t * a.s;
+    }
+    {
+        uint64_t s2 = pair(a.s, 0.0f), u2 = pair(a.u, 0.0f);
+        const uint64_t c2 = pair(c, c);
         uint32_t next[8];
-        if (ch0 < n_chunks) load(ch0, next);
-        for (int64_t ch = ch0; ch - lane < n_chunks; ch += per_round) {
-            const bool live = ch < n_chunks;
-            float v[kChunk];
-            if constexpr (sizeof(T) == 4) {
+        if (first < n_chunks) load_chunk(chunks + first * kChunk, next);
+        for (int64_t ch = first; ch < n_chunks; ch += step) {
+            uint32_t w[8];
 #pragma unroll
-                for (int j = 0; j < 8; j++) v[j] = __uint_as_float(next[j]);
-            } else {
+            for (int j = 0; j < 8; j++) w[j] = next[j];
+            if (ch + step < n_chunks) load_chunk(chunks + (ch + step) * kChunk, next);   // requested before this one's work
+            const float top = Ch::top(w);
+            if (top > a.m) {
+                const float t = fmaxf((a.m - top) * c, -200.0f), e = exp2_fast(t);
+                const uint64_t e2 = pair(e, e);
+                u2 = mul2(fma2(s2, pair(t, t), u2), e2);
+                s2 = mul2(s2, e2);
+                a.m = top;
+            }
+            const uint64_t minus_m = pair(-a.m, -a.m);
 #pragma unroll
-                for (int j = 0; j < 8; j++) {
-                    const float2 f = unpack2<T>(next[j]);
-                    v[2 * j] = f.x;
-                    v[2 * j + 1] = f.y;
+            for (int j = 0; j < kChunk / 2; j++) {
+                float v0, v1, t0, t1;
+                Ch::two(w, j, v0, v1);
+                unpair(mul2(add2(pair(v0, v1), minus_m), c2), t0, t1);
+                t0 = max_nan(t0, -200.0f);     // a masked logit: 2^-200 is 0, and 0 * -200 too
+                t1 = max_nan(t1, -200.0f);
+                const uint64_t e = pair(exp2_fast(t0), exp2_fast(t1));
+                s2 = add2(s2, e);
+                u2 = fma2(pair(t0, t1), e, u2);
+            }
+        }
+        float s0, s1, u0, u1;
+        unpair(s2, s0, s1);
+        unpair(u2, u0, u1);
+        a.s = s0 + s1;
+        a.u = u0 + u1;
+    }
+
+    // block: the maximum first, then the sums relative to it, always in the same order
+    {
+        const bool none = a.s == 0.0f;
+        uint32_t top = none ? 0u : order_of(a.m);
+        float m = a.m;
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, o));
+        if (lane == 0) sh.warp_m[warp] = m;
+        if (n_alt > 0) {
+            top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, 1));
+            if ((lane & 1) == 0) sh.group_top[threadIdx.x >> 1] = top;
+        }
+        if (threadIdx.x == 0) {
+            sh.threshold = kFloor;
+            sh.count = 0;
+        }
+        if (threadIdx.x < kMaxAlt) sh.best[threadIdx.x] = 0ull;
+        __syncthreads();
+        float bm = sh.warp_m[0];
+#pragma unroll
+        for (int w = 1; w < kWarps; w++) bm = fmaxf(bm, sh.warp_m[w]);
+        Sums r = a;
+        r.raise(bm, c);
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) {
+            r.s += __shfl_xor_sync(0xFFFFFFFFu, r.s, o);
+            r.u += __shfl_xor_sync(0xFFFFFFFFu, r.u, o);
+        }
+        if (lane == 0) {
+            sh.warp_s[warp] = r.s;
+            sh.warp_u[warp] = r.u;
+        }
+        // the n_alt-th largest of the pairs' maxima: the one that n_alt - 1 are above (equal ones in the order of their places)
+        if (n_alt > 0 && threadIdx.x < kThreads / 2) {
+            const uint32_t mine = sh.group_top[threadIdx.x];
+            int above = 0;
+#pragma unroll 8
+            for (int j = 0; j < kThreads / 8; j++) {
+                const uint4 o = reinterpret_cast<const uint4*>(sh.group_top)[j];
+                const int at = 4 * j;
+                above += (o.x > mine || (o.x == mine && at < (int)threadIdx.x)) + (o.y > mine || (o.y == mine && at + 1 < (int)threadIdx.x)) +
+                         (o.z > mine || (o.z == mine && at + 2 < (int)threadIdx.x)) + (o.w > mine || (o.w == mine && at + 3 < (int)threadIdx.x));
+            }
+            if (above == n_alt - 1 && mine > kFloor) sh.threshold = mine;
+        }
+        __syncthreads();
+        if (threadIdx.x == 0) {
+            float s = 0.0f, u = 0.0f;
+#pragma unroll
+            for (int w = 0; w < kWarps; w++) {
+                s += sh.warp_s[w];
+                u += sh.warp_u[w];
+            }
+            sh.block_sums[0] = bm;
+            sh.block_sums[1] = s;
+            sh.block_sums[2] = u;
+        }
+    }
+
+    // ---------------------------------------------------------- alternatives
+    if (n_alt > 0) {
+        const float least = value_of(sh.threshold);
+        auto push = [&](float v, int64_t i) {
+            const int at = atomicAdd(&sh.count, 1);
+            if (at < kList) sh.list[at] = key_of(v, (uint32_t)i);
+        };
+        if (has_extra) {
+            const float v = to_f32(x[extra_at]);
+            if (v >= least) push(v, extra_at);
+        }
+        // the warp reads the chunks of each of its threads that qualify, a lane each
+        for (uint32_t q = __ballot_sync(0xFFFFFFFFu, a.s != 0.0f && a.m >= least); q != 0u; q &= q - 1u) {
+            const int64_t from = first - lane + (__ffs(q) - 1);
+            for (int64_t ch = from + lane * step; ch < n_chunks; ch += 32 * step) {
+                uint32_t w[8];
+                load_chunk(chunks + ch * kChunk, w);
+                if (Ch::top(w) >= least) {
+#pragma unroll
+                    for (int j = 0; j < kChunk / 2; j++) {
+                        float v0, v1;
+                        Ch::two(w, j, v0, v1);
+                        if (v0 >= least) push(v0, head + ch * kChunk + 2 * j);
+                        if (v1 >= least) push(v1, head + ch * kChunk + 2 * j + 1);
+                    }
                 }
             }
-            if (ch + per_round < n_chunks) load(ch + per_round, next);
-            float top = v[0];
-#pragma unroll
-            for (int j = 1; j < kChunk; j++) top = fmaxf(top, v[j]);
-            if (live) {
-                if (top > a.m) a.raise(top, c);
-#pragma unroll
-                for (int j = 0; j < kChunk; j++) {
-                    const float t = max_nan((v[j] - a.m) * c, -200.0f), e = exp2_fast(t);
-                    a.s += e;
-                    a.u = fmaf(t, e, a.u);
+        }
+        __syncthreads();
+        if (sh.count <= kList) {
+            rank_list(sh.list, sh.count, n_alt, sh.best);
+        } else {
+            // too many: a second pass over the part, in which a warp keeps its best 32 (one a lane) and lists only what may enter them.
+            // Its chunks come in ascending order, so an equal logit behind a full list is out: rows of equal logits cost one compare each.
+            uint64_t* list = s_warp_list + (size_t)warp * kWarpList;
+            uint64_t mine = 0ull;
+            uint32_t own = sh.threshold;
+            if (lane == 0) sh.pending[warp] = 0;
+            __syncwarp();
+            auto flush = [&](bool all) {   // merge candidates 32 at a time; the rest stays (or goes too, padded with nothing)
+                int pending = *(volatile int*)&sh.pending[warp];
+                if (!all && pending < 32) return;
+                while (pending >= 32 || (all && pending > 0)) {
+                    const int n = min(pending, 32);
+                    const uint64_t k = lane < n ? list[pending - n + lane] : 0ull;
+                    pending -= n;
+                    mine = merge32(mine, sort32(k, lane), lane);
                 }
-            }
-            if (n_alt > 0) {
-                uint32_t bound = max(own, *(volatile uint32_t*)&sh.threshold);
-                if (ch == ch0) {   // first round: n_alt of the 32 chunks reach the n_alt-th largest of their maxima
-                    const uint64_t k = sort32(live && top >= kLowest ? (uint64_t)order_of(top) : 0ull, lane);
-                    bound = max(bound, (uint32_t)__shfl_sync(0xFFFFFFFFu, k, n_alt - 1));
-                    if (lane == 0) atomicMax(&sh.threshold, bound);
-                }
-                const float least = value_of(bound);
-                if (__any_sync(0xFFFFFFFFu, live && top >= least)) {
-                    if (live && top >= least) {
+                __syncwarp();
+                const uint32_t kth = (uint32_t)(__shfl_sync(0xFFFFFFFFu, mine, n_alt - 1) >> 32);
+                if (lane == 0) sh.pending[warp] = pending;
+                if (kth != 0u) own = kth + 1u;
+                __syncwarp();
+            };
+            for (int64_t ch = first; ch - lane < n_chunks; ch += step) {
+                uint32_t w[8];
+                const bool live = ch < n_chunks;
+                if (live) load_chunk(chunks + ch * kChunk, w);
+                const float least = value_of(own);
+                const bool any = live && Ch::top(w) >= least;
+                if (__any_sync(0xFFFFFFFFu, any)) {
+                    if (any) {
 #pragma unroll
-                        for (int j = 0; j < kChunk; j++)
-                            if (v[j] >= least) list[atomicAdd(&sh.pending[warp], 1)] = key_of(v[j], (uint32_t)(head + ch * kChunk + j));
+                        for (int j = 0; j < kChunk / 2; j++) {
+                            float v0, v1;
+                            Ch::two(w, j, v0, v1);
+                            if (v0 >= least) list[atomicAdd(&sh.pending[warp], 1)] = key_of(v0, (uint32_t)(head + ch * kChunk + 2 * j));
+                            if (v1 >= least) list[atomicAdd(&sh.pending[warp], 1)] = key_of(v1, (uint32_t)(head + ch * kChunk + 2 * j + 1));
+                        }
                     }
                     __syncwarp();
                     flush(false);
                 }
             }
-        }
-        // the elements outside the aligned words, fewer than 8 + kChunk: one a lane, first block and warp
-        if (rank == 0 && warp == 0) {
-            const int extra = head + (int)(V - body);
-            const int64_t i = lane < head ? lane : body + (lane - head);
-            if (lane < extra) {
-                const float v = to_f32(x[i]);
-                if (v > a.m) a.raise(v, c);
-                const float t = max_nan((v - a.m) * c, -200.0f), e = exp2_fast(t);
-                a.s += e;
-                a.u = fmaf(t, e, a.u);
-                // some of these come before all others: an equal logit may win
-                if (n_alt > 0 && v >= kLowest) list[atomicAdd(&sh.pending[warp], 1)] = key_of(v, (uint32_t)i);
+            if (has_extra) {   // some of these come before all others: an equal logit may win
+                const float v = to_f32(x[extra_at]);
+                if (v >= kLowest) list[atomicAdd(&sh.pending[warp], 1)] = key_of(v, (uint32_t)extra_at);
             }
             __syncwarp();
-        }
-        if (n_alt > 0) flush(true);
-        // warp, block, cluster: always in the same order
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) {
-            const Sums b{__shfl_xor_sync(0xFFFFFFFFu, a.m, o), __shfl_xor_sync(0xFFFFFFFFu, a.s, o), __shfl_xor_sync(0xFFFFFFFFu, a.u, o)};
-            a.add(b, c);
-        }
-        if (lane == 0) sh.sums[warp] = a;
-        sh.best[warp][lane] = mine;
-        __syncthreads();
-        if (warp == 0) {
-            a = sh.sums[0];
-            for (int w = 1; w < kWarps; w++) a.add(sh.sums[w], c);
-            if (n_alt > 0)
-                for (int w = 1; w < kWarps; w++) mine = merge32(mine, sh.best[w][lane], lane);
-            if (splits > 1) {
-                sh.best[0][lane] = mine;
-                if (lane == 0) sh.block_sums = a;
+            flush(true);
+            __syncthreads();
+            sh.list[threadIdx.x] = mine;   // 256 of them; empty places (0) rank last
+            __syncthreads();
+            if (mine != 0ull) {
+                int r = 0;
+                for (int j = 0; j < kThreads; j++) r += sh.list[j] > mine ? 1 : 0;
+                if (r < n_alt) sh.best[r] = mine;
             }
         }
-        if (splits > 1) {
-            asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-            if (rank == 0 && warp == 0) {
-                const uint32_t sums_at = (uint32_t)__cvta_generic_to_shared(&sh.block_sums), best_at = (uint32_t)__cvta_generic_to_shared(&sh.best[0][lane]);
-                for (int p = 1; p < splits; p++) {
+    }
+    __syncthreads();
+
+    // --------------------------------------------------------------- the row
+    float m = sh.block_sums[0], s = sh.block_sums[1], u = sh.block_sums[2];
+    if (splits > 1) {
+        asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+        if (rank == 0) {
+            // a lane of the first warp per block for the sums; n_alt keys of every block for the alternatives
+            if (warp == 0) {
+                Sums p{kLowest, 0.0f, 0.0f};
+                if (lane < splits) {
                     uint32_t at;
-                    Sums b;
-                    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(sums_at), "r"(p));
-                    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(b.m) : "r"(at) : "memory");
-                    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(b.s) : "r"(at + 4) : "memory");
-                    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(b.u) : "r"(at + 8) : "memory");
-                    a.add(b, c);
-                    if (n_alt > 0) {
-                        uint64_t k;
-                        asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(best_at), "r"(p));
-                        asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(k) : "r"(at) : "memory");
-                        mine = merge32(mine, k, lane);
-                    }
+                    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"((uint32_t)__cvta_generic_to_shared(sh.block_sums)), "r"(lane));
+                    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(p.m) : "r"(at) : "memory");
+                    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(p.s) : "r"(at + 4) : "memory");
+                    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(p.u) : "r"(at + 8) : "memory");
+                }
+                m = p.m;
+#pragma unroll
+                for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, o));
+                p.raise(m, c);
+                s = p.s;
+                u = p.u;
+#pragma unroll
+                for (int o = 16; o > 0; o >>= 1) {
+                    s += __shfl_xor_sync(0xFFFFFFFFu, s, o);
+                    u += __shfl_xor_sync(0xFFFFFFFFu, u, o);
                 }
             }
+            if (n_alt > 0) {
+                for (int i = threadIdx.x; i < splits * n_alt; i += kThreads) {
+                    uint32_t at;
+                    uint64_t k;
+                    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"((uint32_t)__cvta_generic_to_shared(&sh.best[i % n_alt])), "r"(i / n_alt));
+                    asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(k) : "r"(at) : "memory");
+                    sh.list[i] = k;
+                }
+                __syncthreads();
+                for (int i = threadIdx.x; i < splits * n_alt; i += kThreads) {
+                    const uint64_t k = sh.list[i];
+                    int r = 0;
+                    for (int j = 0; j < splits * n_alt; j++) r += sh.list[j] > k ? 1 : 0;
+                    if (k != 0ull && r < n_alt) sh.best[r] = k;
+                }
+                __syncthreads();
+            }
         }
+    }
+    if (rank == 0) {
         // s: NaN where the row holds a NaN or +inf, 0 where it is masked as a whole
         const float nan = __uint_as_float(0x7FC00000u);
-        if (rank == 0) {
-            if (warp == 0) {
-                const bool bad = a.s != a.s, empty = a.s == 0.0f;
-                const float log_s = empty ? 0.0f : logf(a.s), m = bad ? nan : (empty ? 0.0f : a.m);
-                if (lane == 0) {
-                    sh.stats[0] = m;
-                    sh.stats[1] = log_s;
-                    if (entropy != nullptr) entropy[row] = bad ? nan : (empty ? 0.0f : log_s - kLn2 * (a.u / a.s));
-                }
-                if (lane < n_alt) {
-                    const uint32_t o = (uint32_t)(mine >> 32);
-                    const bool none = bad || mine == 0ull;
-                    alts[row * n_alt + lane] = none ? -1 : (int32_t)~(uint32_t)mine;
-                    alt_logprobs[row * n_alt + lane] = bad ? nan : (none ? -INFINITY : (value_of(o) - m) * scale - log_s);
-                }
+        if (warp == 0) {
+            const bool bad = s != s, empty = s == 0.0f;
+            const float log_s = empty ? 0.0f : logf(s);
+            m = bad ? nan : (empty ? 0.0f : m);
+            if (lane == 0) {
+                sh.stats[0] = m;
+                sh.stats[1] = log_s;
+                if (entropy != nullptr) entropy[row] = bad ? nan : (empty ? 0.0f : log_s - kLn2 * (u / s));
             }
+            if (lane < n_alt) {
+                const uint64_t k = sh.best[lane];
+                const bool none = bad || k == 0ull;
+                alts[row * n_alt + lane] = none ? -1 : (int32_t)~(uint32_t)k;
+                alt_logprobs[row * n_alt + lane] = bad ? nan : (none ? -INFINITY : (value_of((uint32_t)(k >> 32)) - m) * scale - log_s);
+            }
+        }
+        if (n_given > 0) {
             __syncthreads();
             for (int g = threadIdx.x; g < n_given; g += kThreads) {
                 const int32_t tok = tokens[row * n_given + g];
                 logprobs[row * n_given + g] = tok >= 0 && tok < V ? (to_f32(x[tok]) - sh.stats[0]) * scale - sh.stats[1] : -INFINITY;
             }
         }
-        // nobody's lists go away (or are overwritten by the next row) while they are read
-        if (splits > 1) asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-        else __syncthreads();
     }
+    // nobody's shared memory goes away while the first block reads it
+    if (splits > 1) asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
 template <int DT>
 int launch(const void* logits, int64_t t, int64_t v, int64_t row_stride, float scale, const int32_t* tokens, int n_given, float* logprobs, float* entropy,
            int n_alt, int32_t* alts, float* alt_logprobs, cudaStream_t stream) {
     using T = typename Elem<DT>::T;
-    int dev = 0, sms = 0;
+    constexpr int kMaxDevices = 64;
+    static std::atomic<int> sm_counts[kMaxDevices];
+    int dev = 0;
     DSX_CUDA(cudaGetDevice(&dev));
-    DSX_CUDA(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev));
-    // few rows: as many blocks a row as still give every thread two chunks, and no more than two blocks an SM in all
+    DSX_REQUIRE(dev >= 0 && dev < kMaxDevices, "token_logprobs: device index %d out of range", dev);
+    int sms = sm_counts[dev].load(std::memory_order_acquire);
+    if (sms == 0) {
+        DSX_CUDA(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev));
+        sm_counts[dev].store(sms, std::memory_order_release);
+    }
+    // few rows: as many blocks a row as still give every thread two chunks, and no more than four blocks an SM in all
     int splits = 1;
-    while (splits < kMaxCluster && t * splits * 2 <= 2 * sms && v >= (int64_t)splits * 2 * 2 * kThreads * Chunk<T>::n) splits *= 2;
+    while (splits < kMaxCluster && t * splits * 2 <= 4 * sms && v >= (int64_t)splits * 2 * 2 * kThreads * Chunk<T>::n) splits *= 2;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)(std::min<int64_t>(t, splits > 1 ? t : (int64_t)1 << 30) * splits));
+    cfg.gridDim = dim3((unsigned)(t * splits));
     cfg.blockDim = dim3(kThreads);
     cfg.dynamicSmemBytes = n_alt > 0 ? sizeof(uint64_t) * kWarps * (64 + 32 * Chunk<T>::n) : 0;
     cfg.stream = stream;
@@ -319,7 +505,7 @@ int launch(const void* logits, int64_t t, int64_t v, int64_t row_stride, float s
     attr[0].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = splits > 1 ? 1 : 0;
-    DSX_CUDA(cudaLaunchKernelEx(&cfg, token_logprobs_kernel<DT>, logits, t, v, row_stride, scale, tokens, n_given, logprobs, entropy, n_alt, alts, alt_logprobs,
+    DSX_CUDA(cudaLaunchKernelEx(&cfg, token_logprobs_kernel<DT>, logits, v, row_stride, scale, tokens, n_given, logprobs, entropy, n_alt, alts, alt_logprobs,
                                 splits));
     DSX_LAUNCHED();
     return DSX_OK;

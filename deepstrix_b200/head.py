@@ -14,54 +14,71 @@ torch is used only for device memory and the current stream; tensors live on the
 from __future__ import annotations
 
 import ctypes as C
-from dataclasses import dataclass
 
 import torch
 
-from .moe import _check, _dptr, _stream, lib
+from .moe import DsxError, lib
 
 DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+_P, _I, _L, _F = C.c_void_p, C.c_int, C.c_int64, C.c_float
+_SIGNATURES = {
+    "dsx_mxfp4_quantize": [_P, _I, _L, _L, _L, _I, _P, _P, _P],
+    "dsx_mxfp4_dequantize": [_P, _P, _L, _L, _I, _P, _I, _L, _P],
+    "dsx_mxfp4_matmul": [_P, _P, _I, _L, _P, _P, _L, _L, _P, _I, _L, _P],
+    "dsx_token_logprobs": [_P, _I, _L, _L, _L, _F, _P, _I, _P, _P, _I, _P, _P, _P],
+    "dsx_head_check": [_P, C.POINTER(C.c_uint32)],
+}
+_functions = {}
 
 
-def _here(*tensors):
-    """All on the current device (kernels run on its current stream)."""
-    for t in tensors:
-        assert t.is_cuda, "tensors must be on the GPU"
-        assert t.device.index == torch.cuda.current_device(), f"tensor on {t.device}, current device is cuda:{torch.cuda.current_device()}"
+def _call(name, *args):
+    """One C call: plain integers for pointers and sizes (a call of this file is a few microseconds of host time; wrapping
+    every argument by hand costs as much again)."""
+    fn = _functions.get(name)
+    if fn is None:
+        fn = getattr(lib(), name)
+        fn.argtypes = _SIGNATURES[name]
+        _functions[name] = fn
+    rc = fn(*args)
+    if rc != 0:
+        raise DsxError(rc, lib().dsx_last_error().decode())
+
+
+def _here(*tensors) -> int:
+    """All on the current device, whose current stream (returned) the kernels run on."""
+    assert all(t.is_cuda for t in tensors), "tensors must be on the GPU"
+    device = torch.cuda.current_device()
+    assert all(t.get_device() == device for t in tensors), f"tensors on {[str(t.device) for t in tensors]}, current device is cuda:{device}"
+    return torch._C._cuda_getCurrentRawStream(device)
 
 
 def _row_stride(t: torch.Tensor) -> int:
     """Elements between rows of a 2-D tensor whose columns are contiguous."""
-    assert t.dim() == 2 and (t.shape[1] <= 1 or t.stride(1) == 1), "rows must have contiguous columns"
-    stride = t.stride(0) if t.shape[0] > 1 else t.shape[1]
-    assert stride >= t.shape[1], "rows must not overlap"
-    return stride
+    assert t.dim() == 2, "a matrix of rows"
+    rows, cols = t.shape
+    row_stride, col_stride = t.stride()
+    assert cols <= 1 or col_stride == 1, "rows must have contiguous columns"
+    if rows <= 1:
+        return cols
+    assert row_stride >= cols, "rows must not overlap"
+    return row_stride
 
 
-@dataclass
 class Mxfp4Rows:
     """Rows as sums of MXFP4 terms: uint8 codes [terms, rows, K / 2] (element 2i in the low nibble) and E8M0 scales
     [terms, rows, K / 32]; two-dimensional tensors are one term (a stored matrix)."""
-    codes: torch.Tensor
-    scales: torch.Tensor
+    __slots__ = ("codes", "scales", "n_terms", "rows", "k")
 
-    def __post_init__(self):
-        c, s = self.codes, self.scales
-        assert c.dtype == torch.uint8 and s.dtype == torch.uint8 and c.is_contiguous() and s.is_contiguous()
-        assert c.dim() in (2, 3) and c.shape[:-1] == s.shape[:-1] and c.shape[-1] == 16 * s.shape[-1], "codes [.., K / 2] and scales [.., K / 32]"
-        assert c.device == s.device
+    def __init__(self, codes: torch.Tensor, scales: torch.Tensor):
+        assert codes.dtype == torch.uint8 and scales.dtype == torch.uint8 and codes.is_contiguous() and scales.is_contiguous()
+        shape = codes.shape
+        assert len(shape) in (2, 3) and shape[:-1] == scales.shape[:-1] and shape[-1] == 16 * scales.shape[-1], "codes [.., K / 2] and scales [.., K / 32]"
+        assert codes.device == scales.device
+        self._set(codes, scales, shape[0] if len(shape) == 3 else 1, shape[-2], 2 * shape[-1])
 
-    @property
-    def n_terms(self) -> int:
-        return self.codes.shape[0] if self.codes.dim() == 3 else 1
-
-    @property
-    def rows(self) -> int:
-        return self.codes.shape[-2]
-
-    @property
-    def k(self) -> int:
-        return self.codes.shape[-1] * 2
+    def _set(self, codes, scales, n_terms, rows, k):
+        self.codes, self.scales, self.n_terms, self.rows, self.k = codes, scales, n_terms, rows, k
+        return self
 
 
 class Mxfp4Quantize:
@@ -70,15 +87,14 @@ class Mxfp4Quantize:
 
     @staticmethod
     def launch(x: torch.Tensor, n_terms: int = 1) -> Mxfp4Rows:
-        assert x.dtype in DTYPES
+        assert x.dtype in DTYPES, f"rows of {x.dtype}"
         stride = _row_stride(x)
-        _here(x)
+        stream = _here(x)
         rows, k = x.shape
         codes = torch.empty((n_terms, rows, k // 2), dtype=torch.uint8, device=x.device)
         scales = torch.empty((n_terms, rows, k // 32), dtype=torch.uint8, device=x.device)
-        _check(lib().dsx_mxfp4_quantize(_dptr(x), DTYPES[x.dtype], C.c_int64(rows), C.c_int64(k), C.c_int64(stride), n_terms, _dptr(codes), _dptr(scales),
-                                        _stream()))
-        return Mxfp4Rows(codes, scales)
+        _call("dsx_mxfp4_quantize", x.data_ptr(), DTYPES[x.dtype], rows, k, stride, n_terms, codes.data_ptr(), scales.data_ptr(), stream)
+        return Mxfp4Rows.__new__(Mxfp4Rows)._set(codes, scales, n_terms, rows, k)
 
 
 class Mxfp4Dequantize:
@@ -86,13 +102,11 @@ class Mxfp4Dequantize:
 
     @staticmethod
     def launch(q: Mxfp4Rows, dtype: torch.dtype = torch.float32, out: torch.Tensor | None = None) -> torch.Tensor:
-        _here(q.codes)
         if out is None:
             out = torch.empty((q.rows, q.k), dtype=dtype, device=q.codes.device)
-        assert out.shape == (q.rows, q.k) and out.dtype == dtype
-        _here(out)
-        _check(lib().dsx_mxfp4_dequantize(_dptr(q.codes), _dptr(q.scales), C.c_int64(q.rows), C.c_int64(q.k), q.n_terms, _dptr(out), DTYPES[dtype],
-                                          C.c_int64(_row_stride(out)), _stream()))
+        assert out.shape == (q.rows, q.k) and out.dtype == dtype and dtype in DTYPES
+        _call("dsx_mxfp4_dequantize", q.codes.data_ptr(), q.scales.data_ptr(), q.rows, q.k, q.n_terms, out.data_ptr(), DTYPES[dtype], _row_stride(out),
+              _here(q.codes, out))
         return out
 
 
@@ -101,23 +115,24 @@ class Mxfp4Matmul:
 
     @staticmethod
     def launch(a: Mxfp4Rows, w: Mxfp4Rows, dtype: torch.dtype = torch.bfloat16, out: torch.Tensor | None = None) -> torch.Tensor:
-        assert w.n_terms == 1 and a.k == w.k
-        _here(a.codes, w.codes)
+        assert w.n_terms == 1, "a weight has one term"
+        assert a.k == w.k, f"rows of {a.k} and of {w.k} columns"
         if out is None:
             out = torch.empty((a.rows, w.rows), dtype=dtype, device=a.codes.device)
-        assert out.shape == (a.rows, w.rows) and out.dtype == dtype
-        _here(out)
-        _check(lib().dsx_mxfp4_matmul(_dptr(a.codes), _dptr(a.scales), a.n_terms, C.c_int64(a.rows), _dptr(w.codes), _dptr(w.scales), C.c_int64(w.rows),
-                                      C.c_int64(a.k), _dptr(out), DTYPES[dtype], C.c_int64(_row_stride(out)), _stream()))
+        assert out.shape == (a.rows, w.rows) and out.dtype == dtype and dtype in DTYPES
+        _call("dsx_mxfp4_matmul", a.codes.data_ptr(), a.scales.data_ptr(), a.n_terms, a.rows, w.codes.data_ptr(), w.scales.data_ptr(), w.rows, a.k,
+              out.data_ptr(), DTYPES[dtype], _row_stride(out), _here(a.codes, w.codes, out))
         return out
 
 
 def check() -> int:
     """The product's device-side error word on the current device (0 = clean).  Clears it; synchronises the stream."""
     w = C.c_uint32()
-    rc = lib().dsx_head_check(_stream(), C.byref(w))
-    if rc != -3:   # DSX_ERR_DEVICE only says that the word is non-zero
-        _check(rc)
+    try:
+        _call("dsx_head_check", torch.cuda.current_stream().cuda_stream, C.byref(w))
+    except DsxError as e:
+        if e.code != -3:   # DSX_ERR_DEVICE only says that the word is non-zero
+            raise
     return w.value
 
 
@@ -129,20 +144,22 @@ class TokenLogprobs:
         """logits [T, V] f32 / bf16 / f16 (any row stride), tokens int32 [T] or [T, n] -> (logprobs f32 like tokens or None,
         entropy f32 [T], ids int32 [T, n_alt], their log probabilities f32 [T, n_alt]).  -inf logits are masked; see
         ``dsx_token_logprobs`` for rows with nothing left and rows that hold a NaN."""
-        assert logits.dtype in DTYPES
+        assert logits.dtype in DTYPES, f"logits of {logits.dtype}"
         stride = _row_stride(logits)
-        _here(logits)
         T, V = logits.shape
         dev = logits.device
-        given, logprobs = 0, None
+        given, logprobs, tokens_at, logprobs_at = 0, None, None, None
         if tokens is not None:
-            assert tokens.dtype == torch.int32 and tokens.is_contiguous() and tokens.dim() in (1, 2) and tokens.shape[0] == T
-            _here(tokens)
+            assert tokens.dtype == torch.int32 and tokens.is_contiguous() and tokens.dim() in (1, 2) and tokens.shape[0] == T, "int32 tokens [T] or [T, n]"
+            stream = _here(logits, tokens)
             given = 1 if tokens.dim() == 1 else tokens.shape[1]
             logprobs = torch.empty(tokens.shape, dtype=torch.float32, device=dev)
+            tokens_at, logprobs_at = tokens.data_ptr(), logprobs.data_ptr()
+        else:
+            stream = _here(logits)
         entropy = torch.empty((T,), dtype=torch.float32, device=dev)
         ids = torch.empty((T, n_alt), dtype=torch.int32, device=dev)
         alternatives = torch.empty((T, n_alt), dtype=torch.float32, device=dev)
-        _check(lib().dsx_token_logprobs(_dptr(logits), DTYPES[logits.dtype], C.c_int64(T), C.c_int64(V), C.c_int64(stride), C.c_float(inv_temperature),
-                                        _dptr(tokens), given, _dptr(logprobs), _dptr(entropy), n_alt, _dptr(ids), _dptr(alternatives), _stream()))
+        _call("dsx_token_logprobs", logits.data_ptr(), DTYPES[logits.dtype], T, V, stride, inv_temperature, tokens_at, given, logprobs_at,
+              entropy.data_ptr(), n_alt, ids.data_ptr(), alternatives.data_ptr(), stream)
         return logprobs, entropy, ids, alternatives
