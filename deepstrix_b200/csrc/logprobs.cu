@@ -152,25 +152,33 @@ struct Sums {
 
 constexpr int kList = 512;   // candidates the block ranks by counting
 
-struct Shared {
+struct alignas(16) Shared {
     float warp_m[kWarps], warp_s[kWarps], warp_u[kWarps];
-    uint32_t group_top[kThreads / 2];       // order of the maxima of pairs of threads, 0 where they saw nothing
-    uint32_t threshold;                     // order of a value that n_alt logits of the row's part reach (kFloor: any)
+    alignas(16) uint32_t group_top[kThreads / 2];       // order of the maxima of pairs of threads, 0 where they saw nothing
+    uint32_t warp_least[kWarps / 2];        // their smallest is the order of a value that n_alt logits of the row's part reach
+    uint32_t readers[kWarps];               // lanes whose chunks are read again
+    int reader[kThreads];                   // and their threads, in order
     int count;                              // candidates that reach it
     int pending[kWarps];                    // second pass: candidates on the warps' lists
-    uint64_t list[kList];
+    alignas(16) uint64_t list[kList + 2];
     uint64_t best[kMaxAlt];                 // the part's best, descending, 0 = nothing
     float block_sums[3];
     float stats[2];                         // the row's m and ln s
 };
 
-// best[0 .. n_alt) = the n_alt largest of the n distinct keys of `list`, descending: a key's place is the number of larger ones.
-__device__ __forceinline__ void rank_list(const uint64_t* list, int n, int n_alt, uint64_t* best) {
+// best[0 .. n_alt) = the n_alt largest of the n keys of `list`, descending: a key's place is the number of larger ones (keys are
+// distinct but for 0, "nothing", which takes no place).  Keys are read two at a time; list[n] is written.
+__device__ __forceinline__ void rank_list(uint64_t* list, int n, int n_alt, uint64_t* best) {
+    if (threadIdx.x == 0) list[n] = 0ull;   // the other half of the last pair
+    __syncthreads();
     for (int i = threadIdx.x; i < n; i += kThreads) {
         const uint64_t k = list[i];
         int r = 0;
-        for (int j = 0; j < n; j++) r += list[j] > k ? 1 : 0;
-        if (r < n_alt) best[r] = k;
+        for (int j = 0; j < n; j += 2) {
+            const ulonglong2 o = *reinterpret_cast<const ulonglong2*>(list + j);
+            r += (o.x > k ? 1 : 0) + (o.y > k ? 1 : 0);
+        }
+        if (k != 0ull && r < n_alt) best[r] = k;
     }
 }
 
@@ -184,7 +192,7 @@ token_logprobs_kernel(const void* __restrict__ logits, int64_t V, int64_t row_st
     constexpr int kChunk = Ch::n;
     constexpr int kWarpList = 64 + 32 * kChunk;  // second pass, candidates of a warp: fewer than 32 left over, a chunk of every lane, the edges
     extern __shared__ uint64_t s_warp_list[];    // [warps][kWarpList]
-    __shared__ __align__(16) Shared sh;
+    __shared__ Shared sh;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int rank = splits > 1 ? (int)(blockIdx.x % (unsigned)splits) : 0;
     const int64_t row = blockIdx.x / (unsigned)splits;
@@ -261,7 +269,6 @@ token_logprobs_kernel(const void* __restrict__ logits, int64_t V, int64_t row_st
             if ((lane & 1) == 0) sh.group_top[threadIdx.x >> 1] = top;
         }
         if (threadIdx.x == 0) {
-            sh.threshold = kFloor;
             sh.count = 0;
         }
         if (threadIdx.x < kMaxAlt) sh.best[threadIdx.x] = 0ull;
@@ -280,18 +287,19 @@ token_logprobs_kernel(const void* __restrict__ logits, int64_t V, int64_t row_st
             sh.warp_s[warp] = r.s;
             sh.warp_u[warp] = r.u;
         }
-        // the n_alt-th largest of the pairs' maxima: the one that n_alt - 1 are above (equal ones in the order of their places)
+        // the n_alt-th largest of the pairs' maxima = the smallest that fewer than n_alt of them are above
         if (n_alt > 0 && threadIdx.x < kThreads / 2) {
             const uint32_t mine = sh.group_top[threadIdx.x];
             int above = 0;
 #pragma unroll 8
             for (int j = 0; j < kThreads / 8; j++) {
                 const uint4 o = reinterpret_cast<const uint4*>(sh.group_top)[j];
-                const int at = 4 * j;
-                above += (o.x > mine || (o.x == mine && at < (int)threadIdx.x)) + (o.y > mine || (o.y == mine && at + 1 < (int)threadIdx.x)) +
-                         (o.z > mine || (o.z == mine && at + 2 < (int)threadIdx.x)) + (o.w > mine || (o.w == mine && at + 3 < (int)threadIdx.x));
+                above += (o.x > mine) + (o.y > mine) + (o.z > mine) + (o.w > mine);
             }
-            if (above == n_alt - 1 && mine > kFloor) sh.threshold = mine;
+            uint32_t least = above < n_alt ? mine : 0xFFFFFFFFu;
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) least = min(least, __shfl_xor_sync(0xFFFFFFFFu, least, o));
+            if (lane == 0) sh.warp_least[warp] = least;
         }
         __syncthreads();
         if (threadIdx.x == 0) {
@@ -309,7 +317,11 @@ token_logprobs_kernel(const void* __restrict__ logits, int64_t V, int64_t row_st
 
     // ---------------------------------------------------------- alternatives
     if (n_alt > 0) {
-        const float least = value_of(sh.threshold);
+        uint32_t threshold = sh.warp_least[0];
+#pragma unroll
+        for (int w = 1; w < kWarps / 2; w++) threshold = min(threshold, sh.warp_least[w]);
+        threshold = max(threshold, kFloor);
+        const float least = value_of(threshold);
         auto push = [&](float v, int64_t i) {
             const int at = atomicAdd(&sh.count, 1);
             if (at < kList) sh.list[at] = key_of(v, (uint32_t)i);
@@ -318,20 +330,33 @@ token_logprobs_kernel(const void* __restrict__ logits, int64_t V, int64_t row_st
             const float v = to_f32(x[extra_at]);
             if (v >= least) push(v, extra_at);
         }
-        // the warp reads the chunks of each of its threads that qualify, a lane each
-        for (uint32_t q = __ballot_sync(0xFFFFFFFFu, a.s != 0.0f && a.m >= least); q != 0u; q &= q - 1u) {
-            const int64_t from = first - lane + (__ffs(q) - 1);
-            for (int64_t ch = from + lane * step; ch < n_chunks; ch += 32 * step) {
-                uint32_t w[8];
-                load_chunk(chunks + ch * kChunk, w);
-                if (Ch::top(w) >= least) {
+        const uint32_t again = __ballot_sync(0xFFFFFFFFu, a.s != 0.0f && a.m >= least);
+        if (lane == 0) sh.readers[warp] = again;
+        __syncthreads();
+        int n_readers = 0, place = 0;
 #pragma unroll
-                    for (int j = 0; j < kChunk / 2; j++) {
-                        float v0, v1;
-                        Ch::two(w, j, v0, v1);
-                        if (v0 >= least) push(v0, head + ch * kChunk + 2 * j);
-                        if (v1 >= least) push(v1, head + ch * kChunk + 2 * j + 1);
-                    }
+        for (int w = 0; w < kWarps; w++) {
+            if (w == warp) place = n_readers;
+            n_readers += __popc(sh.readers[w]);
+        }
+        if ((again >> lane) & 1u) sh.reader[place + __popc(again & ((1u << lane) - 1u))] = (int)threadIdx.x;
+        __syncthreads();
+        // their chunks, shared out over the block: round r of reader i is item i * rounds + r
+        const int64_t part = (int64_t)rank * kThreads;
+        const uint32_t rounds = n_chunks > part ? (uint32_t)((n_chunks - part + step - 1) / step) : 0u, items = (uint32_t)n_readers * rounds;
+        for (uint32_t item = threadIdx.x; item < items; item += kThreads) {
+            const uint32_t i = item / rounds;
+            const int64_t ch = part + sh.reader[i] + (int64_t)(item - i * rounds) * step;
+            if (ch >= n_chunks) continue;
+            uint32_t w[8];
+            load_chunk(chunks + ch * kChunk, w);
+            if (Ch::top(w) >= least) {
+#pragma unroll
+                for (int j = 0; j < kChunk / 2; j++) {
+                    float v0, v1;
+                    Ch::two(w, j, v0, v1);
+                    if (v0 >= least) push(v0, head + ch * kChunk + 2 * j);
+                    if (v1 >= least) push(v1, head + ch * kChunk + 2 * j + 1);
                 }
             }
         }
@@ -343,7 +368,7 @@ token_logprobs_kernel(const void* __restrict__ logits, int64_t V, int64_t row_st
             // Its chunks come in ascending order, so an equal logit behind a full list is out: rows of equal logits cost one compare each.
             uint64_t* list = s_warp_list + (size_t)warp * kWarpList;
             uint64_t mine = 0ull;
-            uint32_t own = sh.threshold;
+            uint32_t own = threshold;
             if (lane == 0) sh.pending[warp] = 0;
             __syncwarp();
             auto flush = [&](bool all) {   // merge candidates 32 at a time; the rest stays (or goes too, padded with nothing)
@@ -388,13 +413,8 @@ token_logprobs_kernel(const void* __restrict__ logits, int64_t V, int64_t row_st
             __syncwarp();
             flush(true);
             __syncthreads();
-            sh.list[threadIdx.x] = mine;   // 256 of them; empty places (0) rank last
-            __syncthreads();
-            if (mine != 0ull) {
-                int r = 0;
-                for (int j = 0; j < kThreads; j++) r += sh.list[j] > mine ? 1 : 0;
-                if (r < n_alt) sh.best[r] = mine;
-            }
+            sh.list[threadIdx.x] = mine;   // 256 of them
+            rank_list(sh.list, kThreads, n_alt, sh.best);
         }
     }
     __syncthreads();
@@ -434,13 +454,7 @@ token_logprobs_kernel(const void* __restrict__ logits, int64_t V, int64_t row_st
                     asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(k) : "r"(at) : "memory");
                     sh.list[i] = k;
                 }
-                __syncthreads();
-                for (int i = threadIdx.x; i < splits * n_alt; i += kThreads) {
-                    const uint64_t k = sh.list[i];
-                    int r = 0;
-                    for (int j = 0; j < splits * n_alt; j++) r += sh.list[j] > k ? 1 : 0;
-                    if (k != 0ull && r < n_alt) sh.best[r] = k;
-                }
+                rank_list(sh.list, splits * n_alt, n_alt, sh.best);
                 __syncthreads();
             }
         }
