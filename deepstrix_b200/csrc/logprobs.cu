@@ -23,8 +23,6 @@
 namespace dsx {
 namespace {
 
-constexpr int kThreads = 256;
-constexpr int kWarps = kThreads / 32;
 constexpr int kMaxAlt = 32;            // one per lane of the warp that holds a list
 constexpr int kMaxCluster = 8;
 constexpr float kLowest = -3.402823466e38f;
@@ -152,14 +150,17 @@ struct Sums {
 
 constexpr int kList = 512;   // candidates the block ranks by counting
 
+template <int NT>
 struct alignas(16) Shared {
+    static constexpr int kWarps = NT / 32;
     float warp_m[kWarps], warp_s[kWarps], warp_u[kWarps];
-    alignas(16) uint32_t group_top[kThreads / 2];       // order of the maxima of pairs of threads, 0 where they saw nothing
-    uint32_t warp_least[kWarps / 2];        // their smallest is the order of a value that n_alt logits of the row's part reach
+    alignas(16) uint32_t group_top[NT / 2];       // order of the maxima of pairs of threads, 0 where they saw nothing
+    uint32_t warp_least[NT / 64];        // their smallest is the order of a value that n_alt logits of the row's part reach
     uint32_t readers[kWarps];               // lanes whose chunks are read again
-    int reader[kThreads];                   // and their threads, in order
+    int reader[NT];                   // and their threads, in order
     int count;                              // candidates that reach it
-    int pending[kWarps];                    // second pass: candidates on the warps' lists
+    int pending[kWarps];                    // second pass: candidates on the warps' lists,
+    uint64_t warp_list[kWarps][96];         // at most 31 left over and two of every lane
     alignas(16) uint64_t list[kList + 2];
     uint64_t best[kMaxAlt];                 // the part's best, descending, 0 = nothing
     float block_sums[3];
@@ -168,10 +169,11 @@ struct alignas(16) Shared {
 
 // best[0 .. n_alt) = the n_alt largest of the n keys of `list`, descending: a key's place is the number of larger ones (keys are
 // distinct but for 0, "nothing", which takes no place).  Keys are read two at a time; list[n] is written.
+template <int NT>
 __device__ __forceinline__ void rank_list(uint64_t* list, int n, int n_alt, uint64_t* best) {
     if (threadIdx.x == 0) list[n] = 0ull;   // the other half of the last pair
     __syncthreads();
-    for (int i = threadIdx.x; i < n; i += kThreads) {
+    for (int i = threadIdx.x; i < n; i += NT) {
         const uint64_t k = list[i];
         int r = 0;
         for (int j = 0; j < n; j += 2) {
@@ -182,17 +184,19 @@ __device__ __forceinline__ void rank_list(uint64_t* list, int n, int n_alt, uint
     }
 }
 
-template <int DT>
-__global__ void __launch_bounds__(kThreads)
+// NT threads a block: 256, or 64 for many short rows, whose time is the part behind the loop.  48 registers a thread (1280 threads an SM, 40 KB
+// of logits in flight): 4096 rows of 131072 bf16 take 199 us; with 64 registers (1024 threads) 206, with 40 (1536, spilling) 201, with
+// 1024 threads that request two chunks ahead 217.
+template <int DT, int NT>
+__global__ void __launch_bounds__(NT, 1280 / NT)
 token_logprobs_kernel(const void* __restrict__ logits, int64_t V, int64_t row_stride, float scale, const int32_t* __restrict__ tokens, int n_given,
                       float* __restrict__ logprobs, float* __restrict__ entropy, int n_alt, int32_t* __restrict__ alts, float* __restrict__ alt_logprobs,
                       int splits) {
     using T = typename Elem<DT>::T;
     using Ch = Chunk<T>;
     constexpr int kChunk = Ch::n;
-    constexpr int kWarpList = 64 + 32 * kChunk;  // second pass, candidates of a warp: fewer than 32 left over, a chunk of every lane, the edges
-    extern __shared__ uint64_t s_warp_list[];    // [warps][kWarpList]
-    __shared__ Shared sh;
+    constexpr int kThreads = NT, kWarps = NT / 32;
+    __shared__ Shared<NT> sh;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int rank = splits > 1 ? (int)(blockIdx.x % (unsigned)splits) : 0;
     const int64_t row = blockIdx.x / (unsigned)splits;
@@ -319,7 +323,7 @@ token_logprobs_kernel(const void* __restrict__ logits, int64_t V, int64_t row_st
     if (n_alt > 0) {
         uint32_t threshold = sh.warp_least[0];
 #pragma unroll
-        for (int w = 1; w < kWarps / 2; w++) threshold = min(threshold, sh.warp_least[w]);
+        for (int w = 1; w < NT / 64; w++) threshold = min(threshold, sh.warp_least[w]);
         threshold = max(threshold, kFloor);
         const float least = value_of(threshold);
         auto push = [&](float v, int64_t i) {
@@ -362,13 +366,13 @@ token_logprobs_kernel(const void* __restrict__ logits, int64_t V, int64_t row_st
         }
         __syncthreads();
         if (sh.count <= kList) {
-            rank_list(sh.list, sh.count, n_alt, sh.best);
+            rank_list<NT>(sh.list, sh.count, n_alt, sh.best);
         } else {
             // too many: a second pass over the part, in which a warp keeps its best 32 (one a lane) and lists only what may enter them.
             // Its chunks come in ascending order, so an equal logit behind a full list is out: rows of equal logits cost one compare each.
-            uint64_t* list = s_warp_list + (size_t)warp * kWarpList;
+            uint64_t* list = sh.warp_list[warp];
             uint64_t mine = 0ull;
-            uint32_t own = threshold;
+            uint32_t kth = 0u, own = threshold;   // order of the list's n_alt-th; the lowest order that may still enter it
             if (lane == 0) sh.pending[warp] = 0;
             __syncwarp();
             auto flush = [&](bool all) {   // merge candidates 32 at a time; the rest stays (or goes too, padded with nothing)
@@ -381,9 +385,8 @@ token_logprobs_kernel(const void* __restrict__ logits, int64_t V, int64_t row_st
                     mine = merge32(mine, sort32(k, lane), lane);
                 }
                 __syncwarp();
-                const uint32_t kth = (uint32_t)(__shfl_sync(0xFFFFFFFFu, mine, n_alt - 1) >> 32);
+                kth = (uint32_t)(__shfl_sync(0xFFFFFFFFu, mine, n_alt - 1) >> 32);
                 if (lane == 0) sh.pending[warp] = pending;
-                if (kth != 0u) own = kth + 1u;
                 __syncwarp();
             };
             for (int64_t ch = first; ch - lane < n_chunks; ch += step) {
@@ -393,17 +396,19 @@ token_logprobs_kernel(const void* __restrict__ logits, int64_t V, int64_t row_st
                 const float least = value_of(own);
                 const bool any = live && Ch::top(w) >= least;
                 if (__any_sync(0xFFFFFFFFu, any)) {
-                    if (any) {
+#pragma unroll 1
+                    for (int j = 0; j < kChunk / 2; j++) {
+                        float v0 = -INFINITY, v1 = -INFINITY;
 #pragma unroll
-                        for (int j = 0; j < kChunk / 2; j++) {
-                            float v0, v1;
-                            Ch::two(w, j, v0, v1);
-                            if (v0 >= least) list[atomicAdd(&sh.pending[warp], 1)] = key_of(v0, (uint32_t)(head + ch * kChunk + 2 * j));
-                            if (v1 >= least) list[atomicAdd(&sh.pending[warp], 1)] = key_of(v1, (uint32_t)(head + ch * kChunk + 2 * j + 1));
-                        }
+                        for (int i = 0; i < kChunk / 2; i++)
+                            if (i == j && any) Ch::two(w, i, v0, v1);
+                        const float bar = value_of(max(own, kth));   // within a round an equal logit may have the lower index
+                        if (v0 >= bar) list[atomicAdd(&sh.pending[warp], 1)] = key_of(v0, (uint32_t)(head + ch * kChunk + 2 * j));
+                        if (v1 >= bar) list[atomicAdd(&sh.pending[warp], 1)] = key_of(v1, (uint32_t)(head + ch * kChunk + 2 * j + 1));
+                        __syncwarp();
+                        flush(false);
                     }
-                    __syncwarp();
-                    flush(false);
+                    own = max(own, kth + 1u);
                 }
             }
             if (has_extra) {   // some of these come before all others: an equal logit may win
@@ -414,7 +419,7 @@ token_logprobs_kernel(const void* __restrict__ logits, int64_t V, int64_t row_st
             flush(true);
             __syncthreads();
             sh.list[threadIdx.x] = mine;   // 256 of them
-            rank_list(sh.list, kThreads, n_alt, sh.best);
+            rank_list<NT>(sh.list, kThreads, n_alt, sh.best);
         }
     }
     __syncthreads();
@@ -454,7 +459,7 @@ token_logprobs_kernel(const void* __restrict__ logits, int64_t V, int64_t row_st
                     asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(k) : "r"(at) : "memory");
                     sh.list[i] = k;
                 }
-                rank_list(sh.list, splits * n_alt, n_alt, sh.best);
+                rank_list<NT>(sh.list, splits * n_alt, n_alt, sh.best);
                 __syncthreads();
             }
         }
@@ -490,10 +495,29 @@ token_logprobs_kernel(const void* __restrict__ logits, int64_t V, int64_t row_st
     if (splits > 1) asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
-template <int DT>
+template <int DT, int NT>
 int launch(const void* logits, int64_t t, int64_t v, int64_t row_stride, float scale, const int32_t* tokens, int n_given, float* logprobs, float* entropy,
-           int n_alt, int32_t* alts, float* alt_logprobs, cudaStream_t stream) {
-    using T = typename Elem<DT>::T;
+           int n_alt, int32_t* alts, float* alt_logprobs, int splits, cudaStream_t stream) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(t * splits));
+    cfg.blockDim = dim3(NT);
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = (unsigned)splits;
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = splits > 1 ? 1 : 0;
+    DSX_CUDA(cudaLaunchKernelEx(&cfg, token_logprobs_kernel<DT, NT>, logits, v, row_stride, scale, tokens, n_given, logprobs, entropy, n_alt, alts,
+                                alt_logprobs, splits));
+    DSX_LAUNCHED();
+    return DSX_OK;
+}
+
+template <int DT>
+int launch_for(const void* logits, int64_t t, int64_t v, int64_t row_stride, float scale, const int32_t* tokens, int n_given, float* logprobs, float* entropy,
+               int n_alt, int32_t* alts, float* alt_logprobs, cudaStream_t stream) {
     constexpr int kMaxDevices = 64;
     static std::atomic<int> sm_counts[kMaxDevices];
     int dev = 0;
@@ -504,25 +528,16 @@ int launch(const void* logits, int64_t t, int64_t v, int64_t row_stride, float s
         DSX_CUDA(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev));
         sm_counts[dev].store(sms, std::memory_order_release);
     }
-    // few rows: as many blocks a row as still give every thread two chunks, and no more than four blocks an SM in all
+    constexpr int kChunk = Chunk<typename Elem<DT>::T>::n;
+    // many rows of at most 16 chunks a thread: the small block (4096 rows of 4096 bf16 16.5 us against 38.8, of 16384 36.8 against 57.9, but
+    // of 32000 with 20 alternatives 114 against 85); also a row that a small block reads in one round
+    const bool small = v <= 64 * kChunk || (t >= 8 * (int64_t)sms && v <= 16 * 64 * kChunk);
+    // few rows: as many blocks a row as still give every thread two chunks, and no more than two blocks an SM in all (64 rows of 131072 f32:
+    // 17.5 / 12.9 / 10.8 / 11.7 us with 1 / 2 / 4 / 8)
     int splits = 1;
-    while (splits < kMaxCluster && t * splits * 2 <= 4 * sms && v >= (int64_t)splits * 2 * 2 * kThreads * Chunk<T>::n) splits *= 2;
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)(t * splits));
-    cfg.blockDim = dim3(kThreads);
-    cfg.dynamicSmemBytes = n_alt > 0 ? sizeof(uint64_t) * kWarps * (64 + 32 * Chunk<T>::n) : 0;
-    cfg.stream = stream;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = (unsigned)splits;
-    attr[0].val.clusterDim.y = 1;
-    attr[0].val.clusterDim.z = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = splits > 1 ? 1 : 0;
-    DSX_CUDA(cudaLaunchKernelEx(&cfg, token_logprobs_kernel<DT>, logits, v, row_stride, scale, tokens, n_given, logprobs, entropy, n_alt, alts, alt_logprobs,
-                                splits));
-    DSX_LAUNCHED();
-    return DSX_OK;
+    while (!small && splits < kMaxCluster && t * splits * 2 <= 2 * (int64_t)sms && v >= (int64_t)splits * 2 * 2 * 256 * kChunk) splits *= 2;
+    if (small) return launch<DT, 64>(logits, t, v, row_stride, scale, tokens, n_given, logprobs, entropy, n_alt, alts, alt_logprobs, splits, stream);
+    return launch<DT, 256>(logits, t, v, row_stride, scale, tokens, n_given, logprobs, entropy, n_alt, alts, alt_logprobs, splits, stream);
 }
 
 }  // namespace
@@ -542,7 +557,7 @@ extern "C" int dsx_token_logprobs(const void* logits, int dtype, int64_t t, int6
     DSX_REQUIRE(logits && (n_given == 0 || (tokens && logprobs)) && (n_alt == 0 || (alts && alt_logprobs)), "token_logprobs: null argument");
     DSX_REQUIRE(((uintptr_t)logits & (dtype_size(dtype) - 1)) == 0, "token_logprobs: logits must be aligned to their elements");
     const cudaStream_t s = (cudaStream_t)stream;
-#define DSX_GO(DT) return launch<DT>(logits, t, v, row_stride, inv_temperature, tokens, n_given, logprobs, entropy, n_alt, alts, alt_logprobs, s)
+#define DSX_GO(DT) return launch_for<DT>(logits, t, v, row_stride, inv_temperature, tokens, n_given, logprobs, entropy, n_alt, alts, alt_logprobs, s)
     if (dtype == DSX_F32) DSX_GO(DSX_F32);
     if (dtype == DSX_BF16) DSX_GO(DSX_BF16);
     DSX_GO(DSX_F16);

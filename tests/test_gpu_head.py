@@ -335,6 +335,29 @@ def test_logprobs_hard_rows(torch_cuda, moe, V, dtype):
         _check_logprobs(torch, dx, tokens, n_alt)
 
 
+@pytest.mark.parametrize("dtype", ["float32", "float16"])
+@pytest.mark.parametrize("V", [3, 700, 5003])
+def test_logprobs_many_short_rows(torch_cuda, moe, V, dtype):
+    """Enough rows for the small blocks; among them equal rows, sorted rows, masked rows, each starting at another address modulo 16."""
+    torch = torch_cuda
+    rng = np.random.default_rng(V)
+    T = 1300
+    wide = rng.standard_normal((T, V + 1)).astype(np.float32)
+    x = wide[:, :V]
+    x[0] = 0.0
+    x[1] = np.linspace(-9, 9, V)
+    x[2] = np.linspace(9, -9, V)
+    x[3] = -np.inf
+    x[4, ::2] = -np.inf
+    x[5, V // 2] = np.nan
+    x[6] = rng.integers(0, 2, V)
+    x[7] = float(torch.finfo(_dtype(torch, dtype)).min)
+    x[8] = np.where(np.arange(V) % 7 == 0, 2.0, 1.0)
+    x[1200:1209] = x[:9]
+    dx = torch.from_numpy(wide).cuda().to(_dtype(torch, dtype))[:, :V]
+    _check_logprobs(torch, dx, rng.integers(-1, V + 1, (T, 2)).astype(np.int32), 20)
+
+
 def test_logprobs_without_tokens_or_alternatives(torch_cuda, moe):
     torch = torch_cuda
     from deepstrix_b200 import head
