@@ -9,11 +9,11 @@
 // few hundred run on the same kernel: a decode batch is an N of 16 under a stream of weights.  The terms of A are further MMAs into
 // the same accumulator: W is read once for all of them.  A pipeline stage is 256 columns: 128-byte rows (128-byte swizzle) of W and of every
 // term, each one TMA box, zero-filled past the operand's edges; and their scale bytes.
-// Scales are read as stored (row-major bytes; nothing is laid out beforehand): two loader warps bring the stage's 8 bytes of
-// every row into shared memory as 4-byte asynchronous copies (single bytes where rows of scales are not 4-byte aligned), in the form of
-// scale-factor chunks -- 128 rows x 4 blocks as 32 lanes x 16 bytes -- and four scale warps, one per lane quarter, move a landed
-// stage's chunks to tensor memory (ld.shared + tcgen05.st; the tensor core's own copy would queue behind its MMAs).
-// Warp roles (12 warps): TMA producer, MMA issue, 2 scale loaders, 4 scale warps, 4 epilogue warps; two accumulators, so that a
+// Scales are read as stored (row-major bytes; nothing is laid out beforehand): four loader warps, a row of every 128-row group a
+// thread, bring the stage's 8 bytes of each row into shared memory -- by 8-byte asynchronous copies where rows of scales are 8-byte
+// aligned, else as the aligned words that hold them, requested a stage ahead and shifted into place -- and four scale warps, one per
+// lane quarter, move a landed stage's scales to tensor memory (ld.shared + tcgen05.st; the tensor core's own copy would queue behind its MMAs).
+// Warp roles: TMA producer, MMA issue, 4 loaders, 4 scale warps, 4 epilogue warps; two accumulators, so that a
 // tile is read out under the next one's MMAs.
 // Few tiles: the columns are split over the CTAs of a cluster; each leaves its partial tile in shared memory and the cluster adds
 // them in rank order through distributed shared memory, so results do not depend on timing and need no workspace.
@@ -31,13 +31,14 @@ namespace {
 
 __device__ uint32_t g_head_error = 0;
 
-constexpr int kThreads = 384;
-constexpr int kLoaders = 64;
+constexpr int kScaleWarp0 = 4, kEpiWarp0 = 8, kLoadWarp0 = 12, kThreads = 512;   // roles start on warp-group boundaries; warps 2 and 3 are idle
+constexpr int kLoaders = 128;
 constexpr int kWRows = 128;          // W rows of a tile
 constexpr int kStageK = 256;         // columns of a stage
 constexpr int kRowBytes = kStageK / 2;
 constexpr int kWBytes = kWRows * kRowBytes;
-constexpr int kChunk = 512;          // scale bytes of 128 rows x 4 blocks
+constexpr int kGroupBytes = 1024;    // scale bytes of a group of 128 rows: 8 a row
+constexpr int kMaxGroups = 4;        // W and up to three term groups
 constexpr int kMaxStages = 8;
 constexpr int kMaxTokens = 208;      // A rows of a tile: two accumulators and four scale slots fill tensor memory
 constexpr uint32_t kSpinLimit = 1u << 22;
@@ -106,10 +107,8 @@ __device__ __forceinline__ void tc_ld16(uint32_t taddr, uint32_t (&r)[16]) {
         : "r"(taddr));
 }
 __device__ __forceinline__ void tc_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
-__device__ __forceinline__ void tc_st8(uint32_t taddr, const uint4& a, const uint4& b) {
-    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(taddr), "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w),
-                 "r"(b.x), "r"(b.y), "r"(b.z), "r"(b.w)
-                 : "memory");
+__device__ __forceinline__ void tc_st4(uint32_t taddr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x4.b32 [%0], {%1,%2,%3,%4};" ::"r"(taddr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
 }
 __device__ __forceinline__ uint32_t cluster_ctarank() {
     uint32_t r;
@@ -153,11 +152,11 @@ struct MatmulArgs {
     int K, terms;
     int tokens;              // A rows of a tile (multiple of 16)
     int stages, stage_bytes; // ring
-    int chunks;              // scale chunks of a stage and 128-column half: 1 (W) + terms * ceil(tokens / 128)
+    int groups;              // 128-row groups of scales: 1 (W) + terms * ceil(tokens / 128)
     int tmem_cols;
     int splits;              // CTAs of a cluster that share a tile's columns
     int tiles_w, tiles;      // tile t: W tile t % tiles_w, token tile t / tiles_w
-    int words;               // rows of scales are 4-byte aligned
+    int aligned;             // rows of scales are 8-byte aligned
 };
 
 template <int DT>
@@ -206,8 +205,9 @@ mxfp4_matmul_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_con
     const int tile0 = (int)blockIdx.x / g.splits, tile_step = (int)gridDim.x / g.splits;
     const int BN = g.tokens;
     const uint32_t b_bytes = (uint32_t)(g.terms * BN * kRowBytes);
-    const uint32_t sc_off = kWBytes + b_bytes;                  // the stage's scale chunks: [128-column half][W, term 0, ...][512]
-    const uint32_t slot0 = tmem + 2u * (uint32_t)BN, slot_cols = 8u * (uint32_t)g.chunks;
+    const uint32_t sc_off = kWBytes + b_bytes;                  // the stage's scales: [W, term 0, ...][row][8]
+    // scale slot of a stage: the two 128-column halves, each 4 columns a group (a term's groups side by side)
+    const uint32_t slot0 = tmem + 2u * (uint32_t)BN, half_cols = 4u * (uint32_t)g.groups, slot_cols = 2u * half_cols;
     const int nb = (BN + 127) >> 7;
 
     if (warp == 0) {
@@ -252,7 +252,7 @@ mxfp4_matmul_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_con
                     const uint32_t a_lo = lo0 + s * ((uint32_t)g.stage_bytes >> 4), b_lo = a_lo + (kWBytes >> 4), sc = slot0 + s * slot_cols;
                     const int steps = min(4, (g.K - kc * kStageK + 63) >> 6);
                     for (int ks = 0; ks < steps; ks++) {
-                        const uint32_t sfw = sc + (uint32_t)(ks >> 1) * 4u * (uint32_t)g.chunks;
+                        const uint32_t sfw = sc + (uint32_t)(ks >> 1) * half_cols;
                         for (int q = 0; q < g.terms; q++)
                             tc_mma_mxf4(acc, a_lo + 2u * ks, b_lo + (uint32_t)q * term_step + 2u * ks, hi, (ks & 1) ? idesc2 : idesc0, sfw,
                                         sfw + 4u + (uint32_t)(q * nb) * 4u, (kc > kc0 || ks > 0 || q > 0) ? 1u : 0u);
@@ -263,57 +263,79 @@ mxfp4_matmul_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_con
                 if (ok) tc_commit(bar(ACC_FULL) + 8u * b);
             }
         }
-    } else if (warp < 4) {
+    } else if (warp >= kLoadWarp0) {
         // --------------------------------------------------------- scale loaders
-        // Thread i brings the rows i and i + 64 of every 128-row group: two words (the stage's two 128-column halves) a row.
-        const int i = threadIdx.x - 64;
+        const int r = threadIdx.x - kLoadWarp0 * 32;   // row of every group
         const int nblk = g.K >> 5;
+        const uint32_t dst0 = sbase + sc_off + (uint32_t)r * 8u;
         uint32_t s = 0, ph = 0;
         bool ok = true;
         for (int tile = tile0; tile < g.tiles && ok; tile += tile_step) {
-            const int64_t w0 = (int64_t)(tile % g.tiles_w) * kWRows, a0 = (int64_t)(tile / g.tiles_w) * BN;
-            for (int kc = kc0; kc < kc1; kc++) {
-                ok = mbar_wait(bar(EMPTY) + 8u * s, ph ^ 1u, abort_flag);
-                if (!ok) break;
-                const uint32_t sc = sbase + s * (uint32_t)g.stage_bytes + sc_off;
-                const int blk = kc * 8;
-                // row r of a chunk: 4 bytes at (r % 32) * 16 + (r / 32) * 4
-                auto bring = [&](const uint8_t* base, int64_t row, int64_t rows_end, int chunk, int r) {
-                    const bool live = row < rows_end;
-                    const uint8_t* src = base + (live ? row : 0) * nblk + blk;
-                    const uint32_t dst = sc + (uint32_t)chunk * kChunk + (uint32_t)((r & 31) * 16 + (r >> 5) * 4);
+            const int64_t w_row = (int64_t)(tile % g.tiles_w) * kWRows + r, a_row0 = (int64_t)(tile / g.tiles_w) * BN;
+            // this thread's row of every group, null where the operand has none
+            const uint8_t* row[kMaxGroups];
+            row[0] = w_row < g.N ? g.w_scales + w_row * nblk : nullptr;
 #pragma unroll
-                    for (int h = 0; h < 2; h++) {
-                        const int n = live ? min(4, max(0, nblk - blk - 4 * h)) : 0;
-                        const uint32_t d = dst + (uint32_t)(h * g.chunks) * kChunk;
-                        if (g.words) {   // a word lies inside the row or past its end; zero-filled there
-                            asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(d), "l"(n ? src + 4 * h : base), "r"(n) : "memory");
-                        } else {
-                            uint32_t v = 0;
-                            for (int j = 0; j < n; j++) v |= (uint32_t)__ldg(src + 4 * h + j) << (8 * j);
-                            asm volatile("st.shared.b32 [%0], %1;" ::"r"(d), "r"(v) : "memory");
-                        }
-                    }
-                };
+            for (int i = 1; i < kMaxGroups; i++) {
+                const int q = nb == 2 ? 0 : i - 1, ra = (nb == 2 ? (i - 1) * 128 : 0) + r;   // nb == 2 only with one term
+                row[i] = i < g.groups && ra < BN && a_row0 + ra < g.M ? g.a_scales + ((int64_t)q * g.M + a_row0 + ra) * nblk : nullptr;
+            }
+            if (g.aligned) {
+                for (int kc = kc0; kc < kc1; kc++) {
+                    ok = mbar_wait(bar(EMPTY) + 8u * s, ph ^ 1u, abort_flag);
+                    if (!ok) break;
+                    const uint32_t dst = dst0 + s * (uint32_t)g.stage_bytes;
 #pragma unroll
-                for (int p = 0; p < 2; p++) {
-                    const int r = i + 64 * p;
-                    bring(g.w_scales, w0 + r, g.N, 0, r);
-                    for (int q = 0; q < g.terms; q++)
-                        for (int c = 0; c < nb; c++) {
-                            const int ra = c * 128 + r;
-                            if (ra < BN) bring(g.a_scales + (int64_t)q * g.M * nblk, a0 + ra, g.M, 1 + q * nb + c, r);
-                        }
+                    for (int i = 0; i < kMaxGroups; i++)
+                        if (i < g.groups)   // zero-filled where there is no row
+                            asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(dst + i * kGroupBytes), "l"(row[i] ? row[i] + kc * 8 : g.w_scales),
+                                         "r"(row[i] ? 8 : 0)
+                                         : "memory");
+                    asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar(FULL) + 8u * s) : "memory");
+                    if (++s == (uint32_t)g.stages) { s = 0; ph ^= 1u; }
                 }
-                const uint32_t full = bar(FULL) + 8u * s;
-                if (g.words) asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(full) : "memory");
-                else mbar_arrive(full);
-                if (++s == (uint32_t)g.stages) { s = 0; ph ^= 1u; }
+            } else {
+                // the aligned words that hold bytes blk .. blk + 7 of a row (the row's last bytes: fewer), at most three
+                auto fetch = [&](const uint8_t* p, int blk, uint32_t (&w)[3]) {
+                    const int n = p ? min(8, nblk - blk) : 0;
+                    const uintptr_t at = (uintptr_t)p + blk;
+                    const uint32_t* q = reinterpret_cast<const uint32_t*>(at & ~(uintptr_t)3);
+                    const int span = n > 0 ? (int)(at & 3) + n : 0;
+#pragma unroll
+                    for (int j = 0; j < 3; j++) w[j] = 4 * j < span ? __ldg(q + j) : 0u;
+                };
+                uint32_t w[kMaxGroups][3];
+#pragma unroll
+                for (int i = 0; i < kMaxGroups; i++) fetch(row[i], kc0 * 8, w[i]);
+                for (int kc = kc0; kc < kc1; kc++) {
+                    uint32_t lo[kMaxGroups], hi[kMaxGroups];
+#pragma unroll
+                    for (int i = 0; i < kMaxGroups; i++) {
+                        const uint32_t sh = ((uint32_t)(uintptr_t)row[i] + kc * 8) * 8u;   // funnel shifts take it modulo 32
+                        lo[i] = __funnelshift_r(w[i][0], w[i][1], sh);
+                        hi[i] = __funnelshift_r(w[i][1], w[i][2], sh);
+                        const int n = nblk - kc * 8;   // bytes past the row's end belong to the next row
+                        if (n < 8) {
+                            lo[i] = n >= 4 ? lo[i] : lo[i] & ((1u << (8 * n)) - 1u);
+                            hi[i] = n > 4 ? hi[i] & ((1u << (8 * (n - 4))) - 1u) : 0u;
+                        }
+                        if (kc + 1 < kc1) fetch(row[i], (kc + 1) * 8, w[i]);
+                    }
+                    ok = mbar_wait(bar(EMPTY) + 8u * s, ph ^ 1u, abort_flag);
+                    if (!ok) break;
+                    const uint32_t dst = dst0 + s * (uint32_t)g.stage_bytes;
+#pragma unroll
+                    for (int i = 0; i < kMaxGroups; i++)
+                        if (i < g.groups) asm volatile("st.shared.v2.b32 [%0], {%1, %2};" ::"r"(dst + i * kGroupBytes), "r"(lo[i]), "r"(hi[i]) : "memory");
+                    mbar_arrive(bar(FULL) + 8u * s);
+                    if (++s == (uint32_t)g.stages) { s = 0; ph ^= 1u; }
+                }
             }
         }
         asm volatile("cp.async.wait_all;" ::: "memory");
-    } else if (warp < 8) {
+    } else if (warp >= kScaleWarp0 && warp < kEpiWarp0) {
         // ----------------------------------------------------------- scale warps
+        // The tensor core wants, in every lane quarter, lane l's column j of a group's half to hold the half's four bytes of row 32 j + l.
         const uint32_t q = (uint32_t)(warp & 3);
         uint32_t s = 0, ph = 0;
         bool ok = true;
@@ -321,19 +343,24 @@ mxfp4_matmul_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_con
             for (int kc = kc0; kc < kc1; kc++) {
                 ok = mbar_wait(bar(FULL) + 8u * s, ph, abort_flag);
                 if (!ok) break;
-                const uint8_t* src = smem + (size_t)s * g.stage_bytes + sc_off + lane * 16;
+                const uint8_t* src = smem + (size_t)s * g.stage_bytes + sc_off + lane * 8;
                 const uint32_t dst = slot0 + s * slot_cols + ((q * 32u) << 16);
-                for (int c = 0; c < g.chunks; c++) {   // 2 * chunks of them, stored two at a time
-                    const uint4 v0 = *reinterpret_cast<const uint4*>(src + (2 * c) * kChunk), v1 = *reinterpret_cast<const uint4*>(src + (2 * c + 1) * kChunk);
-                    tc_st8(dst + 8u * (uint32_t)c, v0, v1);
-                }
+#pragma unroll
+                for (int i = 0; i < kMaxGroups; i++)
+                    if (i < g.groups) {
+                        uint2 v[4];
+#pragma unroll
+                        for (int j = 0; j < 4; j++) v[j] = *reinterpret_cast<const uint2*>(src + i * kGroupBytes + j * 256);
+                        tc_st4(dst + 4u * i, v[0].x, v[1].x, v[2].x, v[3].x);
+                        tc_st4(dst + half_cols + 4u * i, v[0].y, v[1].y, v[2].y, v[3].y);
+                    }
                 asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(bar(SC_FULL) + 8u * s);
                 if (++s == (uint32_t)g.stages) { s = 0; ph ^= 1u; }
             }
-    } else {
+    } else if (warp >= kEpiWarp0) {
         // -------------------------------------------------------------- epilogue
         const uint32_t q = (uint32_t)(warp & 3);
         uint32_t t = 0;
@@ -394,15 +421,15 @@ mxfp4_matmul_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_con
 constexpr int kSmallMin = 77 * 1024, kSmallMax = 112 * 1024, kLargeMin = 160 * 1024, kLargeMax = 225 * 1024;
 
 struct Plan {
-    int tokens, stages, stage_bytes, chunks, tmem_cols, smem, per_sm, splits, tiles_w, tiles_m;
+    int tokens, stages, stage_bytes, groups, tmem_cols, smem, per_sm, splits, tiles_w, tiles_m;
 };
 
 bool plan_block(int terms, int tokens, Plan* p) {
-    const int nb = (tokens + 127) / 128, chunks = 1 + terms * nb;
+    const int nb = (tokens + 127) / 128, groups = 1 + terms * nb;
     p->tokens = tokens;
-    p->chunks = chunks;
-    p->stage_bytes = kWBytes + terms * tokens * kRowBytes + 2 * chunks * kChunk;
-    auto cols = [&](int stages) { return 2 * tokens + stages * 8 * chunks; };
+    p->groups = groups;
+    p->stage_bytes = kWBytes + terms * tokens * kRowBytes + groups * kGroupBytes;
+    auto cols = [&](int stages) { return 2 * tokens + stages * 8 * groups; };
     auto pow2 = [](int c) { int r = 32; while (r < c) r *= 2; return r; };
     int st = std::min(kMaxStages, (kSmallMax - 1024) / p->stage_bytes);
     while (st > 3 && cols(st) > 256) st--;
@@ -536,9 +563,9 @@ int dsx_mxfp4_matmul(const void* a_codes, const void* a_scales, int n_terms, int
     g.out = out;
     g.row_stride = row_stride;
     g.M = m; g.N = n; g.K = (int)k; g.terms = n_terms;
-    g.tokens = p.tokens; g.stages = p.stages; g.stage_bytes = p.stage_bytes; g.chunks = p.chunks; g.tmem_cols = p.tmem_cols; g.splits = p.splits;
+    g.tokens = p.tokens; g.stages = p.stages; g.stage_bytes = p.stage_bytes; g.groups = p.groups; g.tmem_cols = p.tmem_cols; g.splits = p.splits;
     g.tiles_w = p.tiles_w; g.tiles = p.tiles_w * p.tiles_m;
-    g.words = k % 128 == 0 && (((uintptr_t)a_scales | (uintptr_t)w_scales) & 3) == 0;
+    g.aligned = k % kStageK == 0 && (((uintptr_t)a_scales | (uintptr_t)w_scales) & 7) == 0;
     const cudaStream_t s = (cudaStream_t)stream;
     if (dtype == DSX_F32) return launch<DSX_F32>(p, tw, ta, g, sms, s);
     if (dtype == DSX_BF16) return launch<DSX_BF16>(p, tw, ta, g, sms, s);
