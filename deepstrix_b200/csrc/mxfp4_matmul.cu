@@ -83,19 +83,24 @@ __device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map
 }
 __device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
-__device__ __forceinline__ void tc_commit(uint32_t bar) {
-    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+__device__ __forceinline__ void tc_commit(uint32_t leader, uint32_t bar) {
+    asm volatile(
+        "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %1, 0;\n\t"
+        "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(bar), "r"(leader)
+        : "memory");
 }
-// D[128 x N] (+)= A[128 x 64] . B[N x 64]^T, E2M1 operands, one E8M0 scale per 32 columns of either operand.
-__device__ __forceinline__ void tc_mma_mxf4(uint32_t d, uint32_t a_lo, uint32_t b_lo, uint32_t hi, uint32_t idesc, uint32_t sfa, uint32_t sfb,
+// D[128 x N] (+)= A[128 x 64] . B[N x 64]^T, E2M1 operands, one E8M0 scale per 32 columns of either operand; issued by the lanes whose
+// `leader` is set (one of the warp), under a predicate and not a branch: see the MMA warp.
+__device__ __forceinline__ void tc_mma_mxf4(uint32_t leader, uint32_t d, uint32_t a_lo, uint32_t b_lo, uint32_t hi, uint32_t idesc, uint32_t sfa, uint32_t sfb,
                                             uint32_t accumulate) {
     asm volatile(
-        "{\n\t.reg .pred p;\n\t.reg .b64 da, db;\n\t"
+        "{\n\t.reg .pred p, q;\n\t.reg .b64 da, db;\n\t"
         "setp.ne.b32 p, %7, 0;\n\t"
+        "setp.ne.b32 q, %8, 0;\n\t"
         "mov.b64 da, {%1, %3};\n\t"
         "mov.b64 db, {%2, %3};\n\t"
-        "tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], da, db, %4, [%5], [%6], p;\n\t}"
-        ::"r"(d), "r"(a_lo), "r"(b_lo), "r"(hi), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate)
+        "@q tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], da, db, %4, [%5], [%6], p;\n\t}"
+        ::"r"(d), "r"(a_lo), "r"(b_lo), "r"(hi), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate), "r"(leader)
         : "memory");
 }
 __device__ __forceinline__ void tc_ld16(uint32_t taddr, uint32_t (&r)[16]) {
@@ -149,7 +154,7 @@ struct MatmulArgs {
     void* out;
     int64_t row_stride;
     int64_t M, N;
-    int K, terms;
+    int K;
     int tokens;              // A rows of a tile (multiple of 16)
     int stages, stage_bytes; // ring
     int groups;              // 128-row groups of scales: 1 (W) + terms * ceil(tokens / 128)
@@ -159,7 +164,7 @@ struct MatmulArgs {
     int aligned;             // rows of scales are 8-byte aligned
 };
 
-template <int DT>
+template <int DT, int TERMS>
 __global__ void __launch_bounds__(kThreads, 2)
 mxfp4_matmul_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CUtensorMap tmap_a, const MatmulArgs g) {
     using T = typename Elem<DT>::T;
@@ -204,7 +209,7 @@ mxfp4_matmul_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_con
     const int kc0 = (int)((int64_t)n_kc * rank / g.splits), kc1 = (int)((int64_t)n_kc * (rank + 1) / g.splits);
     const int tile0 = (int)blockIdx.x / g.splits, tile_step = (int)gridDim.x / g.splits;
     const int BN = g.tokens;
-    const uint32_t b_bytes = (uint32_t)(g.terms * BN * kRowBytes);
+    const uint32_t b_bytes = (uint32_t)(TERMS * BN * kRowBytes);
     const uint32_t sc_off = kWBytes + b_bytes;                  // the stage's scales: [W, term 0, ...][row][8]
     // scale slot of a stage: the two 128-column halves, each 4 columns a group (a term's groups side by side)
     const uint32_t slot0 = tmem + 2u * (uint32_t)BN, half_cols = 4u * (uint32_t)g.groups, slot_cols = 2u * half_cols;
@@ -233,35 +238,42 @@ mxfp4_matmul_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_con
         }
     } else if (warp == 1) {
         // ------------------------------------------------------------- MMA issue
-        if (lane == 0) {
-            uint32_t s = 0, ph = 0, t = 0;
-            bool ok = true;
-            const uint64_t d0 = operand_desc(sbase);
-            const uint32_t hi = (uint32_t)(d0 >> 32), lo0 = (uint32_t)d0;
-            const uint32_t term_step = (uint32_t)(BN * kRowBytes) >> 4;
-            const uint32_t idesc0 = mxf4_idesc(BN, 0u), idesc2 = mxf4_idesc(BN, 2u);
-            for (int tile = tile0; tile < g.tiles && ok; tile += tile_step, t++) {
-                const uint32_t b = t & 1u, acc = tmem + b * (uint32_t)BN;
-                ok = mbar_wait(bar(ACC_EMPTY) + 8u * b, ((t >> 1) & 1u) ^ 1u, abort_flag);
+        // The whole warp walks the loop and one lane issues, under a predicate: the instruction takes its operands from uniform registers, and
+        // inside a branch of one lane each of them had to be carried there first -- 230 clocks an MMA, whatever its size.  Votes keep the
+        // loop's exits uniform.
+        const uint32_t leader = lane == 0 ? 1u : 0u;
+        uint32_t s = 0, ph = 0, t = 0;
+        bool ok = true;
+        const uint64_t d0 = operand_desc(sbase);
+        const uint32_t hi = (uint32_t)(d0 >> 32), lo0 = __shfl_sync(0xFFFFFFFFu, (uint32_t)d0, 0);
+        const uint32_t tm = __shfl_sync(0xFFFFFFFFu, tmem, 0), slots = tm + 2u * (uint32_t)BN;
+        const uint32_t term_step = (uint32_t)(BN * kRowBytes) >> 4, stage_step = (uint32_t)g.stage_bytes >> 4;
+        const uint32_t idesc0 = mxf4_idesc(BN, 0u), idesc2 = mxf4_idesc(BN, 2u);
+        for (int tile = tile0; tile < g.tiles && ok; tile += tile_step, t++) {
+            const uint32_t b = t & 1u, acc = tm + b * (uint32_t)BN;
+            ok = __all_sync(0xFFFFFFFFu, mbar_wait(bar(ACC_EMPTY) + 8u * b, ((t >> 1) & 1u) ^ 1u, abort_flag));
+            if (!ok) break;
+            tc_fence_after();
+            for (int kc = kc0; kc < kc1; kc++) {
+                ok = __all_sync(0xFFFFFFFFu, mbar_wait(bar(SC_FULL) + 8u * s, ph, abort_flag) && mbar_wait(bar(FULL) + 8u * s, ph, abort_flag));
                 if (!ok) break;
                 tc_fence_after();
-                for (int kc = kc0; kc < kc1; kc++) {
-                    ok = mbar_wait(bar(SC_FULL) + 8u * s, ph, abort_flag) && mbar_wait(bar(FULL) + 8u * s, ph, abort_flag);
-                    if (!ok) break;
-                    tc_fence_after();
-                    const uint32_t a_lo = lo0 + s * ((uint32_t)g.stage_bytes >> 4), b_lo = a_lo + (kWBytes >> 4), sc = slot0 + s * slot_cols;
-                    const int steps = min(4, (g.K - kc * kStageK + 63) >> 6);
-                    for (int ks = 0; ks < steps; ks++) {
+                const uint32_t a_lo = lo0 + s * stage_step, b_lo = a_lo + (kWBytes >> 4), sc = slots + s * slot_cols;
+                const int steps = (g.K - kc * kStageK + 63) >> 6;
+#pragma unroll
+                for (int ks = 0; ks < 4; ks++) {
+                    if (ks < steps) {
                         const uint32_t sfw = sc + (uint32_t)(ks >> 1) * half_cols;
-                        for (int q = 0; q < g.terms; q++)
-                            tc_mma_mxf4(acc, a_lo + 2u * ks, b_lo + (uint32_t)q * term_step + 2u * ks, hi, (ks & 1) ? idesc2 : idesc0, sfw,
+#pragma unroll
+                        for (int q = 0; q < TERMS; q++)
+                            tc_mma_mxf4(leader, acc, a_lo + 2u * ks, b_lo + (uint32_t)q * term_step + 2u * ks, hi, (ks & 1) ? idesc2 : idesc0, sfw,
                                         sfw + 4u + (uint32_t)(q * nb) * 4u, (kc > kc0 || ks > 0 || q > 0) ? 1u : 0u);
                     }
-                    tc_commit(bar(EMPTY) + 8u * s);
-                    if (++s == (uint32_t)g.stages) { s = 0; ph ^= 1u; }
                 }
-                if (ok) tc_commit(bar(ACC_FULL) + 8u * b);
+                tc_commit(leader, bar(EMPTY) + 8u * s);
+                if (++s == (uint32_t)g.stages) { s = 0; ph ^= 1u; }
             }
+            if (ok) tc_commit(leader, bar(ACC_FULL) + 8u * b);
         }
     } else if (warp >= kLoadWarp0) {
         // --------------------------------------------------------- scale loaders
@@ -480,7 +492,7 @@ bool make_plan(int64_t M, int64_t N, int K, int terms, int sms, Plan* best) {
     return best_t < 1e300;
 }
 
-template <int DT>
+template <int DT, int TERMS>
 int launch(const Plan& p, const CUtensorMap& w, const CUtensorMap& a, MatmulArgs g, int sms, cudaStream_t stream) {
     cudaLaunchConfig_t cfg = {};
     const int64_t units = (int64_t)p.tiles_w * p.tiles_m * p.splits;
@@ -497,9 +509,28 @@ int launch(const Plan& p, const CUtensorMap& w, const CUtensorMap& a, MatmulArgs
     attr[1].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = p.splits > 1 ? 2 : 1;
-    DSX_CUDA(cudaLaunchKernelEx(&cfg, mxfp4_matmul_kernel<DT>, w, a, g));
+    DSX_CUDA(cudaLaunchKernelEx(&cfg, mxfp4_matmul_kernel<DT, TERMS>, w, a, g));
     DSX_LAUNCHED();
     return DSX_OK;
+}
+
+template <typename F>
+void for_each_kernel(F f) {
+    f(mxfp4_matmul_kernel<DSX_F32, 1>);
+    f(mxfp4_matmul_kernel<DSX_F32, 2>);
+    f(mxfp4_matmul_kernel<DSX_F32, 3>);
+    f(mxfp4_matmul_kernel<DSX_BF16, 1>);
+    f(mxfp4_matmul_kernel<DSX_BF16, 2>);
+    f(mxfp4_matmul_kernel<DSX_BF16, 3>);
+    f(mxfp4_matmul_kernel<DSX_F16, 1>);
+    f(mxfp4_matmul_kernel<DSX_F16, 2>);
+    f(mxfp4_matmul_kernel<DSX_F16, 3>);
+}
+template <int DT>
+int launch_terms(int terms, const Plan& p, const CUtensorMap& w, const CUtensorMap& a, const MatmulArgs& g, int sms, cudaStream_t stream) {
+    if (terms == 1) return launch<DT, 1>(p, w, a, g, sms, stream);
+    if (terms == 2) return launch<DT, 2>(p, w, a, g, sms, stream);
+    return launch<DT, 3>(p, w, a, g, sms, stream);
 }
 
 // SM count of the current device; the opt-in to large shared memory is made once per device.
@@ -512,9 +543,11 @@ int configure(int* sms) {
     int n = sm_counts[dev].load(std::memory_order_acquire);
     if (n == 0) {
         DSX_CUDA(cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev));
-        DSX_CUDA(cudaFuncSetAttribute(mxfp4_matmul_kernel<DSX_F32>, cudaFuncAttributeMaxDynamicSharedMemorySize, kLargeMax));
-        DSX_CUDA(cudaFuncSetAttribute(mxfp4_matmul_kernel<DSX_BF16>, cudaFuncAttributeMaxDynamicSharedMemorySize, kLargeMax));
-        DSX_CUDA(cudaFuncSetAttribute(mxfp4_matmul_kernel<DSX_F16>, cudaFuncAttributeMaxDynamicSharedMemorySize, kLargeMax));
+        int rc = DSX_OK;
+        for_each_kernel([&](auto* kernel) {
+            if (rc == DSX_OK) rc = [&]() -> int { DSX_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kLargeMax)); return DSX_OK; }();
+        });
+        if (rc != DSX_OK) return rc;
         sm_counts[dev].store(n, std::memory_order_release);
     }
     *sms = n;
@@ -562,14 +595,14 @@ int dsx_mxfp4_matmul(const void* a_codes, const void* a_scales, int n_terms, int
     g.a_scales = (const uint8_t*)a_scales;
     g.out = out;
     g.row_stride = row_stride;
-    g.M = m; g.N = n; g.K = (int)k; g.terms = n_terms;
+    g.M = m; g.N = n; g.K = (int)k;
     g.tokens = p.tokens; g.stages = p.stages; g.stage_bytes = p.stage_bytes; g.groups = p.groups; g.tmem_cols = p.tmem_cols; g.splits = p.splits;
     g.tiles_w = p.tiles_w; g.tiles = p.tiles_w * p.tiles_m;
     g.aligned = k % kStageK == 0 && (((uintptr_t)a_scales | (uintptr_t)w_scales) & 7) == 0;
     const cudaStream_t s = (cudaStream_t)stream;
-    if (dtype == DSX_F32) return launch<DSX_F32>(p, tw, ta, g, sms, s);
-    if (dtype == DSX_BF16) return launch<DSX_BF16>(p, tw, ta, g, sms, s);
-    return launch<DSX_F16>(p, tw, ta, g, sms, s);
+    if (dtype == DSX_F32) return launch_terms<DSX_F32>(n_terms, p, tw, ta, g, sms, s);
+    if (dtype == DSX_BF16) return launch_terms<DSX_BF16>(n_terms, p, tw, ta, g, sms, s);
+    return launch_terms<DSX_F16>(n_terms, p, tw, ta, g, sms, s);
 }
 
 int dsx_head_check(dsx_stream_t stream_, uint32_t* error_word) {
