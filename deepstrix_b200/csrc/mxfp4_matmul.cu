@@ -112,8 +112,51 @@ __device__ __forceinline__ void tc_ld16(uint32_t taddr, uint32_t (&r)[16]) {
         : "r"(taddr));
 }
 __device__ __forceinline__ void tc_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
-__device__ __forceinline__ void tc_st4(uint32_t taddr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
-    asm volatile("tcgen05.st.sync.aligned.32x32b.x4.b32 [%0], {%1,%2,%3,%4};" ::"r"(taddr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
+// lane l of the warp writes N columns of its tensor-memory lane
+__device__ __forceinline__ void tc_st(uint32_t taddr, const uint32_t (&r)[8]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]),
+                 "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+                 : "memory");
+}
+__device__ __forceinline__ void tc_st(uint32_t taddr, const uint32_t (&r)[16]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr), "r"(r[0]),
+                 "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]),
+                 "r"(r[13]), "r"(r[14]), "r"(r[15])
+                 : "memory");
+}
+__device__ __forceinline__ void tc_st(uint32_t taddr, const uint32_t (&r)[32]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
+        "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(taddr),
+        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]),
+        "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]),
+        "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+        : "memory");
+}
+// Scales of a landed stage, this lane's rows (row 32 j + lane of group i at src + i * kGroupBytes + j * 256), to the stage's slot: both
+// 128-column halves, 4 columns a group each -- one or two wide stores (a 4-column store a group and half took 100 clocks apiece).
+template <int GROUPS>
+__device__ __forceinline__ void store_scales(const uint8_t* src, uint32_t dst) {
+    uint32_t v[8 * GROUPS];
+#pragma unroll
+    for (int i = 0; i < GROUPS; i++)
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            const uint2 two = *reinterpret_cast<const uint2*>(src + i * kGroupBytes + j * 256);
+            v[4 * i + j] = two.x;
+            v[4 * GROUPS + 4 * i + j] = two.y;
+        }
+    if constexpr (GROUPS == 3) {
+        uint32_t lo[16], hi[8];
+#pragma unroll
+        for (int i = 0; i < 16; i++) lo[i] = v[i];
+#pragma unroll
+        for (int i = 0; i < 8; i++) hi[i] = v[16 + i];
+        tc_st(dst, lo);
+        tc_st(dst + 16u, hi);
+    } else {
+        tc_st(dst, v);
+    }
 }
 __device__ __forceinline__ uint32_t cluster_ctarank() {
     uint32_t r;
@@ -148,6 +191,32 @@ __device__ __forceinline__ uint32_t mxf4_idesc(int n, uint32_t sf) {
     return (1u << 7) | (1u << 10) | ((uint32_t)(n >> 3) << 17) | (1u << 23) | ((128u >> 4) << 24) | (sf << 4) | (sf << 29);
 }
 
+// Sixteen tokens of the lane's output column (32 neighbouring columns a warp).  16-bit results leave in pairs of columns where the rows
+// allow 4-byte stores: even lanes take the even tokens of their own and the next lane's column, odd lanes the odd ones, so a store
+// instruction carries two tokens.
+template <typename T>
+__device__ __forceinline__ void store_tokens(T* __restrict__ o, int64_t stride, const uint32_t (&v)[16], int rows, bool live, int pairs, int lane) {
+    if constexpr (sizeof(T) == 2) {
+        if (pairs) {   // N is even: both columns of a pair exist or neither does
+            const bool odd = lane & 1;
+            uint32_t* p = reinterpret_cast<uint32_t*>(o + (odd ? stride - 1 : 0));
+            const int64_t step = stride;   // two rows, in 32-bit words
+#pragma unroll
+            for (int j = 0; j < 16; j += 2) {
+                const float mine = __uint_as_float(odd ? v[j + 1] : v[j]), theirs = __uint_as_float(odd ? v[j] : v[j + 1]);
+                const float got = __shfl_xor_sync(0xFFFFFFFFu, theirs, 1);
+                const uint32_t w = odd ? pack2<T>(got, mine) : pack2<T>(mine, got);
+                if (live && j + (odd ? 1 : 0) < rows) *p = w;
+                p += step;
+            }
+            return;
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < 16; j++)
+        if (live && j < rows) o[j * stride] = from_f32<T>(__uint_as_float(v[j]));
+}
+
 struct MatmulArgs {
     const uint8_t* w_scales;
     const uint8_t* a_scales;
@@ -162,6 +231,7 @@ struct MatmulArgs {
     int splits;              // CTAs of a cluster that share a tile's columns
     int tiles_w, tiles;      // tile t: W tile t % tiles_w, token tile t / tiles_w
     int aligned;             // rows of scales are 8-byte aligned
+    int pairs;               // results are 16-bit and pairs of columns 4-byte aligned in every row
 };
 
 template <int DT, int TERMS>
@@ -357,15 +427,12 @@ mxfp4_matmul_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_con
                 if (!ok) break;
                 const uint8_t* src = smem + (size_t)s * g.stage_bytes + sc_off + lane * 8;
                 const uint32_t dst = slot0 + s * slot_cols + ((q * 32u) << 16);
-#pragma unroll
-                for (int i = 0; i < kMaxGroups; i++)
-                    if (i < g.groups) {
-                        uint2 v[4];
-#pragma unroll
-                        for (int j = 0; j < 4; j++) v[j] = *reinterpret_cast<const uint2*>(src + i * kGroupBytes + j * 256);
-                        tc_st4(dst + 4u * i, v[0].x, v[1].x, v[2].x, v[3].x);
-                        tc_st4(dst + half_cols + 4u * i, v[0].y, v[1].y, v[2].y, v[3].y);
-                    }
+if constexpr (TERMS == 1) {
+                    if (nb == 1) store_scales<2>(src, dst);
+                    else store_scales<3>(src, dst);
+                } else {
+                    store_scales<1 + TERMS>(src, dst);   // two or three terms: one group each
+                }
                 asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
                 tc_fence_before();
                 __syncwarp();
@@ -383,6 +450,8 @@ mxfp4_matmul_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_con
             ok = mbar_wait(bar(ACC_FULL) + 8u * b, (t >> 1) & 1u, abort_flag);
             if (!ok) break;
             tc_fence_after();
+            const int rows = (int)min((int64_t)BN, g.M - m0);         // tokens that exist
+            T* o = reinterpret_cast<T*>(g.out) + m0 * g.row_stride + n;
             for (int c0 = 0; c0 < BN; c0 += 16) {
                 uint32_t v[16];
                 tc_ld16(acc + (uint32_t)c0, v);
@@ -391,11 +460,9 @@ mxfp4_matmul_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_con
                     float* p = reinterpret_cast<float*>(smem) + (size_t)c0 * kWRows + q * 32 + lane;
 #pragma unroll
                     for (int j = 0; j < 16; j++) p[j * kWRows] = __uint_as_float(v[j]);
-                } else if (n < g.N) {
-                    T* o = reinterpret_cast<T*>(g.out) + (m0 + c0) * g.row_stride + n;
-#pragma unroll
-                    for (int j = 0; j < 16; j++)
-                        if (m0 + c0 + j < g.M) o[j * g.row_stride] = from_f32<T>(__uint_as_float(v[j]));
+                } else {
+                    store_tokens<T>(o, g.row_stride, v, rows - c0, n < g.N, g.pairs, lane);
+                    o += 16 * g.row_stride;
                 }
             }
             tc_fence_before();
@@ -599,6 +666,7 @@ int dsx_mxfp4_matmul(const void* a_codes, const void* a_scales, int n_terms, int
     g.tokens = p.tokens; g.stages = p.stages; g.stage_bytes = p.stage_bytes; g.groups = p.groups; g.tmem_cols = p.tmem_cols; g.splits = p.splits;
     g.tiles_w = p.tiles_w; g.tiles = p.tiles_w * p.tiles_m;
     g.aligned = k % kStageK == 0 && (((uintptr_t)a_scales | (uintptr_t)w_scales) & 7) == 0;
+    g.pairs = dtype != DSX_F32 && n % 2 == 0 && (row_stride % 2 == 0 || m == 1) && ((uintptr_t)out & 3) == 0;
     const cudaStream_t s = (cudaStream_t)stream;
     if (dtype == DSX_F32) return launch_terms<DSX_F32>(n_terms, p, tw, ta, g, sms, s);
     if (dtype == DSX_BF16) return launch_terms<DSX_BF16>(n_terms, p, tw, ta, g, sms, s);
