@@ -83,25 +83,51 @@ __device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map
 }
 __device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+// Arrives on a barrier (of either CTA of a pair) when the MMAs issued so far have completed.
+template <bool PAIR>
 __device__ __forceinline__ void tc_commit(uint32_t leader, uint32_t bar) {
-    asm volatile(
-        "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %1, 0;\n\t"
-        "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(bar), "r"(leader)
-        : "memory");
+    if constexpr (PAIR)
+        asm volatile(
+            "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %1, 0;\n\t"
+            "@q tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(bar), "r"(leader)
+            : "memory");
+    else
+        asm volatile(
+            "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %1, 0;\n\t"
+            "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(bar), "r"(leader)
+            : "memory");
 }
-// D[128 x N] (+)= A[128 x 64] . B[N x 64]^T, E2M1 operands, one E8M0 scale per 32 columns of either operand; issued by the lanes whose
-// `leader` is set (one of the warp), under a predicate and not a branch: see the MMA warp.
+// Arrival on a barrier of the other CTA of a pair.  Relaxed: what it reports (tensor-memory accesses this warp has waited for) is finished
+// before it issues, and a release at cluster scope holds the thread for about a microsecond.
+__device__ __forceinline__ void mbar_arrive_cluster(uint32_t cluster_bar) {
+    asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_bar) : "memory");
+}
+// D[M x N] (+)= A[M x 64] . B[N x 64]^T, E2M1 operands, one E8M0 scale per 32 columns of either operand; M = 128, or 256 over the two
+// CTAs of a pair (rows 0 .. 127 of A and D in the even one, each holding N / 2 rows of B).  Issued by the lanes whose `leader` is set (one
+// of the warp), under a predicate and not a branch: see the MMA warp.
+template <bool PAIR>
 __device__ __forceinline__ void tc_mma_mxf4(uint32_t leader, uint32_t d, uint32_t a_lo, uint32_t b_lo, uint32_t hi, uint32_t idesc, uint32_t sfa, uint32_t sfb,
                                             uint32_t accumulate) {
-    asm volatile(
-        "{\n\t.reg .pred p, q;\n\t.reg .b64 da, db;\n\t"
-        "setp.ne.b32 p, %7, 0;\n\t"
-        "setp.ne.b32 q, %8, 0;\n\t"
-        "mov.b64 da, {%1, %3};\n\t"
-        "mov.b64 db, {%2, %3};\n\t"
-        "@q tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], da, db, %4, [%5], [%6], p;\n\t}"
-        ::"r"(d), "r"(a_lo), "r"(b_lo), "r"(hi), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate), "r"(leader)
-        : "memory");
+    if constexpr (PAIR)
+        asm volatile(
+            "{\n\t.reg .pred p, q;\n\t.reg .b64 da, db;\n\t"
+            "setp.ne.b32 p, %7, 0;\n\t"
+            "setp.ne.b32 q, %8, 0;\n\t"
+            "mov.b64 da, {%1, %3};\n\t"
+            "mov.b64 db, {%2, %3};\n\t"
+            "@q tcgen05.mma.cta_group::2.kind::mxf4.block_scale.scale_vec::2X [%0], da, db, %4, [%5], [%6], p;\n\t}"
+            ::"r"(d), "r"(a_lo), "r"(b_lo), "r"(hi), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate), "r"(leader)
+            : "memory");
+    else
+        asm volatile(
+            "{\n\t.reg .pred p, q;\n\t.reg .b64 da, db;\n\t"
+            "setp.ne.b32 p, %7, 0;\n\t"
+            "setp.ne.b32 q, %8, 0;\n\t"
+            "mov.b64 da, {%1, %3};\n\t"
+            "mov.b64 db, {%2, %3};\n\t"
+            "@q tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], da, db, %4, [%5], [%6], p;\n\t}"
+            ::"r"(d), "r"(a_lo), "r"(b_lo), "r"(hi), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate), "r"(leader)
+            : "memory");
 }
 __device__ __forceinline__ void tc_ld16(uint32_t taddr, uint32_t (&r)[16]) {
     asm volatile(
@@ -185,10 +211,10 @@ __device__ __forceinline__ uint64_t operand_desc(uint32_t saddr) {
     d |= (uint64_t)2 << 61;                         // 128-byte swizzle
     return d;
 }
-// kind::mxf4: E2M1 x E2M1 -> f32, E8M0 scales, K-major operands, M = 128, K = 64; sf = byte (0 or 2) of the 4-byte scale words
+// kind::mxf4: E2M1 x E2M1 -> f32, E8M0 scales, K-major operands, K = 64; sf = byte (0 or 2) of the 4-byte scale words
 // that holds this k step's first block.
-__device__ __forceinline__ uint32_t mxf4_idesc(int n, uint32_t sf) {
-    return (1u << 7) | (1u << 10) | ((uint32_t)(n >> 3) << 17) | (1u << 23) | ((128u >> 4) << 24) | (sf << 4) | (sf << 29);
+__device__ __forceinline__ uint32_t mxf4_idesc(uint32_t m, int n, uint32_t sf) {
+    return (1u << 7) | (1u << 10) | ((uint32_t)(n >> 3) << 17) | (1u << 23) | ((m >> 4) << 24) | (sf << 4) | (sf << 29);
 }
 
 // Sixteen tokens of the lane's output column (32 neighbouring columns a warp).  16-bit results leave in pairs of columns where the rows
@@ -234,8 +260,11 @@ struct MatmulArgs {
     int pairs;               // results are 16-bit and pairs of columns 4-byte aligned in every row
 };
 
-template <int DT, int TERMS>
-__global__ void __launch_bounds__(kThreads, 2)
+// PAIR: clusters of two CTAs.  A pair takes 256 W rows, 128 each, and every MMA spans both; each CTA loads and holds half of the tile's A
+// rows (and the scales of all of them).  The even CTA issues; each CTA's loads count on its own barriers, the scale warps of both report to
+// the even one, commits arrive in both.  No load is broadcast.
+template <int DT, int TERMS, bool PAIR>
+__global__ void __launch_bounds__(kThreads, PAIR ? 1 : 2)
 mxfp4_matmul_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CUtensorMap tmap_a, const MatmulArgs g) {
     using T = typename Elem<DT>::T;
     extern __shared__ uint8_t smem_raw[];
@@ -252,12 +281,12 @@ mxfp4_matmul_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_con
     if (threadIdx.x == 0) {
         for (int i = 0; i < kMaxStages; i++) {
             mbar_init(bar(FULL + i), 1 + kLoaders);
-            mbar_init(bar(SC_FULL + i), 4);
+            mbar_init(bar(SC_FULL + i), PAIR ? 8 : 4);
             mbar_init(bar(EMPTY + i), 1);
         }
         for (int b = 0; b < 2; b++) {
             mbar_init(bar(ACC_FULL + b), 1);
-            mbar_init(bar(ACC_EMPTY + b), 4);
+            mbar_init(bar(ACC_EMPTY + b), PAIR ? 8 : 4);
         }
         *abort_flag = 0u;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -265,21 +294,30 @@ mxfp4_matmul_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_con
         asm volatile("prefetch.tensormap [%0];" ::"l"(&tmap_a) : "memory");
     }
     if (warp == 1) {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(s_misc)), "r"(g.tmem_cols) : "memory");
-        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+        if constexpr (PAIR) {
+            asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(s_misc)), "r"(g.tmem_cols) : "memory");
+            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+        } else {
+            asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(s_misc)), "r"(g.tmem_cols) : "memory");
+            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+        }
     }
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = *(volatile uint32_t*)s_misc;
+    if constexpr (PAIR) cluster_sync_all();   // both CTAs' barriers exist before either signals the other
     pdl_wait();   // the operands may come from the kernel before this one
 
-    const int rank = g.splits > 1 ? (int)cluster_ctarank() : 0;
+    const int half = PAIR ? (int)cluster_ctarank() : 0;   // of a pair
+    const int rank = !PAIR && g.splits > 1 ? (int)cluster_ctarank() : 0;   // among the splits of a tile
     const int n_kc = (g.K + kStageK - 1) / kStageK;
     const int kc0 = (int)((int64_t)n_kc * rank / g.splits), kc1 = (int)((int64_t)n_kc * (rank + 1) / g.splits);
-    const int tile0 = (int)blockIdx.x / g.splits, tile_step = (int)gridDim.x / g.splits;
-    const int BN = g.tokens;
-    const uint32_t b_bytes = (uint32_t)(TERMS * BN * kRowBytes);
+    const int per_tile = PAIR ? 2 : g.splits;               // CTAs
+    const int tile0 = (int)blockIdx.x / per_tile, tile_step = (int)gridDim.x / per_tile;
+    const int BN = g.tokens, held = PAIR ? BN / 2 : BN;    // A rows of a tile, and of them in this CTA
+    constexpr int kTileW = PAIR ? 2 * kWRows : kWRows;
+    const uint32_t b_bytes = (uint32_t)(TERMS * held * kRowBytes);
     const uint32_t sc_off = kWBytes + b_bytes;                  // the stage's scales: [W, term 0, ...][row][8]
     // scale slot of a stage: the two 128-column halves, each 4 columns a group (a term's groups side by side)
     const uint32_t slot0 = tmem + 2u * (uint32_t)BN, half_cols = 4u * (uint32_t)g.groups, slot_cols = 2u * half_cols;
@@ -291,7 +329,7 @@ mxfp4_matmul_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_con
             uint32_t s = 0, ph = 0;
             bool ok = true;
             for (int tile = tile0; tile < g.tiles && ok; tile += tile_step) {
-                const int w0 = (tile % g.tiles_w) * kWRows, a0 = (tile / g.tiles_w) * BN;
+                const int w0 = (tile % g.tiles_w) * kTileW + half * kWRows, a0 = (tile / g.tiles_w) * BN + half * held;
                 for (int kc = kc0; kc < kc1; kc++) {
                     ok = mbar_wait(bar(EMPTY) + 8u * s, ph ^ 1u, abort_flag);
                     if (!ok) break;
@@ -311,15 +349,15 @@ mxfp4_matmul_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_con
         // The whole warp walks the loop and one lane issues, under a predicate: the instruction takes its operands from uniform registers, and
         // inside a branch of one lane each of them had to be carried there first -- 230 clocks an MMA, whatever its size.  Votes keep the
         // loop's exits uniform.
-        const uint32_t leader = lane == 0 ? 1u : 0u;
+        const uint32_t leader = lane == 0 ? 1u : 0u, peer = PAIR ? map_to_cta(bar0, 1u) - bar0 : 0u;   // from a barrier here to the odd CTA's
         uint32_t s = 0, ph = 0, t = 0;
         bool ok = true;
         const uint64_t d0 = operand_desc(sbase);
         const uint32_t hi = (uint32_t)(d0 >> 32), lo0 = __shfl_sync(0xFFFFFFFFu, (uint32_t)d0, 0);
         const uint32_t tm = __shfl_sync(0xFFFFFFFFu, tmem, 0), slots = tm + 2u * (uint32_t)BN;
-        const uint32_t term_step = (uint32_t)(BN * kRowBytes) >> 4, stage_step = (uint32_t)g.stage_bytes >> 4;
-        const uint32_t idesc0 = mxf4_idesc(BN, 0u), idesc2 = mxf4_idesc(BN, 2u);
-        for (int tile = tile0; tile < g.tiles && ok; tile += tile_step, t++) {
+        const uint32_t term_step = (uint32_t)(held * kRowBytes) >> 4, stage_step = (uint32_t)g.stage_bytes >> 4;
+        const uint32_t idesc0 = mxf4_idesc(kTileW, BN, 0u), idesc2 = mxf4_idesc(kTileW, BN, 2u);
+        for (int tile = tile0; tile < g.tiles && ok && half == 0; tile += tile_step, t++) {
             const uint32_t b = t & 1u, acc = tm + b * (uint32_t)BN;
             ok = __all_sync(0xFFFFFFFFu, mbar_wait(bar(ACC_EMPTY) + 8u * b, ((t >> 1) & 1u) ^ 1u, abort_flag));
             if (!ok) break;
@@ -336,14 +374,18 @@ mxfp4_matmul_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_con
                         const uint32_t sfw = sc + (uint32_t)(ks >> 1) * half_cols;
 #pragma unroll
                         for (int q = 0; q < TERMS; q++)
-                            tc_mma_mxf4(leader, acc, a_lo + 2u * ks, b_lo + (uint32_t)q * term_step + 2u * ks, hi, (ks & 1) ? idesc2 : idesc0, sfw,
+                            tc_mma_mxf4<PAIR>(leader, acc, a_lo + 2u * ks, b_lo + (uint32_t)q * term_step + 2u * ks, hi, (ks & 1) ? idesc2 : idesc0, sfw,
                                         sfw + 4u + (uint32_t)(q * nb) * 4u, (kc > kc0 || ks > 0 || q > 0) ? 1u : 0u);
                     }
                 }
-                tc_commit(leader, bar(EMPTY) + 8u * s);
+                tc_commit<PAIR>(leader, bar(EMPTY) + 8u * s);
+                if constexpr (PAIR) tc_commit<PAIR>(leader, peer + bar(EMPTY) + 8u * s);
                 if (++s == (uint32_t)g.stages) { s = 0; ph ^= 1u; }
             }
-            if (ok) tc_commit(leader, bar(ACC_FULL) + 8u * b);
+            if (ok) {
+                tc_commit<PAIR>(leader, bar(ACC_FULL) + 8u * b);
+                if constexpr (PAIR) tc_commit<PAIR>(leader, peer + bar(ACC_FULL) + 8u * b);
+            }
         }
     } else if (warp >= kLoadWarp0) {
         // --------------------------------------------------------- scale loaders
@@ -353,7 +395,7 @@ mxfp4_matmul_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_con
         uint32_t s = 0, ph = 0;
         bool ok = true;
         for (int tile = tile0; tile < g.tiles && ok; tile += tile_step) {
-            const int64_t w_row = (int64_t)(tile % g.tiles_w) * kWRows + r, a_row0 = (int64_t)(tile / g.tiles_w) * BN;
+            const int64_t w_row = (int64_t)(tile % g.tiles_w) * kTileW + half * kWRows + r, a_row0 = (int64_t)(tile / g.tiles_w) * BN;
             // this thread's row of every group, null where the operand has none
             const uint8_t* row[kMaxGroups];
             row[0] = w_row < g.N ? g.w_scales + w_row * nblk : nullptr;
@@ -436,7 +478,10 @@ if constexpr (TERMS == 1) {
                 asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
                 tc_fence_before();
                 __syncwarp();
-                if (lane == 0) mbar_arrive(bar(SC_FULL) + 8u * s);
+                if (lane == 0) {
+                    if (PAIR && half != 0) mbar_arrive_cluster(map_to_cta(bar(SC_FULL) + 8u * s, 0u));
+                    else mbar_arrive(bar(SC_FULL) + 8u * s);
+                }
                 if (++s == (uint32_t)g.stages) { s = 0; ph ^= 1u; }
             }
     } else if (warp >= kEpiWarp0) {
@@ -445,7 +490,7 @@ if constexpr (TERMS == 1) {
         uint32_t t = 0;
         bool ok = true;
         for (int tile = tile0; tile < g.tiles && ok; tile += tile_step, t++) {
-            const int64_t n = (int64_t)(tile % g.tiles_w) * kWRows + q * 32 + lane, m0 = (int64_t)(tile / g.tiles_w) * BN;
+            const int64_t n = (int64_t)(tile % g.tiles_w) * kTileW + half * kWRows + q * 32 + lane, m0 = (int64_t)(tile / g.tiles_w) * BN;
             const uint32_t b = t & 1u, acc = tmem + b * (uint32_t)BN + ((q * 32u) << 16);
             ok = mbar_wait(bar(ACC_FULL) + 8u * b, (t >> 1) & 1u, abort_flag);
             if (!ok) break;
@@ -456,7 +501,7 @@ if constexpr (TERMS == 1) {
                 uint32_t v[16];
                 tc_ld16(acc + (uint32_t)c0, v);
                 tc_wait_ld();
-                if (g.splits > 1) {   // the partial tile, token-major, in the ring's memory (every stage has been consumed)
+                if (!PAIR && g.splits > 1) {   // the partial tile, token-major, in the ring's memory (every stage has been consumed)
                     float* p = reinterpret_cast<float*>(smem) + (size_t)c0 * kWRows + q * 32 + lane;
 #pragma unroll
                     for (int j = 0; j < 16; j++) p[j * kWRows] = __uint_as_float(v[j]);
@@ -467,14 +512,18 @@ if constexpr (TERMS == 1) {
             }
             tc_fence_before();
             __syncwarp();
-            if (lane == 0) mbar_arrive(bar(ACC_EMPTY) + 8u * b);
+            if (lane == 0) {
+                if (PAIR && half != 0) mbar_arrive_cluster(map_to_cta(bar(ACC_EMPTY) + 8u * b, 0u));
+                else mbar_arrive(bar(ACC_EMPTY) + 8u * b);
+            }
         }
     }
 
     tc_fence_before();
     __syncthreads();
     if (threadIdx.x == 0 && *abort_flag) atomicOr(&g_head_error, 1u);
-    if (g.splits > 1) {
+    if constexpr (PAIR) cluster_sync_all();   // neither CTA's shared or tensor memory goes away while the other may still use it
+    if (!PAIR && g.splits > 1) {
         cluster_sync_all();
         // CTA `rank` adds the tokens rank, rank + splits, ... of all partial tiles, in rank order
         const int64_t w0 = (int64_t)(tile0 % g.tiles_w) * kWRows, m0 = (int64_t)(tile0 / g.tiles_w) * BN;
@@ -490,7 +539,8 @@ if constexpr (TERMS == 1) {
     }
     if (warp == 1) {
         tc_fence_after();
-        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(g.tmem_cols) : "memory");
+        if constexpr (PAIR) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(g.tmem_cols) : "memory");
+        else asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(g.tmem_cols) : "memory");
     }
 }
 
@@ -501,18 +551,20 @@ constexpr int kSmallMin = 77 * 1024, kSmallMax = 112 * 1024, kLargeMin = 160 * 1
 
 struct Plan {
     int tokens, stages, stage_bytes, groups, tmem_cols, smem, per_sm, splits, tiles_w, tiles_m;
+    bool pair;
 };
 
-bool plan_block(int terms, int tokens, Plan* p) {
+bool plan_block(int terms, int tokens, bool pair, Plan* p) {
     const int nb = (tokens + 127) / 128, groups = 1 + terms * nb;
     p->tokens = tokens;
+    p->pair = pair;
     p->groups = groups;
-    p->stage_bytes = kWBytes + terms * tokens * kRowBytes + groups * kGroupBytes;
+    p->stage_bytes = kWBytes + terms * (pair ? tokens / 2 : tokens) * kRowBytes + groups * kGroupBytes;
     auto cols = [&](int stages) { return 2 * tokens + stages * 8 * groups; };
     auto pow2 = [](int c) { int r = 32; while (r < c) r *= 2; return r; };
     int st = std::min(kMaxStages, (kSmallMax - 1024) / p->stage_bytes);
     while (st > 3 && cols(st) > 256) st--;
-    if (st >= 3 && cols(st) <= 256) {
+    if (!pair && st >= 3 && cols(st) <= 256) {
         p->stages = st;
         p->smem = std::max(kSmallMin, st * p->stage_bytes + 1024);
         p->per_sm = 2;
@@ -528,42 +580,48 @@ bool plan_block(int terms, int tokens, Plan* p) {
     return p->stages * p->stage_bytes >= tokens * kWRows * 4;   // a partial tile fits into the ring
 }
 
-// Tokens a tile and splits of the columns, from a model of the time in clocks: a stage costs an SM its MMAs (tokens / 2 clocks per 64
-// columns and term) or its copies (about 40 bytes a clock and SM from L2), whichever is longer; a block about 3000 clocks before and
-// after its stages, a joined tile another 1500; and the operands come from HBM at about 23 bytes a clock and SM.
-bool make_plan(int64_t M, int64_t N, int K, int terms, int sms, Plan* best) {
+// Tokens a tile, pairs or single CTAs, and splits of the columns, from a model of the time in clocks.  A stage costs its MMAs (tokens / 2
+// clocks per 64 columns and term) or its shared-memory traffic -- operand reads of the MMAs, what lands, four reads of the scales -- at 128
+// bytes a clock with a third on top, or its copies at about 45 bytes a clock from L2; a block about 3000 clocks before and after its stages, a
+// joined tile another 1500; and the operands come from HBM at about 23 bytes a clock and SM.
+bool make_plan(int64_t M, int64_t N, int K, int terms, int sms, bool pairs_run, Plan* best) {
     const int n_kc = (K + kStageK - 1) / kStageK;
-    const int tiles_w = (int)((N + kWRows - 1) / kWRows);
     double best_t = 1e300;
     const int most = terms == 1 ? kMaxTokens : 128;
-    for (int tokens = 16; tokens <= most && tokens < M + 16; tokens += 16) {
-        Plan p;
-        if (!plan_block(terms, tokens, &p)) continue;
-        p.tiles_w = tiles_w;
-        p.tiles_m = (int)((M + tokens - 1) / tokens);
-        for (int s = 1; s <= 8 && s <= n_kc; s *= 2) {
-            const int64_t units = (int64_t)p.tiles_w * p.tiles_m * s;
-            if (s > 1 && units > (int64_t)sms * p.per_sm) break;
-            const double stage = std::max(4.0 * terms * tokens / 2, p.stage_bytes / 40.0);
-            const double busiest = (double)((units + sms - 1) / sms);
+    for (int pair = 0; pair <= (pairs_run ? 1 : 0); pair++)
+        for (int tokens = 16; tokens <= most && tokens < M + 16; tokens += 16) {
+            Plan p;
+            if (!plan_block(terms, tokens, pair != 0, &p)) continue;
+            const int ctas = pair ? 2 : 1;
+            p.tiles_w = (int)((N + kWRows * ctas - 1) / (kWRows * ctas));
+            p.tiles_m = (int)((M + tokens - 1) / tokens);
+            const int held = pair ? tokens / 2 : tokens;
+            const double mma = 4.0 * terms * tokens / 2;
+            const double shared = 1.33 * (4.0 * terms * (4096 + 32.0 * held) + p.stage_bytes + 4.0 * p.groups * kGroupBytes) / 128;
+            const double stage = std::max(std::max(mma, shared), p.stage_bytes / 45.0);
             const double hbm = ((double)N + (double)terms * M) * K * 17 / 32 / (23.0 * sms);
-            const double t = std::max(busiest * ((n_kc + s - 1) / s) * stage, hbm) + 3000.0 * ((units + (int64_t)sms * p.per_sm - 1) / ((int64_t)sms * p.per_sm)) +
-                             (s > 1 ? 1500.0 + 20.0 * tokens : 0.0) + 30.0 * tokens;
-            if (t < best_t) {
-                best_t = t;
-                p.splits = s;
-                *best = p;
+            for (int s = 1; s <= (pair ? 1 : 8) && s <= n_kc; s *= 2) {
+                const int64_t units = (int64_t)p.tiles_w * p.tiles_m * s, slots = (int64_t)sms / ctas;
+                if (s > 1 && units > slots * p.per_sm) break;
+                const double busiest = (double)((units + slots - 1) / slots);
+                const double t = std::max(busiest * ((n_kc + s - 1) / s) * stage, hbm) + 3000.0 * ((units + slots * p.per_sm - 1) / (slots * p.per_sm)) +
+                                 (s > 1 ? 1500.0 + 20.0 * tokens : 0.0) + 30.0 * tokens;
+                if (t < best_t) {
+                    best_t = t;
+                    p.splits = s;
+                    *best = p;
+                }
             }
         }
-    }
     return best_t < 1e300;
 }
 
-template <int DT, int TERMS>
-int launch(const Plan& p, const CUtensorMap& w, const CUtensorMap& a, MatmulArgs g, int sms, cudaStream_t stream) {
+template <int DT, int TERMS, bool PAIR>
+int launch(const Plan& p, const CUtensorMap& w, const CUtensorMap& a, const MatmulArgs& g, int sms, cudaStream_t stream) {
+    const int cluster = PAIR ? 2 : p.splits;
+    const int64_t tiles = (int64_t)p.tiles_w * p.tiles_m;
     cudaLaunchConfig_t cfg = {};
-    const int64_t units = (int64_t)p.tiles_w * p.tiles_m * p.splits;
-    cfg.gridDim = dim3((unsigned)(p.splits > 1 ? units : std::min<int64_t>(units, (int64_t)sms * p.per_sm)));
+    cfg.gridDim = dim3((unsigned)(cluster * (p.splits > 1 ? tiles : std::min<int64_t>(tiles, (int64_t)sms / cluster * p.per_sm))));
     cfg.blockDim = dim3(kThreads);
     cfg.dynamicSmemBytes = (size_t)p.smem;
     cfg.stream = stream;
@@ -571,53 +629,70 @@ int launch(const Plan& p, const CUtensorMap& w, const CUtensorMap& a, MatmulArgs
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     attr[1].id = cudaLaunchAttributeClusterDimension;
-    attr[1].val.clusterDim.x = (unsigned)p.splits;
+    attr[1].val.clusterDim.x = (unsigned)cluster;
     attr[1].val.clusterDim.y = 1;
     attr[1].val.clusterDim.z = 1;
     cfg.attrs = attr;
-    cfg.numAttrs = p.splits > 1 ? 2 : 1;
-    DSX_CUDA(cudaLaunchKernelEx(&cfg, mxfp4_matmul_kernel<DT, TERMS>, w, a, g));
+    cfg.numAttrs = cluster > 1 ? 2 : 1;
+    DSX_CUDA(cudaLaunchKernelEx(&cfg, mxfp4_matmul_kernel<DT, TERMS, PAIR>, w, a, g));
     DSX_LAUNCHED();
     return DSX_OK;
 }
 
-template <typename F>
-void for_each_kernel(F f) {
-    f(mxfp4_matmul_kernel<DSX_F32, 1>);
-    f(mxfp4_matmul_kernel<DSX_F32, 2>);
-    f(mxfp4_matmul_kernel<DSX_F32, 3>);
-    f(mxfp4_matmul_kernel<DSX_BF16, 1>);
-    f(mxfp4_matmul_kernel<DSX_BF16, 2>);
-    f(mxfp4_matmul_kernel<DSX_BF16, 3>);
-    f(mxfp4_matmul_kernel<DSX_F16, 1>);
-    f(mxfp4_matmul_kernel<DSX_F16, 2>);
-    f(mxfp4_matmul_kernel<DSX_F16, 3>);
-}
 template <int DT>
-int launch_terms(int terms, const Plan& p, const CUtensorMap& w, const CUtensorMap& a, const MatmulArgs& g, int sms, cudaStream_t stream) {
-    if (terms == 1) return launch<DT, 1>(p, w, a, g, sms, stream);
-    if (terms == 2) return launch<DT, 2>(p, w, a, g, sms, stream);
-    return launch<DT, 3>(p, w, a, g, sms, stream);
+int launch_for(int terms, const Plan& p, const CUtensorMap& w, const CUtensorMap& a, const MatmulArgs& g, int sms, cudaStream_t stream) {
+    if (terms == 1) return p.pair ? launch<DT, 1, true>(p, w, a, g, sms, stream) : launch<DT, 1, false>(p, w, a, g, sms, stream);
+    if (terms == 2) return p.pair ? launch<DT, 2, true>(p, w, a, g, sms, stream) : launch<DT, 2, false>(p, w, a, g, sms, stream);
+    return p.pair ? launch<DT, 3, true>(p, w, a, g, sms, stream) : launch<DT, 3, false>(p, w, a, g, sms, stream);
 }
 
-// SM count of the current device; the opt-in to large shared memory is made once per device.
-int configure(int* sms) {
+template <int DT, int TERMS>
+int allow_shared() {
+    DSX_CUDA(cudaFuncSetAttribute(mxfp4_matmul_kernel<DT, TERMS, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, kLargeMax));
+    DSX_CUDA(cudaFuncSetAttribute(mxfp4_matmul_kernel<DT, TERMS, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, kLargeMax));
+    return DSX_OK;
+}
+template <int DT>
+int allow_shared_all() {
+    if (int rc = allow_shared<DT, 1>()) return rc;
+    if (int rc = allow_shared<DT, 2>()) return rc;
+    return allow_shared<DT, 3>();
+}
+
+// SM count of the current device and whether it runs CTA pairs (a partition of a device may not hold a cluster of two); looked up,
+// and the opt-in to large shared memory made, once per device.
+int configure(int* sms, bool* pairs_run) {
     constexpr int kMaxDevices = 64;
-    static std::atomic<int> sm_counts[kMaxDevices];
+    static std::atomic<int> known[kMaxDevices];   // SM count, its sign bit saying that pairs do not run
     int dev = 0;
     DSX_CUDA(cudaGetDevice(&dev));
     DSX_REQUIRE(dev >= 0 && dev < kMaxDevices, "mxfp4_matmul: device index %d out of range", dev);
-    int n = sm_counts[dev].load(std::memory_order_acquire);
+    int n = known[dev].load(std::memory_order_acquire);
     if (n == 0) {
         DSX_CUDA(cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev));
-        int rc = DSX_OK;
-        for_each_kernel([&](auto* kernel) {
-            if (rc == DSX_OK) rc = [&]() -> int { DSX_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kLargeMax)); return DSX_OK; }();
-        });
-        if (rc != DSX_OK) return rc;
-        sm_counts[dev].store(n, std::memory_order_release);
+        if (int rc = allow_shared_all<DSX_F32>()) return rc;
+        if (int rc = allow_shared_all<DSX_BF16>()) return rc;
+        if (int rc = allow_shared_all<DSX_F16>()) return rc;
+        cudaLaunchConfig_t lc = {};
+        lc.gridDim = dim3(2);
+        lc.blockDim = dim3(kThreads);
+        lc.dynamicSmemBytes = kLargeMax;
+        cudaLaunchAttribute attr[1];
+        attr[0].id = cudaLaunchAttributeClusterDimension;
+        attr[0].val.clusterDim.x = 2;
+        attr[0].val.clusterDim.y = 1;
+        attr[0].val.clusterDim.z = 1;
+        lc.attrs = attr;
+        lc.numAttrs = 1;
+        int clusters = 0;
+        if (cudaOccupancyMaxActiveClusters(&clusters, mxfp4_matmul_kernel<DSX_F32, 1, true>, &lc) != cudaSuccess || clusters < 1) {
+            (void)cudaGetLastError();
+            n = -n;
+        }
+        known[dev].store(n, std::memory_order_release);
     }
-    *sms = n;
+    *sms = n < 0 ? -n : n;
+    *pairs_run = n > 0;
     return DSX_OK;
 }
 
@@ -640,9 +715,10 @@ int dsx_mxfp4_matmul(const void* a_codes, const void* a_scales, int n_terms, int
     DSX_REQUIRE((((uintptr_t)a_codes | (uintptr_t)w_codes) & 15) == 0 && ((uintptr_t)out & (dtype_size(dtype) - 1)) == 0,
                 "mxfp4_matmul: codes must be 16-byte aligned, out aligned to its elements");
     int sms = 0;
-    if (int rc = configure(&sms)) return rc;
+    bool pairs_run = false;
+    if (int rc = configure(&sms, &pairs_run)) return rc;
     Plan p;
-    if (!make_plan(m, n, (int)k, n_terms, sms, &p)) return set_error(DSX_ERR_UNSUPPORTED, "mxfp4_matmul: no tile for %d terms", n_terms);
+    if (!make_plan(m, n, (int)k, n_terms, sms, pairs_run, &p)) return set_error(DSX_ERR_UNSUPPORTED, "mxfp4_matmul: no tile for %d terms", n_terms);
     DSX_REQUIRE((int64_t)p.tiles_w * p.tiles_m < ((int64_t)1 << 30), "mxfp4_matmul: too many tiles");
     CUtensorMap tw, ta;
     {
@@ -654,7 +730,7 @@ int dsx_mxfp4_matmul(const void* a_codes, const void* a_scales, int n_terms, int
     {
         const cuuint64_t dims[3] = {(cuuint64_t)(k / 2), (cuuint64_t)m, (cuuint64_t)n_terms};
         const cuuint64_t strides[2] = {(cuuint64_t)(k / 2), (cuuint64_t)(m * (k / 2))};
-        const cuuint32_t box[3] = {(cuuint32_t)kRowBytes, (cuuint32_t)p.tokens, (cuuint32_t)n_terms};
+        const cuuint32_t box[3] = {(cuuint32_t)kRowBytes, (cuuint32_t)(p.pair ? p.tokens / 2 : p.tokens), (cuuint32_t)n_terms};
         if (int rc = tmap_encode(&ta, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, a_codes, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B)) return rc;
     }
     MatmulArgs g{};
@@ -668,9 +744,9 @@ int dsx_mxfp4_matmul(const void* a_codes, const void* a_scales, int n_terms, int
     g.aligned = k % kStageK == 0 && (((uintptr_t)a_scales | (uintptr_t)w_scales) & 7) == 0;
     g.pairs = dtype != DSX_F32 && n % 2 == 0 && (row_stride % 2 == 0 || m == 1) && ((uintptr_t)out & 3) == 0;
     const cudaStream_t s = (cudaStream_t)stream;
-    if (dtype == DSX_F32) return launch_terms<DSX_F32>(n_terms, p, tw, ta, g, sms, s);
-    if (dtype == DSX_BF16) return launch_terms<DSX_BF16>(n_terms, p, tw, ta, g, sms, s);
-    return launch_terms<DSX_F16>(n_terms, p, tw, ta, g, sms, s);
+    if (dtype == DSX_F32) return launch_for<DSX_F32>(n_terms, p, tw, ta, g, sms, s);
+    if (dtype == DSX_BF16) return launch_for<DSX_BF16>(n_terms, p, tw, ta, g, sms, s);
+    return launch_for<DSX_F16>(n_terms, p, tw, ta, g, sms, s);
 }
 
 int dsx_head_check(dsx_stream_t stream_, uint32_t* error_word) {
