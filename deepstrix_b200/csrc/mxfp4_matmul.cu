@@ -9,11 +9,12 @@
 // few hundred run on the same kernel: a decode batch is an N of 16 under a stream of weights.  The terms of A are further MMAs into
 // the same accumulator: W is read once for all of them.  A pipeline stage is 256 columns: 128-byte rows (128-byte swizzle) of W and of every
 // term, each one TMA box, zero-filled past the operand's edges; and their scale bytes.
-// Scales are read as stored (row-major bytes; nothing is laid out beforehand): four loader warps, a row of every 128-row group a
-// thread, bring the stage's 8 bytes of each row into shared memory -- by 8-byte asynchronous copies where rows of scales are 8-byte
-// aligned, else as the aligned words that hold them, requested a stage ahead and shifted into place -- and four scale warps, one per
-// lane quarter, move a landed stage's scales to tensor memory (ld.shared + tcgen05.st; the tensor core's own copy would queue behind its MMAs).
-// Warp roles: TMA producer, MMA issue, 4 loaders, 4 scale warps, 4 epilogue warps; two accumulators, so that a
+// Scales are read as stored (row-major bytes; nothing is laid out beforehand), 16 bytes of every row -- 512 columns, two stages -- at a time
+// into a ring of their own: by TMA where rows of scales are 16-byte aligned (K a multiple of 512), else by four loader warps, a row of
+// every 128-row group a thread, as the aligned words that hold them, requested ahead and shifted into place.  (Asynchronous copies of 8 bytes
+// a row and stage kept the shared-memory pipe 60 % busy with 32 lines an instruction.)  Four scale warps, one per lane quarter, move them to
+// tensor memory a stage at a time (ld.shared + tcgen05.st; the tensor core's own copy would queue behind its MMAs).
+// Warp roles: TMA of codes, MMA issue, TMA of scales, 4 scale warps, 4 epilogue warps, 4 loaders; two accumulators, so that a
 // tile is read out under the next one's MMAs.
 // Few tiles: the columns are split over the CTAs of a cluster; each leaves its partial tile in shared memory and the cluster adds
 // them in rank order through distributed shared memory, so results do not depend on timing and need no workspace.
@@ -31,13 +32,14 @@ namespace {
 
 __device__ uint32_t g_head_error = 0;
 
-constexpr int kScaleWarp0 = 4, kEpiWarp0 = 8, kLoadWarp0 = 12, kThreads = 512;   // roles start on warp-group boundaries; warps 2 and 3 are idle
+constexpr int kScaleWarp0 = 4, kEpiWarp0 = 8, kLoadWarp0 = 12, kThreads = 512;   // roles start on warp-group boundaries; warp 3 is idle
 constexpr int kLoaders = 128;
 constexpr int kWRows = 128;          // W rows of a tile
 constexpr int kStageK = 256;         // columns of a stage
 constexpr int kRowBytes = kStageK / 2;
 constexpr int kWBytes = kWRows * kRowBytes;
-constexpr int kGroupBytes = 1024;    // scale bytes of a group of 128 rows: 8 a row
+constexpr int kGroupBytes = 2048;    // scale bytes of a group of 128 rows: 16 a row, two stages
+constexpr int kMaxScaleBufs = 3;
 constexpr int kMaxGroups = 4;        // W and up to three term groups
 constexpr int kMaxStages = 8;
 constexpr int kMaxTokens = 208;      // A rows of a tile: two accumulators and four scale slots fill tensor memory
@@ -159,16 +161,16 @@ __device__ __forceinline__ void tc_st(uint32_t taddr, const uint32_t (&r)[32]) {
         "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
         : "memory");
 }
-// Scales of a landed stage, this lane's rows (row 32 j + lane of group i at src + i * kGroupBytes + j * 256), to the stage's slot: both
+// Scales of a landed stage, this lane's rows (row 32 j + lane of group i at src + group i + j * 512), to the stage's slot: both
 // 128-column halves, 4 columns a group each -- one or two wide stores (a 4-column store a group and half took 100 clocks apiece).
 template <int GROUPS>
-__device__ __forceinline__ void store_scales(const uint8_t* src, uint32_t dst) {
+__device__ __forceinline__ void store_scales(const uint8_t* src, uint32_t group_step, uint32_t dst) {
     uint32_t v[8 * GROUPS];
 #pragma unroll
     for (int i = 0; i < GROUPS; i++)
 #pragma unroll
         for (int j = 0; j < 4; j++) {
-            const uint2 two = *reinterpret_cast<const uint2*>(src + i * kGroupBytes + j * 256);
+            const uint2 two = *reinterpret_cast<const uint2*>(src + (i ? kGroupBytes + (i - 1) * group_step : 0u) + j * 512);
             v[4 * i + j] = two.x;
             v[4 * GROUPS + 4 * i + j] = two.y;
         }
@@ -251,12 +253,13 @@ struct MatmulArgs {
     int64_t M, N;
     int K;
     int tokens;              // A rows of a tile (multiple of 16)
-    int stages, stage_bytes; // ring
+    int stages, stage_bytes; // ring of codes, and of scale slots in tensor memory
+    int scale_bufs;          // ring of scales, kGroupBytes a group
     int groups;              // 128-row groups of scales: 1 (W) + terms * ceil(tokens / 128)
     int tmem_cols;
     int splits;              // CTAs of a cluster that share a tile's columns
     int tiles_w, tiles;      // tile t: W tile t % tiles_w, token tile t / tiles_w
-    int aligned;             // rows of scales are 8-byte aligned
+    int scale_tma;           // rows of scales are 16-byte aligned: TMA brings them
     int pairs;               // results are 16-bit and pairs of columns 4-byte aligned in every row
 };
 
@@ -265,28 +268,35 @@ struct MatmulArgs {
 // the even one, commits arrive in both.  No load is broadcast.
 template <int DT, int TERMS, bool PAIR>
 __global__ void __launch_bounds__(kThreads, PAIR ? 1 : 2)
-mxfp4_matmul_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CUtensorMap tmap_a, const MatmulArgs g) {
+mxfp4_matmul_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_ws,
+                    const __grid_constant__ CUtensorMap tmap_as, const MatmulArgs g) {
     using T = typename Elem<DT>::T;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
-    __shared__ __align__(8) uint64_t s_bars[3 * kMaxStages + 4];
+    __shared__ __align__(8) uint64_t s_bars[3 * kMaxStages + 4 + 2 * kMaxScaleBufs];
     __shared__ uint32_t s_misc[2];
     const uint32_t sbase = smem_u32(smem), bar0 = smem_u32(s_bars);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    // FULL[s]: codes (TMA bytes) and scales (loaders) of the stage have landed; SC_FULL[s]: its scales are in tensor memory;
-    // EMPTY[s]: the MMAs that read it have completed; ACC_FULL / ACC_EMPTY[b]: accumulator b is complete / read out.
-    constexpr int FULL = 0, SC_FULL = kMaxStages, EMPTY = 2 * kMaxStages, ACC_FULL = 3 * kMaxStages, ACC_EMPTY = ACC_FULL + 2;
+    // FULL[s]: the codes of the stage have landed; SC_FULL[s]: its scales are in tensor memory (a pair: those of both CTAs, and the odd CTA's
+    // codes have landed); EMPTY[s]: the MMAs that read it have completed; ACC_FULL / ACC_EMPTY[b]: accumulator b is complete / read out;
+    // RAW_FULL / RAW_EMPTY[d]: two stages' scales have landed / are in tensor memory.
+    constexpr int FULL = 0, SC_FULL = kMaxStages, EMPTY = 2 * kMaxStages, ACC_FULL = 3 * kMaxStages, ACC_EMPTY = ACC_FULL + 2, RAW_FULL = ACC_EMPTY + 2,
+                  RAW_EMPTY = RAW_FULL + kMaxScaleBufs;
     auto bar = [&](int i) { return bar0 + 8u * (uint32_t)i; };
     volatile uint32_t* abort_flag = s_misc + 1;
     if (threadIdx.x == 0) {
         for (int i = 0; i < kMaxStages; i++) {
-            mbar_init(bar(FULL + i), 1 + kLoaders);
+            mbar_init(bar(FULL + i), 1);
             mbar_init(bar(SC_FULL + i), PAIR ? 8 : 4);
             mbar_init(bar(EMPTY + i), 1);
         }
         for (int b = 0; b < 2; b++) {
             mbar_init(bar(ACC_FULL + b), 1);
             mbar_init(bar(ACC_EMPTY + b), PAIR ? 8 : 4);
+        }
+        for (int d = 0; d < kMaxScaleBufs; d++) {
+            mbar_init(bar(RAW_FULL + d), g.scale_tma ? 1 : kLoaders);
+            mbar_init(bar(RAW_EMPTY + d), 4);
         }
         *abort_flag = 0u;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -318,7 +328,9 @@ mxfp4_matmul_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_con
     const int BN = g.tokens, held = PAIR ? BN / 2 : BN;    // A rows of a tile, and of them in this CTA
     constexpr int kTileW = PAIR ? 2 * kWRows : kWRows;
     const uint32_t b_bytes = (uint32_t)(TERMS * held * kRowBytes);
-    const uint32_t sc_off = kWBytes + b_bytes;                  // the stage's scales: [W, term 0, ...][row][8]
+    // scales behind the ring of codes: [buffer][W, term 0, ...][row][16]; a term's group has room for 128 rows behind the previous one's rows
+    const uint32_t raw0 = (uint32_t)(g.stages * g.stage_bytes), raw_bytes = (uint32_t)(g.groups * kGroupBytes);
+    const uint32_t group_step = BN > 128 ? (uint32_t)kGroupBytes : (uint32_t)BN * 16u;
     // scale slot of a stage: the two 128-column halves, each 4 columns a group (a term's groups side by side)
     const uint32_t slot0 = tmem + 2u * (uint32_t)BN, half_cols = 4u * (uint32_t)g.groups, slot_cols = 2u * half_cols;
     const int nb = (BN + 127) >> 7;
@@ -387,100 +399,116 @@ mxfp4_matmul_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_con
                 if constexpr (PAIR) tc_commit<PAIR>(leader, peer + bar(ACC_FULL) + 8u * b);
             }
         }
+    } else if (warp == 2) {
+        // --------------------------------------------------------- TMA of scales
+        if (lane == 0 && g.scale_tma) {
+            uint32_t d = 0, ph = 0;
+            bool ok = true;
+            for (int tile = tile0; tile < g.tiles && ok; tile += tile_step) {
+                const int w0 = (tile % g.tiles_w) * kTileW + half * kWRows, a0 = (tile / g.tiles_w) * BN;
+                for (int kc = kc0 & ~1; kc < kc1; kc += 2) {
+                    ok = mbar_wait(bar(RAW_EMPTY) + 8u * d, ph ^ 1u, abort_flag);
+                    if (!ok) break;
+                    const uint32_t dst = sbase + raw0 + d * raw_bytes, full = bar(RAW_FULL) + 8u * d;
+                    mbar_expect_tx(full, kGroupBytes + (uint32_t)(TERMS * BN * 16));
+                    tma_load_2d(dst, &tmap_ws, kc * 8, w0, full);
+                    tma_load_3d(dst + kGroupBytes, &tmap_as, kc * 8, a0, 0, full);
+                    if (++d == (uint32_t)g.scale_bufs) { d = 0; ph ^= 1u; }
+                }
+            }
+            if (!ok)
+                for (uint32_t i = 0; i < (uint32_t)g.scale_bufs; i++)
+                    for (uint32_t n = 0; n < kSpinLimit / 64 && !mbar_try(bar(RAW_FULL) + 8u * i, i < d ? ph : ph ^ 1u); n++) {}
+        }
     } else if (warp >= kLoadWarp0) {
         // --------------------------------------------------------- scale loaders
-        const int r = threadIdx.x - kLoadWarp0 * 32;   // row of every group
-        const int nblk = g.K >> 5;
-        const uint32_t dst0 = sbase + sc_off + (uint32_t)r * 8u;
-        uint32_t s = 0, ph = 0;
-        bool ok = true;
-        for (int tile = tile0; tile < g.tiles && ok; tile += tile_step) {
-            const int64_t w_row = (int64_t)(tile % g.tiles_w) * kTileW + half * kWRows + r, a_row0 = (int64_t)(tile / g.tiles_w) * BN;
-            // this thread's row of every group, null where the operand has none
-            const uint8_t* row[kMaxGroups];
-            row[0] = w_row < g.N ? g.w_scales + w_row * nblk : nullptr;
+        if (!g.scale_tma) {
+            const int r = threadIdx.x - kLoadWarp0 * 32;   // row of every group
+            const int nblk = g.K >> 5;
+            uint32_t d = 0, ph = 0;
+            bool ok = true;
+            for (int tile = tile0; tile < g.tiles && ok; tile += tile_step) {
+                const int64_t w_row = (int64_t)(tile % g.tiles_w) * kTileW + half * kWRows + r, a_row0 = (int64_t)(tile / g.tiles_w) * BN;
+                // this thread's row of every group, null where the operand has none
+                const uint8_t* row[kMaxGroups];
+                bool place[kMaxGroups];   // the group has room for it
+                row[0] = w_row < g.N ? g.w_scales + w_row * nblk : nullptr;
+                place[0] = true;
 #pragma unroll
-            for (int i = 1; i < kMaxGroups; i++) {
-                const int q = nb == 2 ? 0 : i - 1, ra = (nb == 2 ? (i - 1) * 128 : 0) + r;   // nb == 2 only with one term
-                row[i] = i < g.groups && ra < BN && a_row0 + ra < g.M ? g.a_scales + ((int64_t)q * g.M + a_row0 + ra) * nblk : nullptr;
-            }
-            if (g.aligned) {
-                for (int kc = kc0; kc < kc1; kc++) {
-                    ok = mbar_wait(bar(EMPTY) + 8u * s, ph ^ 1u, abort_flag);
-                    if (!ok) break;
-                    const uint32_t dst = dst0 + s * (uint32_t)g.stage_bytes;
-#pragma unroll
-                    for (int i = 0; i < kMaxGroups; i++)
-                        if (i < g.groups)   // zero-filled where there is no row
-                            asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(dst + i * kGroupBytes), "l"(row[i] ? row[i] + kc * 8 : g.w_scales),
-                                         "r"(row[i] ? 8 : 0)
-                                         : "memory");
-                    asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar(FULL) + 8u * s) : "memory");
-                    if (++s == (uint32_t)g.stages) { s = 0; ph ^= 1u; }
+                for (int i = 1; i < kMaxGroups; i++) {
+                    const int q = nb == 2 ? 0 : i - 1, ra = (nb == 2 ? (i - 1) * 128 : 0) + r;   // nb == 2 only with one term
+                    place[i] = i < g.groups && ra < BN;
+                    row[i] = place[i] && a_row0 + ra < g.M ? g.a_scales + ((int64_t)q * g.M + a_row0 + ra) * nblk : nullptr;
                 }
-            } else {
-                // the aligned words that hold bytes blk .. blk + 7 of a row (the row's last bytes: fewer), at most three
-                auto fetch = [&](const uint8_t* p, int blk, uint32_t (&w)[3]) {
-                    const int n = p ? min(8, nblk - blk) : 0;
+                // the aligned words that hold bytes blk .. blk + 15 of a row (the row's last bytes: fewer), at most five
+                auto fetch = [&](const uint8_t* p, int blk, uint32_t (&w)[5]) {
+                    const int n = p ? min(16, nblk - blk) : 0;
                     const uintptr_t at = (uintptr_t)p + blk;
                     const uint32_t* q = reinterpret_cast<const uint32_t*>(at & ~(uintptr_t)3);
                     const int span = n > 0 ? (int)(at & 3) + n : 0;
 #pragma unroll
-                    for (int j = 0; j < 3; j++) w[j] = 4 * j < span ? __ldg(q + j) : 0u;
+                    for (int j = 0; j < 5; j++) w[j] = 4 * j < span ? __ldg(q + j) : 0u;
                 };
-                uint32_t w[kMaxGroups][3];
+                for (int kc = kc0 & ~1; kc < kc1; kc += 2) {
+                    uint32_t w[kMaxGroups][5];
 #pragma unroll
-                for (int i = 0; i < kMaxGroups; i++) fetch(row[i], kc0 * 8, w[i]);
-                for (int kc = kc0; kc < kc1; kc++) {
-                    uint32_t lo[kMaxGroups], hi[kMaxGroups];
+                    for (int i = 0; i < kMaxGroups; i++) fetch(row[i], kc * 8, w[i]);   // requested before the wait
+                    ok = mbar_wait(bar(RAW_EMPTY) + 8u * d, ph ^ 1u, abort_flag);
+                    if (!ok) break;
+                    const uint32_t dst = sbase + raw0 + d * raw_bytes + (uint32_t)r * 16u;
+                    const int n = nblk - kc * 8;   // bytes past the row's end belong to the next row
 #pragma unroll
                     for (int i = 0; i < kMaxGroups; i++) {
                         const uint32_t sh = ((uint32_t)(uintptr_t)row[i] + kc * 8) * 8u;   // funnel shifts take it modulo 32
-                        lo[i] = __funnelshift_r(w[i][0], w[i][1], sh);
-                        hi[i] = __funnelshift_r(w[i][1], w[i][2], sh);
-                        const int n = nblk - kc * 8;   // bytes past the row's end belong to the next row
-                        if (n < 8) {
-                            lo[i] = n >= 4 ? lo[i] : lo[i] & ((1u << (8 * n)) - 1u);
-                            hi[i] = n > 4 ? hi[i] & ((1u << (8 * (n - 4))) - 1u) : 0u;
-                        }
-                        if (kc + 1 < kc1) fetch(row[i], (kc + 1) * 8, w[i]);
-                    }
-                    ok = mbar_wait(bar(EMPTY) + 8u * s, ph ^ 1u, abort_flag);
-                    if (!ok) break;
-                    const uint32_t dst = dst0 + s * (uint32_t)g.stage_bytes;
+                        uint32_t v[4];
 #pragma unroll
-                    for (int i = 0; i < kMaxGroups; i++)
-                        if (i < g.groups) asm volatile("st.shared.v2.b32 [%0], {%1, %2};" ::"r"(dst + i * kGroupBytes), "r"(lo[i]), "r"(hi[i]) : "memory");
-                    mbar_arrive(bar(FULL) + 8u * s);
-                    if (++s == (uint32_t)g.stages) { s = 0; ph ^= 1u; }
+                        for (int j = 0; j < 4; j++) {
+                            v[j] = __funnelshift_r(w[i][j], w[i][j + 1], sh);
+                            if (n < 4 * j + 4) v[j] = n > 4 * j ? v[j] & ((1u << (8 * (n - 4 * j))) - 1u) : 0u;
+                        }
+                        if (place[i])
+                            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(dst + (i ? kGroupBytes + (i - 1) * group_step : 0u)), "r"(v[0]), "r"(v[1]),
+                                         "r"(v[2]), "r"(v[3])
+                                         : "memory");
+                    }
+                    mbar_arrive(bar(RAW_FULL) + 8u * d);
+                    if (++d == (uint32_t)g.scale_bufs) { d = 0; ph ^= 1u; }
                 }
             }
         }
-        asm volatile("cp.async.wait_all;" ::: "memory");
     } else if (warp >= kScaleWarp0 && warp < kEpiWarp0) {
         // ----------------------------------------------------------- scale warps
         // The tensor core wants, in every lane quarter, lane l's column j of a group's half to hold the half's four bytes of row 32 j + l.
         const uint32_t q = (uint32_t)(warp & 3);
-        uint32_t s = 0, ph = 0;
+        uint32_t s = 0, ph = 0, d = 0, dph = 0;
         bool ok = true;
         for (int tile = tile0; tile < g.tiles && ok; tile += tile_step)
             for (int kc = kc0; kc < kc1; kc++) {
-                ok = mbar_wait(bar(FULL) + 8u * s, ph, abort_flag);
+                if (kc == kc0 || (kc & 1) == 0) ok = mbar_wait(bar(RAW_FULL) + 8u * d, dph, abort_flag);
+                ok = ok && mbar_wait(bar(EMPTY) + 8u * s, ph ^ 1u, abort_flag);   // the slot's last MMAs are done
                 if (!ok) break;
-                const uint8_t* src = smem + (size_t)s * g.stage_bytes + sc_off + lane * 8;
+                const uint8_t* src = smem + raw0 + d * raw_bytes + (kc & 1) * 8 + lane * 16;
                 const uint32_t dst = slot0 + s * slot_cols + ((q * 32u) << 16);
-if constexpr (TERMS == 1) {
-                    if (nb == 1) store_scales<2>(src, dst);
-                    else store_scales<3>(src, dst);
+                if constexpr (TERMS == 1) {
+                    if (nb == 1) store_scales<2>(src, group_step, dst);
+                    else store_scales<3>(src, group_step, dst);
                 } else {
-                    store_scales<1 + TERMS>(src, dst);   // two or three terms: one group each
+                    store_scales<1 + TERMS>(src, group_step, dst);   // two or three terms: one group each
                 }
                 asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
                 tc_fence_before();
                 __syncwarp();
+                if (PAIR && half != 0) {
+                    ok = mbar_wait(bar(FULL) + 8u * s, ph, abort_flag);
+                    if (!ok) break;
+                }
                 if (lane == 0) {
                     if (PAIR && half != 0) mbar_arrive_cluster(map_to_cta(bar(SC_FULL) + 8u * s, 0u));
                     else mbar_arrive(bar(SC_FULL) + 8u * s);
+                }
+                if (kc + 1 == kc1 || (kc & 1) != 0) {
+                    if (lane == 0) mbar_arrive(bar(RAW_EMPTY) + 8u * d);
+                    if (++d == (uint32_t)g.scale_bufs) { d = 0; dph ^= 1u; }
                 }
                 if (++s == (uint32_t)g.stages) { s = 0; ph ^= 1u; }
             }
@@ -550,7 +578,7 @@ if constexpr (TERMS == 1) {
 constexpr int kSmallMin = 77 * 1024, kSmallMax = 112 * 1024, kLargeMin = 160 * 1024, kLargeMax = 225 * 1024;
 
 struct Plan {
-    int tokens, stages, stage_bytes, groups, tmem_cols, smem, per_sm, splits, tiles_w, tiles_m;
+    int tokens, stages, stage_bytes, scale_bufs, groups, tmem_cols, smem, per_sm, splits, tiles_w, tiles_m;
     bool pair;
 };
 
@@ -559,23 +587,25 @@ bool plan_block(int terms, int tokens, bool pair, Plan* p) {
     p->tokens = tokens;
     p->pair = pair;
     p->groups = groups;
-    p->stage_bytes = kWBytes + terms * (pair ? tokens / 2 : tokens) * kRowBytes + groups * kGroupBytes;
+    p->stage_bytes = kWBytes + terms * (pair ? tokens / 2 : tokens) * kRowBytes;
     auto cols = [&](int stages) { return 2 * tokens + stages * 8 * groups; };
     auto pow2 = [](int c) { int r = 32; while (r < c) r *= 2; return r; };
-    int st = std::min(kMaxStages, (kSmallMax - 1024) / p->stage_bytes);
-    while (st > 3 && cols(st) > 256) st--;
-    if (!pair && st >= 3 && cols(st) <= 256) {
+    // most stages that fit behind `bufs` buffers of scales
+    auto fit = [&](int smem, int bufs, int most_cols) {
+        int st = std::min(kMaxStages, (smem - 1024 - bufs * groups * kGroupBytes) / p->stage_bytes);
+        while (st > 2 && cols(st) > most_cols) st--;
+        return cols(st) <= most_cols ? st : 0;
+    };
+    auto set = [&](int smem_min, int bufs, int st, int per_sm) {
         p->stages = st;
-        p->smem = std::max(kSmallMin, st * p->stage_bytes + 1024);
-        p->per_sm = 2;
-    } else {
-        st = std::min(kMaxStages, (kLargeMax - 1024) / p->stage_bytes);
-        while (st > 2 && cols(st) > 512) st--;
-        if (st < 2 || cols(st) > 512) return false;
-        p->stages = st;
-        p->smem = std::max(kLargeMin, st * p->stage_bytes + 1024);
-        p->per_sm = 1;
-    }
+        p->scale_bufs = bufs;
+        p->smem = std::max(smem_min, st * p->stage_bytes + bufs * groups * kGroupBytes + 1024);
+        p->per_sm = per_sm;
+    };
+    int st;
+    if (!pair && (st = fit(kSmallMax, 2, 256)) >= 3) set(kSmallMin, 2, st, 2);
+    else if ((st = fit(kLargeMax, 3, 512)) >= 2) set(kLargeMin, 3, st, 1);
+    else return false;
     p->tmem_cols = pow2(cols(p->stages));
     return p->stages * p->stage_bytes >= tokens * kWRows * 4;   // a partial tile fits into the ring
 }
@@ -617,7 +647,7 @@ bool make_plan(int64_t M, int64_t N, int K, int terms, int sms, bool pairs_run, 
 }
 
 template <int DT, int TERMS, bool PAIR>
-int launch(const Plan& p, const CUtensorMap& w, const CUtensorMap& a, const MatmulArgs& g, int sms, cudaStream_t stream) {
+int launch(const Plan& p, const CUtensorMap (&maps)[4], const MatmulArgs& g, int sms, cudaStream_t stream) {
     const int cluster = PAIR ? 2 : p.splits;
     const int64_t tiles = (int64_t)p.tiles_w * p.tiles_m;
     cudaLaunchConfig_t cfg = {};
@@ -634,16 +664,16 @@ int launch(const Plan& p, const CUtensorMap& w, const CUtensorMap& a, const Matm
     attr[1].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = cluster > 1 ? 2 : 1;
-    DSX_CUDA(cudaLaunchKernelEx(&cfg, mxfp4_matmul_kernel<DT, TERMS, PAIR>, w, a, g));
+    DSX_CUDA(cudaLaunchKernelEx(&cfg, mxfp4_matmul_kernel<DT, TERMS, PAIR>, maps[0], maps[1], maps[2], maps[3], g));
     DSX_LAUNCHED();
     return DSX_OK;
 }
 
 template <int DT>
-int launch_for(int terms, const Plan& p, const CUtensorMap& w, const CUtensorMap& a, const MatmulArgs& g, int sms, cudaStream_t stream) {
-    if (terms == 1) return p.pair ? launch<DT, 1, true>(p, w, a, g, sms, stream) : launch<DT, 1, false>(p, w, a, g, sms, stream);
-    if (terms == 2) return p.pair ? launch<DT, 2, true>(p, w, a, g, sms, stream) : launch<DT, 2, false>(p, w, a, g, sms, stream);
-    return p.pair ? launch<DT, 3, true>(p, w, a, g, sms, stream) : launch<DT, 3, false>(p, w, a, g, sms, stream);
+int launch_for(int terms, const Plan& p, const CUtensorMap (&maps)[4], const MatmulArgs& g, int sms, cudaStream_t stream) {
+    if (terms == 1) return p.pair ? launch<DT, 1, true>(p, maps, g, sms, stream) : launch<DT, 1, false>(p, maps, g, sms, stream);
+    if (terms == 2) return p.pair ? launch<DT, 2, true>(p, maps, g, sms, stream) : launch<DT, 2, false>(p, maps, g, sms, stream);
+    return p.pair ? launch<DT, 3, true>(p, maps, g, sms, stream) : launch<DT, 3, false>(p, maps, g, sms, stream);
 }
 
 template <int DT, int TERMS>
@@ -720,18 +750,28 @@ int dsx_mxfp4_matmul(const void* a_codes, const void* a_scales, int n_terms, int
     Plan p;
     if (!make_plan(m, n, (int)k, n_terms, sms, pairs_run, &p)) return set_error(DSX_ERR_UNSUPPORTED, "mxfp4_matmul: no tile for %d terms", n_terms);
     DSX_REQUIRE((int64_t)p.tiles_w * p.tiles_m < ((int64_t)1 << 30), "mxfp4_matmul: too many tiles");
-    CUtensorMap tw, ta;
-    {
-        const cuuint64_t dims[2] = {(cuuint64_t)(k / 2), (cuuint64_t)n};
-        const cuuint64_t strides[1] = {(cuuint64_t)(k / 2)};
-        const cuuint32_t box[2] = {(cuuint32_t)kRowBytes, (cuuint32_t)kWRows};
-        if (int rc = tmap_encode(&tw, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, w_codes, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B)) return rc;
-    }
-    {
-        const cuuint64_t dims[3] = {(cuuint64_t)(k / 2), (cuuint64_t)m, (cuuint64_t)n_terms};
-        const cuuint64_t strides[2] = {(cuuint64_t)(k / 2), (cuuint64_t)(m * (k / 2))};
-        const cuuint32_t box[3] = {(cuuint32_t)kRowBytes, (cuuint32_t)(p.pair ? p.tokens / 2 : p.tokens), (cuuint32_t)n_terms};
-        if (int rc = tmap_encode(&ta, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, a_codes, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B)) return rc;
+    // codes and scales of both operands as (bytes, row) and (bytes, row, term); the maps of scales only where TMA can read them
+    const bool scale_tma = k % 512 == 0 && (((uintptr_t)a_scales | (uintptr_t)w_scales) & 15) == 0;
+    CUtensorMap maps[4];
+    auto encode_w = [&](CUtensorMap* map, const void* base, int64_t row_bytes, int box_bytes, CUtensorMapSwizzle swizzle) {
+        const cuuint64_t dims[2] = {(cuuint64_t)row_bytes, (cuuint64_t)n};
+        const cuuint64_t strides[1] = {(cuuint64_t)row_bytes};
+        const cuuint32_t box[2] = {(cuuint32_t)box_bytes, (cuuint32_t)kWRows};
+        return tmap_encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, base, dims, strides, box, swizzle);
+    };
+    auto encode_a = [&](CUtensorMap* map, const void* base, int64_t row_bytes, int box_bytes, int box_rows, CUtensorMapSwizzle swizzle) {
+        const cuuint64_t dims[3] = {(cuuint64_t)row_bytes, (cuuint64_t)m, (cuuint64_t)n_terms};
+        const cuuint64_t strides[2] = {(cuuint64_t)row_bytes, (cuuint64_t)(m * row_bytes)};
+        const cuuint32_t box[3] = {(cuuint32_t)box_bytes, (cuuint32_t)box_rows, (cuuint32_t)n_terms};
+        return tmap_encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, base, dims, strides, box, swizzle);
+    };
+    if (int rc = encode_w(&maps[0], w_codes, k / 2, kRowBytes, CU_TENSOR_MAP_SWIZZLE_128B)) return rc;
+    if (int rc = encode_a(&maps[1], a_codes, k / 2, kRowBytes, p.pair ? p.tokens / 2 : p.tokens, CU_TENSOR_MAP_SWIZZLE_128B)) return rc;
+    maps[2] = maps[0];
+    maps[3] = maps[1];
+    if (scale_tma) {
+        if (int rc = encode_w(&maps[2], w_scales, k / 32, 16, CU_TENSOR_MAP_SWIZZLE_NONE)) return rc;
+        if (int rc = encode_a(&maps[3], a_scales, k / 32, 16, p.tokens, CU_TENSOR_MAP_SWIZZLE_NONE)) return rc;
     }
     MatmulArgs g{};
     g.w_scales = (const uint8_t*)w_scales;
@@ -741,12 +781,13 @@ int dsx_mxfp4_matmul(const void* a_codes, const void* a_scales, int n_terms, int
     g.M = m; g.N = n; g.K = (int)k;
     g.tokens = p.tokens; g.stages = p.stages; g.stage_bytes = p.stage_bytes; g.groups = p.groups; g.tmem_cols = p.tmem_cols; g.splits = p.splits;
     g.tiles_w = p.tiles_w; g.tiles = p.tiles_w * p.tiles_m;
-    g.aligned = k % kStageK == 0 && (((uintptr_t)a_scales | (uintptr_t)w_scales) & 7) == 0;
+    g.scale_tma = scale_tma;
+    g.scale_bufs = p.scale_bufs;
     g.pairs = dtype != DSX_F32 && n % 2 == 0 && (row_stride % 2 == 0 || m == 1) && ((uintptr_t)out & 3) == 0;
     const cudaStream_t s = (cudaStream_t)stream;
-    if (dtype == DSX_F32) return launch_for<DSX_F32>(n_terms, p, tw, ta, g, sms, s);
-    if (dtype == DSX_BF16) return launch_for<DSX_BF16>(n_terms, p, tw, ta, g, sms, s);
-    return launch_for<DSX_F16>(n_terms, p, tw, ta, g, sms, s);
+    if (dtype == DSX_F32) return launch_for<DSX_F32>(n_terms, p, maps, g, sms, s);
+    if (dtype == DSX_BF16) return launch_for<DSX_BF16>(n_terms, p, maps, g, sms, s);
+    return launch_for<DSX_F16>(n_terms, p, maps, g, sms, s);
 }
 
 int dsx_head_check(dsx_stream_t stream_, uint32_t* error_word) {
