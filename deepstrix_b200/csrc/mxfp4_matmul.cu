@@ -12,9 +12,10 @@
 // Scales are read as stored (row-major bytes; nothing is laid out beforehand), 16 bytes of every row -- 512 columns, two stages -- at a time
 // into a ring of their own: by TMA where rows of scales are 16-byte aligned (K a multiple of 512), else by four loader warps, a row of
 // every 128-row group a thread, as the aligned words that hold them, requested ahead and shifted into place.  (Asynchronous copies of 8 bytes
-// a row and stage kept the shared-memory pipe 60 % busy with 32 lines an instruction.)  Four scale warps, one per lane quarter, move them to
-// tensor memory a stage at a time (ld.shared + tcgen05.st; the tensor core's own copy would queue behind its MMAs).
-// Warp roles: TMA of codes, MMA issue, TMA of scales, 4 scale warps, 4 epilogue warps, 4 loaders; two accumulators, so that a
+// a row and stage kept the shared-memory pipe 60 % busy with 32 lines an instruction.)  Scale warps, one per lane quarter, move a
+// buffer to a slot of tensor memory at a time (ld.shared + tcgen05.st; the tensor core's own copy would queue behind its MMAs); where TMA
+// brings the scales the loader warps are a second set of them, and the sets take alternate buffers: one set alone needed 800 clocks a stage.
+// Warp roles: TMA of codes, MMA issue, TMA of scales, 4 scale warps, 4 epilogue warps, 4 loaders or scale warps; two accumulators, so that a
 // tile is read out under the next one's MMAs.
 // Few tiles: the columns are split over the CTAs of a cluster; each leaves its partial tile in shared memory and the cluster adds
 // them in rank order through distributed shared memory, so results do not depend on timing and need no workspace.
@@ -32,7 +33,7 @@ namespace {
 
 __device__ uint32_t g_head_error = 0;
 
-constexpr int kScaleWarp0 = 4, kEpiWarp0 = 8, kLoadWarp0 = 12, kThreads = 512;   // roles start on warp-group boundaries; warp 3 is idle
+constexpr int kEpiWarp0 = 8, kLoadWarp0 = 12, kThreads = 512;   // roles start on warp-group boundaries
 constexpr int kLoaders = 128;
 constexpr int kWRows = 128;          // W rows of a tile
 constexpr int kStageK = 256;         // columns of a stage
@@ -40,6 +41,7 @@ constexpr int kRowBytes = kStageK / 2;
 constexpr int kWBytes = kWRows * kRowBytes;
 constexpr int kGroupBytes = 2048;    // scale bytes of a group of 128 rows: 16 a row, two stages
 constexpr int kMaxScaleBufs = 3;
+constexpr int kMaxSlots = 4;         // of scales in tensor memory, two stages each
 constexpr int kMaxGroups = 4;        // W and up to three term groups
 constexpr int kMaxStages = 8;
 constexpr int kMaxTokens = 208;      // A rows of a tile: two accumulators and four scale slots fill tensor memory
@@ -58,6 +60,18 @@ __device__ __forceinline__ bool mbar_try(uint32_t bar, uint32_t parity) {
     asm volatile(
         "{\n\t.reg .pred p;\n\t"
         "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(bar), "r"(parity)
+        : "memory");
+    return ok != 0;
+}
+// Has the phase completed?  (try_wait above may hold the thread for microseconds where it has not.)
+__device__ __forceinline__ bool mbar_test(uint32_t bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
         "selp.u32 %0, 1, 0, p;\n\t}"
         : "=r"(ok)
         : "r"(bar), "r"(parity)
@@ -85,13 +99,14 @@ __device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map
 }
 __device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
-// Arrives on a barrier (of either CTA of a pair) when the MMAs issued so far have completed.
+// Arrives on a barrier -- a pair: on the same one of both CTAs -- when the MMAs issued so far have completed.
 template <bool PAIR>
 __device__ __forceinline__ void tc_commit(uint32_t leader, uint32_t bar) {
     if constexpr (PAIR)
         asm volatile(
             "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %1, 0;\n\t"
-            "@q tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(bar), "r"(leader)
+            "@q tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %2;\n\t}" ::"r"(bar), "r"(leader),
+            "h"((uint16_t)3)
             : "memory");
     else
         asm volatile(
@@ -141,11 +156,6 @@ __device__ __forceinline__ void tc_ld16(uint32_t taddr, uint32_t (&r)[16]) {
 }
 __device__ __forceinline__ void tc_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 // lane l of the warp writes N columns of its tensor-memory lane
-__device__ __forceinline__ void tc_st(uint32_t taddr, const uint32_t (&r)[8]) {
-    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]),
-                 "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
-                 : "memory");
-}
 __device__ __forceinline__ void tc_st(uint32_t taddr, const uint32_t (&r)[16]) {
     asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr), "r"(r[0]),
                  "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]),
@@ -161,30 +171,22 @@ __device__ __forceinline__ void tc_st(uint32_t taddr, const uint32_t (&r)[32]) {
         "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
         : "memory");
 }
-// Scales of a landed stage, this lane's rows (row 32 j + lane of group i at src + group i + j * 512), to the stage's slot: both
-// 128-column halves, 4 columns a group each -- one or two wide stores (a 4-column store a group and half took 100 clocks apiece).
+// Scales of two landed stages, GROUPS groups of this lane's rows (row 32 j + lane of group i at src + i * kGroupBytes + j * 512, 16 bytes), to
+// 16 * GROUPS columns of a slot: quarter k of the 512 columns (a scale-factor chunk) takes 4 columns a group, the groups side by side.
 template <int GROUPS>
-__device__ __forceinline__ void store_scales(const uint8_t* src, uint32_t group_step, uint32_t dst) {
-    uint32_t v[8 * GROUPS];
+__device__ __forceinline__ void store_scales(const uint8_t* src, uint32_t dst) {
+    uint32_t v[16 * GROUPS];
 #pragma unroll
     for (int i = 0; i < GROUPS; i++)
 #pragma unroll
         for (int j = 0; j < 4; j++) {
-            const uint2 two = *reinterpret_cast<const uint2*>(src + (i ? kGroupBytes + (i - 1) * group_step : 0u) + j * 512);
-            v[4 * i + j] = two.x;
-            v[4 * GROUPS + 4 * i + j] = two.y;
+            const uint4 row = *reinterpret_cast<const uint4*>(src + i * kGroupBytes + j * 512);
+            v[4 * i + j] = row.x;
+            v[4 * GROUPS + 4 * i + j] = row.y;
+            v[8 * GROUPS + 4 * i + j] = row.z;
+            v[12 * GROUPS + 4 * i + j] = row.w;
         }
-    if constexpr (GROUPS == 3) {
-        uint32_t lo[16], hi[8];
-#pragma unroll
-        for (int i = 0; i < 16; i++) lo[i] = v[i];
-#pragma unroll
-        for (int i = 0; i < 8; i++) hi[i] = v[16 + i];
-        tc_st(dst, lo);
-        tc_st(dst + 16u, hi);
-    } else {
-        tc_st(dst, v);
-    }
+    tc_st(dst, v);
 }
 __device__ __forceinline__ uint32_t cluster_ctarank() {
     uint32_t r;
@@ -253,7 +255,8 @@ struct MatmulArgs {
     int64_t M, N;
     int K;
     int tokens;              // A rows of a tile (multiple of 16)
-    int stages, stage_bytes; // ring of codes, and of scale slots in tensor memory
+    int stages, stage_bytes; // ring of codes
+    int slots;               // ring of scale slots in tensor memory, two stages each
     int scale_bufs;          // ring of scales, kGroupBytes a group
     int groups;              // 128-row groups of scales: 1 (W) + terms * ceil(tokens / 128)
     int tmem_cols;
@@ -273,21 +276,20 @@ mxfp4_matmul_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_con
     using T = typename Elem<DT>::T;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
-    __shared__ __align__(8) uint64_t s_bars[3 * kMaxStages + 4 + 2 * kMaxScaleBufs];
+    __shared__ __align__(8) uint64_t s_bars[2 * kMaxStages + 4 + 2 * kMaxScaleBufs + 2 * kMaxSlots];
     __shared__ uint32_t s_misc[2];
     const uint32_t sbase = smem_u32(smem), bar0 = smem_u32(s_bars);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    // FULL[s]: the codes of the stage have landed; SC_FULL[s]: its scales are in tensor memory (a pair: those of both CTAs, and the odd CTA's
-    // codes have landed); EMPTY[s]: the MMAs that read it have completed; ACC_FULL / ACC_EMPTY[b]: accumulator b is complete / read out;
-    // RAW_FULL / RAW_EMPTY[d]: two stages' scales have landed / are in tensor memory.
-    constexpr int FULL = 0, SC_FULL = kMaxStages, EMPTY = 2 * kMaxStages, ACC_FULL = 3 * kMaxStages, ACC_EMPTY = ACC_FULL + 2, RAW_FULL = ACC_EMPTY + 2,
-                  RAW_EMPTY = RAW_FULL + kMaxScaleBufs;
+    // FULL[s]: the codes of the stage have landed (even CTA of a pair: in both); EMPTY[s]: the MMAs that read it have completed;
+    // ACC_FULL / ACC_EMPTY[b]: accumulator b is complete / read out; RAW_FULL / RAW_EMPTY[d]: two stages' scales have landed / are in tensor
+    // memory; SLOT_FULL / SLOT_EMPTY[v]: and lie in slot v (a pair: of both CTAs) / the MMAs that used them have completed.
+    constexpr int FULL = 0, EMPTY = FULL + kMaxStages, ACC_FULL = EMPTY + kMaxStages, ACC_EMPTY = ACC_FULL + 2, RAW_FULL = ACC_EMPTY + 2,
+                  RAW_EMPTY = RAW_FULL + kMaxScaleBufs, SLOT_FULL = RAW_EMPTY + kMaxScaleBufs, SLOT_EMPTY = SLOT_FULL + kMaxSlots;
     auto bar = [&](int i) { return bar0 + 8u * (uint32_t)i; };
     volatile uint32_t* abort_flag = s_misc + 1;
     if (threadIdx.x == 0) {
         for (int i = 0; i < kMaxStages; i++) {
-            mbar_init(bar(FULL + i), 1);
-            mbar_init(bar(SC_FULL + i), PAIR ? 8 : 4);
+            mbar_init(bar(FULL + i), PAIR && cluster_ctarank() == 0 ? 2 : 1);   // + the odd CTA's report
             mbar_init(bar(EMPTY + i), 1);
         }
         for (int b = 0; b < 2; b++) {
@@ -297,6 +299,10 @@ mxfp4_matmul_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_con
         for (int d = 0; d < kMaxScaleBufs; d++) {
             mbar_init(bar(RAW_FULL + d), g.scale_tma ? 1 : kLoaders);
             mbar_init(bar(RAW_EMPTY + d), 4);
+        }
+        for (int v = 0; v < kMaxSlots; v++) {
+            mbar_init(bar(SLOT_FULL + v), PAIR ? 8 : 4);
+            mbar_init(bar(SLOT_EMPTY + v), 1);
         }
         *abort_flag = 0u;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -331,8 +337,8 @@ mxfp4_matmul_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_con
     // scales behind the ring of codes: [buffer][W, term 0, ...][row][16]; a term's group has room for 128 rows behind the previous one's rows
     const uint32_t raw0 = (uint32_t)(g.stages * g.stage_bytes), raw_bytes = (uint32_t)(g.groups * kGroupBytes);
     const uint32_t group_step = BN > 128 ? (uint32_t)kGroupBytes : (uint32_t)BN * 16u;
-    // scale slot of a stage: the two 128-column halves, each 4 columns a group (a term's groups side by side)
-    const uint32_t slot0 = tmem + 2u * (uint32_t)BN, half_cols = 4u * (uint32_t)g.groups, slot_cols = 2u * half_cols;
+    // scale slots behind the accumulators: W's 16 columns, then the terms' (nb == 2, one term: its two groups interleaved by quarter)
+    const uint32_t slot0 = tmem + 2u * (uint32_t)BN, slot_cols = 16u * (uint32_t)g.groups;
     const int nb = (BN + 127) >> 7;
 
     if (warp == 0) {
@@ -361,43 +367,49 @@ mxfp4_matmul_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_con
         // The whole warp walks the loop and one lane issues, under a predicate: the instruction takes its operands from uniform registers, and
         // inside a branch of one lane each of them had to be carried there first -- 230 clocks an MMA, whatever its size.  Votes keep the
         // loop's exits uniform.
-        const uint32_t leader = lane == 0 ? 1u : 0u, peer = PAIR ? map_to_cta(bar0, 1u) - bar0 : 0u;   // from a barrier here to the odd CTA's
-        uint32_t s = 0, ph = 0, t = 0;
+        const uint32_t leader = lane == 0 ? 1u : 0u;
+        uint32_t s = 0, ph = 0, t = 0, v = 0, vph = 0;
         bool ok = true;
         const uint64_t d0 = operand_desc(sbase);
         const uint32_t hi = (uint32_t)(d0 >> 32), lo0 = __shfl_sync(0xFFFFFFFFu, (uint32_t)d0, 0);
         const uint32_t tm = __shfl_sync(0xFFFFFFFFu, tmem, 0), slots = tm + 2u * (uint32_t)BN;
         const uint32_t term_step = (uint32_t)(held * kRowBytes) >> 4, stage_step = (uint32_t)g.stage_bytes >> 4;
+        const uint32_t quarter = nb == 2 ? 8u : 4u;   // columns of a quarter of A's scales
         const uint32_t idesc0 = mxf4_idesc(kTileW, BN, 0u), idesc2 = mxf4_idesc(kTileW, BN, 2u);
         for (int tile = tile0; tile < g.tiles && ok && half == 0; tile += tile_step, t++) {
             const uint32_t b = t & 1u, acc = tm + b * (uint32_t)BN;
             ok = __all_sync(0xFFFFFFFFu, mbar_wait(bar(ACC_EMPTY) + 8u * b, ((t >> 1) & 1u) ^ 1u, abort_flag));
             if (!ok) break;
             tc_fence_after();
+            bool ready = false;
             for (int kc = kc0; kc < kc1; kc++) {
-                ok = __all_sync(0xFFFFFFFFu, mbar_wait(bar(SC_FULL) + 8u * s, ph, abort_flag) && mbar_wait(bar(FULL) + 8u * s, ph, abort_flag));
+                const bool last = (kc & 1) != 0 || kc + 1 == kc1;   // of its slot
+                if (kc == kc0 || (kc & 1) == 0) ok = __all_sync(0xFFFFFFFFu, mbar_wait(bar(SLOT_FULL) + 8u * v, vph, abort_flag));
+                if (ok && !__all_sync(0xFFFFFFFFu, ready)) ok = __all_sync(0xFFFFFFFFu, mbar_wait(bar(FULL) + 8u * s, ph, abort_flag));
                 if (!ok) break;
                 tc_fence_after();
-                const uint32_t a_lo = lo0 + s * stage_step, b_lo = a_lo + (kWBytes >> 4), sc = slots + s * slot_cols;
+                const uint32_t a_lo = lo0 + s * stage_step, b_lo = a_lo + (kWBytes >> 4), sc = slots + v * slot_cols, empty = bar(EMPTY) + 8u * s;
+                const uint32_t k0 = 2u * (uint32_t)(kc & 1);        // first quarter of the stage
                 const int steps = (g.K - kc * kStageK + 63) >> 6;
+                if (++s == (uint32_t)g.stages) { s = 0; ph ^= 1u; }
+                ready = kc + 1 < kc1 && mbar_test(bar(FULL) + 8u * s, ph);   // asked for ahead of this stage's MMAs
 #pragma unroll
                 for (int ks = 0; ks < 4; ks++) {
                     if (ks < steps) {
-                        const uint32_t sfw = sc + (uint32_t)(ks >> 1) * half_cols;
+                        const uint32_t k = k0 + (uint32_t)(ks >> 1);
 #pragma unroll
                         for (int q = 0; q < TERMS; q++)
-                            tc_mma_mxf4<PAIR>(leader, acc, a_lo + 2u * ks, b_lo + (uint32_t)q * term_step + 2u * ks, hi, (ks & 1) ? idesc2 : idesc0, sfw,
-                                        sfw + 4u + (uint32_t)(q * nb) * 4u, (kc > kc0 || ks > 0 || q > 0) ? 1u : 0u);
+                            tc_mma_mxf4<PAIR>(leader, acc, a_lo + 2u * ks, b_lo + (uint32_t)q * term_step + 2u * ks, hi, (ks & 1) ? idesc2 : idesc0, sc + 4u * k,
+                                              sc + 16u + 16u * (uint32_t)q + quarter * k, (kc > kc0 || ks > 0 || q > 0) ? 1u : 0u);
                     }
                 }
-                tc_commit<PAIR>(leader, bar(EMPTY) + 8u * s);
-                if constexpr (PAIR) tc_commit<PAIR>(leader, peer + bar(EMPTY) + 8u * s);
-                if (++s == (uint32_t)g.stages) { s = 0; ph ^= 1u; }
+                tc_commit<PAIR>(leader, empty);
+                if (last) {
+                    tc_commit<PAIR>(leader, bar(SLOT_EMPTY) + 8u * v);
+                    if (++v == (uint32_t)g.slots) { v = 0; vph ^= 1u; }
+                }
             }
-            if (ok) {
-                tc_commit<PAIR>(leader, bar(ACC_FULL) + 8u * b);
-                if constexpr (PAIR) tc_commit<PAIR>(leader, peer + bar(ACC_FULL) + 8u * b);
-            }
+            if (ok) tc_commit<PAIR>(leader, bar(ACC_FULL) + 8u * b);
         }
     } else if (warp == 2) {
         // --------------------------------------------------------- TMA of scales
@@ -420,9 +432,22 @@ mxfp4_matmul_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_con
                 for (uint32_t i = 0; i < (uint32_t)g.scale_bufs; i++)
                     for (uint32_t n = 0; n < kSpinLimit / 64 && !mbar_try(bar(RAW_FULL) + 8u * i, i < d ? ph : ph ^ 1u); n++) {}
         }
-    } else if (warp >= kLoadWarp0) {
+    } else if (warp == 3) {
+        // ------------------------------ odd CTA of a pair: its landed stages reported to the even one
+        if (PAIR && half != 0 && lane == 0) {
+            uint32_t s = 0, ph = 0;
+            bool ok = true;
+            for (int tile = tile0; tile < g.tiles && ok; tile += tile_step)
+                for (int kc = kc0; kc < kc1; kc++) {
+                    ok = mbar_wait(bar(FULL) + 8u * s, ph, abort_flag);
+                    if (!ok) break;
+                    mbar_arrive_cluster(map_to_cta(bar(FULL) + 8u * s, 0u));
+                    if (++s == (uint32_t)g.stages) { s = 0; ph ^= 1u; }
+                }
+        }
+    } else if (warp >= kLoadWarp0 && !g.scale_tma) {
         // --------------------------------------------------------- scale loaders
-        if (!g.scale_tma) {
+        {
             const int r = threadIdx.x - kLoadWarp0 * 32;   // row of every group
             const int nblk = g.K >> 5;
             uint32_t d = 0, ph = 0;
@@ -476,43 +501,7 @@ mxfp4_matmul_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_con
                 }
             }
         }
-    } else if (warp >= kScaleWarp0 && warp < kEpiWarp0) {
-        // ----------------------------------------------------------- scale warps
-        // The tensor core wants, in every lane quarter, lane l's column j of a group's half to hold the half's four bytes of row 32 j + l.
-        const uint32_t q = (uint32_t)(warp & 3);
-        uint32_t s = 0, ph = 0, d = 0, dph = 0;
-        bool ok = true;
-        for (int tile = tile0; tile < g.tiles && ok; tile += tile_step)
-            for (int kc = kc0; kc < kc1; kc++) {
-                if (kc == kc0 || (kc & 1) == 0) ok = mbar_wait(bar(RAW_FULL) + 8u * d, dph, abort_flag);
-                ok = ok && mbar_wait(bar(EMPTY) + 8u * s, ph ^ 1u, abort_flag);   // the slot's last MMAs are done
-                if (!ok) break;
-                const uint8_t* src = smem + raw0 + d * raw_bytes + (kc & 1) * 8 + lane * 16;
-                const uint32_t dst = slot0 + s * slot_cols + ((q * 32u) << 16);
-                if constexpr (TERMS == 1) {
-                    if (nb == 1) store_scales<2>(src, group_step, dst);
-                    else store_scales<3>(src, group_step, dst);
-                } else {
-                    store_scales<1 + TERMS>(src, group_step, dst);   // two or three terms: one group each
-                }
-                asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
-                tc_fence_before();
-                __syncwarp();
-                if (PAIR && half != 0) {
-                    ok = mbar_wait(bar(FULL) + 8u * s, ph, abort_flag);
-                    if (!ok) break;
-                }
-                if (lane == 0) {
-                    if (PAIR && half != 0) mbar_arrive_cluster(map_to_cta(bar(SC_FULL) + 8u * s, 0u));
-                    else mbar_arrive(bar(SC_FULL) + 8u * s);
-                }
-                if (kc + 1 == kc1 || (kc & 1) != 0) {
-                    if (lane == 0) mbar_arrive(bar(RAW_EMPTY) + 8u * d);
-                    if (++d == (uint32_t)g.scale_bufs) { d = 0; dph ^= 1u; }
-                }
-                if (++s == (uint32_t)g.stages) { s = 0; ph ^= 1u; }
-            }
-    } else if (warp >= kEpiWarp0) {
+    } else if (warp >= kEpiWarp0 && warp < kLoadWarp0) {
         // -------------------------------------------------------------- epilogue
         const uint32_t q = (uint32_t)(warp & 3);
         uint32_t t = 0;
@@ -545,6 +534,38 @@ mxfp4_matmul_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_con
                 else mbar_arrive(bar(ACC_EMPTY) + 8u * b);
             }
         }
+    } else {
+        // ----------------------------------------------------------- scale warps
+        // The tensor core wants, in every lane quarter, lane l's column j of a scale-factor chunk to hold the chunk's four bytes of row 32 j + l.
+        const uint32_t q = (uint32_t)(warp & 3);
+        const uint32_t set = warp >= kLoadWarp0 ? 1u : 0u, sets = g.scale_tma ? 2u : 1u;
+        uint32_t u = 0, d = 0, dph = 0, v = 0, vph = 0;   // buffers so far; ring positions
+        bool ok = true;
+        for (int tile = tile0; tile < g.tiles && ok; tile += tile_step)
+            for (int kc = kc0; kc < kc1; kc = (kc | 1) + 1, u++) {
+                if (sets == 1u || (u & 1u) == set) {
+                    ok = mbar_wait(bar(RAW_FULL) + 8u * d, dph, abort_flag) && mbar_wait(bar(SLOT_EMPTY) + 8u * v, vph ^ 1u, abort_flag);
+                    if (!ok) break;
+                    const uint8_t* src = smem + raw0 + d * raw_bytes + lane * 16;
+                    const uint32_t dst = slot0 + v * slot_cols + ((q * 32u) << 16);
+                    store_scales<1>(src, dst);
+                    if (TERMS == 1 && nb == 2) store_scales<2>(src + kGroupBytes, dst + 16u);
+                    else {
+#pragma unroll 1
+                        for (int i = 0; i < TERMS; i++) store_scales<1>(src + kGroupBytes + i * group_step, dst + 16u + 16u * (uint32_t)i);
+                    }
+                    asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) {
+                        mbar_arrive(bar(RAW_EMPTY) + 8u * d);
+                        if (PAIR && half != 0) mbar_arrive_cluster(map_to_cta(bar(SLOT_FULL) + 8u * v, 0u));
+                        else mbar_arrive(bar(SLOT_FULL) + 8u * v);
+                    }
+                }
+                if (++d == (uint32_t)g.scale_bufs) { d = 0; dph ^= 1u; }
+                if (++v == (uint32_t)g.slots) { v = 0; vph ^= 1u; }
+            }
     }
 
     tc_fence_before();
@@ -578,7 +599,7 @@ mxfp4_matmul_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_con
 constexpr int kSmallMin = 77 * 1024, kSmallMax = 112 * 1024, kLargeMin = 160 * 1024, kLargeMax = 225 * 1024;
 
 struct Plan {
-    int tokens, stages, stage_bytes, scale_bufs, groups, tmem_cols, smem, per_sm, splits, tiles_w, tiles_m;
+    int tokens, stages, slots, stage_bytes, scale_bufs, groups, tmem_cols, smem, per_sm, splits, tiles_w, tiles_m;
     bool pair;
 };
 
@@ -588,25 +609,19 @@ bool plan_block(int terms, int tokens, bool pair, Plan* p) {
     p->pair = pair;
     p->groups = groups;
     p->stage_bytes = kWBytes + terms * (pair ? tokens / 2 : tokens) * kRowBytes;
-    auto cols = [&](int stages) { return 2 * tokens + stages * 8 * groups; };
     auto pow2 = [](int c) { int r = 32; while (r < c) r *= 2; return r; };
-    // most stages that fit behind `bufs` buffers of scales
-    auto fit = [&](int smem, int bufs, int most_cols) {
-        int st = std::min(kMaxStages, (smem - 1024 - bufs * groups * kGroupBytes) / p->stage_bytes);
-        while (st > 2 && cols(st) > most_cols) st--;
-        return cols(st) <= most_cols ? st : 0;
-    };
-    auto set = [&](int smem_min, int bufs, int st, int per_sm) {
-        p->stages = st;
+    // stages and scale slots that fit behind `bufs` buffers of scales into `smem` bytes and `cols` columns
+    auto fit = [&](int smem, int bufs, int cols, int per_sm) {
+        p->stages = std::min(kMaxStages, (smem - 1024 - bufs * groups * kGroupBytes) / p->stage_bytes);
+        p->slots = std::min(kMaxSlots, (cols - 2 * tokens) / (16 * groups));
         p->scale_bufs = bufs;
-        p->smem = std::max(smem_min, st * p->stage_bytes + bufs * groups * kGroupBytes + 1024);
         p->per_sm = per_sm;
+        return p->stages >= (per_sm == 2 ? 3 : 2) && p->slots >= 2;
     };
-    int st;
-    if (!pair && (st = fit(kSmallMax, 2, 256)) >= 3) set(kSmallMin, 2, st, 2);
-    else if ((st = fit(kLargeMax, 3, 512)) >= 2) set(kLargeMin, 3, st, 1);
-    else return false;
-    p->tmem_cols = pow2(cols(p->stages));
+    // three buffers of scales (six stages) only where a ring of that length is to be fed
+    if (!(!pair && fit(kSmallMax, 2, 256, 2)) && !(fit(kLargeMax, 3, 512, 1) && p->stages > 4) && !fit(kLargeMax, 2, 512, 1)) return false;
+    p->smem = std::max(p->per_sm == 2 ? kSmallMin : kLargeMin, p->stages * p->stage_bytes + p->scale_bufs * groups * kGroupBytes + 1024);
+    p->tmem_cols = pow2(2 * tokens + p->slots * 16 * groups);
     return p->stages * p->stage_bytes >= tokens * kWRows * 4;   // a partial tile fits into the ring
 }
 
@@ -779,7 +794,7 @@ int dsx_mxfp4_matmul(const void* a_codes, const void* a_scales, int n_terms, int
     g.out = out;
     g.row_stride = row_stride;
     g.M = m; g.N = n; g.K = (int)k;
-    g.tokens = p.tokens; g.stages = p.stages; g.stage_bytes = p.stage_bytes; g.groups = p.groups; g.tmem_cols = p.tmem_cols; g.splits = p.splits;
+    g.tokens = p.tokens; g.stages = p.stages; g.slots = p.slots; g.stage_bytes = p.stage_bytes; g.groups = p.groups; g.tmem_cols = p.tmem_cols; g.splits = p.splits;
     g.tiles_w = p.tiles_w; g.tiles = p.tiles_w * p.tiles_m;
     g.scale_tma = scale_tma;
     g.scale_bufs = p.scale_bufs;
