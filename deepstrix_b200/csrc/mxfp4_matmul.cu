@@ -66,18 +66,6 @@ __device__ __forceinline__ bool mbar_try(uint32_t bar, uint32_t parity) {
         : "memory");
     return ok != 0;
 }
-// Has the phase completed?  (try_wait above may hold the thread for microseconds where it has not.)
-__device__ __forceinline__ bool mbar_test(uint32_t bar, uint32_t parity) {
-    uint32_t ok;
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
-        "selp.u32 %0, 1, 0, p;\n\t}"
-        : "=r"(ok)
-        : "r"(bar), "r"(parity)
-        : "memory");
-    return ok != 0;
-}
 // Bounded wait that also gives up when another role of the block has.
 __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatile uint32_t* abort_flag) {
     for (uint32_t i = 0; i < kSpinLimit; i++) {
@@ -86,6 +74,15 @@ __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatil
     }
     *abort_flag = 1u;
     return false;
+}
+// The same for a warp that must stay together: it goes on when the wait runs out (what it computes then is reported as missing), so
+// no branch depends on the outcome.
+__device__ __forceinline__ void mbar_wait_on(uint32_t bar, uint32_t parity, volatile uint32_t* abort_flag) {
+    for (uint32_t i = 0; i < kSpinLimit; i++) {
+        if (mbar_try(bar, parity)) return;
+        if ((i & 255u) == 255u && *abort_flag) return;
+    }
+    *abort_flag = 1u;
 }
 __device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap* map, int c0, int c1, uint32_t bar) {
     asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(dst), "l"(map),
@@ -365,51 +362,55 @@ mxfp4_matmul_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_con
     } else if (warp == 1) {
         // ------------------------------------------------------------- MMA issue
         // The whole warp walks the loop and one lane issues, under a predicate: the instruction takes its operands from uniform registers, and
-        // inside a branch of one lane each of them had to be carried there first -- 230 clocks an MMA, whatever its size.  Votes keep the
-        // loop's exits uniform.
+        // inside a branch of one lane each of them had to be carried there first -- 230 clocks an MMA, whatever its size.  Everything between the
+        // MMAs counts: this warp's instructions, not the tensor core, bound the loop.
         const uint32_t leader = lane == 0 ? 1u : 0u;
         uint32_t s = 0, ph = 0, t = 0, v = 0, vph = 0;
-        bool ok = true;
         const uint64_t d0 = operand_desc(sbase);
         const uint32_t hi = (uint32_t)(d0 >> 32), lo0 = __shfl_sync(0xFFFFFFFFu, (uint32_t)d0, 0);
         const uint32_t tm = __shfl_sync(0xFFFFFFFFu, tmem, 0), slots = tm + 2u * (uint32_t)BN;
         const uint32_t term_step = (uint32_t)(held * kRowBytes) >> 4, stage_step = (uint32_t)g.stage_bytes >> 4;
         const uint32_t quarter = nb == 2 ? 8u : 4u;   // columns of a quarter of A's scales
         const uint32_t idesc0 = mxf4_idesc(kTileW, BN, 0u), idesc2 = mxf4_idesc(kTileW, BN, 2u);
-        for (int tile = tile0; tile < g.tiles && ok && half == 0; tile += tile_step, t++) {
+        for (int tile = tile0; tile < g.tiles && half == 0; tile += tile_step, t++) {
             const uint32_t b = t & 1u, acc = tm + b * (uint32_t)BN;
-            ok = __all_sync(0xFFFFFFFFu, mbar_wait(bar(ACC_EMPTY) + 8u * b, ((t >> 1) & 1u) ^ 1u, abort_flag));
-            if (!ok) break;
+            uint32_t started = 0u;
+            mbar_wait_on(bar(ACC_EMPTY) + 8u * b, ((t >> 1) & 1u) ^ 1u, abort_flag);
             tc_fence_after();
-            bool ready = false;
-            for (int kc = kc0; kc < kc1; kc++) {
-                const bool last = (kc & 1) != 0 || kc + 1 == kc1;   // of its slot
-                if (kc == kc0 || (kc & 1) == 0) ok = __all_sync(0xFFFFFFFFu, mbar_wait(bar(SLOT_FULL) + 8u * v, vph, abort_flag));
-                if (ok && !__all_sync(0xFFFFFFFFu, ready)) ok = __all_sync(0xFFFFFFFFu, mbar_wait(bar(FULL) + 8u * s, ph, abort_flag));
-                if (!ok) break;
+            // one stage, the slot's first or second half
+            auto stage = [&](int kc, int h) {
+                mbar_wait_on(bar(FULL) + 8u * s, ph, abort_flag);
                 tc_fence_after();
-                const uint32_t a_lo = lo0 + s * stage_step, b_lo = a_lo + (kWBytes >> 4), sc = slots + v * slot_cols, empty = bar(EMPTY) + 8u * s;
-                const uint32_t k0 = 2u * (uint32_t)(kc & 1);        // first quarter of the stage
-                const int steps = (g.K - kc * kStageK + 63) >> 6;
-                if (++s == (uint32_t)g.stages) { s = 0; ph ^= 1u; }
-                ready = kc + 1 < kc1 && mbar_test(bar(FULL) + 8u * s, ph);   // asked for ahead of this stage's MMAs
+                const uint32_t a_lo = lo0 + s * stage_step, b_lo = a_lo + (kWBytes >> 4), sc = slots + v * slot_cols;
+                auto step = [&](int ks) {
+                    const uint32_t k = 2u * (uint32_t)h + (uint32_t)(ks >> 1);
 #pragma unroll
-                for (int ks = 0; ks < 4; ks++) {
-                    if (ks < steps) {
-                        const uint32_t k = k0 + (uint32_t)(ks >> 1);
-#pragma unroll
-                        for (int q = 0; q < TERMS; q++)
-                            tc_mma_mxf4<PAIR>(leader, acc, a_lo + 2u * ks, b_lo + (uint32_t)q * term_step + 2u * ks, hi, (ks & 1) ? idesc2 : idesc0, sc + 4u * k,
-                                              sc + 16u + 16u * (uint32_t)q + quarter * k, (kc > kc0 || ks > 0 || q > 0) ? 1u : 0u);
+                    for (int q = 0; q < TERMS; q++) {
+                        tc_mma_mxf4<PAIR>(leader, acc, a_lo + 2u * ks, b_lo + (uint32_t)q * term_step + 2u * ks, hi, (ks & 1) ? idesc2 : idesc0, sc + 4u * k,
+                                          sc + 16u + 16u * (uint32_t)q + quarter * k, ks == 0 && q == 0 ? started : 1u);
                     }
+                };
+                if ((kc + 1) * kStageK <= g.K) {
+#pragma unroll
+                    for (int ks = 0; ks < 4; ks++) step(ks);
+                } else {   // the columns' end
+                    const int steps = (g.K - kc * kStageK + 63) >> 6;
+#pragma unroll
+                    for (int ks = 0; ks < 4; ks++)
+                        if (ks < steps) step(ks);
                 }
-                tc_commit<PAIR>(leader, empty);
-                if (last) {
-                    tc_commit<PAIR>(leader, bar(SLOT_EMPTY) + 8u * v);
-                    if (++v == (uint32_t)g.slots) { v = 0; vph ^= 1u; }
-                }
+                started = 1u;
+                tc_commit<PAIR>(leader, bar(EMPTY) + 8u * s);
+                if (++s == (uint32_t)g.stages) { s = 0; ph ^= 1u; }
+            };
+            for (int kc = kc0; kc < kc1;) {
+                mbar_wait_on(bar(SLOT_FULL) + 8u * v, vph, abort_flag);
+                if ((kc & 1) == 0) stage(kc++, 0);
+                if ((kc & 1) != 0 && kc < kc1) stage(kc++, 1);
+                tc_commit<PAIR>(leader, bar(SLOT_EMPTY) + 8u * v);
+                if (++v == (uint32_t)g.slots) { v = 0; vph ^= 1u; }
             }
-            if (ok) tc_commit<PAIR>(leader, bar(ACC_FULL) + 8u * b);
+            tc_commit<PAIR>(leader, bar(ACC_FULL) + 8u * b);
         }
     } else if (warp == 2) {
         // --------------------------------------------------------- TMA of scales
