@@ -78,11 +78,13 @@ __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatil
 // The same for a warp that must stay together: it goes on when the wait runs out (what it computes then is reported as missing), so
 // no branch depends on the outcome.
 __device__ __forceinline__ void mbar_wait_on(uint32_t bar, uint32_t parity, volatile uint32_t* abort_flag) {
-    for (uint32_t i = 0; i < kSpinLimit; i++) {
-        if (mbar_try(bar, parity)) return;
-        if ((i & 255u) == 255u && *abort_flag) return;
+    uint32_t i = 0;
+    for (; i < kSpinLimit; i++) {
+        if (mbar_try(bar, parity)) break;
+        if ((i & 255u) == 255u && *abort_flag) break;
     }
-    *abort_flag = 1u;
+    if (i == kSpinLimit) *abort_flag = 1u;
+    __syncwarp();   // tells the compiler too that the warp is together: what follows may stay in uniform registers
 }
 __device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap* map, int c0, int c1, uint32_t bar) {
     asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(dst), "l"(map),
@@ -367,8 +369,9 @@ mxfp4_matmul_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_con
         const uint32_t leader = lane == 0 ? 1u : 0u;
         uint32_t s = 0, ph = 0, t = 0, v = 0, vph = 0;
         const uint64_t d0 = operand_desc(sbase);
-        const uint32_t hi = (uint32_t)(d0 >> 32), lo0 = __shfl_sync(0xFFFFFFFFu, (uint32_t)d0, 0);
-        const uint32_t tm = __shfl_sync(0xFFFFFFFFu, tmem, 0), slots = tm + 2u * (uint32_t)BN;
+        const uint32_t hi = (uint32_t)(d0 >> 32), lo0 = (uint32_t)d0;
+        const uint32_t tm = __ballot_sync(0xFFFFFFFFu, (tmem >> lane) & 1u);   // tmem itself, as a value known to be uniform
+        const uint32_t slots = tm + 2u * (uint32_t)BN;
         const uint32_t term_step = (uint32_t)(held * kRowBytes) >> 4, stage_step = (uint32_t)g.stage_bytes >> 4;
         const uint32_t quarter = nb == 2 ? 8u : 4u;   // columns of a quarter of A's scales
         const uint32_t idesc0 = mxf4_idesc(kTileW, BN, 0u), idesc2 = mxf4_idesc(kTileW, BN, 2u);
