@@ -5,10 +5,11 @@
 // (crates/v4flash-kernels/kernels/q8_0_matvec.hip:64-150, f16_gemm_wmma.hip) and the FP4 product of its CPU model
 // (scripts/v41_oracle/kernel.py:161-167).
 //
-// Tile.  128 rows of W are the MMA's M side (a tensor-memory lane each), up to 208 rows of A its N side, so that one token and a
-// few hundred run on the same kernel: a decode batch is an N of 16 under a stream of weights.  The terms of A are further MMAs into
-// the same accumulator: W is read once for all of them.  A pipeline stage is 256 columns: 128-byte rows (128-byte swizzle) of W and of every
-// term, each one TMA box, zero-filled past the operand's edges; and their scale bytes.
+// Tile.  128 rows of W are the MMA's M side (a tensor-memory lane each), A's rows its N side, so that one token and a few hundred run on the
+// same kernel: a decode batch is a narrow N under a stream of weights.  Terms of A: a single CTA takes up to 208 rows of all terms together
+// as N -- an MMA costs 50 clocks to issue and no less, so one of N = 48 replaces three of N = 16 -- and the read-out adds each token's terms; a
+// pair of CTAs takes up to 128 tokens and runs a term after the other into the same accumulator.  Either way W is read once for all terms.
+// A pipeline stage is 256 columns: 128-byte rows (128-byte swizzle) of W and of A, each one TMA box, zero-filled past the operand's edges.
 // Scales are read as stored (row-major bytes; nothing is laid out beforehand), 16 bytes of every row -- 512 columns, two stages -- at a time
 // into a ring of their own: by TMA where rows of scales are 16-byte aligned (K a multiple of 512), else by four loader warps, a row of
 // every 128-row group a thread, as the aligned words that hold them, requested ahead and shifted into place.  (Asynchronous copies of 8 bytes
@@ -44,7 +45,7 @@ constexpr int kMaxScaleBufs = 3;
 constexpr int kMaxSlots = 4;         // of scales in tensor memory, two stages each
 constexpr int kMaxGroups = 4;        // W and up to three term groups
 constexpr int kMaxStages = 8;
-constexpr int kMaxTokens = 208;      // A rows of a tile: two accumulators and four scale slots fill tensor memory
+constexpr int kMaxN = 208;           // of an MMA: two accumulators and two scale slots fill tensor memory
 constexpr uint32_t kSpinLimit = 1u << 22;
 
 __device__ __forceinline__ uint32_t smem_u32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
@@ -253,11 +254,12 @@ struct MatmulArgs {
     int64_t row_stride;
     int64_t M, N;
     int K;
-    int tokens;              // A rows of a tile (multiple of 16)
+    int tokens;              // tokens of a tile (multiple of 16)
+    int fold;                // terms laid side by side in N (single CTAs; TERMS is 1 then), or 1
     int stages, stage_bytes; // ring of codes
     int slots;               // ring of scale slots in tensor memory, two stages each
     int scale_bufs;          // ring of scales, kGroupBytes a group
-    int groups;              // 128-row groups of scales: 1 (W) + terms * ceil(tokens / 128)
+    int groups;              // 128-row groups of scales: 1 (W) + TERMS * ceil(tokens * fold / 128)
     int tmem_cols;
     int splits;              // CTAs of a cluster that share a tile's columns
     int tiles_w, tiles;      // tile t: W tile t % tiles_w, token tile t / tiles_w
@@ -330,7 +332,7 @@ mxfp4_matmul_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_con
     const int kc0 = (int)((int64_t)n_kc * rank / g.splits), kc1 = (int)((int64_t)n_kc * (rank + 1) / g.splits);
     const int per_tile = PAIR ? 2 : g.splits;               // CTAs
     const int tile0 = (int)blockIdx.x / per_tile, tile_step = (int)gridDim.x / per_tile;
-    const int BN = g.tokens, held = PAIR ? BN / 2 : BN;    // A rows of a tile, and of them in this CTA
+    const int tokens = g.tokens, BN = tokens * g.fold, held = PAIR ? BN / 2 : BN;   // of a tile; N of its MMAs; rows of that in this CTA
     constexpr int kTileW = PAIR ? 2 * kWRows : kWRows;
     const uint32_t b_bytes = (uint32_t)(TERMS * held * kRowBytes);
     // scales behind the ring of codes: [buffer][W, term 0, ...][row][16]; a term's group has room for 128 rows behind the previous one's rows
@@ -346,7 +348,7 @@ mxfp4_matmul_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_con
             uint32_t s = 0, ph = 0;
             bool ok = true;
             for (int tile = tile0; tile < g.tiles && ok; tile += tile_step) {
-                const int w0 = (tile % g.tiles_w) * kTileW + half * kWRows, a0 = (tile / g.tiles_w) * BN + half * held;
+                const int w0 = (tile % g.tiles_w) * kTileW + half * kWRows, a0 = (tile / g.tiles_w) * tokens + half * held;
                 for (int kc = kc0; kc < kc1; kc++) {
                     ok = mbar_wait(bar(EMPTY) + 8u * s, ph ^ 1u, abort_flag);
                     if (!ok) break;
@@ -421,7 +423,7 @@ mxfp4_matmul_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_con
             uint32_t d = 0, ph = 0;
             bool ok = true;
             for (int tile = tile0; tile < g.tiles && ok; tile += tile_step) {
-                const int w0 = (tile % g.tiles_w) * kTileW + half * kWRows, a0 = (tile / g.tiles_w) * BN;
+                const int w0 = (tile % g.tiles_w) * kTileW + half * kWRows, a0 = (tile / g.tiles_w) * tokens;
                 for (int kc = kc0 & ~1; kc < kc1; kc += 2) {
                     ok = mbar_wait(bar(RAW_EMPTY) + 8u * d, ph ^ 1u, abort_flag);
                     if (!ok) break;
@@ -457,7 +459,7 @@ mxfp4_matmul_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_con
             uint32_t d = 0, ph = 0;
             bool ok = true;
             for (int tile = tile0; tile < g.tiles && ok; tile += tile_step) {
-                const int64_t w_row = (int64_t)(tile % g.tiles_w) * kTileW + half * kWRows + r, a_row0 = (int64_t)(tile / g.tiles_w) * BN;
+                const int64_t w_row = (int64_t)(tile % g.tiles_w) * kTileW + half * kWRows + r, a_row0 = (int64_t)(tile / g.tiles_w) * tokens;
                 // this thread's row of every group, null where the operand has none
                 const uint8_t* row[kMaxGroups];
                 bool place[kMaxGroups];   // the group has room for it
@@ -465,8 +467,9 @@ mxfp4_matmul_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_con
                 place[0] = true;
 #pragma unroll
                 for (int i = 1; i < kMaxGroups; i++) {
-                    const int q = nb == 2 ? 0 : i - 1, ra = (nb == 2 ? (i - 1) * 128 : 0) + r;   // nb == 2 only with one term
-                    place[i] = i < g.groups && ra < BN;
+                    const int rn = (TERMS == 1 ? (i - 1) * 128 : 0) + r;   // row of N; the term it belongs to and its token
+                    const int q = TERMS == 1 ? rn / tokens : i - 1, ra = TERMS == 1 ? rn % tokens : rn;
+                    place[i] = i < g.groups && rn < BN;
                     row[i] = place[i] && a_row0 + ra < g.M ? g.a_scales + ((int64_t)q * g.M + a_row0 + ra) * nblk : nullptr;
                 }
                 // the aligned words that hold bytes blk .. blk + 15 of a row (the row's last bytes: fewer), at most five
@@ -511,17 +514,25 @@ mxfp4_matmul_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_con
         uint32_t t = 0;
         bool ok = true;
         for (int tile = tile0; tile < g.tiles && ok; tile += tile_step, t++) {
-            const int64_t n = (int64_t)(tile % g.tiles_w) * kTileW + half * kWRows + q * 32 + lane, m0 = (int64_t)(tile / g.tiles_w) * BN;
+            const int64_t n = (int64_t)(tile % g.tiles_w) * kTileW + half * kWRows + q * 32 + lane, m0 = (int64_t)(tile / g.tiles_w) * tokens;
             const uint32_t b = t & 1u, acc = tmem + b * (uint32_t)BN + ((q * 32u) << 16);
             ok = mbar_wait(bar(ACC_FULL) + 8u * b, (t >> 1) & 1u, abort_flag);
             if (!ok) break;
             tc_fence_after();
-            const int rows = (int)min((int64_t)BN, g.M - m0);         // tokens that exist
+            const int rows = (int)min((int64_t)tokens, g.M - m0);     // tokens that exist
             T* o = reinterpret_cast<T*>(g.out) + m0 * g.row_stride + n;
-            for (int c0 = 0; c0 < BN; c0 += 16) {
+            for (int c0 = 0; c0 < tokens; c0 += 16) {
                 uint32_t v[16];
                 tc_ld16(acc + (uint32_t)c0, v);
                 tc_wait_ld();
+                if constexpr (!PAIR)
+                    for (int f = 1; f < g.fold; f++) {   // the token's further terms
+                        uint32_t more[16];
+                        tc_ld16(acc + (uint32_t)(f * tokens + c0), more);
+                        tc_wait_ld();
+#pragma unroll
+                        for (int j = 0; j < 16; j++) v[j] = __float_as_uint(__uint_as_float(v[j]) + __uint_as_float(more[j]));
+                    }
                 if (!PAIR && g.splits > 1) {   // the partial tile, token-major, in the ring's memory (every stage has been consumed)
                     float* p = reinterpret_cast<float*>(smem) + (size_t)c0 * kWRows + q * 32 + lane;
 #pragma unroll
@@ -579,9 +590,9 @@ mxfp4_matmul_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_con
     if (!PAIR && g.splits > 1) {
         cluster_sync_all();
         // CTA `rank` adds the tokens rank, rank + splits, ... of all partial tiles, in rank order
-        const int64_t w0 = (int64_t)(tile0 % g.tiles_w) * kWRows, m0 = (int64_t)(tile0 / g.tiles_w) * BN;
+        const int64_t w0 = (int64_t)(tile0 % g.tiles_w) * kWRows, m0 = (int64_t)(tile0 / g.tiles_w) * tokens;
         const int r = threadIdx.x & 127;
-        for (int c = rank + g.splits * (int)(threadIdx.x >> 7); c < BN; c += g.splits * (kThreads / 128)) {
+        for (int c = rank + g.splits * (int)(threadIdx.x >> 7); c < tokens; c += g.splits * (kThreads / 128)) {
             if (m0 + c >= g.M || w0 + r >= g.N) continue;
             const uint32_t at = sbase + (uint32_t)(c * kWRows + r) * 4u;
             float sum = 0.0f;
@@ -603,21 +614,24 @@ mxfp4_matmul_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_con
 constexpr int kSmallMin = 77 * 1024, kSmallMax = 112 * 1024, kLargeMin = 160 * 1024, kLargeMax = 225 * 1024;
 
 struct Plan {
-    int tokens, stages, slots, stage_bytes, scale_bufs, groups, tmem_cols, smem, per_sm, splits, tiles_w, tiles_m;
+    int tokens, fold, stages, slots, stage_bytes, scale_bufs, groups, tmem_cols, smem, per_sm, splits, tiles_w, tiles_m;
     bool pair;
 };
 
 bool plan_block(int terms, int tokens, bool pair, Plan* p) {
-    const int nb = (tokens + 127) / 128, groups = 1 + terms * nb;
     p->tokens = tokens;
     p->pair = pair;
+    p->fold = pair ? 1 : terms;
+    const int n = tokens * p->fold;
+    if (n > kMaxN || (pair && terms > 1 && n > 128)) return false;   // a pair's terms have one group of scales each
+    const int groups = 1 + (pair ? terms : 1) * ((n + 127) / 128);
     p->groups = groups;
     p->stage_bytes = kWBytes + terms * (pair ? tokens / 2 : tokens) * kRowBytes;
     auto pow2 = [](int c) { int r = 32; while (r < c) r *= 2; return r; };
     // stages and scale slots that fit behind `bufs` buffers of scales into `smem` bytes and `cols` columns
     auto fit = [&](int smem, int bufs, int cols, int per_sm) {
         p->stages = std::min(kMaxStages, (smem - 1024 - bufs * groups * kGroupBytes) / p->stage_bytes);
-        p->slots = std::min(kMaxSlots, (cols - 2 * tokens) / (16 * groups));
+        p->slots = std::min(kMaxSlots, (cols - 2 * n) / (16 * groups));
         p->scale_bufs = bufs;
         p->per_sm = per_sm;
         return p->stages >= (per_sm == 2 ? 3 : 2) && p->slots >= 2;
@@ -625,29 +639,26 @@ bool plan_block(int terms, int tokens, bool pair, Plan* p) {
     // three buffers of scales (six stages) only where a ring of that length is to be fed
     if (!(!pair && fit(kSmallMax, 2, 256, 2)) && !(fit(kLargeMax, 3, 512, 1) && p->stages > 4) && !fit(kLargeMax, 2, 512, 1)) return false;
     p->smem = std::max(p->per_sm == 2 ? kSmallMin : kLargeMin, p->stages * p->stage_bytes + p->scale_bufs * groups * kGroupBytes + 1024);
-    p->tmem_cols = pow2(2 * tokens + p->slots * 16 * groups);
+    p->tmem_cols = pow2(2 * n + p->slots * 16 * groups);
     return p->stages * p->stage_bytes >= tokens * kWRows * 4;   // a partial tile fits into the ring
 }
 
-// Tokens a tile, pairs or single CTAs, and splits of the columns, from a model of the time in clocks.  A stage costs its MMAs (tokens / 2
-// clocks per 64 columns and term) or its shared-memory traffic -- operand reads of the MMAs, what lands, four reads of the scales -- at 128
-// bytes a clock with a third on top, or its copies at about 45 bytes a clock from L2; a block about 3000 clocks before and after its stages, a
-// joined tile another 1500; and the operands come from HBM at about 23 bytes a clock and SM.
+// Tokens a tile, pairs or single CTAs, and splits of the columns, from a model of the time in clocks.  A stage costs its MMAs and 150 clocks
+// of the issuing warp around them, or its copies at about 32 bytes a clock and SM from L2; a block about 3000 clocks before and after its
+// stages, a joined tile another 1500; and the operands come from HBM at about 23 bytes a clock and SM.
 bool make_plan(int64_t M, int64_t N, int K, int terms, int sms, bool pairs_run, Plan* best) {
     const int n_kc = (K + kStageK - 1) / kStageK;
     double best_t = 1e300;
-    const int most = terms == 1 ? kMaxTokens : 128;
     for (int pair = 0; pair <= (pairs_run ? 1 : 0); pair++)
-        for (int tokens = 16; tokens <= most && tokens < M + 16; tokens += 16) {
+        for (int tokens = 16; tokens <= kMaxN && tokens < M + 16; tokens += 16) {
             Plan p;
             if (!plan_block(terms, tokens, pair != 0, &p)) continue;
             const int ctas = pair ? 2 : 1;
             p.tiles_w = (int)((N + kWRows * ctas - 1) / (kWRows * ctas));
             p.tiles_m = (int)((M + tokens - 1) / tokens);
-            const int held = pair ? tokens / 2 : tokens;
-            const double mma = 4.0 * terms * tokens / 2;
-            const double shared = 1.33 * (4.0 * terms * (4096 + 32.0 * held) + p.stage_bytes + 4.0 * p.groups * kGroupBytes) / 128;
-            const double stage = std::max(std::max(mma, shared), p.stage_bytes / 45.0);
+            // an MMA: N / 2 clocks, 50 at least; what surrounds a stage's runs under the other block's where two share an SM
+            const double mma = 4.0 * (pair ? terms : 1) * std::max(50.0, tokens * p.fold / 2.0) + (p.per_sm == 2 ? 0.0 : 150.0);
+            const double stage = std::max(mma, p.stage_bytes / 32.0);
             const double hbm = ((double)N + (double)terms * M) * K * 17 / 32 / (23.0 * sms);
             for (int s = 1; s <= (pair ? 1 : 8) && s <= n_kc; s *= 2) {
                 const int64_t units = (int64_t)p.tiles_w * p.tiles_m * s, slots = (int64_t)sms / ctas;
@@ -690,22 +701,19 @@ int launch(const Plan& p, const CUtensorMap (&maps)[4], const MatmulArgs& g, int
 
 template <int DT>
 int launch_for(int terms, const Plan& p, const CUtensorMap (&maps)[4], const MatmulArgs& g, int sms, cudaStream_t stream) {
-    if (terms == 1) return p.pair ? launch<DT, 1, true>(p, maps, g, sms, stream) : launch<DT, 1, false>(p, maps, g, sms, stream);
-    if (terms == 2) return p.pair ? launch<DT, 2, true>(p, maps, g, sms, stream) : launch<DT, 2, false>(p, maps, g, sms, stream);
-    return p.pair ? launch<DT, 3, true>(p, maps, g, sms, stream) : launch<DT, 3, false>(p, maps, g, sms, stream);
+    if (!p.pair) return launch<DT, 1, false>(p, maps, g, sms, stream);
+    if (terms == 1) return launch<DT, 1, true>(p, maps, g, sms, stream);
+    if (terms == 2) return launch<DT, 2, true>(p, maps, g, sms, stream);
+    return launch<DT, 3, true>(p, maps, g, sms, stream);
 }
 
-template <int DT, int TERMS>
-int allow_shared() {
-    DSX_CUDA(cudaFuncSetAttribute(mxfp4_matmul_kernel<DT, TERMS, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, kLargeMax));
-    DSX_CUDA(cudaFuncSetAttribute(mxfp4_matmul_kernel<DT, TERMS, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, kLargeMax));
-    return DSX_OK;
-}
 template <int DT>
-int allow_shared_all() {
-    if (int rc = allow_shared<DT, 1>()) return rc;
-    if (int rc = allow_shared<DT, 2>()) return rc;
-    return allow_shared<DT, 3>();
+int allow_shared() {
+    DSX_CUDA(cudaFuncSetAttribute(mxfp4_matmul_kernel<DT, 1, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, kLargeMax));
+    DSX_CUDA(cudaFuncSetAttribute(mxfp4_matmul_kernel<DT, 1, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, kLargeMax));
+    DSX_CUDA(cudaFuncSetAttribute(mxfp4_matmul_kernel<DT, 2, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, kLargeMax));
+    DSX_CUDA(cudaFuncSetAttribute(mxfp4_matmul_kernel<DT, 3, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, kLargeMax));
+    return DSX_OK;
 }
 
 // SM count of the current device and whether it runs CTA pairs (a partition of a device may not hold a cluster of two); looked up,
@@ -719,9 +727,9 @@ int configure(int* sms, bool* pairs_run) {
     int n = known[dev].load(std::memory_order_acquire);
     if (n == 0) {
         DSX_CUDA(cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev));
-        if (int rc = allow_shared_all<DSX_F32>()) return rc;
-        if (int rc = allow_shared_all<DSX_BF16>()) return rc;
-        if (int rc = allow_shared_all<DSX_F16>()) return rc;
+        if (int rc = allow_shared<DSX_F32>()) return rc;
+        if (int rc = allow_shared<DSX_BF16>()) return rc;
+        if (int rc = allow_shared<DSX_F16>()) return rc;
         cudaLaunchConfig_t lc = {};
         lc.gridDim = dim3(2);
         lc.blockDim = dim3(kThreads);
@@ -798,7 +806,7 @@ int dsx_mxfp4_matmul(const void* a_codes, const void* a_scales, int n_terms, int
     g.out = out;
     g.row_stride = row_stride;
     g.M = m; g.N = n; g.K = (int)k;
-    g.tokens = p.tokens; g.stages = p.stages; g.slots = p.slots; g.stage_bytes = p.stage_bytes; g.groups = p.groups; g.tmem_cols = p.tmem_cols; g.splits = p.splits;
+    g.tokens = p.tokens; g.fold = p.fold; g.stages = p.stages; g.slots = p.slots; g.stage_bytes = p.stage_bytes; g.groups = p.groups; g.tmem_cols = p.tmem_cols; g.splits = p.splits;
     g.tiles_w = p.tiles_w; g.tiles = p.tiles_w * p.tiles_m;
     g.scale_tma = scale_tma;
     g.scale_bufs = p.scale_bufs;
