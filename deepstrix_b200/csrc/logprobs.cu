@@ -75,6 +75,11 @@ __device__ __forceinline__ uint64_t merge32(uint64_t a, uint64_t b, int lane) {
     return k;
 }
 
+__device__ __forceinline__ void cluster_sync_all() {
+    __syncwarp();   // the .aligned forms want the warp together, whatever branch came before
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
 // Two f32 in one register pair.
 __device__ __forceinline__ uint64_t pair(float a, float b) {
     uint64_t r;
@@ -427,7 +432,7 @@ token_logprobs_kernel(const void* __restrict__ logits, int64_t V, int64_t row_st
     // --------------------------------------------------------------- the row
     float m = sh.block_sums[0], s = sh.block_sums[1], u = sh.block_sums[2];
     if (splits > 1) {
-        asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+        cluster_sync_all();
         if (rank == 0) {
             // a lane of the first warp per block for the sums; n_alt keys of every block for the alternatives
             if (warp == 0) {
@@ -492,7 +497,7 @@ token_logprobs_kernel(const void* __restrict__ logits, int64_t V, int64_t row_st
         }
     }
     // nobody's shared memory goes away while the first block reads it
-    if (splits > 1) asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+    if (splits > 1) cluster_sync_all();
 }
 
 template <int DT, int NT>

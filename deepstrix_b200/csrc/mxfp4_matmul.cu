@@ -76,8 +76,9 @@ __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatil
     *abort_flag = 1u;
     return false;
 }
-// The same for a warp that must stay together: it goes on when the wait runs out (what it computes then is reported as missing), so
-// no branch depends on the outcome.
+// The same for a warp that goes on as one.  Its lanes may see the phase complete at different polls, and what follows (tcgen05 loads and
+// stores, MMAs from uniform registers) wants them together: hence the __syncwarp, and no branch on the outcome -- when the wait runs out the
+// warp goes on, and what it then computes is reported as missing.
 __device__ __forceinline__ void mbar_wait_on(uint32_t bar, uint32_t parity, volatile uint32_t* abort_flag) {
     uint32_t i = 0;
     for (; i < kSpinLimit; i++) {
@@ -85,7 +86,7 @@ __device__ __forceinline__ void mbar_wait_on(uint32_t bar, uint32_t parity, vola
         if ((i & 255u) == 255u && *abort_flag) break;
     }
     if (i == kSpinLimit) *abort_flag = 1u;
-    __syncwarp();   // tells the compiler too that the warp is together: what follows may stay in uniform registers
+    __syncwarp();
 }
 __device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap* map, int c0, int c1, uint32_t bar) {
     asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(dst), "l"(map),
@@ -204,6 +205,7 @@ __device__ __forceinline__ float ld_cluster_f32(uint32_t addr) {
     return v;
 }
 __device__ __forceinline__ void cluster_sync_all() {
+    __syncwarp();   // the .aligned forms want the warp together, whatever branch came before
     asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 // K-major operand tile of 128-byte rows, 128-byte swizzle: 8-row groups of 1024 bytes.
@@ -311,6 +313,7 @@ mxfp4_matmul_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_con
         asm volatile("prefetch.tensormap [%0];" ::"l"(&tmap_a) : "memory");
     }
     if (warp == 1) {
+        __syncwarp();
         if constexpr (PAIR) {
             asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(s_misc)), "r"(g.tmem_cols) : "memory");
             asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
@@ -417,6 +420,9 @@ mxfp4_matmul_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_con
             }
             tc_commit<PAIR>(leader, bar(ACC_FULL) + 8u * b);
         }
+        if (*abort_flag && t > 0)   // somebody gave up: let the MMAs in flight finish before tensor memory goes away
+            for (uint32_t n = 0; n < kSpinLimit / 64 && !mbar_try(bar(ACC_FULL) + 8u * ((t - 1u) & 1u), ((t - 1u) >> 1) & 1u); n++) {}
+        __syncwarp();
     } else if (warp == 2) {
         // --------------------------------------------------------- TMA of scales
         if (lane == 0 && g.scale_tma) {
@@ -512,17 +518,16 @@ mxfp4_matmul_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_con
         // -------------------------------------------------------------- epilogue
         const uint32_t q = (uint32_t)(warp & 3);
         uint32_t t = 0;
-        bool ok = true;
-        for (int tile = tile0; tile < g.tiles && ok; tile += tile_step, t++) {
+        for (int tile = tile0; tile < g.tiles; tile += tile_step, t++) {
             const int64_t n = (int64_t)(tile % g.tiles_w) * kTileW + half * kWRows + q * 32 + lane, m0 = (int64_t)(tile / g.tiles_w) * tokens;
             const uint32_t b = t & 1u, acc = tmem + b * (uint32_t)BN + ((q * 32u) << 16);
-            ok = mbar_wait(bar(ACC_FULL) + 8u * b, (t >> 1) & 1u, abort_flag);
-            if (!ok) break;
+            mbar_wait_on(bar(ACC_FULL) + 8u * b, (t >> 1) & 1u, abort_flag);
             tc_fence_after();
             const int rows = (int)min((int64_t)tokens, g.M - m0);     // tokens that exist
             T* o = reinterpret_cast<T*>(g.out) + m0 * g.row_stride + n;
             for (int c0 = 0; c0 < tokens; c0 += 16) {
                 uint32_t v[16];
+                __syncwarp();   // stores above may have parted the lanes
                 tc_ld16(acc + (uint32_t)c0, v);
                 tc_wait_ld();
                 if constexpr (!PAIR)
@@ -555,12 +560,12 @@ mxfp4_matmul_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_con
         const uint32_t q = (uint32_t)(warp & 3);
         const uint32_t set = warp >= kLoadWarp0 ? 1u : 0u, sets = g.scale_tma ? 2u : 1u;
         uint32_t u = 0, d = 0, dph = 0, v = 0, vph = 0;   // buffers so far; ring positions
-        bool ok = true;
-        for (int tile = tile0; tile < g.tiles && ok; tile += tile_step)
+        for (int tile = tile0; tile < g.tiles; tile += tile_step)
             for (int kc = kc0; kc < kc1; kc = (kc | 1) + 1, u++) {
                 if (sets == 1u || (u & 1u) == set) {
-                    ok = mbar_wait(bar(RAW_FULL) + 8u * d, dph, abort_flag) && mbar_wait(bar(SLOT_EMPTY) + 8u * v, vph ^ 1u, abort_flag);
-                    if (!ok) break;
+                    mbar_wait_on(bar(RAW_FULL) + 8u * d, dph, abort_flag);
+                    mbar_wait_on(bar(SLOT_EMPTY) + 8u * v, vph ^ 1u, abort_flag);
+                    tc_fence_after();
                     const uint8_t* src = smem + raw0 + d * raw_bytes + lane * 16;
                     const uint32_t dst = slot0 + v * slot_cols + ((q * 32u) << 16);
                     store_scales<1>(src, dst);
@@ -583,6 +588,7 @@ mxfp4_matmul_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_con
             }
     }
 
+    __syncwarp();
     tc_fence_before();
     __syncthreads();
     if (threadIdx.x == 0 && *abort_flag) atomicOr(&g_head_error, 1u);
@@ -602,6 +608,7 @@ mxfp4_matmul_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_con
         cluster_sync_all();   // nobody's shared memory goes away while another CTA reads it
     }
     if (warp == 1) {
+        __syncwarp();
         tc_fence_after();
         if constexpr (PAIR) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(g.tmem_cols) : "memory");
         else asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(g.tmem_cols) : "memory");
