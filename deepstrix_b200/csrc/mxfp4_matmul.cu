@@ -41,7 +41,7 @@ constexpr int kStageK = 256;         // columns of a stage
 constexpr int kRowBytes = kStageK / 2;
 constexpr int kWBytes = kWRows * kRowBytes;
 constexpr int kGroupBytes = 2048;    // scale bytes of a group of 128 rows: 16 a row, two stages
-constexpr int kMaxScaleBufs = 3;
+constexpr int kMaxScaleBufs = 4;     // two or four: see plan_block
 constexpr int kMaxSlots = 4;         // of scales in tensor memory, two stages each
 constexpr int kMaxGroups = 4;        // W and up to three term groups
 constexpr int kMaxStages = 8;
@@ -643,8 +643,11 @@ bool plan_block(int terms, int tokens, bool pair, Plan* p) {
         p->per_sm = per_sm;
         return p->stages >= (per_sm == 2 ? 3 : 2) && p->slots >= 2;
     };
-    // three buffers of scales (six stages) only where a ring of that length is to be fed
-    if (!(!pair && fit(kSmallMax, 2, 256, 2)) && !(fit(kLargeMax, 3, 512, 1) && p->stages > 4) && !fit(kLargeMax, 2, 512, 1)) return false;
+    // An even number of buffers of scales, so that each belongs to one of the two sets of scale warps: a set that shared a buffer with the other
+    // could ask for a phase of its barrier whose predecessor had not completed yet, and a parity wait lets that pass.  (Slots: the set that
+    // comes to a slot has waited for one that the tensor core finished behind the slot's last use but one.)  Four only where a ring of that
+    // length is to be fed.
+    if (!(!pair && fit(kSmallMax, 2, 256, 2)) && !(fit(kLargeMax, 4, 512, 1) && p->stages > 4) && !fit(kLargeMax, 2, 512, 1)) return false;
     p->smem = std::max(p->per_sm == 2 ? kSmallMin : kLargeMin, p->stages * p->stage_bytes + p->scale_bufs * groups * kGroupBytes + 1024);
     p->tmem_cols = pow2(2 * n + p->slots * 16 * groups);
     return p->stages * p->stage_bytes >= tokens * kWRows * 4;   // a partial tile fits into the ring
