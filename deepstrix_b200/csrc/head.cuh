@@ -1,5 +1,7 @@
 // Shared by the kernels of the quantised head: element types, MXFP4 rows, the error word.
 #pragma once
+#include <atomic>
+
 #include "dsx_common.cuh"
 
 namespace dsx {
@@ -38,6 +40,22 @@ template <> __device__ __forceinline__ float2 unpack2<__nv_bfloat16>(uint32_t w)
     return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xFFFF0000u));
 }
 template <> __device__ __forceinline__ float2 unpack2<__half>(uint32_t w) { return __half22float2(*reinterpret_cast<const __half2*>(&w)); }
+
+// SM count of the current device, looked up once per device.
+inline int head_sm_count(int* sms) {
+    constexpr int kMaxDevices = 64;
+    static std::atomic<int> known[kMaxDevices];
+    int dev = 0;
+    DSX_CUDA(cudaGetDevice(&dev));
+    DSX_REQUIRE(dev >= 0 && dev < kMaxDevices, "device index %d out of range", dev);
+    int n = known[dev].load(std::memory_order_relaxed);
+    if (n == 0) {
+        DSX_CUDA(cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev));
+        known[dev].store(n, std::memory_order_relaxed);
+    }
+    *sms = n;
+    return DSX_OK;
+}
 
 // -------------------------------------------------------------- MXFP4 values
 // 2^(e - 127); e = 0 is the subnormal 2^-127, e = 255 is NaN (the E8M0 encoding).

@@ -16,8 +16,6 @@
 // distributed shared memory: one launch, no workspace, and the order of every addition is fixed.
 //
 // Bound: HBM; bf16 and f16 rows at the full rate are 11.6 elements a clock and SM, of which the exponentials can take 16.
-#include <atomic>
-
 #include "head.cuh"
 
 namespace dsx {
@@ -523,16 +521,8 @@ int launch(const void* logits, int64_t t, int64_t v, int64_t row_stride, float s
 template <int DT>
 int launch_for(const void* logits, int64_t t, int64_t v, int64_t row_stride, float scale, const int32_t* tokens, int n_given, float* logprobs, float* entropy,
                int n_alt, int32_t* alts, float* alt_logprobs, cudaStream_t stream) {
-    constexpr int kMaxDevices = 64;
-    static std::atomic<int> sm_counts[kMaxDevices];
-    int dev = 0;
-    DSX_CUDA(cudaGetDevice(&dev));
-    DSX_REQUIRE(dev >= 0 && dev < kMaxDevices, "token_logprobs: device index %d out of range", dev);
-    int sms = sm_counts[dev].load(std::memory_order_acquire);
-    if (sms == 0) {
-        DSX_CUDA(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev));
-        sm_counts[dev].store(sms, std::memory_order_release);
-    }
+    int sms = 0;
+    if (int rc = head_sm_count(&sms)) return rc;
     constexpr int kChunk = Chunk<typename Elem<DT>::T>::n;
     // many rows of at most 16 chunks a thread: the small block (4096 rows of 4096 bf16 16.5 us against 38.8, of 16384 36.8 against 57.9, but
     // of 32000 with 20 alternatives 114 against 85); also a row that a small block reads in one round

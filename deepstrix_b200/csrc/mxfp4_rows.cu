@@ -135,9 +135,8 @@ mxfp4_dequantize_kernel(const uint32_t* __restrict__ codes, const uint8_t* __res
 }
 
 int grid_of(int64_t n_threads, unsigned* blocks) {
-    int dev = 0, sms = 0;
-    DSX_CUDA(cudaGetDevice(&dev));
-    DSX_CUDA(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev));
+    int sms = 0;
+    if (int rc = head_sm_count(&sms)) return rc;
     const int64_t want = (n_threads + kThreads - 1) / kThreads, cap = (int64_t)sms * 8;
     *blocks = (unsigned)(want < cap ? want : cap);
     return DSX_OK;

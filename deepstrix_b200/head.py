@@ -46,9 +46,10 @@ def _call(name, *args):
 
 def _here(*tensors) -> int:
     """All on the current device, whose current stream (returned) the kernels run on."""
-    assert all(t.is_cuda for t in tensors), "tensors must be on the GPU"
-    device = torch.cuda.current_device()
-    assert all(t.get_device() == device for t in tensors), f"tensors on {[str(t.device) for t in tensors]}, current device is cuda:{device}"
+    device = torch.cuda.current_device() if tensors[0].is_cuda else None
+    for t in tensors:
+        assert t.is_cuda, "tensors must be on the GPU"
+        assert t.get_device() == device, f"tensor on {t.device}, current device is cuda:{device}"
     return torch._C._cuda_getCurrentRawStream(device)
 
 
@@ -65,20 +66,48 @@ def _row_stride(t: torch.Tensor) -> int:
 
 
 class Mxfp4Rows:
-    """Rows as sums of MXFP4 terms: uint8 codes [terms, rows, K / 2] (element 2i in the low nibble) and E8M0 scales
+    """Rows as sums of MXFP4 terms: uint8 ``codes`` [terms, rows, K / 2] (element 2i in the low nibble) and E8M0 ``scales``
     [terms, rows, K / 32]; two-dimensional tensors are one term (a stored matrix)."""
-    __slots__ = ("codes", "scales", "n_terms", "rows", "k")
+    __slots__ = ("n_terms", "rows", "k", "codes_at", "scales_at", "_buffer", "_codes", "_scales")
 
     def __init__(self, codes: torch.Tensor, scales: torch.Tensor):
         assert codes.dtype == torch.uint8 and scales.dtype == torch.uint8 and codes.is_contiguous() and scales.is_contiguous()
         shape = codes.shape
         assert len(shape) in (2, 3) and shape[:-1] == scales.shape[:-1] and shape[-1] == 16 * scales.shape[-1], "codes [.., K / 2] and scales [.., K / 32]"
         assert codes.device == scales.device
-        self._set(codes, scales, shape[0] if len(shape) == 3 else 1, shape[-2], 2 * shape[-1])
+        self.n_terms, self.rows, self.k = shape[0] if len(shape) == 3 else 1, shape[-2], 2 * shape[-1]
+        self._buffer, self._codes, self._scales = codes, codes, scales
+        self.codes_at, self.scales_at = codes.data_ptr(), scales.data_ptr()
 
-    def _set(self, codes, scales, n_terms, rows, k):
-        self.codes, self.scales, self.n_terms, self.rows, self.k = codes, scales, n_terms, rows, k
-        return self
+    @classmethod
+    def _empty(cls, n_terms: int, rows: int, k: int, device) -> "Mxfp4Rows":
+        """Room for the quantiser's result: one allocation, the tensors made when they are asked for."""
+        assert n_terms >= 1 and k % 32 == 0, f"{n_terms} terms of rows of {k} columns (a multiple of 32)"
+        q = cls.__new__(cls)
+        n = n_terms * rows * k
+        q.n_terms, q.rows, q.k, q._codes, q._scales = n_terms, rows, k, None, None
+        q._buffer = torch.empty(n // 2 + n // 32, dtype=torch.uint8, device=device)
+        q.codes_at = q._buffer.data_ptr()
+        q.scales_at = q.codes_at + n // 2
+        return q
+
+    @property
+    def device(self) -> torch.device:
+        return self._buffer.device
+
+    @property
+    def codes(self) -> torch.Tensor:
+        if self._codes is None:
+            row = self.k // 2
+            self._codes = self._buffer.as_strided((self.n_terms, self.rows, row), (self.rows * row, row, 1), 0)
+        return self._codes
+
+    @property
+    def scales(self) -> torch.Tensor:
+        if self._scales is None:
+            row = self.k // 32
+            self._scales = self._buffer.as_strided((self.n_terms, self.rows, row), (self.rows * row, row, 1), self.n_terms * self.rows * self.k // 2)
+        return self._scales
 
 
 class Mxfp4Quantize:
@@ -91,10 +120,9 @@ class Mxfp4Quantize:
         stride = _row_stride(x)
         stream = _here(x)
         rows, k = x.shape
-        codes = torch.empty((n_terms, rows, k // 2), dtype=torch.uint8, device=x.device)
-        scales = torch.empty((n_terms, rows, k // 32), dtype=torch.uint8, device=x.device)
-        _call("dsx_mxfp4_quantize", x.data_ptr(), DTYPES[x.dtype], rows, k, stride, n_terms, codes.data_ptr(), scales.data_ptr(), stream)
-        return Mxfp4Rows.__new__(Mxfp4Rows)._set(codes, scales, n_terms, rows, k)
+        q = Mxfp4Rows._empty(n_terms, rows, k, x.device)
+        _call("dsx_mxfp4_quantize", x.data_ptr(), DTYPES[x.dtype], rows, k, stride, n_terms, q.codes_at, q.scales_at, stream)
+        return q
 
 
 class Mxfp4Dequantize:
@@ -103,10 +131,10 @@ class Mxfp4Dequantize:
     @staticmethod
     def launch(q: Mxfp4Rows, dtype: torch.dtype = torch.float32, out: torch.Tensor | None = None) -> torch.Tensor:
         if out is None:
-            out = torch.empty((q.rows, q.k), dtype=dtype, device=q.codes.device)
+            out = torch.empty(q.rows, q.k, dtype=dtype, device=q.device)
         assert out.shape == (q.rows, q.k) and out.dtype == dtype and dtype in DTYPES
-        _call("dsx_mxfp4_dequantize", q.codes.data_ptr(), q.scales.data_ptr(), q.rows, q.k, q.n_terms, out.data_ptr(), DTYPES[dtype], _row_stride(out),
-              _here(q.codes, out))
+        _call("dsx_mxfp4_dequantize", q.codes_at, q.scales_at, q.rows, q.k, q.n_terms, out.data_ptr(), DTYPES[dtype], _row_stride(out),
+              _here(q._buffer, out))
         return out
 
 
@@ -118,10 +146,10 @@ class Mxfp4Matmul:
         assert w.n_terms == 1, "a weight has one term"
         assert a.k == w.k, f"rows of {a.k} and of {w.k} columns"
         if out is None:
-            out = torch.empty((a.rows, w.rows), dtype=dtype, device=a.codes.device)
+            out = torch.empty(a.rows, w.rows, dtype=dtype, device=a.device)
         assert out.shape == (a.rows, w.rows) and out.dtype == dtype and dtype in DTYPES
-        _call("dsx_mxfp4_matmul", a.codes.data_ptr(), a.scales.data_ptr(), a.n_terms, a.rows, w.codes.data_ptr(), w.scales.data_ptr(), w.rows, a.k,
-              out.data_ptr(), DTYPES[dtype], _row_stride(out), _here(a.codes, w.codes, out))
+        _call("dsx_mxfp4_matmul", a.codes_at, a.scales_at, a.n_terms, a.rows, w.codes_at, w.scales_at, w.rows, a.k, out.data_ptr(), DTYPES[dtype],
+              _row_stride(out), _here(a._buffer, w._buffer, out))
         return out
 
 
@@ -153,13 +181,13 @@ class TokenLogprobs:
             assert tokens.dtype == torch.int32 and tokens.is_contiguous() and tokens.dim() in (1, 2) and tokens.shape[0] == T, "int32 tokens [T] or [T, n]"
             stream = _here(logits, tokens)
             given = 1 if tokens.dim() == 1 else tokens.shape[1]
-            logprobs = torch.empty(tokens.shape, dtype=torch.float32, device=dev)
+            logprobs = torch.empty_like(tokens, dtype=torch.float32)
             tokens_at, logprobs_at = tokens.data_ptr(), logprobs.data_ptr()
         else:
             stream = _here(logits)
-        entropy = torch.empty((T,), dtype=torch.float32, device=dev)
-        ids = torch.empty((T, n_alt), dtype=torch.int32, device=dev)
-        alternatives = torch.empty((T, n_alt), dtype=torch.float32, device=dev)
+        entropy = torch.empty(T, dtype=torch.float32, device=dev)
+        ids = torch.empty(T, n_alt, dtype=torch.int32, device=dev)
+        alternatives = torch.empty_like(ids, dtype=torch.float32)
         _call("dsx_token_logprobs", logits.data_ptr(), DTYPES[logits.dtype], T, V, stride, inv_temperature, tokens_at, given, logprobs_at,
               entropy.data_ptr(), n_alt, ids.data_ptr(), alternatives.data_ptr(), stream)
         return logprobs, entropy, ids, alternatives
