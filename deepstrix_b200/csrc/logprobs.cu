@@ -205,6 +205,7 @@ token_logprobs_kernel(const void* __restrict__ logits, int64_t V, int64_t row_st
     const int64_t row = blockIdx.x / (unsigned)splits;
     const float c = scale * kLog2e;
     const T* __restrict__ x = reinterpret_cast<const T*>(logits) + row * row_stride;
+    pdl_wait();   // the logits may come from the kernel before this one
     // whole 16-byte words from the row's first aligned element on; the few elements before and after them one by one
     const int head = (int)min((int64_t)(((16u - (uint32_t)((uintptr_t)x & 15u)) & 15u) / sizeof(T)), V);
     const int64_t n_chunks = (V - head) / kChunk;
@@ -505,13 +506,15 @@ int launch(const void* logits, int64_t t, int64_t v, int64_t row_stride, float s
     cfg.gridDim = dim3((unsigned)(t * splits));
     cfg.blockDim = dim3(NT);
     cfg.stream = stream;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = (unsigned)splits;
-    attr[0].val.clusterDim.y = 1;
-    attr[0].val.clusterDim.z = 1;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = (unsigned)splits;
+    attr[1].val.clusterDim.y = 1;
+    attr[1].val.clusterDim.z = 1;
     cfg.attrs = attr;
-    cfg.numAttrs = splits > 1 ? 1 : 0;
+    cfg.numAttrs = splits > 1 ? 2 : 1;
     DSX_CUDA(cudaLaunchKernelEx(&cfg, token_logprobs_kernel<DT, NT>, logits, v, row_stride, scale, tokens, n_given, logprobs, entropy, n_alt, alts,
                                 alt_logprobs, splits));
     DSX_LAUNCHED();

@@ -8,6 +8,8 @@
 // the nearest E2M1 value (ties to the even code), and the next term does the same with what is left over, r - value.  Every step
 // is exact in f32, so the bytes can be restated on a CPU.  A block with a NaN or an infinity is NaN as a whole: its first
 // scale byte is 255 (E8M0's NaN), its codes are 0, and its later terms are 0.
+#include <algorithm>
+
 #include "head.cuh"
 
 namespace dsx {
@@ -61,92 +63,137 @@ __device__ __forceinline__ void store8(T* __restrict__ p, const float (&v)[8]) {
     }
 }
 
+// max |.| of eight values as f32, NaN if one of them is
+__device__ __forceinline__ float abs_max_nan(float a, float b) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(fabsf(a)), "f"(fabsf(b)));
+    return r;
+}
+__device__ __forceinline__ float abs_max8(const float (&v)[8]) {
+    return abs_max_nan(abs_max_nan(abs_max_nan(v[0], v[1]), abs_max_nan(v[2], v[3])), abs_max_nan(abs_max_nan(v[4], v[5]), abs_max_nan(v[6], v[7])));
+}
+
 // A lane holds 8 consecutive values, four neighbouring lanes a block of 32: loads are 16 (f32: 32) bytes a lane and coalesced, the
 // block's maximum is two shuffles away, and a warp stores 128 bytes of codes.  Groups of 8 are numbered through all rows, so a
-// short row wastes no lane; K / 8 is a multiple of 4, so a block never straddles two quads.
-template <int DT, int TERMS, bool VEC>
+// short row wastes no lane; K / 8 is a multiple of 4, so a block never straddles two quads.  ITEMS groups a lane are requested before the
+// first is worked on: a full grid (8 blocks of 256 an SM) of one 16-byte load a lane is 32 KB in flight an SM, too little for HBM.
+template <int DT, int TERMS, bool VEC, int ITEMS>
 __global__ void __launch_bounds__(kThreads)
 mxfp4_quantize_kernel(const void* __restrict__ x_, int64_t n_groups, uint32_t groups_per_row, int64_t row_stride, uint32_t* __restrict__ codes,
                       uint8_t* __restrict__ scales) {
     using T = typename Elem<DT>::T;
+    pdl_wait();
+    if (ITEMS == 1) pdl_launch_dependents();   // a small launch leaves room for the next kernel to set itself up
     const T* __restrict__ x = reinterpret_cast<const T*>(x_);
     const bool dense = row_stride == (int64_t)groups_per_row * 8;
     // n_groups is a multiple of 4, so the four lanes of a block are in range or out of it together; the mask of a quad
     const uint32_t quad = 0xFu << (threadIdx.x & 28u);
-    for (int64_t g = (int64_t)blockIdx.x * kThreads + threadIdx.x; g < n_groups; g += (int64_t)gridDim.x * kThreads) {
-        int64_t off = g * 8;
-        if (!dense) {
-            const int64_t row = g / groups_per_row;
-            off = row * row_stride + (g - row * groups_per_row) * 8;
+    for (int64_t g0 = (int64_t)blockIdx.x * (kThreads * ITEMS) + threadIdx.x; g0 < n_groups; g0 += (int64_t)gridDim.x * (kThreads * ITEMS)) {
+        float v[ITEMS][8];
+#pragma unroll
+        for (int i = 0; i < ITEMS; i++) {
+            const int64_t g = g0 + i * kThreads;
+            int64_t off = g * 8;
+            if (!dense) {
+                const int64_t row = g / groups_per_row;
+                off = row * row_stride + (g - row * groups_per_row) * 8;
+            }
+            if (g < n_groups) load8<T, VEC>(x + off, v[i]);
         }
-        float v[8];
-        load8<T, VEC>(x + off, v);
 #pragma unroll
-        for (int t = 0; t < TERMS; t++) {
-            uint32_t amax = 0u;   // magnitudes compare as integers; NaNs are above the infinity's bits
+        for (int i = 0; i < ITEMS; i++) {
+            const int64_t g = g0 + i * kThreads;
+            if (g >= n_groups) break;
 #pragma unroll
-            for (int j = 0; j < 8; j++) amax = max(amax, __float_as_uint(v[j]) & 0x7FFFFFFFu);
-            amax = max(amax, __shfl_xor_sync(quad, amax, 1));
-            amax = max(amax, __shfl_xor_sync(quad, amax, 2));
-            const bool bad = amax >= 0x7F800000u;
-            const int e = min(max((int)(amax >> 23) - 2 + ((amax & 0x7FFFFFu) > 0x400000u ? 1 : 0), 1), 253);
-            const float inv = __uint_as_float((uint32_t)(254 - e) << 23);
-            float sv[8];
+            for (int t = 0; t < TERMS; t++) {
+                float m = abs_max8(v[i]);
+                m = abs_max_nan(m, __shfl_xor_sync(quad, m, 1));
+                m = abs_max_nan(m, __shfl_xor_sync(quad, m, 2));
+                const uint32_t amax = __float_as_uint(m);
+                const bool bad = amax >= 0x7F800000u;   // infinite or NaN (whose sign bit is clear behind max.NaN)
+                const int e = min(max((int)(amax >> 23) - 2 + ((amax & 0x7FFFFFu) > 0x400000u ? 1 : 0), 1), 253);
+                const float inv = __uint_as_float((uint32_t)(254 - e) << 23);
+                float sv[8];
 #pragma unroll
-            for (int j = 0; j < 8; j++) sv[j] = bad ? 0.0f : v[j] * inv;
-            const uint32_t w = e2m1_encode8(sv);
-            codes[(int64_t)t * n_groups + g] = w;
-            if ((threadIdx.x & 3u) == 0u) scales[(int64_t)t * (n_groups >> 2) + (g >> 2)] = bad ? 255u : (uint8_t)e;
-            if (t + 1 < TERMS) {
-                // value = code * 2^(e - 127): the codes' f32 forms are scaled by 2^-126, hence two exact multiplications
-                const float scl = __uint_as_float((uint32_t)e << 23);
+                for (int j = 0; j < 8; j++) sv[j] = v[i][j] * inv;
+                const uint32_t w = bad ? 0u : e2m1_encode8(sv);
+                codes[(int64_t)t * n_groups + g] = w;
+                if ((threadIdx.x & 3u) == 0u) scales[(int64_t)t * (n_groups >> 2) + (g >> 2)] = bad ? 255u : (uint8_t)e;
+                if (t + 1 < TERMS) {
+                    // value = code * 2^(e - 127): the codes' f32 forms are scaled by 2^-126, hence two exact multiplications
+                    const float scl = __uint_as_float((uint32_t)e << 23);
 #pragma unroll
-                for (int j = 0; j < 8; j++) v[j] = bad ? 0.0f : __fmaf_rn(-e2m1_to_f32(w >> (4 * j)), scl, v[j]);   // exact: the residual
+                    for (int j = 0; j < 8; j++) v[i][j] = bad ? 0.0f : __fmaf_rn(-e2m1_to_f32(w >> (4 * j)), scl, v[i][j]);   // exact: the residual
+                }
             }
         }
     }
 }
 
-template <int DT, bool VEC>
+template <int DT, bool VEC, int ITEMS>
 __global__ void __launch_bounds__(kThreads)
 mxfp4_dequantize_kernel(const uint32_t* __restrict__ codes, const uint8_t* __restrict__ scales, int64_t n_groups, uint32_t groups_per_row, int terms,
                         void* __restrict__ out_, int64_t row_stride) {
     using T = typename Elem<DT>::T;
+    pdl_wait();
+    if (ITEMS == 1) pdl_launch_dependents();
     T* __restrict__ out = reinterpret_cast<T*>(out_);
     const bool dense = row_stride == (int64_t)groups_per_row * 8;
-    for (int64_t g = (int64_t)blockIdx.x * kThreads + threadIdx.x; g < n_groups; g += (int64_t)gridDim.x * kThreads) {
-        float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    for (int64_t g0 = (int64_t)blockIdx.x * (kThreads * ITEMS) + threadIdx.x; g0 < n_groups; g0 += (int64_t)gridDim.x * (kThreads * ITEMS)) {
+        float v[ITEMS][8];
         for (int t = 0; t < terms; t++) {
-            const uint32_t w = __ldg(codes + (int64_t)t * n_groups + g);
-            const float s = e8m0_value(__ldg(scales + (int64_t)t * (n_groups >> 2) + (g >> 2)));
+            uint32_t w[ITEMS], e[ITEMS];
 #pragma unroll
-            for (int j = 0; j < 8; j++) {
-                const float d = e2m1_to_f32(w >> (4 * j)) * s;
-                v[j] = t == 0 ? d : v[j] + d;
+            for (int i = 0; i < ITEMS; i++) {
+                const int64_t g = min(g0 + i * kThreads, n_groups - 1);
+                w[i] = __ldg(codes + (int64_t)t * n_groups + g);
+                e[i] = __ldg(scales + (int64_t)t * (n_groups >> 2) + (g >> 2));
+            }
+#pragma unroll
+            for (int i = 0; i < ITEMS; i++) {
+                const float s = e8m0_value(e[i]);
+#pragma unroll
+                for (int j = 0; j < 8; j++) {
+                    const float d = e2m1_to_f32(w[i] >> (4 * j)) * s;
+                    v[i][j] = t == 0 ? d : v[i][j] + d;
+                }
             }
         }
-        int64_t off = g * 8;
-        if (!dense) {
-            const int64_t row = g / groups_per_row;
-            off = row * row_stride + (g - row * groups_per_row) * 8;
+#pragma unroll
+        for (int i = 0; i < ITEMS; i++) {
+            const int64_t g = g0 + i * kThreads;
+            if (g >= n_groups) break;
+            int64_t off = g * 8;
+            if (!dense) {
+                const int64_t row = g / groups_per_row;
+                off = row * row_stride + (g - row * groups_per_row) * 8;
+            }
+            store8<T, VEC>(out + off, v[i]);
         }
-        store8<T, VEC>(out + off, v);
     }
 }
 
-int grid_of(int64_t n_threads, unsigned* blocks) {
+// Launches `small` (a group a lane, at most 8 blocks an SM) or, where that would go round more than once, `large` (four groups).
+template <typename K, typename... A>
+int launch_rows(K small, K large, int64_t n_groups, cudaStream_t s, A... args) {
     int sms = 0;
     if (int rc = head_sm_count(&sms)) return rc;
-    const int64_t want = (n_threads + kThreads - 1) / kThreads, cap = (int64_t)sms * 8;
-    *blocks = (unsigned)(want < cap ? want : cap);
+    const int64_t cap = (int64_t)sms * 8, blocks = (n_groups + kThreads - 1) / kThreads;
+    const bool big = blocks > cap;
+    DSX_CUDA(launch_pdl(big ? large : small, dim3((unsigned)(big ? std::min(cap, (blocks + 3) / 4) : blocks)), dim3(kThreads), 0, s, args...));
+    DSX_LAUNCHED();
     return DSX_OK;
 }
 
+template <int DT, bool VEC, int TERMS>
+int launch_quantize(cudaStream_t s, const void* x, int64_t n_groups, uint32_t gpr, int64_t stride, uint32_t* codes, uint8_t* scales) {
+    return launch_rows(mxfp4_quantize_kernel<DT, TERMS, VEC, 1>, mxfp4_quantize_kernel<DT, TERMS, VEC, 4>, n_groups, s, x, n_groups, gpr, stride, codes, scales);
+}
 template <int DT, bool VEC>
-void launch_quantize(int terms, unsigned blocks, cudaStream_t s, const void* x, int64_t n_groups, uint32_t gpr, int64_t stride, uint32_t* codes, uint8_t* scales) {
-    if (terms == 1) mxfp4_quantize_kernel<DT, 1, VEC><<<blocks, kThreads, 0, s>>>(x, n_groups, gpr, stride, codes, scales);
-    else if (terms == 2) mxfp4_quantize_kernel<DT, 2, VEC><<<blocks, kThreads, 0, s>>>(x, n_groups, gpr, stride, codes, scales);
-    else mxfp4_quantize_kernel<DT, 3, VEC><<<blocks, kThreads, 0, s>>>(x, n_groups, gpr, stride, codes, scales);
+int launch_quantize_terms(int terms, cudaStream_t s, const void* x, int64_t n_groups, uint32_t gpr, int64_t stride, uint32_t* codes, uint8_t* scales) {
+    if (terms == 1) return launch_quantize<DT, VEC, 1>(s, x, n_groups, gpr, stride, codes, scales);
+    if (terms == 2) return launch_quantize<DT, VEC, 2>(s, x, n_groups, gpr, stride, codes, scales);
+    return launch_quantize<DT, VEC, 3>(s, x, n_groups, gpr, stride, codes, scales);
 }
 
 int check_rows(const char* what, int dtype, int64_t rows, int64_t k, int64_t row_stride, int n_terms) {
@@ -172,20 +219,14 @@ int dsx_mxfp4_quantize(const void* x, int dtype, int64_t rows, int64_t k, int64_
     DSX_REQUIRE(((uintptr_t)x & (dtype_size(dtype) - 1)) == 0 && ((uintptr_t)codes & 15) == 0, "mxfp4_quantize: x must be aligned to its elements, codes to 16 bytes");
     const int64_t n_groups = rows * (k / 8);
     const bool vec = (((uintptr_t)x | (uintptr_t)(rows > 1 ? row_stride * dtype_size(dtype) : 0)) & 15) == 0;
-    unsigned blocks;
-    if (int rc = grid_of(n_groups, &blocks)) return rc;
     const cudaStream_t s = (cudaStream_t)stream;
-#define DSX_GO(DT)                                                                                                                              \
-    do {                                                                                                                                        \
-        if (vec) launch_quantize<DT, true>(n_terms, blocks, s, x, n_groups, (uint32_t)(k / 8), row_stride, (uint32_t*)codes, (uint8_t*)scales); \
-        else launch_quantize<DT, false>(n_terms, blocks, s, x, n_groups, (uint32_t)(k / 8), row_stride, (uint32_t*)codes, (uint8_t*)scales);    \
-    } while (0)
+#define DSX_GO(DT)                                                                                                                                \
+    return vec ? launch_quantize_terms<DT, true>(n_terms, s, x, n_groups, (uint32_t)(k / 8), row_stride, (uint32_t*)codes, (uint8_t*)scales)        \
+               : launch_quantize_terms<DT, false>(n_terms, s, x, n_groups, (uint32_t)(k / 8), row_stride, (uint32_t*)codes, (uint8_t*)scales)
     if (dtype == DSX_F32) DSX_GO(DSX_F32);
-    else if (dtype == DSX_BF16) DSX_GO(DSX_BF16);
-    else DSX_GO(DSX_F16);
+    if (dtype == DSX_BF16) DSX_GO(DSX_BF16);
+    DSX_GO(DSX_F16);
 #undef DSX_GO
-    DSX_LAUNCHED();
-    return DSX_OK;
 }
 
 int dsx_mxfp4_dequantize(const void* codes, const void* scales, int64_t rows, int64_t k, int n_terms, void* out, int dtype, int64_t row_stride,
@@ -197,20 +238,17 @@ int dsx_mxfp4_dequantize(const void* codes, const void* scales, int64_t rows, in
                 "mxfp4_dequantize: out must be aligned to its elements, codes to 16 bytes");
     const int64_t n_groups = rows * (k / 8);
     const bool vec = (((uintptr_t)out | (uintptr_t)(rows > 1 ? row_stride * dtype_size(dtype) : 0)) & 15) == 0;
-    unsigned blocks;
-    if (int rc = grid_of(n_groups, &blocks)) return rc;
     const cudaStream_t s = (cudaStream_t)stream;
-#define DSX_GO(DT)                                                                                                                                             \
-    do {                                                                                                                                                       \
-        if (vec) mxfp4_dequantize_kernel<DT, true><<<blocks, kThreads, 0, s>>>((const uint32_t*)codes, (const uint8_t*)scales, n_groups, (uint32_t)(k / 8), n_terms, out, row_stride); \
-        else mxfp4_dequantize_kernel<DT, false><<<blocks, kThreads, 0, s>>>((const uint32_t*)codes, (const uint8_t*)scales, n_groups, (uint32_t)(k / 8), n_terms, out, row_stride);    \
-    } while (0)
+    const uint32_t* c = (const uint32_t*)codes;
+    const uint8_t* e = (const uint8_t*)scales;
+    const uint32_t gpr = (uint32_t)(k / 8);
+#define DSX_GO(DT)                                                                                                                                \
+    return vec ? launch_rows(mxfp4_dequantize_kernel<DT, true, 1>, mxfp4_dequantize_kernel<DT, true, 4>, n_groups, s, c, e, n_groups, gpr, n_terms, out, row_stride) \
+               : launch_rows(mxfp4_dequantize_kernel<DT, false, 1>, mxfp4_dequantize_kernel<DT, false, 4>, n_groups, s, c, e, n_groups, gpr, n_terms, out, row_stride)
     if (dtype == DSX_F32) DSX_GO(DSX_F32);
-    else if (dtype == DSX_BF16) DSX_GO(DSX_BF16);
-    else DSX_GO(DSX_F16);
+    if (dtype == DSX_BF16) DSX_GO(DSX_BF16);
+    DSX_GO(DSX_F16);
 #undef DSX_GO
-    DSX_LAUNCHED();
-    return DSX_OK;
 }
 
 }  // extern "C"
