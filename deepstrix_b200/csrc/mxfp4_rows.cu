@@ -15,7 +15,7 @@
 namespace dsx {
 namespace {
 
-constexpr int kThreads = 256;
+constexpr int kThreads = 128;
 
 // Eight floats -> eight E2M1 codes (round to nearest even, saturating), element i in nibble i.
 __device__ __forceinline__ uint32_t e2m1_encode8(const float (&v)[8]) {
@@ -31,129 +31,129 @@ __device__ __forceinline__ uint32_t e2m1_encode8(const float (&v)[8]) {
     return out;
 }
 
-// Eight consecutive values of a row, as f32.
-template <typename T, bool VEC>
-__device__ __forceinline__ void load8(const T* __restrict__ p, float (&v)[8]) {
+// N consecutive values of a row, as f32, in 16-byte loads where they are aligned.
+template <typename T, bool VEC, int N>
+__device__ __forceinline__ void load_values(const T* __restrict__ p, float (&v)[N]) {
     if constexpr (!VEC) {
 #pragma unroll
-        for (int j = 0; j < 8; j++) v[j] = to_f32(p[j]);
+        for (int j = 0; j < N; j++) v[j] = to_f32(p[j]);
     } else if constexpr (sizeof(T) == 4) {
-        const float4 a = __ldg(reinterpret_cast<const float4*>(p)), b = __ldg(reinterpret_cast<const float4*>(p) + 1);
-        v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
-    } else {
-        const uint4 a = __ldg(reinterpret_cast<const uint4*>(p));
-        const uint32_t w[4] = {a.x, a.y, a.z, a.w};
 #pragma unroll
-        for (int j = 0; j < 4; j++) {
-            const float2 f = unpack2<T>(w[j]);
-            v[2 * j] = f.x; v[2 * j + 1] = f.y;
+        for (int i = 0; i < N / 4; i++) {
+            const float4 a = __ldg(reinterpret_cast<const float4*>(p) + i);
+            v[4 * i] = a.x; v[4 * i + 1] = a.y; v[4 * i + 2] = a.z; v[4 * i + 3] = a.w;
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < N / 8; i++) {
+            const uint4 a = __ldg(reinterpret_cast<const uint4*>(p) + i);
+            const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                const float2 f = unpack2<T>(w[j]);
+                v[8 * i + 2 * j] = f.x; v[8 * i + 2 * j + 1] = f.y;
+            }
         }
     }
 }
-template <typename T, bool VEC>
-__device__ __forceinline__ void store8(T* __restrict__ p, const float (&v)[8]) {
-    if constexpr (!VEC) {
-#pragma unroll
-        for (int j = 0; j < 8; j++) p[j] = from_f32<T>(v[j]);
-    } else if constexpr (sizeof(T) == 4) {
-        reinterpret_cast<float4*>(p)[0] = make_float4(v[0], v[1], v[2], v[3]);
-        reinterpret_cast<float4*>(p)[1] = make_float4(v[4], v[5], v[6], v[7]);
-    } else {
-        *reinterpret_cast<uint4*>(p) = make_uint4(pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3]), pack2<T>(v[4], v[5]), pack2<T>(v[6], v[7]));
-    }
-}
 
-// max |.| of eight values as f32, NaN if one of them is
+// |.| compared with a NaN winning
 __device__ __forceinline__ float abs_max_nan(float a, float b) {
     float r;
     asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(fabsf(a)), "f"(fabsf(b)));
     return r;
 }
-__device__ __forceinline__ float abs_max8(const float (&v)[8]) {
-    return abs_max_nan(abs_max_nan(abs_max_nan(v[0], v[1]), abs_max_nan(v[2], v[3])), abs_max_nan(abs_max_nan(v[4], v[5]), abs_max_nan(v[6], v[7])));
-}
 
-// A lane holds 8 consecutive values, four neighbouring lanes a block of 32: loads are 16 (f32: 32) bytes a lane and coalesced, the
-// block's maximum is two shuffles away, and a warp stores 128 bytes of codes.  Groups of 8 are numbered through all rows, so a
-// short row wastes no lane; K / 8 is a multiple of 4, so a block never straddles two quads.  ITEMS groups a lane are requested before the
-// first is worked on: a full grid (8 blocks of 256 an SM) of one 16-byte load a lane is 32 KB in flight an SM, too little for HBM.
-template <int DT, int TERMS, bool VEC, int ITEMS>
+// A lane holds PER consecutive values -- 8 f32 or 16 of 16 bits, 32 bytes -- so four or two neighbouring lanes make a block of 32: loads
+// are coalesced, the block's maximum is a shuffle or two away, and what a block costs beside its values is shared by as many as registers
+// allow.  Units of PER are numbered through all rows, so a short row wastes no lane; a block never straddles two quads or pairs.  48 KB
+// of loads are in flight an SM; the arithmetic (7 instructions a value and term, 25 a lane and term) is what bounds two and three terms.
+template <int DT> constexpr int kPer = DT == DSX_F32 ? 8 : 16;
+
+template <int DT, int TERMS, bool VEC>
 __global__ void __launch_bounds__(kThreads)
-mxfp4_quantize_kernel(const void* __restrict__ x_, int64_t n_groups, uint32_t groups_per_row, int64_t row_stride, uint32_t* __restrict__ codes,
-                      uint8_t* __restrict__ scales) {
+mxfp4_quantize_kernel(const void* __restrict__ x_, int64_t n_units, uint32_t units_per_row, int64_t row_stride, uint32_t* __restrict__ codes,
+                      uint8_t* __restrict__ scales, int release) {
     using T = typename Elem<DT>::T;
+    constexpr int PER = kPer<DT>, LANES = 32 / PER;   // of a block
     pdl_wait();
-    if (ITEMS == 1) pdl_launch_dependents();   // a small launch leaves room for the next kernel to set itself up
+    if (release) pdl_launch_dependents();   // a small launch leaves room for the next kernel to set itself up
     const T* __restrict__ x = reinterpret_cast<const T*>(x_);
-    const bool dense = row_stride == (int64_t)groups_per_row * 8;
-    // n_groups is a multiple of 4, so the four lanes of a block are in range or out of it together; the mask of a quad
-    const uint32_t quad = 0xFu << (threadIdx.x & 28u);
-    for (int64_t g0 = (int64_t)blockIdx.x * (kThreads * ITEMS) + threadIdx.x; g0 < n_groups; g0 += (int64_t)gridDim.x * (kThreads * ITEMS)) {
-        float v[ITEMS][8];
-#pragma unroll
-        for (int i = 0; i < ITEMS; i++) {
-            const int64_t g = g0 + i * kThreads;
-            int64_t off = g * 8;
-            if (!dense) {
-                const int64_t row = g / groups_per_row;
-                off = row * row_stride + (g - row * groups_per_row) * 8;
-            }
-            if (g < n_groups) load8<T, VEC>(x + off, v[i]);
+    const bool dense = row_stride == (int64_t)units_per_row * PER;
+    // n_units is a multiple of LANES, so the lanes of a block are in range or out of it together; their mask
+    const uint32_t mates = ((1u << LANES) - 1u) << (threadIdx.x & (32u - LANES));
+    for (int64_t g = (int64_t)blockIdx.x * kThreads + threadIdx.x; g < n_units; g += (int64_t)gridDim.x * kThreads) {
+        int64_t off = g * PER;
+        if (!dense) {
+            const int64_t row = g / units_per_row;
+            off = row * row_stride + (g - row * units_per_row) * PER;
         }
+        float v[PER];
+        load_values<T, VEC, PER>(x + off, v);
+        bool bad = false;
 #pragma unroll
-        for (int i = 0; i < ITEMS; i++) {
-            const int64_t g = g0 + i * kThreads;
-            if (g >= n_groups) break;
+        for (int t = 0; t < TERMS; t++) {
+            float m = abs_max_nan(v[0], v[1]);
 #pragma unroll
-            for (int t = 0; t < TERMS; t++) {
-                float m = abs_max8(v[i]);
-                m = abs_max_nan(m, __shfl_xor_sync(quad, m, 1));
-                m = abs_max_nan(m, __shfl_xor_sync(quad, m, 2));
-                const uint32_t amax = __float_as_uint(m);
-                const bool bad = amax >= 0x7F800000u;   // infinite or NaN (whose sign bit is clear behind max.NaN)
-                const int e = min(max((int)(amax >> 23) - 2 + ((amax & 0x7FFFFFu) > 0x400000u ? 1 : 0), 1), 253);
-                const float inv = __uint_as_float((uint32_t)(254 - e) << 23);
+            for (int j = 2; j < PER; j++) m = abs_max_nan(m, v[j]);
+#pragma unroll
+            for (int o = 1; o < LANES; o *= 2) m = abs_max_nan(m, __shfl_xor_sync(mates, m, o));
+            const uint32_t amax = __float_as_uint(m);
+            if (t == 0) bad = amax >= 0x7F800000u;   // infinite or NaN (whose sign bit is clear behind max.NaN)
+            const int e = min(max((int)(amax >> 23) - 2 + ((amax & 0x7FFFFFu) > 0x400000u ? 1 : 0), 1), 253);
+            const float inv = __uint_as_float((uint32_t)(254 - e) << 23), scl = __uint_as_float((uint32_t)e << 23);
+            uint32_t w[PER / 8];
+#pragma unroll
+            for (int i = 0; i < PER / 8; i++) {
                 float sv[8];
 #pragma unroll
-                for (int j = 0; j < 8; j++) sv[j] = v[i][j] * inv;
-                const uint32_t w = bad ? 0u : e2m1_encode8(sv);
-                codes[(int64_t)t * n_groups + g] = w;
-                if ((threadIdx.x & 3u) == 0u) scales[(int64_t)t * (n_groups >> 2) + (g >> 2)] = bad ? 255u : (uint8_t)e;
+                for (int j = 0; j < 8; j++) sv[j] = v[8 * i + j] * inv;
+                const uint32_t c = e2m1_encode8(sv);
+                w[i] = bad ? 0u : c;
                 if (t + 1 < TERMS) {
-                    // value = code * 2^(e - 127): the codes' f32 forms are scaled by 2^-126, hence two exact multiplications
-                    const float scl = __uint_as_float((uint32_t)e << 23);
+                    // value = code * 2^(e - 127): the codes' f32 forms are scaled by 2^-126, hence two exact multiplications.  (In a bad block
+                    // the rest is as bad, and its codes are 0 from here on.)
 #pragma unroll
-                    for (int j = 0; j < 8; j++) v[i][j] = bad ? 0.0f : __fmaf_rn(-e2m1_to_f32(w >> (4 * j)), scl, v[i][j]);   // exact: the residual
+                    for (int j = 0; j < 8; j++) v[8 * i + j] = __fmaf_rn(-e2m1_to_f32(c >> (4 * j)), scl, v[8 * i + j]);   // exact: the residual
                 }
             }
+            uint32_t* to = codes + ((int64_t)t * n_units + g) * (PER / 8);
+            if constexpr (PER == 16) *reinterpret_cast<uint2*>(to) = make_uint2(w[0], w[1]);
+            else *to = w[0];
+            if ((threadIdx.x & (LANES - 1)) == 0) scales[((int64_t)t * n_units + g) / LANES] = bad ? (t == 0 ? 255u : 1u) : (uint8_t)e;
         }
     }
 }
 
+// A lane makes 16 bytes of the result (4 f32 or 8 values of 16 bits), so that a warp's stores are whole sectors; ITEMS of them, whose codes
+// and scales -- a few bytes a lane -- are requested together.
+template <int DT> constexpr int kOut = DT == DSX_F32 ? 4 : 8;
+
 template <int DT, bool VEC, int ITEMS>
 __global__ void __launch_bounds__(kThreads)
-mxfp4_dequantize_kernel(const uint32_t* __restrict__ codes, const uint8_t* __restrict__ scales, int64_t n_groups, uint32_t groups_per_row, int terms,
-                        void* __restrict__ out_, int64_t row_stride) {
+mxfp4_dequantize_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales, int64_t n_units, uint32_t units_per_row, int terms,
+                        void* __restrict__ out_, int64_t row_stride, int release) {
     using T = typename Elem<DT>::T;
+    constexpr int PER = kOut<DT>, LANES = 32 / PER;
     pdl_wait();
-    if (ITEMS == 1) pdl_launch_dependents();
+    if (release) pdl_launch_dependents();
     T* __restrict__ out = reinterpret_cast<T*>(out_);
-    const bool dense = row_stride == (int64_t)groups_per_row * 8;
-    for (int64_t g0 = (int64_t)blockIdx.x * (kThreads * ITEMS) + threadIdx.x; g0 < n_groups; g0 += (int64_t)gridDim.x * (kThreads * ITEMS)) {
-        float v[ITEMS][8];
+    const bool dense = row_stride == (int64_t)units_per_row * PER;
+    for (int64_t g0 = (int64_t)blockIdx.x * (kThreads * ITEMS) + threadIdx.x; g0 < n_units; g0 += (int64_t)gridDim.x * (kThreads * ITEMS)) {
+        float v[ITEMS][PER];
         for (int t = 0; t < terms; t++) {
             uint32_t w[ITEMS], e[ITEMS];
 #pragma unroll
             for (int i = 0; i < ITEMS; i++) {
-                const int64_t g = min(g0 + i * kThreads, n_groups - 1);
-                w[i] = __ldg(codes + (int64_t)t * n_groups + g);
-                e[i] = __ldg(scales + (int64_t)t * (n_groups >> 2) + (g >> 2));
+                const int64_t g = (int64_t)t * n_units + min(g0 + i * kThreads, n_units - 1);
+                w[i] = PER == 8 ? __ldg(reinterpret_cast<const uint32_t*>(codes) + g) : (uint32_t)__ldg(reinterpret_cast<const uint16_t*>(codes) + g);
+                e[i] = __ldg(scales + g / LANES);
             }
 #pragma unroll
             for (int i = 0; i < ITEMS; i++) {
                 const float s = e8m0_value(e[i]);
 #pragma unroll
-                for (int j = 0; j < 8; j++) {
+                for (int j = 0; j < PER; j++) {
                     const float d = e2m1_to_f32(w[i] >> (4 * j)) * s;
                     v[i][j] = t == 0 ? d : v[i][j] + d;
                 }
@@ -162,38 +162,56 @@ mxfp4_dequantize_kernel(const uint32_t* __restrict__ codes, const uint8_t* __res
 #pragma unroll
         for (int i = 0; i < ITEMS; i++) {
             const int64_t g = g0 + i * kThreads;
-            if (g >= n_groups) break;
-            int64_t off = g * 8;
+            if (g >= n_units) break;
+            int64_t off = g * PER;
             if (!dense) {
-                const int64_t row = g / groups_per_row;
-                off = row * row_stride + (g - row * groups_per_row) * 8;
+                const int64_t row = g / units_per_row;
+                off = row * row_stride + (g - row * units_per_row) * PER;
             }
-            store8<T, VEC>(out + off, v[i]);
+            if constexpr (!VEC) {
+#pragma unroll
+                for (int j = 0; j < PER; j++) out[off + j] = from_f32<T>(v[i][j]);
+            } else if constexpr (sizeof(T) == 4) {
+                *reinterpret_cast<float4*>(out + off) = make_float4(v[i][0], v[i][1], v[i][2], v[i][3]);
+            } else {
+                *reinterpret_cast<uint4*>(out + off) = make_uint4(pack2<T>(v[i][0], v[i][1]), pack2<T>(v[i][2], v[i][3]), pack2<T>(v[i][4], v[i][5]),
+                                                                  pack2<T>(v[i][6], v[i][7]));
+            }
         }
     }
 }
 
-// Launches `small` (a group a lane, at most 8 blocks an SM) or, where that would go round more than once, `large` (four groups).
+// A grid of at most `per_sm` blocks an SM.
 template <typename K, typename... A>
-int launch_rows(K small, K large, int64_t n_groups, cudaStream_t s, A... args) {
+int launch_rows(K kernel, int64_t n_threads, int per_sm, cudaStream_t s, A... args) {
     int sms = 0;
     if (int rc = head_sm_count(&sms)) return rc;
-    const int64_t cap = (int64_t)sms * 8, blocks = (n_groups + kThreads - 1) / kThreads;
-    const bool big = blocks > cap;
-    DSX_CUDA(launch_pdl(big ? large : small, dim3((unsigned)(big ? std::min(cap, (blocks + 3) / 4) : blocks)), dim3(kThreads), 0, s, args...));
+    const int64_t cap = (int64_t)sms * per_sm, blocks = (n_threads + kThreads - 1) / kThreads;
+    DSX_CUDA(launch_pdl(kernel, dim3((unsigned)std::min(cap, blocks)), dim3(kThreads), 0, s, args..., blocks <= cap / 4 ? 1 : 0));
     DSX_LAUNCHED();
     return DSX_OK;
 }
 
-template <int DT, bool VEC, int TERMS>
-int launch_quantize(cudaStream_t s, const void* x, int64_t n_groups, uint32_t gpr, int64_t stride, uint32_t* codes, uint8_t* scales) {
-    return launch_rows(mxfp4_quantize_kernel<DT, TERMS, VEC, 1>, mxfp4_quantize_kernel<DT, TERMS, VEC, 4>, n_groups, s, x, n_groups, gpr, stride, codes, scales);
-}
+constexpr int kPerSm = 2048 / kThreads;
+
 template <int DT, bool VEC>
-int launch_quantize_terms(int terms, cudaStream_t s, const void* x, int64_t n_groups, uint32_t gpr, int64_t stride, uint32_t* codes, uint8_t* scales) {
-    if (terms == 1) return launch_quantize<DT, VEC, 1>(s, x, n_groups, gpr, stride, codes, scales);
-    if (terms == 2) return launch_quantize<DT, VEC, 2>(s, x, n_groups, gpr, stride, codes, scales);
-    return launch_quantize<DT, VEC, 3>(s, x, n_groups, gpr, stride, codes, scales);
+int launch_quantize(int terms, cudaStream_t s, const void* x, int64_t rows, int64_t k, int64_t stride, uint32_t* codes, uint8_t* scales) {
+    const int64_t n = rows * (k / kPer<DT>);
+    const uint32_t per_row = (uint32_t)(k / kPer<DT>);
+    if (terms == 1) return launch_rows(mxfp4_quantize_kernel<DT, 1, VEC>, n, kPerSm, s, x, n, per_row, stride, codes, scales);
+    if (terms == 2) return launch_rows(mxfp4_quantize_kernel<DT, 2, VEC>, n, kPerSm, s, x, n, per_row, stride, codes, scales);
+    return launch_rows(mxfp4_quantize_kernel<DT, 3, VEC>, n, kPerSm, s, x, n, per_row, stride, codes, scales);
+}
+
+template <int DT, bool VEC>
+int launch_dequantize(int terms, cudaStream_t s, const uint8_t* codes, const uint8_t* scales, int64_t rows, int64_t k, void* out, int64_t stride) {
+    const int64_t n = rows * (k / kOut<DT>);
+    const uint32_t per_row = (uint32_t)(k / kOut<DT>);
+    int sms = 0;
+    if (int rc = head_sm_count(&sms)) return rc;
+    // four items a lane once there are more than one for every lane of a full grid
+    if (n <= (int64_t)sms * 2048) return launch_rows(mxfp4_dequantize_kernel<DT, VEC, 1>, n, kPerSm, s, codes, scales, n, per_row, terms, out, stride);
+    return launch_rows(mxfp4_dequantize_kernel<DT, VEC, 4>, (n + 3) / 4, kPerSm, s, codes, scales, n, per_row, terms, out, stride);
 }
 
 int check_rows(const char* what, int dtype, int64_t rows, int64_t k, int64_t row_stride, int n_terms) {
@@ -217,12 +235,11 @@ int dsx_mxfp4_quantize(const void* x, int dtype, int64_t rows, int64_t k, int64_
     if (rows == 0) return DSX_OK;
     DSX_REQUIRE(x && codes && scales, "mxfp4_quantize: null argument");
     DSX_REQUIRE(((uintptr_t)x & (dtype_size(dtype) - 1)) == 0 && ((uintptr_t)codes & 15) == 0, "mxfp4_quantize: x must be aligned to its elements, codes to 16 bytes");
-    const int64_t n_groups = rows * (k / 8);
     const bool vec = (((uintptr_t)x | (uintptr_t)(rows > 1 ? row_stride * dtype_size(dtype) : 0)) & 15) == 0;
     const cudaStream_t s = (cudaStream_t)stream;
-#define DSX_GO(DT)                                                                                                                                \
-    return vec ? launch_quantize_terms<DT, true>(n_terms, s, x, n_groups, (uint32_t)(k / 8), row_stride, (uint32_t*)codes, (uint8_t*)scales)        \
-               : launch_quantize_terms<DT, false>(n_terms, s, x, n_groups, (uint32_t)(k / 8), row_stride, (uint32_t*)codes, (uint8_t*)scales)
+#define DSX_GO(DT)                                                                                                        \
+    return vec ? launch_quantize<DT, true>(n_terms, s, x, rows, k, row_stride, (uint32_t*)codes, (uint8_t*)scales)          \
+               : launch_quantize<DT, false>(n_terms, s, x, rows, k, row_stride, (uint32_t*)codes, (uint8_t*)scales)
     if (dtype == DSX_F32) DSX_GO(DSX_F32);
     if (dtype == DSX_BF16) DSX_GO(DSX_BF16);
     DSX_GO(DSX_F16);
@@ -236,15 +253,11 @@ int dsx_mxfp4_dequantize(const void* codes, const void* scales, int64_t rows, in
     DSX_REQUIRE(codes && scales && out, "mxfp4_dequantize: null argument");
     DSX_REQUIRE(((uintptr_t)out & (dtype_size(dtype) - 1)) == 0 && ((uintptr_t)codes & 15) == 0,
                 "mxfp4_dequantize: out must be aligned to its elements, codes to 16 bytes");
-    const int64_t n_groups = rows * (k / 8);
     const bool vec = (((uintptr_t)out | (uintptr_t)(rows > 1 ? row_stride * dtype_size(dtype) : 0)) & 15) == 0;
     const cudaStream_t s = (cudaStream_t)stream;
-    const uint32_t* c = (const uint32_t*)codes;
-    const uint8_t* e = (const uint8_t*)scales;
-    const uint32_t gpr = (uint32_t)(k / 8);
-#define DSX_GO(DT)                                                                                                                                \
-    return vec ? launch_rows(mxfp4_dequantize_kernel<DT, true, 1>, mxfp4_dequantize_kernel<DT, true, 4>, n_groups, s, c, e, n_groups, gpr, n_terms, out, row_stride) \
-               : launch_rows(mxfp4_dequantize_kernel<DT, false, 1>, mxfp4_dequantize_kernel<DT, false, 4>, n_groups, s, c, e, n_groups, gpr, n_terms, out, row_stride)
+#define DSX_GO(DT)                                                                                                                \
+    return vec ? launch_dequantize<DT, true>(n_terms, s, (const uint8_t*)codes, (const uint8_t*)scales, rows, k, out, row_stride)   \
+               : launch_dequantize<DT, false>(n_terms, s, (const uint8_t*)codes, (const uint8_t*)scales, rows, k, out, row_stride)
     if (dtype == DSX_F32) DSX_GO(DSX_F32);
     if (dtype == DSX_BF16) DSX_GO(DSX_BF16);
     DSX_GO(DSX_F16);
