@@ -62,11 +62,26 @@ inline int head_sm_count(int* sms) {
 __device__ __forceinline__ float e8m0_value(uint32_t e) {
     return e == 255u ? __uint_as_float(0x7FC00000u) : (e == 0u ? __uint_as_float(0x00400000u) : __uint_as_float(e << 23));
 }
-// Value of the E2M1 code in the low four bits of n, times 2^-126: two exponent bits and the mantissa bit sit where an f32 has
-// its lowest exponent bits and its highest mantissa bit (code 1 is the f32 subnormal 2^-127, as it is E2M1's own subnormal 0.5).
-__device__ __forceinline__ float e2m1_scaled(uint32_t n) { return __uint_as_float(((n & 7u) << 22) | ((n & 8u) << 28)); }
-// * 2^126, exact; adding +0 turns code 8 (minus zero) into plain zero, as the CPU quantiser's integer table has it, so that the sign of a
-// zero residual -- and with it the code of the next term -- is the same there
-__device__ __forceinline__ float e2m1_to_f32(uint32_t n) { return __fmaf_rn(e2m1_scaled(n), 8.507059173023462e37f, 0.0f); }
+// The codes in nibble k of either half of x as two f16 values: the two exponent bits and the mantissa bit of a code sit where an f16 has its
+// lowest exponent bits and its highest mantissa bit (code 1 is an f16 subnormal there, as it is E2M1's own), so what is left is a factor of 2^14.
+// Four integer instructions a pair.  (The hardware's decoder, cvt.rn.f16x2.e2m1x2, is two instructions shorter, but gave zeros or wrong
+// values inside two kernels of this library although it is right in isolation: CUDA 12.9, sm_100a.)
+template <int K>
+__device__ __forceinline__ float2 e2m1_pair(uint32_t x) {
+    const uint32_t mag = K == 0 ? x << 9 : (K == 1 ? x << 5 : (K == 2 ? x << 1 : x >> 3));
+    const uint32_t sign = K == 0 ? x << 12 : (K == 1 ? x << 8 : (K == 2 ? x << 4 : x));
+    const uint32_t h = (mag & 0x0E000E00u) | (sign & 0x80008000u);
+    return __half22float2(__hmul2(*reinterpret_cast<const __half2*>(&h), __half2half2(__ushort_as_half((unsigned short)0x7400))));   // * 2^14
+}
+// The values of eight codes (element i in nibble i), and of four in the low half of w.  Exact.
+__device__ __forceinline__ void e2m1_values(uint32_t w, float (&d)[8]) {
+    const float2 a = e2m1_pair<0>(w), b = e2m1_pair<1>(w), c = e2m1_pair<2>(w), e = e2m1_pair<3>(w);
+    d[0] = a.x; d[4] = a.y; d[1] = b.x; d[5] = b.y; d[2] = c.x; d[6] = c.y; d[3] = e.x; d[7] = e.y;
+}
+__device__ __forceinline__ void e2m1_values(uint32_t w, float (&d)[4]) {
+    const uint32_t x = __byte_perm(w, 0u, 0x4140);   // byte 0 to the low half, byte 1 to the high one
+    const float2 a = e2m1_pair<0>(x), b = e2m1_pair<1>(x);
+    d[0] = a.x; d[2] = a.y; d[1] = b.x; d[3] = b.y;
+}
 
 }  // namespace dsx

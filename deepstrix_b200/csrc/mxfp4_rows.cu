@@ -111,10 +111,12 @@ mxfp4_quantize_kernel(const void* __restrict__ x_, int64_t n_units, uint32_t uni
                 const uint32_t c = e2m1_encode8(sv);
                 w[i] = bad ? 0u : c;
                 if (t + 1 < TERMS) {
-                    // value = code * 2^(e - 127): the codes' f32 forms are scaled by 2^-126, hence two exact multiplications.  (In a bad block
-                    // the rest is as bad, and its codes are 0 from here on.)
+                    // Adding +0 makes minus zero plain zero, as in the CPU quantiser's integer table: the sign of a zero residual, and with it the
+                    // next term's code, is the same there.  (In a bad block the rest is as bad, and its codes are 0 from here on.)
+                    float d[8];
+                    e2m1_values(c, d);
 #pragma unroll
-                    for (int j = 0; j < 8; j++) v[8 * i + j] = __fmaf_rn(-e2m1_to_f32(c >> (4 * j)), scl, v[8 * i + j]);   // exact: the residual
+                    for (int j = 0; j < 8; j++) v[8 * i + j] = __fmaf_rn(-(d[j] + 0.0f), scl, v[8 * i + j]);   // exact: the residual
                 }
             }
             uint32_t* to = codes + ((int64_t)t * n_units + g) * (PER / 8);
@@ -152,11 +154,10 @@ mxfp4_dequantize_kernel(const uint8_t* __restrict__ codes, const uint8_t* __rest
 #pragma unroll
             for (int i = 0; i < ITEMS; i++) {
                 const float s = e8m0_value(e[i]);
+                float d[PER];
+                e2m1_values(w[i], d);
 #pragma unroll
-                for (int j = 0; j < PER; j++) {
-                    const float d = e2m1_to_f32(w[i] >> (4 * j)) * s;
-                    v[i][j] = t == 0 ? d : v[i][j] + d;
-                }
+                for (int j = 0; j < PER; j++) v[i][j] = t == 0 ? d[j] * s : __fmaf_rn(d[j], s, v[i][j]);   // the product is exact
             }
         }
 #pragma unroll
