@@ -131,9 +131,9 @@ mxfp4_quantize_kernel(const void* __restrict__ x_, int64_t n_units, uint32_t uni
 // and scales -- a few bytes a lane -- are requested together.
 template <int DT> constexpr int kOut = DT == DSX_F32 ? 4 : 8;
 
-template <int DT, bool VEC, int ITEMS>
+template <int DT, int TERMS, bool VEC, int ITEMS>
 __global__ void __launch_bounds__(kThreads)
-mxfp4_dequantize_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales, int64_t n_units, uint32_t units_per_row, int terms,
+mxfp4_dequantize_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales, int64_t n_units, uint32_t units_per_row,
                         void* __restrict__ out_, int64_t row_stride, int release) {
     using T = typename Elem<DT>::T;
     constexpr int PER = kOut<DT>, LANES = 32 / PER;
@@ -142,28 +142,28 @@ mxfp4_dequantize_kernel(const uint8_t* __restrict__ codes, const uint8_t* __rest
     T* __restrict__ out = reinterpret_cast<T*>(out_);
     const bool dense = row_stride == (int64_t)units_per_row * PER;
     for (int64_t g0 = (int64_t)blockIdx.x * (kThreads * ITEMS) + threadIdx.x; g0 < n_units; g0 += (int64_t)gridDim.x * (kThreads * ITEMS)) {
-        float v[ITEMS][PER];
-        for (int t = 0; t < terms; t++) {
-            uint32_t w[ITEMS], e[ITEMS];
+        uint32_t w[ITEMS][TERMS], e[ITEMS][TERMS];
 #pragma unroll
-            for (int i = 0; i < ITEMS; i++) {
+        for (int i = 0; i < ITEMS; i++)
+#pragma unroll
+            for (int t = 0; t < TERMS; t++) {
                 const int64_t g = (int64_t)t * n_units + min(g0 + i * kThreads, n_units - 1);
-                w[i] = PER == 8 ? __ldg(reinterpret_cast<const uint32_t*>(codes) + g) : (uint32_t)__ldg(reinterpret_cast<const uint16_t*>(codes) + g);
-                e[i] = __ldg(scales + g / LANES);
+                w[i][t] = PER == 8 ? __ldg(reinterpret_cast<const uint32_t*>(codes) + g) : (uint32_t)__ldg(reinterpret_cast<const uint16_t*>(codes) + g);
+                e[i][t] = __ldg(scales + g / LANES);
             }
-#pragma unroll
-            for (int i = 0; i < ITEMS; i++) {
-                const float s = e8m0_value(e[i]);
-                float d[PER];
-                e2m1_values(w[i], d);
-#pragma unroll
-                for (int j = 0; j < PER; j++) v[i][j] = t == 0 ? d[j] * s : __fmaf_rn(d[j], s, v[i][j]);   // the product is exact
-            }
-        }
 #pragma unroll
         for (int i = 0; i < ITEMS; i++) {
             const int64_t g = g0 + i * kThreads;
             if (g >= n_units) break;
+            float v[PER];
+#pragma unroll
+            for (int t = 0; t < TERMS; t++) {
+                const float s = e8m0_value(e[i][t]);
+                float d[PER];
+                e2m1_values(w[i][t], d);
+#pragma unroll
+                for (int j = 0; j < PER; j++) v[j] = t == 0 ? d[j] * s : __fmaf_rn(d[j], s, v[j]);   // the product is exact
+            }
             int64_t off = g * PER;
             if (!dense) {
                 const int64_t row = g / units_per_row;
@@ -171,12 +171,11 @@ mxfp4_dequantize_kernel(const uint8_t* __restrict__ codes, const uint8_t* __rest
             }
             if constexpr (!VEC) {
 #pragma unroll
-                for (int j = 0; j < PER; j++) out[off + j] = from_f32<T>(v[i][j]);
+                for (int j = 0; j < PER; j++) out[off + j] = from_f32<T>(v[j]);
             } else if constexpr (sizeof(T) == 4) {
-                *reinterpret_cast<float4*>(out + off) = make_float4(v[i][0], v[i][1], v[i][2], v[i][3]);
+                *reinterpret_cast<float4*>(out + off) = make_float4(v[0], v[1], v[2], v[3]);
             } else {
-                *reinterpret_cast<uint4*>(out + off) = make_uint4(pack2<T>(v[i][0], v[i][1]), pack2<T>(v[i][2], v[i][3]), pack2<T>(v[i][4], v[i][5]),
-                                                                  pack2<T>(v[i][6], v[i][7]));
+                *reinterpret_cast<uint4*>(out + off) = make_uint4(pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3]), pack2<T>(v[4], v[5]), pack2<T>(v[6], v[7]));
             }
         }
     }
@@ -204,15 +203,22 @@ int launch_quantize(int terms, cudaStream_t s, const void* x, int64_t rows, int6
     return launch_rows(mxfp4_quantize_kernel<DT, 3, VEC>, n, kPerSm, s, x, n, per_row, stride, codes, scales);
 }
 
-template <int DT, bool VEC>
-int launch_dequantize(int terms, cudaStream_t s, const uint8_t* codes, const uint8_t* scales, int64_t rows, int64_t k, void* out, int64_t stride) {
+template <int DT, int TERMS, bool VEC>
+int launch_dequantize_terms(cudaStream_t s, const uint8_t* codes, const uint8_t* scales, int64_t rows, int64_t k, void* out, int64_t stride) {
     const int64_t n = rows * (k / kOut<DT>);
     const uint32_t per_row = (uint32_t)(k / kOut<DT>);
     int sms = 0;
     if (int rc = head_sm_count(&sms)) return rc;
-    // four items a lane once there are more than one for every lane of a full grid
-    if (n <= (int64_t)sms * 2048) return launch_rows(mxfp4_dequantize_kernel<DT, VEC, 1>, n, kPerSm, s, codes, scales, n, per_row, terms, out, stride);
-    return launch_rows(mxfp4_dequantize_kernel<DT, VEC, 4>, (n + 3) / 4, kPerSm, s, codes, scales, n, per_row, terms, out, stride);
+    // four items a lane once there are more than one for every lane of a full grid, and more blocks than run at once (65536 x 2048 to bf16: 65 us,
+    // 70 us in a grid of what runs at once; two items 68, one 81)
+    if (n <= (int64_t)sms * 2048) return launch_rows(mxfp4_dequantize_kernel<DT, TERMS, VEC, 1>, n, kPerSm, s, codes, scales, n, per_row, out, stride);
+    return launch_rows(mxfp4_dequantize_kernel<DT, TERMS, VEC, 4>, (n + 3) / 4, 4 * kPerSm, s, codes, scales, n, per_row, out, stride);
+}
+template <int DT, bool VEC>
+int launch_dequantize(int terms, cudaStream_t s, const uint8_t* codes, const uint8_t* scales, int64_t rows, int64_t k, void* out, int64_t stride) {
+    if (terms == 1) return launch_dequantize_terms<DT, 1, VEC>(s, codes, scales, rows, k, out, stride);
+    if (terms == 2) return launch_dequantize_terms<DT, 2, VEC>(s, codes, scales, rows, k, out, stride);
+    return launch_dequantize_terms<DT, 3, VEC>(s, codes, scales, rows, k, out, stride);
 }
 
 int check_rows(const char* what, int dtype, int64_t rows, int64_t k, int64_t row_stride, int n_terms) {
