@@ -77,7 +77,9 @@ mxfp4_quantize_kernel(const void* __restrict__ x_, int64_t n_units, uint32_t uni
     using T = typename Elem<DT>::T;
     constexpr int PER = kPer<DT>, LANES = 32 / PER;   // of a block
     pdl_wait();
-    if (release) pdl_launch_dependents();   // a small launch leaves room for the next kernel to set itself up
+    // A small launch leaves room for the next kernel to set itself up.  What comes after the wait is all this kernel writes, and no kernel of
+    // the library reads codes before its own wait.
+    if (release) pdl_launch_dependents();
     const T* __restrict__ x = reinterpret_cast<const T*>(x_);
     const bool dense = row_stride == (int64_t)units_per_row * PER;
     // n_units is a multiple of LANES, so the lanes of a block are in range or out of it together; their mask
@@ -134,11 +136,10 @@ template <int DT> constexpr int kOut = DT == DSX_F32 ? 4 : 8;
 template <int DT, int TERMS, bool VEC, int ITEMS>
 __global__ void __launch_bounds__(kThreads)
 mxfp4_dequantize_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales, int64_t n_units, uint32_t units_per_row,
-                        void* __restrict__ out_, int64_t row_stride, int release) {
+                        void* __restrict__ out_, int64_t row_stride) {
     using T = typename Elem<DT>::T;
     constexpr int PER = kOut<DT>, LANES = 32 / PER;
-    pdl_wait();
-    if (release) pdl_launch_dependents();
+    pdl_wait();   // and no early release: the result may be router weights, which the router copies before its own wait
     T* __restrict__ out = reinterpret_cast<T*>(out_);
     const bool dense = row_stride == (int64_t)units_per_row * PER;
     for (int64_t g0 = (int64_t)blockIdx.x * (kThreads * ITEMS) + threadIdx.x; g0 < n_units; g0 += (int64_t)gridDim.x * (kThreads * ITEMS)) {
@@ -181,26 +182,26 @@ mxfp4_dequantize_kernel(const uint8_t* __restrict__ codes, const uint8_t* __rest
     }
 }
 
-// A grid of at most `per_sm` blocks an SM.
+constexpr int kPerSm = 2048 / kThreads;   // blocks an SM holds
+
 template <typename K, typename... A>
-int launch_rows(K kernel, int64_t n_threads, int per_sm, cudaStream_t s, A... args) {
-    int sms = 0;
-    if (int rc = head_sm_count(&sms)) return rc;
-    const int64_t cap = (int64_t)sms * per_sm, blocks = (n_threads + kThreads - 1) / kThreads;
-    DSX_CUDA(launch_pdl(kernel, dim3((unsigned)std::min(cap, blocks)), dim3(kThreads), 0, s, args..., blocks <= cap / 4 ? 1 : 0));
+int launch_rows(K kernel, int64_t blocks, cudaStream_t s, A... args) {
+    DSX_CUDA(launch_pdl(kernel, dim3((unsigned)blocks), dim3(kThreads), 0, s, args...));
     DSX_LAUNCHED();
     return DSX_OK;
 }
-
-constexpr int kPerSm = 2048 / kThreads;
 
 template <int DT, bool VEC>
 int launch_quantize(int terms, cudaStream_t s, const void* x, int64_t rows, int64_t k, int64_t stride, uint32_t* codes, uint8_t* scales) {
     const int64_t n = rows * (k / kPer<DT>);
     const uint32_t per_row = (uint32_t)(k / kPer<DT>);
-    if (terms == 1) return launch_rows(mxfp4_quantize_kernel<DT, 1, VEC>, n, kPerSm, s, x, n, per_row, stride, codes, scales);
-    if (terms == 2) return launch_rows(mxfp4_quantize_kernel<DT, 2, VEC>, n, kPerSm, s, x, n, per_row, stride, codes, scales);
-    return launch_rows(mxfp4_quantize_kernel<DT, 3, VEC>, n, kPerSm, s, x, n, per_row, stride, codes, scales);
+    int sms = 0;
+    if (int rc = head_sm_count(&sms)) return rc;
+    const int64_t cap = (int64_t)sms * kPerSm, blocks = std::min(cap, (n + kThreads - 1) / kThreads);
+    const int release = blocks <= cap / 4;
+    if (terms == 1) return launch_rows(mxfp4_quantize_kernel<DT, 1, VEC>, blocks, s, x, n, per_row, stride, codes, scales, release);
+    if (terms == 2) return launch_rows(mxfp4_quantize_kernel<DT, 2, VEC>, blocks, s, x, n, per_row, stride, codes, scales, release);
+    return launch_rows(mxfp4_quantize_kernel<DT, 3, VEC>, blocks, s, x, n, per_row, stride, codes, scales, release);
 }
 
 template <int DT, int TERMS, bool VEC>
@@ -211,8 +212,10 @@ int launch_dequantize_terms(cudaStream_t s, const uint8_t* codes, const uint8_t*
     if (int rc = head_sm_count(&sms)) return rc;
     // four items a lane once there are more than one for every lane of a full grid, and more blocks than run at once (65536 x 2048 to bf16: 65 us,
     // 70 us in a grid of what runs at once; two items 68, one 81)
-    if (n <= (int64_t)sms * 2048) return launch_rows(mxfp4_dequantize_kernel<DT, TERMS, VEC, 1>, n, kPerSm, s, codes, scales, n, per_row, out, stride);
-    return launch_rows(mxfp4_dequantize_kernel<DT, TERMS, VEC, 4>, (n + 3) / 4, 4 * kPerSm, s, codes, scales, n, per_row, out, stride);
+    const int64_t lanes = (int64_t)sms * kPerSm * kThreads;
+    if (n <= lanes) return launch_rows(mxfp4_dequantize_kernel<DT, TERMS, VEC, 1>, (n + kThreads - 1) / kThreads, s, codes, scales, n, per_row, out, stride);
+    const int64_t blocks = std::min<int64_t>((n + 4 * kThreads - 1) / (4 * kThreads), 4 * sms * kPerSm);
+    return launch_rows(mxfp4_dequantize_kernel<DT, TERMS, VEC, 4>, blocks, s, codes, scales, n, per_row, out, stride);
 }
 template <int DT, bool VEC>
 int launch_dequantize(int terms, cudaStream_t s, const uint8_t* codes, const uint8_t* scales, int64_t rows, int64_t k, void* out, int64_t stride) {
@@ -223,8 +226,8 @@ int launch_dequantize(int terms, cudaStream_t s, const uint8_t* codes, const uin
 
 int check_rows(const char* what, int dtype, int64_t rows, int64_t k, int64_t row_stride, int n_terms) {
     DSX_REQUIRE(dtype_ok(dtype), "%s: unknown element type %d", what, dtype);
-    DSX_REQUIRE(rows >= 0 && k >= 32 && k % 32 == 0 && k <= ((int64_t)1 << 30), "%s: %lld rows of %lld columns (a multiple of 32)", what, (long long)rows,
-                (long long)k);
+    DSX_REQUIRE(k >= 32 && k % 32 == 0 && k <= ((int64_t)1 << 30) && rows >= 0 && rows <= ((int64_t)1 << 46) / k,
+                "%s: %lld rows of %lld columns (a multiple of 32, at most 2^30; 2^46 values)", what, (long long)rows, (long long)k);
     DSX_REQUIRE(n_terms >= 1 && n_terms <= 3, "%s: %d terms (1 to 3)", what, n_terms);
     DSX_REQUIRE(row_stride >= k || rows <= 1, "%s: row stride %lld below the %lld columns of a row", what, (long long)row_stride, (long long)k);
     return DSX_OK;

@@ -391,6 +391,35 @@ def test_expert_store_from_float_weights(torch_cuda, moe, oracle):
     st.close()
 
 
+@pytest.mark.parametrize("T", [2, 40])
+def test_router_weights_dequantised_right_before_the_layer(torch_cuda, moe, T):
+    """The layer's router may copy its weights before the kernel ahead of it has ended: what the dequantiser writes is complete all the same."""
+    torch = torch_cuda
+    from deepstrix_b200 import head, synth
+    from deepstrix_b200.config import MoeConfig, RouterConfig
+    cfg = MoeConfig(hidden=512, ffn=256, shared_ffn=256,
+                    router=RouterConfig(n_expert=32, n_used=4, n_group=1, topk_group=1, score_fn=1, route_scale=2.5))
+    w = synth.make_layer(cfg, 4)
+    routers = [head.Mxfp4Quantize.launch(torch.from_numpy(w["router_w"]).cuda().roll(i, 0), 3) for i in range(2)]
+    buffer = torch.empty((32, 512), dtype=torch.float32, device="cuda")
+    store = moe.RoutedExpertWeights.from_host(cfg.fmt, cfg.hidden, cfg.ffn, w["gate"], w["up"], w["down"])
+    shared = moe.RoutedExpertWeights.from_host(cfg.fmt, cfg.hidden, cfg.shared_ffn, w["shared_gate"], w["shared_up"], w["shared_down"])
+    layer = moe.MoeLayer(cfg, store, shared, buffer, torch.from_numpy(w["router_bias"]).cuda(), max_tokens=T)
+    x = torch.from_numpy(synth.make_tokens(cfg, 4, T).view(np.int16)).cuda().view(torch.bfloat16)
+    want = []
+    for q in routers:
+        head.Mxfp4Dequantize.launch(q, torch.float32, out=buffer)
+        torch.cuda.synchronize()
+        want.append(layer.forward(x))
+        torch.cuda.synchronize()
+    assert not torch.equal(want[0], want[1])
+    got = []
+    for i in range(40):
+        head.Mxfp4Dequantize.launch(routers[i % 2], torch.float32, out=buffer)
+        got.append(layer.forward(x))
+    assert all(torch.equal(g, want[i % 2]) for i, g in enumerate(got)) and layer.check() == 0
+
+
 def _head_inputs(torch, T, H, V, seed):
     g = torch.Generator(device="cuda").manual_seed(seed)
     return (torch.randn((T, H), generator=g, device="cuda"), torch.rand((H,), generator=g, device="cuda") + 0.5,
@@ -414,8 +443,7 @@ def test_norm_head_logprobs_together(torch_cuda, moe, T):
     rows, logits, lp, ent, ids, alp = _head_step(torch, moe, x, norm, w, tokens, torch.float32)
     w64 = torch.from_numpy(_values64(w.codes[0].cpu().numpy(), w.scales[0].cpu().numpy())).cuda()
     exact = rows.double() @ w64.T
-    # three terms leave at most 2^-2 of a step each: a value of a block is off by at most 6 / 6 * (1/6)^... -- bounded per block by
-    # (1/4)^3 of its largest magnitude; here the measured norm of the dropped rest, |x - sum of terms|, bounds the logits through Cauchy-Schwarz
+    # what three terms drop, x minus their sum, is measured; Cauchy-Schwarz turns its norm into a bound on the logits
     rest = rows.double() - head.Mxfp4Dequantize.launch(head.Mxfp4Quantize.launch(rows, 3), torch.float32).double()
     slack = rest.norm(dim=1, keepdim=True) * w64.norm(dim=1)[None] + 3 * 2048 * 2.0 ** -23 * (rows.double().abs() @ w64.abs().T) * 1.1
     assert bool(((logits.double() - exact).abs() <= slack).all())
