@@ -553,7 +553,8 @@ extern "C" int dsx_token_logprobs(const void* logits, int dtype, int64_t t, int6
     if (t == 0) return DSX_OK;
     DSX_REQUIRE(row_stride >= v || t == 1, "token_logprobs: row stride %lld below the %lld logits of a row", (long long)row_stride, (long long)v);
     DSX_REQUIRE(logits && (n_given == 0 || (tokens && logprobs)) && (n_alt == 0 || (alts && alt_logprobs)), "token_logprobs: null argument");
-    DSX_REQUIRE(((uintptr_t)logits & (dtype_size(dtype) - 1)) == 0, "token_logprobs: logits must be aligned to their elements");
+    const uintptr_t words = (n_given ? (uintptr_t)tokens | (uintptr_t)logprobs : 0) | (uintptr_t)entropy | (n_alt ? (uintptr_t)alts | (uintptr_t)alt_logprobs : 0);
+    DSX_REQUIRE(((uintptr_t)logits & (dtype_size(dtype) - 1)) == 0 && (words & 3) == 0, "token_logprobs: every array must be aligned to its elements");
     const cudaStream_t s = (cudaStream_t)stream;
 #define DSX_GO(DT) return launch_for<DT>(logits, t, v, row_stride, inv_temperature, tokens, n_given, logprobs, entropy, n_alt, alts, alt_logprobs, s)
     if (dtype == DSX_F32) DSX_GO(DSX_F32);

@@ -617,7 +617,8 @@ mxfp4_matmul_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_con
 
 // Two sizes of block, so that tensor memory is never over-committed by blocks of this kernel that share an SM (a cluster whose
 // blocks wait for tensor memory held by another such cluster could wait for ever): at most 112 KB of shared memory and 256
-// columns (two blocks an SM, a third does not fit beside 77 KB or more), or at least 160 KB (alone on its SM).
+// columns (two blocks an SM, a third does not fit beside 77 KB or more), or at least 160 KB (alone on its SM).  Nor does either fit beside the
+// layer's own kernel of CTA pairs (225 KB); the layer's single-CTA kernels wait for no other block, so they give their columns back.
 constexpr int kSmallMin = 77 * 1024, kSmallMax = 112 * 1024, kLargeMin = 160 * 1024, kLargeMax = 225 * 1024;
 
 struct Plan {
@@ -773,8 +774,9 @@ extern "C" {
 int dsx_mxfp4_matmul(const void* a_codes, const void* a_scales, int n_terms, int64_t m, const void* w_codes, const void* w_scales, int64_t n,
                      int64_t k, void* out, int dtype, int64_t row_stride, dsx_stream_t stream) {
     DSX_REQUIRE(dtype_ok(dtype), "mxfp4_matmul: unknown element type %d", dtype);
-    DSX_REQUIRE(m >= 0 && n >= 0 && k >= 32 && k % 32 == 0 && m < ((int64_t)1 << 22) && n < ((int64_t)1 << 31) && k <= ((int64_t)1 << 30),
-                "mxfp4_matmul: %lld x %lld x %lld (k a multiple of 32)", (long long)m, (long long)n, (long long)k);
+    // 2^24 columns: the longest a wait lasts (a tile's MMAs, 20 ms) stays far inside its limit
+    DSX_REQUIRE(m >= 0 && n >= 0 && k >= 32 && k % 32 == 0 && m < ((int64_t)1 << 22) && n < ((int64_t)1 << 31) && k <= ((int64_t)1 << 24),
+                "mxfp4_matmul: %lld x %lld x %lld (k a multiple of 32, at most 2^24; m below 2^22)", (long long)m, (long long)n, (long long)k);
     DSX_REQUIRE(n_terms >= 1 && n_terms <= 3, "mxfp4_matmul: %d terms (1 to 3)", n_terms);
     if (m == 0 || n == 0) return DSX_OK;
     DSX_REQUIRE(a_codes && a_scales && w_codes && w_scales && out, "mxfp4_matmul: null argument");

@@ -521,14 +521,14 @@ enum dsx_dtype { DSX_F32 = 0, DSX_BF16 = 1, DSX_F16 = 2 };
  * quantize: term 0 holds x, each further term what the earlier ones leave over, per block of 32 with the scale
  * 2^ceil(log2(max|.| / 6)) (byte kept in 1..253) and codes rounded to nearest, ties to even.  Relative error of a row of normal
  * values about 0.11 / 0.013 / 0.0016 for 1 / 2 / 3 terms.  A block holding a NaN or an infinity gets scale byte 255.
- * x: rows of `dtype`, row_stride elements apart; any stride of at least k. */
+ * x: rows of `dtype`, row_stride elements apart; any stride of at least k.  k <= 2^30, rows * k <= 2^46. */
 DSX_API int dsx_mxfp4_quantize(const void* x, int dtype, int64_t rows, int64_t k, int64_t row_stride, int n_terms, void* codes,
                                void* scales, dsx_stream_t stream);
 /* The values the rows stand for: terms added in f32 in order, rounded once to `dtype`. */
 DSX_API int dsx_mxfp4_dequantize(const void* codes, const void* scales, int64_t rows, int64_t k, int n_terms, void* out, int dtype,
                                  int64_t row_stride, dsx_stream_t stream);
 /* out[m, n] = sum over a's terms and k of a[m, k] * w[n, k]; a: n_terms x [m, k], w: one term [n, k]; f32 accumulation, one
- * rounding to `dtype`; rows of out row_stride elements apart (columns past n are left as they are).  m < 2^22. */
+ * rounding to `dtype`; rows of out row_stride elements apart (columns past n are left as they are).  m < 2^22, k <= 2^24. */
 DSX_API int dsx_mxfp4_matmul(const void* a_codes, const void* a_scales, int n_terms, int64_t m, const void* w_codes,
                              const void* w_scales, int64_t n, int64_t k, void* out, int dtype, int64_t row_stride,
                              dsx_stream_t stream);
@@ -542,7 +542,7 @@ DSX_API int dsx_head_check(dsx_stream_t stream, uint32_t* error_word);
  *   alt_logprobs f32 [t, n_alt]    their log probabilities
  * A logit of -inf is masked: no weight, never an alternative (ids run out as -1 with -inf).  A row that is masked as a whole:
  * logprobs -inf, entropy 0, ids -1.  A row that holds a NaN or +inf: every number NaN (tokens outside [0, v): -inf), ids -1.
- * n_given <= 1024, n_alt <= 32. */
+ * t < 2^28, n_given <= 1024, n_alt <= 32, inv_temperature in 1e-6 .. 1e6. */
 DSX_API int dsx_token_logprobs(const void* logits, int dtype, int64_t t, int64_t v, int64_t row_stride, float inv_temperature,
                                const int32_t* tokens, int n_given, float* logprobs, float* entropy, int n_alt, int32_t* alts,
                                float* alt_logprobs, dsx_stream_t stream);

@@ -62,6 +62,17 @@ def test_logprobs_refusals(moe):
     assert "aligned" in f(x=ODD)
 
 
+def test_refused_sizes_and_alignments(moe):
+    """Sizes whose products would pass 64 bits, rows longer than a wait is meant to last, arrays that are not aligned to their elements."""
+    assert "values" in _refused(moe, "dsx_mxfp4_quantize", P, F32, L(1 << 58), L(64), L(64), 1, P, P, N)
+    assert "values" in _refused(moe, "dsx_mxfp4_dequantize", P, P, L(1 << 58), L(64), 1, P, F32, L(64), N)
+    assert "2^24" in _refused(moe, "dsx_mxfp4_matmul", P, P, 1, L(1), P, P, L(8), L((1 << 24) + 32), P, F32, L(8), N)
+    arrays = [P, P, P, P, P]
+    for i in range(5):
+        tok, lp, ent, ids, alp = arrays[:i] + [ODD] + arrays[i + 1:]
+        assert "aligned" in _refused(moe, "dsx_token_logprobs", P, F32, L(2), L(100), L(100), C.c_float(1.0), tok, 1, lp, ent, 1, ids, alp, N)
+
+
 def test_nothing_to_do_is_not_an_error(moe):
     lib = moe.lib()
     assert lib.dsx_mxfp4_quantize(N, BF16, L(0), L(64), L(64), 1, N, N, N) == 0
