@@ -369,8 +369,9 @@ mxfp4_matmul_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_con
     } else if (warp == 1) {
         // ------------------------------------------------------------- MMA issue
         // The whole warp walks the loop and one lane issues, under a predicate: the instruction takes its operands from uniform registers, and
-        // inside a branch of one lane each of them had to be carried there first -- 230 clocks an MMA, whatever its size.  Everything between the
-        // MMAs counts: this warp's instructions, not the tensor core, bound the loop.
+        // inside a branch of one lane each of them had to be carried there first -- 230 clocks an MMA, whatever its size, against 50.  This
+        // warp bounds large products: a pair's stage takes it 580 clocks (four MMAs 200, a satisfied wait 80 each, a commit 35) with MMAs of
+        // N = 208, which run 424, as of N = 16, with and without the copies and the scales.  Two warps that took turns were no faster.
         const uint32_t leader = lane == 0 ? 1u : 0u;
         uint32_t s = 0, ph = 0, t = 0, v = 0, vph = 0;
         const uint64_t d0 = operand_desc(sbase);
@@ -385,11 +386,9 @@ mxfp4_matmul_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_con
             uint32_t started = 0u;
             mbar_wait_on(bar(ACC_EMPTY) + 8u * b, ((t >> 1) & 1u) ^ 1u, abort_flag);
             tc_fence_after();
-            // one stage, the slot's first or second half
-            auto stage = [&](int kc, int h) {
-                mbar_wait_on(bar(FULL) + 8u * s, ph, abort_flag);
-                tc_fence_after();
-                const uint32_t a_lo = lo0 + s * stage_step, b_lo = a_lo + (kWBytes >> 4), sc = slots + v * slot_cols;
+            // the MMAs of one stage, the slot's first or second half
+            auto stage = [&](uint32_t at, int kc, int h) {
+                const uint32_t a_lo = lo0 + at * stage_step, b_lo = a_lo + (kWBytes >> 4), sc = slots + v * slot_cols;
                 auto step = [&](int ks) {
                     const uint32_t k = 2u * (uint32_t)h + (uint32_t)(ks >> 1);
 #pragma unroll
@@ -408,13 +407,27 @@ mxfp4_matmul_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_con
                         if (ks < steps) step(ks);
                 }
                 started = 1u;
-                tc_commit<PAIR>(leader, bar(EMPTY) + 8u * s);
-                if (++s == (uint32_t)g.stages) { s = 0; ph ^= 1u; }
             };
-            for (int kc = kc0; kc < kc1;) {
+            for (int kc = kc0; kc < kc1;) {   // a slot of scales at a time: its waits first, then the MMAs of both stages
                 mbar_wait_on(bar(SLOT_FULL) + 8u * v, vph, abort_flag);
-                if ((kc & 1) == 0) stage(kc++, 0);
-                if ((kc & 1) != 0 && kc < kc1) stage(kc++, 1);
+                mbar_wait_on(bar(FULL) + 8u * s, ph, abort_flag);
+                const uint32_t s0 = s;
+                if (++s == (uint32_t)g.stages) { s = 0; ph ^= 1u; }
+                if ((kc & 1) == 0 && kc + 1 < kc1) {
+                    mbar_wait_on(bar(FULL) + 8u * s, ph, abort_flag);
+                    tc_fence_after();
+                    stage(s0, kc, 0);
+                    tc_commit<PAIR>(leader, bar(EMPTY) + 8u * s0);
+                    stage(s, kc + 1, 1);
+                    tc_commit<PAIR>(leader, bar(EMPTY) + 8u * s);
+                    if (++s == (uint32_t)g.stages) { s = 0; ph ^= 1u; }
+                    kc += 2;
+                } else {
+                    tc_fence_after();
+                    stage(s0, kc, kc & 1);
+                    tc_commit<PAIR>(leader, bar(EMPTY) + 8u * s0);
+                    kc++;
+                }
                 tc_commit<PAIR>(leader, bar(SLOT_EMPTY) + 8u * v);
                 if (++v == (uint32_t)g.slots) { v = 0; vph ^= 1u; }
             }
