@@ -8,6 +8,9 @@
 // the nearest E2M1 value (ties to the even code), and the next term does the same with what is left over, r - value.  Every step
 // is exact in f32, so the bytes can be restated on a CPU.  A block with a NaN or an infinity is NaN as a whole: its first
 // scale byte is 255 (E8M0's NaN), its codes are 0, and its later terms are 0.
+//
+// Both directions are bound by HBM where there is one term (65536 x 2048 f32: 88.7 us to codes, 6.85 TB/s, 97 us back, 6.25; bf16 52 and 54 us),
+// by arithmetic for more (8192 x 4096 bf16: 13.6 and 12.9 us with one term, 35.8 and 28.7 with three), and by latency below a megabyte (2 us).
 #include <algorithm>
 
 #include "head.cuh"
