@@ -26,6 +26,7 @@ namespace {
 
 constexpr int kMaxAlt = 32;            // one per lane of the warp that holds a list
 constexpr int kMaxCluster = 8;
+constexpr int kMaxGiven = 1024;
 constexpr float kLowest = -3.402823466e38f;
 constexpr uint32_t kFloor = 0x00800000u;   // order_of(kLowest): nothing finite is below it
 constexpr float kLn2 = 0.6931471805599453f, kLog2e = 1.4426950408889634f;
@@ -162,29 +163,27 @@ struct alignas(16) Shared {
     float warp_m[kWarps], warp_s[kWarps], warp_u[kWarps];
     alignas(16) uint32_t group_top[NT / 2];       // order of the maxima of pairs of threads, 0 where they saw nothing
     uint32_t warp_least[NT / 64];        // their smallest is the order of a value that n_alt logits of the row's part reach
-    uint32_t readers[kWarps];               // lanes whose chunks are read again
-    int reader[NT];                   // and their threads, in order
+    int n_readers;                          // threads whose chunks are read again,
+    int reader[NT];                         // in any order
     int count;                              // candidates that reach it
     int pending[kWarps];                    // second pass: candidates on the warps' lists,
     uint64_t warp_list[kWarps][96];         // at most 31 left over and two of every lane
     alignas(16) uint64_t list[kList + 2];
     uint64_t best[kMaxAlt];                 // the part's best, descending, 0 = nothing
     float block_sums[3];
-    float stats[2];                         // the row's m and ln s
+    float given[kMaxGiven];                 // logits of the given tokens
 };
 
 // best[0 .. n_alt) = the n_alt largest of the n keys of `list`, descending: a key's place is the number of larger ones (keys are
-// distinct but for 0, "nothing", which takes no place).  Keys are read two at a time; list[n] is written.
+// distinct but for 0, "nothing", which takes no place).  Keys are read two at a time; what lies behind an odd end is not counted.
 template <int NT>
-__device__ __forceinline__ void rank_list(uint64_t* list, int n, int n_alt, uint64_t* best) {
-    if (threadIdx.x == 0) list[n] = 0ull;   // the other half of the last pair
-    __syncthreads();
+__device__ __forceinline__ void rank_list(const uint64_t* list, int n, int n_alt, uint64_t* best) {
     for (int i = threadIdx.x; i < n; i += NT) {
         const uint64_t k = list[i];
         int r = 0;
         for (int j = 0; j < n; j += 2) {
             const ulonglong2 o = *reinterpret_cast<const ulonglong2*>(list + j);
-            r += (o.x > k ? 1 : 0) + (o.y > k ? 1 : 0);
+            r += (o.x > k ? 1 : 0) + (o.y > k && j + 1 < n ? 1 : 0);
         }
         if (k != 0ull && r < n_alt) best[r] = k;
     }
@@ -234,6 +233,11 @@ token_logprobs_kernel(const void* __restrict__ logits, int64_t V, int64_t row_st
         const uint64_t c2 = pair(c, c);
         uint32_t next[8];
         if (first < n_chunks) load_chunk(chunks + first * kChunk, next);
+        if (rank == 0)   // two dependent loads that the first chunk's latency covers
+            for (int g = threadIdx.x; g < n_given; g += kThreads) {
+                const int32_t tok = tokens[row * n_given + g];
+                sh.given[g] = tok >= 0 && tok < V ? to_f32(x[tok]) : 0.0f;
+            }
         for (int64_t ch = first; ch < n_chunks; ch += step) {
             uint32_t w[8];
 #pragma unroll
@@ -281,6 +285,7 @@ token_logprobs_kernel(const void* __restrict__ logits, int64_t V, int64_t row_st
         }
         if (threadIdx.x == 0) {
             sh.count = 0;
+            sh.n_readers = 0;
         }
         if (threadIdx.x < kMaxAlt) sh.best[threadIdx.x] = 0ull;
         __syncthreads();
@@ -342,19 +347,16 @@ token_logprobs_kernel(const void* __restrict__ logits, int64_t V, int64_t row_st
             if (v >= least) push(v, extra_at);
         }
         const uint32_t again = __ballot_sync(0xFFFFFFFFu, a.s != 0.0f && a.m >= least);
-        if (lane == 0) sh.readers[warp] = again;
-        __syncthreads();
-        int n_readers = 0, place = 0;
-#pragma unroll
-        for (int w = 0; w < kWarps; w++) {
-            if (w == warp) place = n_readers;
-            n_readers += __popc(sh.readers[w]);
+        if (again) {
+            int place = 0;
+            if (lane == 0) place = atomicAdd(&sh.n_readers, __popc(again));
+            place = __shfl_sync(0xFFFFFFFFu, place, 0);
+            if ((again >> lane) & 1u) sh.reader[place + __popc(again & ((1u << lane) - 1u))] = (int)threadIdx.x;
         }
-        if ((again >> lane) & 1u) sh.reader[place + __popc(again & ((1u << lane) - 1u))] = (int)threadIdx.x;
         __syncthreads();
         // their chunks, shared out over the block: round r of reader i is item i * rounds + r
         const int64_t part = (int64_t)rank * kThreads;
-        const uint32_t rounds = n_chunks > part ? (uint32_t)((n_chunks - part + step - 1) / step) : 0u, items = (uint32_t)n_readers * rounds;
+        const uint32_t rounds = n_chunks > part ? (uint32_t)((n_chunks - part + step - 1) / step) : 0u, items = (uint32_t)sh.n_readers * rounds;
         for (uint32_t item = threadIdx.x; item < items; item += kThreads) {
             const uint32_t i = item / rounds;
             const int64_t ch = part + sh.reader[i] + (int64_t)(item - i * rounds) * step;
@@ -426,6 +428,7 @@ token_logprobs_kernel(const void* __restrict__ logits, int64_t V, int64_t row_st
             flush(true);
             __syncthreads();
             sh.list[threadIdx.x] = mine;   // 256 of them
+            __syncthreads();
             rank_list<NT>(sh.list, kThreads, n_alt, sh.best);
         }
     }
@@ -466,36 +469,28 @@ token_logprobs_kernel(const void* __restrict__ logits, int64_t V, int64_t row_st
                     asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(k) : "r"(at) : "memory");
                     sh.list[i] = k;
                 }
+                __syncthreads();
                 rank_list<NT>(sh.list, splits * n_alt, n_alt, sh.best);
                 __syncthreads();
             }
         }
     }
-    if (rank == 0) {
+    if (rank == 0 && warp == 0) {
         // s: NaN where the row holds a NaN or +inf, 0 where it is masked as a whole
         const float nan = __uint_as_float(0x7FC00000u);
-        if (warp == 0) {
-            const bool bad = s != s, empty = s == 0.0f;
-            const float log_s = empty ? 0.0f : logf(s);
-            m = bad ? nan : (empty ? 0.0f : m);
-            if (lane == 0) {
-                sh.stats[0] = m;
-                sh.stats[1] = log_s;
-                if (entropy != nullptr) entropy[row] = bad ? nan : (empty ? 0.0f : log_s - kLn2 * (u / s));
-            }
-            if (lane < n_alt) {
-                const uint64_t k = sh.best[lane];
-                const bool none = bad || k == 0ull;
-                alts[row * n_alt + lane] = none ? -1 : (int32_t)~(uint32_t)k;
-                alt_logprobs[row * n_alt + lane] = bad ? nan : (none ? -INFINITY : (value_of((uint32_t)(k >> 32)) - m) * scale - log_s);
-            }
+        const bool bad = s != s, empty = s == 0.0f;
+        const float log_s = empty ? 0.0f : logf(s);
+        m = bad ? nan : (empty ? 0.0f : m);
+        if (lane == 0 && entropy != nullptr) entropy[row] = bad ? nan : (empty ? 0.0f : log_s - kLn2 * (u / s));
+        if (lane < n_alt) {
+            const uint64_t k = sh.best[lane];
+            const bool none = bad || k == 0ull;
+            alts[row * n_alt + lane] = none ? -1 : (int32_t)~(uint32_t)k;
+            alt_logprobs[row * n_alt + lane] = bad ? nan : (none ? -INFINITY : (value_of((uint32_t)(k >> 32)) - m) * scale - log_s);
         }
-        if (n_given > 0) {
-            __syncthreads();
-            for (int g = threadIdx.x; g < n_given; g += kThreads) {
-                const int32_t tok = tokens[row * n_given + g];
-                logprobs[row * n_given + g] = tok >= 0 && tok < V ? (to_f32(x[tok]) - sh.stats[0]) * scale - sh.stats[1] : -INFINITY;
-            }
+        for (int g = lane; g < n_given; g += 32) {
+            const int32_t tok = tokens[row * n_given + g];
+            logprobs[row * n_given + g] = tok >= 0 && tok < V ? (sh.given[g] - m) * scale - log_s : -INFINITY;
         }
     }
     // nobody's shared memory goes away while the first block reads it
@@ -550,7 +545,7 @@ extern "C" int dsx_token_logprobs(const void* logits, int dtype, int64_t t, int6
                                   int n_given, float* logprobs, float* entropy, int n_alt, int32_t* alts, float* alt_logprobs, dsx_stream_t stream) {
     DSX_REQUIRE(dtype_ok(dtype), "token_logprobs: unknown element type %d", dtype);
     DSX_REQUIRE(t >= 0 && t <= 0x0FFFFFFF && v >= 1 && v <= 0x7FFFFFFF, "token_logprobs: %lld rows of %lld logits", (long long)t, (long long)v);
-    DSX_REQUIRE(n_given >= 0 && n_given <= 1024 && n_alt >= 0 && n_alt <= kMaxAlt, "token_logprobs: %d given tokens (at most 1024), %d alternatives (at most 32)",
+    DSX_REQUIRE(n_given >= 0 && n_given <= kMaxGiven && n_alt >= 0 && n_alt <= kMaxAlt, "token_logprobs: %d given tokens (at most 1024), %d alternatives (at most 32)",
                 n_given, n_alt);
     DSX_REQUIRE(inv_temperature >= 1.0e-6f && inv_temperature <= 1.0e6f, "token_logprobs: inverse temperature %g (1e-6 to 1e6)", inv_temperature);
     if (t == 0) return DSX_OK;
