@@ -493,8 +493,12 @@ token_logprobs_kernel(const void* __restrict__ logits, int64_t V, int64_t row_st
             logprobs[row * n_given + g] = tok >= 0 && tok < V ? (sh.given[g] - m) * scale - log_s : -INFINITY;
         }
     }
-    // nobody's shared memory goes away while the first block reads it
-    if (splits > 1) cluster_sync_all();
+    // Nobody's shared memory goes away while the first block reads it (what it read has gone into its stores by then; a release would
+    // wait for those).
+    if (splits > 1) {
+        __syncwarp();
+        asm volatile("barrier.cluster.arrive.relaxed.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+    }
 }
 
 template <int DT, int NT>

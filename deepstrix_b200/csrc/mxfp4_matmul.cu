@@ -204,14 +204,19 @@ __device__ __forceinline__ uint32_t map_to_cta(uint32_t saddr, uint32_t cta) {
     asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(saddr), "r"(cta));
     return r;
 }
-__device__ __forceinline__ float ld_cluster_f32(uint32_t addr) {
-    float v;
-    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+__device__ __forceinline__ float4 ld_cluster_f32x4(uint32_t addr) {
+    float4 v;
+    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
     return v;
 }
 __device__ __forceinline__ void cluster_sync_all() {
     __syncwarp();   // the .aligned forms want the warp together, whatever branch came before
     asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// The same where nothing written is read behind it: a release would wait for the stores of results, most of a microsecond.
+__device__ __forceinline__ void cluster_sync_relaxed() {
+    __syncwarp();
+    asm volatile("barrier.cluster.arrive.relaxed.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 // K-major operand tile of 128-byte rows, 128-byte swizzle: 8-row groups of 1024 bytes.
 __device__ __forceinline__ uint64_t operand_desc(uint32_t saddr) {
@@ -331,7 +336,7 @@ mxfp4_matmul_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_con
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = *(volatile uint32_t*)s_misc;
-    if constexpr (PAIR) cluster_sync_all();   // both CTAs' barriers exist before either signals the other
+    if constexpr (PAIR) cluster_sync_relaxed();   // both CTAs' barriers exist before either signals the other
     pdl_wait();   // the operands may come from the kernel before this one
 
     const int half = PAIR ? (int)cluster_ctarank() : 0;   // of a pair
@@ -610,20 +615,34 @@ mxfp4_matmul_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_con
     tc_fence_before();
     __syncthreads();
     if (threadIdx.x == 0 && *abort_flag) atomicOr(&g_head_error, 1u);
-    if constexpr (PAIR) cluster_sync_all();   // neither CTA's shared or tensor memory goes away while the other may still use it
+    if constexpr (PAIR) cluster_sync_relaxed();   // neither CTA's shared or tensor memory goes away while the other may still use it
     if (!PAIR && g.splits > 1) {
         cluster_sync_all();
         // CTA `rank` adds the tokens rank, rank + splits, ... of all partial tiles, in rank order
         const int64_t w0 = (int64_t)(tile0 % g.tiles_w) * kWRows, m0 = (int64_t)(tile0 / g.tiles_w) * tokens;
-        const int r = threadIdx.x & 127;
-        for (int c = rank + g.splits * (int)(threadIdx.x >> 7); c < tokens; c += g.splits * (kThreads / 128)) {
-            if (m0 + c >= g.M || w0 + r >= g.N) continue;
-            const uint32_t at = sbase + (uint32_t)(c * kWRows + r) * 4u;
-            float sum = 0.0f;
-            for (int p = 0; p < g.splits; p++) sum += ld_cluster_f32(map_to_cta(at, (uint32_t)p));
-            reinterpret_cast<T*>(g.out)[(m0 + c) * g.row_stride + w0 + r] = from_f32<T>(sum);
+        // (a warp a token, four columns a lane; the parts are requested together)
+        for (int c = rank + g.splits * warp; c < tokens && m0 + c < g.M; c += g.splits * (kThreads / 32)) {
+            const uint32_t at = sbase + (uint32_t)(c * kWRows + lane * 4) * 4u;
+            float4 part[8], sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+            for (int p = 0; p < 8; p++)
+                if (p < g.splits) part[p] = ld_cluster_f32x4(map_to_cta(at, (uint32_t)p));
+#pragma unroll
+            for (int p = 0; p < 8; p++)
+                if (p < g.splits) {
+                    sum.x += part[p].x;
+                    sum.y += part[p].y;
+                    sum.z += part[p].z;
+                    sum.w += part[p].w;
+                }
+            const int64_t n = w0 + lane * 4;
+            T* o = reinterpret_cast<T*>(g.out) + (m0 + c) * g.row_stride + n;
+            if (n < g.N) o[0] = from_f32<T>(sum.x);
+            if (n + 1 < g.N) o[1] = from_f32<T>(sum.y);
+            if (n + 2 < g.N) o[2] = from_f32<T>(sum.z);
+            if (n + 3 < g.N) o[3] = from_f32<T>(sum.w);
         }
-        cluster_sync_all();   // nobody's shared memory goes away while another CTA reads it
+        cluster_sync_relaxed();   // nobody's shared memory goes away while another CTA reads it (what it read has gone into its stores)
     }
     if (warp == 1) {
         __syncwarp();
