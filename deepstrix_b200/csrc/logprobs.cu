@@ -26,7 +26,7 @@ namespace {
 
 constexpr int kMaxAlt = 32;            // one per lane of the warp that holds a list
 constexpr int kMaxCluster = 8;
-constexpr int kMaxGiven = 1024;
+constexpr int kMaxGiven = 1024, kFetched = 64;   // given tokens of a row; of which are fetched ahead
 constexpr float kLowest = -3.402823466e38f;
 constexpr uint32_t kFloor = 0x00800000u;   // order_of(kLowest): nothing finite is below it
 constexpr float kLn2 = 0.6931471805599453f, kLog2e = 1.4426950408889634f;
@@ -80,6 +80,12 @@ __device__ __forceinline__ uint64_t merge32(uint64_t a, uint64_t b, int lane) {
 __device__ __forceinline__ void cluster_sync_all() {
     __syncwarp();   // the .aligned forms want the warp together, whatever branch came before
     asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// where the first block of the cluster has `p`
+__device__ __forceinline__ uint32_t in_first_block(const void* p) {
+    uint32_t r;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(r) : "r"((uint32_t)__cvta_generic_to_shared(p)));
+    return r;
 }
 
 // Two f32 in one register pair.
@@ -160,18 +166,19 @@ constexpr int kList = 512;   // candidates the block ranks by counting
 template <int NT>
 struct alignas(16) Shared {
     static constexpr int kWarps = NT / 32;
+    alignas(16) uint32_t group_top[32];     // order of the maxima of 32 groups of threads, 0 where they saw nothing
     float warp_m[kWarps], warp_s[kWarps], warp_u[kWarps];
-    alignas(16) uint32_t group_top[NT / 2];       // order of the maxima of pairs of threads, 0 where they saw nothing
-    uint32_t warp_least[NT / 64];        // their smallest is the order of a value that n_alt logits of the row's part reach
-    int n_readers;                          // threads whose chunks are read again,
+    int n_readers;                          // threads whose maximum reaches the threshold,
     int reader[NT];                         // in any order
     int count;                              // candidates that reach it
     int pending[kWarps];                    // second pass: candidates on the warps' lists,
     uint64_t warp_list[kWarps][96];         // at most 31 left over and two of every lane
     alignas(16) uint64_t list[kList + 2];
+    alignas(16) uint64_t cluster_list[NT == 64 ? 2 : kMaxCluster * kMaxAlt];   // first block of a cluster: the bests of all blocks,
+    float sums[kMaxCluster][3];                                 // and their sums
     uint64_t best[kMaxAlt];                 // the part's best, descending, 0 = nothing
-    float block_sums[3];
-    float given[kMaxGiven];                 // logits of the given tokens
+    float given[kFetched];                  // logits of the first given tokens
+    bool outside[kFetched];                 // no such token
 };
 
 // best[0 .. n_alt) = the n_alt largest of the n keys of `list`, descending: a key's place is the number of larger ones (keys are
@@ -207,16 +214,17 @@ token_logprobs_kernel(const void* __restrict__ logits, int64_t V, int64_t row_st
     const int64_t row = blockIdx.x / (unsigned)splits;
     const float c = scale * kLog2e;
     const T* __restrict__ x = reinterpret_cast<const T*>(logits) + row * row_stride;
+    if (splits > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");   // this block has started; waited for behind the loop
     pdl_wait();   // the logits may come from the kernel before this one
     // whole 16-byte words from the row's first aligned element on; the few elements before and after them one by one
     const int head = (int)min((int64_t)(((16u - (uint32_t)((uintptr_t)x & 15u)) & 15u) / sizeof(T)), V);
-    const int64_t n_chunks = (V - head) / kChunk;
-    const int64_t body = head + n_chunks * kChunk;
+    const uint32_t n_chunks = (uint32_t)((V - head) / kChunk);   // below 2^28
+    const int64_t body = head + (int64_t)n_chunks * kChunk;
     const int extra = rank == 0 ? head + (int)(V - body) : 0;          // fewer than 8 + kChunk, one a lane of the first block's first warp
-    const int64_t extra_at = lane < head ? lane : body + (lane - head);
+    const uint32_t extra_at = lane < head ? (uint32_t)lane : (uint32_t)body + (uint32_t)(lane - head);
     const bool has_extra = warp == 0 && lane < extra;
     // chunk i of this thread is first + i * step
-    const int64_t step = (int64_t)kThreads * splits, first = (int64_t)rank * kThreads + threadIdx.x;
+    const uint32_t step = (uint32_t)(kThreads * splits), part = (uint32_t)(rank * kThreads), first = part + threadIdx.x;
     const T* chunks = x + head;
 
     // ------------------------------------------------------------------ sums
@@ -232,17 +240,19 @@ token_logprobs_kernel(const void* __restrict__ logits, int64_t V, int64_t row_st
         uint64_t s2 = pair(a.s, 0.0f), u2 = pair(a.u, 0.0f);
         const uint64_t c2 = pair(c, c);
         uint32_t next[8];
-        if (first < n_chunks) load_chunk(chunks + first * kChunk, next);
+        if (first < n_chunks) load_chunk(chunks + (int64_t)first * kChunk, next);
         if (rank == 0)   // two dependent loads that the first chunk's latency covers
-            for (int g = threadIdx.x; g < n_given; g += kThreads) {
+            for (int g = threadIdx.x; g < min(n_given, kFetched); g += kThreads) {
                 const int32_t tok = tokens[row * n_given + g];
-                sh.given[g] = tok >= 0 && tok < V ? to_f32(x[tok]) : 0.0f;
+                const bool in = tok >= 0 && tok < V;
+                sh.given[g] = in ? to_f32(x[tok]) : 0.0f;
+                sh.outside[g] = !in;
             }
-        for (int64_t ch = first; ch < n_chunks; ch += step) {
+        for (uint32_t ch = first; ch < n_chunks; ch += step) {
             uint32_t w[8];
 #pragma unroll
             for (int j = 0; j < 8; j++) w[j] = next[j];
-            if (ch + step < n_chunks) load_chunk(chunks + (ch + step) * kChunk, next);   // requested before this one's work
+            if (ch + step < n_chunks) load_chunk(chunks + (int64_t)(ch + step) * kChunk, next);   // requested before this one's work
             const float top = Ch::top(w);
             if (top > a.m) {
                 const float t = fmaxf((a.m - top) * c, -200.0f), e = exp2_fast(t);
@@ -271,105 +281,100 @@ token_logprobs_kernel(const void* __restrict__ logits, int64_t V, int64_t row_st
         a.u = u0 + u1;
     }
 
-    // block: the maximum first, then the sums relative to it, always in the same order
+    // A warp's sums, and the maxima of 32 groups of threads.  All sums are added in an order that does not depend on timing.
+    __syncwarp();
+    if (splits > 1) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");   // every block of the cluster has started
     {
-        const bool none = a.s == 0.0f;
-        uint32_t top = none ? 0u : order_of(a.m);
         float m = a.m;
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, o));
-        if (lane == 0) sh.warp_m[warp] = m;
-        if (n_alt > 0) {
-            top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, 1));
-            if ((lane & 1) == 0) sh.group_top[threadIdx.x >> 1] = top;
-        }
-        if (threadIdx.x == 0) {
-            sh.count = 0;
-            sh.n_readers = 0;
-        }
-        if (threadIdx.x < kMaxAlt) sh.best[threadIdx.x] = 0ull;
-        __syncthreads();
-        float bm = sh.warp_m[0];
+        uint32_t top = a.s == 0.0f ? 0u : order_of(a.m);
 #pragma unroll
-        for (int w = 1; w < kWarps; w++) bm = fmaxf(bm, sh.warp_m[w]);
+        for (int o = kWarps / 2; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
+        if (threadIdx.x % kWarps == 0) sh.group_top[threadIdx.x / kWarps] = top;
         Sums r = a;
-        r.raise(bm, c);
+        r.raise(m, c);
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) {
             r.s += __shfl_xor_sync(0xFFFFFFFFu, r.s, o);
             r.u += __shfl_xor_sync(0xFFFFFFFFu, r.u, o);
         }
         if (lane == 0) {
+            sh.warp_m[warp] = m;
             sh.warp_s[warp] = r.s;
             sh.warp_u[warp] = r.u;
         }
-        // the n_alt-th largest of the pairs' maxima = the smallest that fewer than n_alt of them are above
-        if (n_alt > 0 && threadIdx.x < kThreads / 2) {
-            const uint32_t mine = sh.group_top[threadIdx.x];
-            int above = 0;
-#pragma unroll 8
-            for (int j = 0; j < kThreads / 8; j++) {
-                const uint4 o = reinterpret_cast<const uint4*>(sh.group_top)[j];
-                above += (o.x > mine) + (o.y > mine) + (o.z > mine) + (o.w > mine);
-            }
-            uint32_t least = above < n_alt ? mine : 0xFFFFFFFFu;
-#pragma unroll
-            for (int o = 16; o > 0; o >>= 1) least = min(least, __shfl_xor_sync(0xFFFFFFFFu, least, o));
-            if (lane == 0) sh.warp_least[warp] = least;
-        }
-        __syncthreads();
         if (threadIdx.x == 0) {
-            float s = 0.0f, u = 0.0f;
-#pragma unroll
-            for (int w = 0; w < kWarps; w++) {
-                s += sh.warp_s[w];
-                u += sh.warp_u[w];
-            }
-            sh.block_sums[0] = bm;
-            sh.block_sums[1] = s;
-            sh.block_sums[2] = u;
+            sh.count = 0;
+            sh.n_readers = 0;
         }
+        if (threadIdx.x < kMaxAlt) sh.best[threadIdx.x] = 0ull;
+    }
+    __syncthreads();
+    if (warp == kWarps - 1) {   // the part's sums, to the row's first block
+        Sums p{kLowest, 0.0f, 0.0f};
+        if (lane < kWarps) p = Sums{sh.warp_m[lane], sh.warp_s[lane], sh.warp_u[lane]};
+        float m = p.m;
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, o));
+        p.raise(m, c);
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) {
+            p.s += __shfl_xor_sync(0xFFFFFFFFu, p.s, o);
+            p.u += __shfl_xor_sync(0xFFFFFFFFu, p.u, o);
+        }
+        const float v = lane == 0 ? m : (lane == 1 ? p.s : p.u);
+        if (lane < 3) {
+            if (splits > 1) asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(in_first_block(&sh.sums[rank][lane])), "f"(v) : "memory");
+            else sh.sums[0][lane] = v;
+        }
+        __syncwarp();
     }
 
     // ---------------------------------------------------------- alternatives
     if (n_alt > 0) {
-        uint32_t threshold = sh.warp_least[0];
+        // the n_alt-th largest of the groups' maxima = the smallest that fewer than n_alt of them are above: n_alt logits reach it
+        const uint32_t mine = sh.group_top[lane];
+        int above = 0;
 #pragma unroll
-        for (int w = 1; w < NT / 64; w++) threshold = min(threshold, sh.warp_least[w]);
-        threshold = max(threshold, kFloor);
+        for (int j = 0; j < 8; j++) {
+            const uint4 o = reinterpret_cast<const uint4*>(sh.group_top)[j];
+            above += (o.x > mine) + (o.y > mine) + (o.z > mine) + (o.w > mine);
+        }
+        const uint32_t threshold = max(__reduce_min_sync(0xFFFFFFFFu, above < n_alt ? mine : 0xFFFFFFFFu), kFloor);
         const float least = value_of(threshold);
-        auto push = [&](float v, int64_t i) {
+        auto push = [&](float v, uint32_t i) {
             const int at = atomicAdd(&sh.count, 1);
-            if (at < kList) sh.list[at] = key_of(v, (uint32_t)i);
+            if (at < kList) sh.list[at] = key_of(v, i);
         };
         if (has_extra) {
             const float v = to_f32(x[extra_at]);
-            if (v >= least) push(v, extra_at);
+            if (v >= least) push(v, (uint32_t)extra_at);
         }
-        const uint32_t again = __ballot_sync(0xFFFFFFFFu, a.s != 0.0f && a.m >= least);
+        const bool reaches = a.s != 0.0f && a.m >= least;
+        const uint32_t again = __ballot_sync(0xFFFFFFFFu, reaches);
         if (again) {
             int place = 0;
             if (lane == 0) place = atomicAdd(&sh.n_readers, __popc(again));
             place = __shfl_sync(0xFFFFFFFFu, place, 0);
-            if ((again >> lane) & 1u) sh.reader[place + __popc(again & ((1u << lane) - 1u))] = (int)threadIdx.x;
+            if (reaches) sh.reader[place + __popc(again & ((1u << lane) - 1u))] = (int)threadIdx.x;
         }
         __syncthreads();
         // their chunks, shared out over the block: round r of reader i is item i * rounds + r
-        const int64_t part = (int64_t)rank * kThreads;
-        const uint32_t rounds = n_chunks > part ? (uint32_t)((n_chunks - part + step - 1) / step) : 0u, items = (uint32_t)sh.n_readers * rounds;
+        const uint32_t rounds = n_chunks > part ? (n_chunks - part + step - 1) / step : 0u, items = (uint32_t)sh.n_readers * rounds;
         for (uint32_t item = threadIdx.x; item < items; item += kThreads) {
             const uint32_t i = item / rounds;
-            const int64_t ch = part + sh.reader[i] + (int64_t)(item - i * rounds) * step;
+            const uint32_t ch = part + (uint32_t)sh.reader[i] + (item - i * rounds) * step;
             if (ch >= n_chunks) continue;
             uint32_t w[8];
-            load_chunk(chunks + ch * kChunk, w);
+            load_chunk(chunks + (int64_t)ch * kChunk, w);
             if (Ch::top(w) >= least) {
 #pragma unroll
                 for (int j = 0; j < kChunk / 2; j++) {
                     float v0, v1;
                     Ch::two(w, j, v0, v1);
-                    if (v0 >= least) push(v0, head + ch * kChunk + 2 * j);
-                    if (v1 >= least) push(v1, head + ch * kChunk + 2 * j + 1);
+                    if (v0 >= least) push(v0, head + ch * (uint32_t)kChunk + 2 * j);
+                    if (v1 >= least) push(v1, head + ch * (uint32_t)kChunk + 2 * j + 1);
                 }
             }
         }
@@ -398,10 +403,10 @@ token_logprobs_kernel(const void* __restrict__ logits, int64_t V, int64_t row_st
                 if (lane == 0) sh.pending[warp] = pending;
                 __syncwarp();
             };
-            for (int64_t ch = first; ch - lane < n_chunks; ch += step) {
+            for (uint32_t ch = first; ch - lane < n_chunks; ch += step) {
                 uint32_t w[8];
                 const bool live = ch < n_chunks;
-                if (live) load_chunk(chunks + ch * kChunk, w);
+                if (live) load_chunk(chunks + (int64_t)ch * kChunk, w);
                 const float least = value_of(own);
                 const bool any = live && Ch::top(w) >= least;
                 if (__any_sync(0xFFFFFFFFu, any)) {
@@ -412,8 +417,8 @@ token_logprobs_kernel(const void* __restrict__ logits, int64_t V, int64_t row_st
                         for (int i = 0; i < kChunk / 2; i++)
                             if (i == j && any) Ch::two(w, i, v0, v1);
                         const float bar = value_of(max(own, kth));   // within a round an equal logit may have the lower index
-                        if (v0 >= bar) list[atomicAdd(&sh.pending[warp], 1)] = key_of(v0, (uint32_t)(head + ch * kChunk + 2 * j));
-                        if (v1 >= bar) list[atomicAdd(&sh.pending[warp], 1)] = key_of(v1, (uint32_t)(head + ch * kChunk + 2 * j + 1));
+                        if (v0 >= bar) list[atomicAdd(&sh.pending[warp], 1)] = key_of(v0, head + ch * (uint32_t)kChunk + 2 * j);
+                        if (v1 >= bar) list[atomicAdd(&sh.pending[warp], 1)] = key_of(v1, head + ch * (uint32_t)kChunk + 2 * j + 1);
                         __syncwarp();
                         flush(false);
                     }
@@ -435,47 +440,29 @@ token_logprobs_kernel(const void* __restrict__ logits, int64_t V, int64_t row_st
     __syncthreads();
 
     // --------------------------------------------------------------- the row
-    float m = sh.block_sums[0], s = sh.block_sums[1], u = sh.block_sums[2];
     if (splits > 1) {
-        cluster_sync_all();
-        if (rank == 0) {
-            // a lane of the first warp per block for the sums; n_alt keys of every block for the alternatives
-            if (warp == 0) {
-                Sums p{kLowest, 0.0f, 0.0f};
-                if (lane < splits) {
-                    uint32_t at;
-                    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"((uint32_t)__cvta_generic_to_shared(sh.block_sums)), "r"(lane));
-                    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(p.m) : "r"(at) : "memory");
-                    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(p.s) : "r"(at + 4) : "memory");
-                    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(p.u) : "r"(at + 8) : "memory");
-                }
-                m = p.m;
-#pragma unroll
-                for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, o));
-                p.raise(m, c);
-                s = p.s;
-                u = p.u;
-#pragma unroll
-                for (int o = 16; o > 0; o >>= 1) {
-                    s += __shfl_xor_sync(0xFFFFFFFFu, s, o);
-                    u += __shfl_xor_sync(0xFFFFFFFFu, u, o);
-                }
-            }
-            if (n_alt > 0) {
-                for (int i = threadIdx.x; i < splits * n_alt; i += kThreads) {
-                    uint32_t at;
-                    uint64_t k;
-                    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"((uint32_t)__cvta_generic_to_shared(&sh.best[i % n_alt])), "r"(i / n_alt));
-                    asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(k) : "r"(at) : "memory");
-                    sh.list[i] = k;
-                }
-                __syncthreads();
-                rank_list<NT>(sh.list, splits * n_alt, n_alt, sh.best);
-                __syncthreads();
-            }
+        if (warp == 0 && lane < n_alt)
+            asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(in_first_block(&sh.cluster_list[rank * n_alt + lane])), "l"(sh.best[lane]) : "memory");
+        cluster_sync_all();   // nothing is read from or written to another block behind it
+        if (rank != 0) return;
+        if (n_alt > 0) {
+            rank_list<NT>(sh.cluster_list, splits * n_alt, n_alt, sh.best);
+            __syncthreads();
         }
     }
-    if (rank == 0 && warp == 0) {
+    if (warp == 0) {
+        Sums p{kLowest, 0.0f, 0.0f};   // a lane per part
+        if (lane < splits) p = Sums{sh.sums[lane][0], sh.sums[lane][1], sh.sums[lane][2]};
+        float m = p.m;
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, o));
+        p.raise(m, c);
+        float s = p.s, u = p.u;
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) {
+            s += __shfl_xor_sync(0xFFFFFFFFu, s, o);
+            u += __shfl_xor_sync(0xFFFFFFFFu, u, o);
+        }
         // s: NaN where the row holds a NaN or +inf, 0 where it is masked as a whole
         const float nan = __uint_as_float(0x7FC00000u);
         const bool bad = s != s, empty = s == 0.0f;
@@ -489,15 +476,18 @@ token_logprobs_kernel(const void* __restrict__ logits, int64_t V, int64_t row_st
             alt_logprobs[row * n_alt + lane] = bad ? nan : (none ? -INFINITY : (value_of((uint32_t)(k >> 32)) - m) * scale - log_s);
         }
         for (int g = lane; g < n_given; g += 32) {
-            const int32_t tok = tokens[row * n_given + g];
-            logprobs[row * n_given + g] = tok >= 0 && tok < V ? (sh.given[g] - m) * scale - log_s : -INFINITY;
+            float v;
+            bool in;
+            if (g < kFetched) {
+                v = sh.given[g];
+                in = !sh.outside[g];
+            } else {
+                const int32_t tok = tokens[row * n_given + g];
+                in = tok >= 0 && tok < V;
+                v = in ? to_f32(x[tok]) : 0.0f;
+            }
+            logprobs[row * n_given + g] = in ? (v - m) * scale - log_s : -INFINITY;
         }
-    }
-    // Nobody's shared memory goes away while the first block reads it (what it read has gone into its stores by then; a release would
-    // wait for those).
-    if (splits > 1) {
-        __syncwarp();
-        asm volatile("barrier.cluster.arrive.relaxed.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
     }
 }
 
