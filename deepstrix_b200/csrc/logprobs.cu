@@ -8,7 +8,7 @@
 // One pass.  A thread keeps its own running maximum and its s and u relative to it; it takes 32 bytes of logits at a time and rescales
 // only when their maximum is new.  Pairs of f32 go through the packed add, multiply and fused multiply-add of sm_100: an element costs
 // about five and a half issue slots, one of them the exponential.
-// The alternatives cost the loop nothing: afterwards the n_alt-th largest of the threads' maxima (of pairs of threads) is a value that
+// The alternatives cost the loop nothing: afterwards the n_alt-th largest of the maxima of 32 or 64 groups of threads is a value that
 // at least n_alt logits reach, and hardly more do, so only the threads whose maximum reaches it have their chunks read again (from L2) for
 // the few logits that do; those are ranked by counting.  Where more than the list holds reach it -- a row of equal logits, say, or one masked with the
 // lowest value -- a second pass keeps the best 32 of every warp in registers, sorting candidates 32 at a time.
@@ -16,9 +16,10 @@
 // distributed shared memory: one launch, no workspace, and the order of every addition is fixed.
 //
 // Bound: HBM; bf16 and f16 rows at the full rate are 11.6 elements a clock and SM, of which the exponentials can take 16.  2048 rows of 131072
-// f32 take 174 us, 6.2 TB/s; 4096 of bf16 180 without alternatives and 198 with five (the part behind the loop of one block in five at a time);
-// 64 rows of f32 12, one row of 32000 7 us, latency.  A ring of asynchronous copies that ran on into the next row was slower (227 us: its
-// instructions, not the loads in flight, were what the loop lacked), and so were chunks requested 2 to 6 ahead for a few rows (12.4 to 13.6).
+// f32 take 172 us, 6.25 TB/s; 4096 of bf16 177 without alternatives and 191 with five (the part behind the loop of one block in five at a
+// time); 64 rows of f32 with twenty 11 us, one row of 32000 5.8, latency.  A ring of asynchronous copies that ran on into the next row was
+// slower (227 us when the loop took 199: its instructions, not the loads in flight, were what the loop lacked), and so were chunks requested 2 to 6
+// ahead for a few rows (0.1 to 1.3 us more), and keeping the chunk of every thread's maximum so that it need not be read again (loop 5 to 10 % longer).
 #include "head.cuh"
 
 namespace dsx {
@@ -166,7 +167,7 @@ constexpr int kList = 512;   // candidates the block ranks by counting
 template <int NT>
 struct alignas(16) Shared {
     static constexpr int kWarps = NT / 32;
-    alignas(16) uint32_t group_top[32];     // order of the maxima of 32 groups of threads, 0 where they saw nothing
+    alignas(16) uint32_t group_top[64];     // order of the maxima of 32 or 64 groups of threads, 0 where they saw nothing
     float warp_m[kWarps], warp_s[kWarps], warp_u[kWarps];
     int n_readers;                          // threads whose maximum reaches the threshold,
     int reader[NT];                         // in any order
@@ -197,8 +198,7 @@ __device__ __forceinline__ void rank_list(const uint64_t* list, int n, int n_alt
 }
 
 // NT threads a block: 256, or 64 for many short rows, whose time is the part behind the loop.  48 registers a thread (1280 threads an SM, 40 KB
-// of logits in flight): 4096 rows of 131072 bf16 take 199 us; with 64 registers (1024 threads) 206, with 40 (1536, spilling) 201, with
-// 1024 threads that request two chunks ahead 217.
+// of logits in flight): 4096 rows of 131072 bf16 take 191 us, 2048 of f32 172; with 64 registers (1024 threads) 198 and 191.
 template <int DT, int NT>
 __global__ void __launch_bounds__(NT, 1280 / NT)
 token_logprobs_kernel(const void* __restrict__ logits, int64_t V, int64_t row_stride, float scale, const int32_t* __restrict__ tokens, int n_given,
@@ -214,6 +214,13 @@ token_logprobs_kernel(const void* __restrict__ logits, int64_t V, int64_t row_st
     const int64_t row = blockIdx.x / (unsigned)splits;
     const float c = scale * kLog2e;
     const T* __restrict__ x = reinterpret_cast<const T*>(logits) + row * row_stride;
+    if (threadIdx.x < 64) sh.group_top[threadIdx.x] = 0u;
+    if (threadIdx.x < kMaxAlt) sh.best[threadIdx.x] = 0ull;
+    if (threadIdx.x == 0) {
+        sh.count = 0;
+        sh.n_readers = 0;
+    }
+    __syncthreads();
     if (splits > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");   // this block has started; waited for behind the loop
     pdl_wait();   // the logits may come from the kernel before this one
     // whole 16-byte words from the row's first aligned element on; the few elements before and after them one by one
@@ -281,17 +288,16 @@ token_logprobs_kernel(const void* __restrict__ logits, int64_t V, int64_t row_st
         a.u = u0 + u1;
     }
 
-    // A warp's sums, and the maxima of 32 groups of threads.  All sums are added in an order that does not depend on timing.
+    // A warp's sums, and the maxima of 32 groups of threads, or of 64 for many alternatives (a threshold that is the least of few maxima lets
+    // more than four times as many candidates through: 64 rows of 131072 with 32 alternatives 13 us, 21 with 32 groups).  All sums are added in an order that does not depend on timing.
+    const bool many = n_alt > 16;
     __syncwarp();
     if (splits > 1) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");   // every block of the cluster has started
     {
         float m = a.m;
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, o));
-        uint32_t top = a.s == 0.0f ? 0u : order_of(a.m);
-#pragma unroll
-        for (int o = kWarps / 2; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
-        if (threadIdx.x % kWarps == 0) sh.group_top[threadIdx.x / kWarps] = top;
+        if (n_alt > 0 && a.s != 0.0f) atomicMax(&sh.group_top[threadIdx.x & (many ? 63 : 31)], order_of(a.m));
         Sums r = a;
         r.raise(m, c);
 #pragma unroll
@@ -304,11 +310,6 @@ token_logprobs_kernel(const void* __restrict__ logits, int64_t V, int64_t row_st
             sh.warp_s[warp] = r.s;
             sh.warp_u[warp] = r.u;
         }
-        if (threadIdx.x == 0) {
-            sh.count = 0;
-            sh.n_readers = 0;
-        }
-        if (threadIdx.x < kMaxAlt) sh.best[threadIdx.x] = 0ull;
     }
     __syncthreads();
     if (warp == kWarps - 1) {   // the part's sums, to the row's first block
@@ -334,14 +335,18 @@ token_logprobs_kernel(const void* __restrict__ logits, int64_t V, int64_t row_st
     // ---------------------------------------------------------- alternatives
     if (n_alt > 0) {
         // the n_alt-th largest of the groups' maxima = the smallest that fewer than n_alt of them are above: n_alt logits reach it
-        const uint32_t mine = sh.group_top[lane];
-        int above = 0;
-#pragma unroll
-        for (int j = 0; j < 8; j++) {
-            const uint4 o = reinterpret_cast<const uint4*>(sh.group_top)[j];
-            above += (o.x > mine) + (o.y > mine) + (o.z > mine) + (o.w > mine);
-        }
-        const uint32_t threshold = max(__reduce_min_sync(0xFFFFFFFFu, above < n_alt ? mine : 0xFFFFFFFFu), kFloor);
+        auto reached = [&](uint32_t mine, int groups) {
+            int above = 0;
+#pragma unroll 8
+            for (int j = 0; j < groups / 4; j++) {
+                const uint4 o = reinterpret_cast<const uint4*>(sh.group_top)[j];
+                above += (o.x > mine) + (o.y > mine) + (o.z > mine) + (o.w > mine);
+            }
+            return above < n_alt ? mine : 0xFFFFFFFFu;
+        };
+        uint32_t reach = reached(sh.group_top[lane], many ? 64 : 32);
+        if (many) reach = min(reach, reached(sh.group_top[lane + 32], 64));
+        const uint32_t threshold = max(__reduce_min_sync(0xFFFFFFFFu, reach), kFloor);
         const float least = value_of(threshold);
         auto push = [&](float v, uint32_t i) {
             const int at = atomicAdd(&sh.count, 1);
@@ -519,11 +524,11 @@ int launch_for(const void* logits, int64_t t, int64_t v, int64_t row_stride, flo
     int sms = 0;
     if (int rc = head_sm_count(&sms)) return rc;
     constexpr int kChunk = Chunk<typename Elem<DT>::T>::n;
-    // many rows of at most 16 chunks a thread: the small block (4096 rows of 4096 bf16 16.5 us against 38.8, of 16384 36.8 against 57.9, but
-    // of 32000 with 20 alternatives 114 against 85); also a row that a small block reads in one round
+    // many rows of at most 16 chunks a thread: the small block (4096 rows of 4096 bf16 15.6 us against 28.4, of 16384 34.2 against 44.7, but
+    // of 32000 with 20 alternatives 98 against 72); also a row that a small block reads in one round
     const bool small = v <= 64 * kChunk || (t >= 8 * (int64_t)sms && v <= 16 * 64 * kChunk);
-    // few rows: as many blocks a row as still give every thread two chunks, and no more than two blocks an SM in all (64 rows of 131072 f32:
-    // 17.5 / 12.9 / 10.8 / 11.7 us with 1 / 2 / 4 / 8)
+    // few rows: as many blocks a row as still give every thread two chunks, and no more than two blocks an SM in all (64 rows of 131072 f32
+    // 20.5 / 14.0 / 11.1 / 13.6 us with 1 / 2 / 4 / 8, 148 of bf16 13.0 / 12.2 / 14.3 / 17.6, one row of 32000 f32 7.0 / 6.6 / 5.8 / 5.4)
     int splits = 1;
     while (!small && splits < kMaxCluster && t * splits * 2 <= 2 * (int64_t)sms && v >= (int64_t)splits * 2 * 2 * 256 * kChunk) splits *= 2;
     if (small) return launch<DT, 64>(logits, t, v, row_stride, scale, tokens, n_given, logprobs, entropy, n_alt, alts, alt_logprobs, splits, stream);
