@@ -359,6 +359,19 @@ def test_logprobs_many_short_rows(torch_cuda, moe, V, dtype):
     _check_logprobs(torch, dx, rng.integers(-1, V + 1, (T, 2)).astype(np.int32), 20)
 
 
+@pytest.mark.parametrize("T,V,given,n_alt", [(2, 40000, 1024, 16), (1300, 900, 70, 17), (64, 2048, 65, 32), (9, 300, 64, 16), (160, 20011, 63, 17)])
+def test_logprobs_many_given_tokens(torch_cuda, moe, T, V, given, n_alt):
+    """More given tokens than are fetched ahead, the same token more than once, tokens outside; both counts of threshold groups."""
+    torch = torch_cuda
+    rng = np.random.default_rng(V)
+    x = (rng.standard_normal((T, V)) * 4).astype(np.float32)
+    x[0, rng.random(V) < 0.5] = -np.inf
+    x[1, 3] = np.nan
+    tokens = rng.integers(-2, V + 2, (T, given)).astype(np.int32)
+    tokens[:, given // 2:given // 2 + 3] = tokens[:, :3]
+    _check_logprobs(torch, torch.from_numpy(x).cuda(), tokens, n_alt, 0.9)
+
+
 def test_logprobs_without_tokens_or_alternatives(torch_cuda, moe):
     torch = torch_cuda
     from deepstrix_b200 import head
