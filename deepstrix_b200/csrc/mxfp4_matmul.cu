@@ -12,8 +12,8 @@
 // A pipeline stage is 256 columns: 128-byte rows (128-byte swizzle) of W and of A, each one TMA box, zero-filled past the operand's edges.
 // Scales are read as stored (row-major bytes; nothing is laid out beforehand), 16 bytes of every row -- 512 columns, two stages -- at a time
 // into a ring of their own: by TMA where rows of scales are 16-byte aligned (K a multiple of 512), else by four loader warps, a row of
-// every 128-row group a thread, as the aligned words that hold them, requested ahead and shifted into place.  (Asynchronous copies of 8 bytes
-// a row and stage kept the shared-memory pipe 60 % busy with 32 lines an instruction.)  Scale warps, one per lane quarter, move a
+// every 128-row group a thread, as the aligned 16-byte words that hold them, requested a step ahead and shifted into place (8192 x 8192 x 4128
+// takes 160 us, as words of 4 bytes 178; with K of 4096 and TMA 121.  Loaders that moved every other buffer to tensor memory as well: 168).  Scale warps, one per lane quarter, move a
 // buffer to a slot of tensor memory at a time (ld.shared + tcgen05.st; the tensor core's own copy would queue behind its MMAs); where TMA
 // brings the scales the loader warps are a second set of them, and the sets take alternate buffers: one set alone needed 800 clocks a stage.
 // Warp roles: TMA of codes, MMA issue, TMA of scales, 4 scale warps, 4 epilogue warps, 4 loaders or scale warps; two accumulators, so that a
@@ -48,7 +48,6 @@ constexpr int kWBytes = kWRows * kRowBytes;
 constexpr int kGroupBytes = 2048;    // scale bytes of a group of 128 rows: 16 a row, two stages
 constexpr int kMaxScaleBufs = 4;     // two or four: see plan_block
 constexpr int kMaxSlots = 4;         // of scales in tensor memory, two stages each
-constexpr int kMaxGroups = 4;        // W and up to three term groups
 constexpr int kMaxStages = 8;
 constexpr int kMaxN = 208;           // of an MMA: two accumulators and two scale slots fill tensor memory
 constexpr uint32_t kSpinLimit = 1u << 22;
@@ -485,48 +484,56 @@ mxfp4_matmul_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_con
         {
             const int r = threadIdx.x - kLoadWarp0 * 32;   // row of every group
             const int nblk = g.K >> 5;
+            constexpr int kGroups = PAIR && TERMS == 3 ? 4 : 3;   // at most: W and a group a term, or two of one term
             uint32_t d = 0, ph = 0;
             bool ok = true;
             for (int tile = tile0; tile < g.tiles && ok; tile += tile_step) {
                 const int64_t w_row = (int64_t)(tile % g.tiles_w) * kTileW + half * kWRows + r, a_row0 = (int64_t)(tile / g.tiles_w) * tokens;
                 // this thread's row of every group, null where the operand has none
-                const uint8_t* row[kMaxGroups];
-                bool place[kMaxGroups];   // the group has room for it
+                const uint8_t* row[kGroups];
+                bool place[kGroups];   // the group has room for it
                 row[0] = w_row < g.N ? g.w_scales + w_row * nblk : nullptr;
                 place[0] = true;
 #pragma unroll
-                for (int i = 1; i < kMaxGroups; i++) {
+                for (int i = 1; i < kGroups; i++) {
                     const int rn = (TERMS == 1 ? (i - 1) * 128 : 0) + r;   // row of N; the term it belongs to and its token
                     const int q = TERMS == 1 ? rn / tokens : i - 1, ra = TERMS == 1 ? rn % tokens : rn;
                     place[i] = i < g.groups && rn < BN;
                     row[i] = place[i] && a_row0 + ra < g.M ? g.a_scales + ((int64_t)q * g.M + a_row0 + ra) * nblk : nullptr;
                 }
-                // the aligned words that hold bytes blk .. blk + 15 of a row (the row's last bytes: fewer), at most five
-                auto fetch = [&](const uint8_t* p, int blk, uint32_t (&w)[5]) {
-                    const int n = p ? min(16, nblk - blk) : 0;
-                    const uintptr_t at = (uintptr_t)p + blk;
-                    const uint32_t* q = reinterpret_cast<const uint32_t*>(at & ~(uintptr_t)3);
-                    const int span = n > 0 ? (int)(at & 3) + n : 0;
-#pragma unroll
-                    for (int j = 0; j < 5; j++) w[j] = 4 * j < span ? __ldg(q + j) : 0u;
+                // A row is a stream of aligned 16-byte words, one a step -- an instruction that touches 32 lines takes as long for 4 bytes of each
+                // as for 16 -- of which two hold the step's bytes; words without a byte of the row are not read.
+                auto word = [&](const uint8_t* p, int i) {   // the word with byte 16 i of the row and those before it up to the boundary
+                    const uintptr_t at = ((uintptr_t)p & ~(uintptr_t)15) + 16 * (uintptr_t)i;
+                    return p && at < (uintptr_t)p + nblk ? __ldg(reinterpret_cast<const uint4*>(at)) : make_uint4(0, 0, 0, 0);
                 };
-                for (int kc = kc0 & ~1; kc < kc1; kc += 2) {
-                    uint32_t w[kMaxGroups][5];
+                uint4 cur[kGroups], next[kGroups];
 #pragma unroll
-                    for (int i = 0; i < kMaxGroups; i++) fetch(row[i], kc * 8, w[i]);   // requested before the wait
+                for (int i = 0; i < kGroups; i++) {
+                    cur[i] = word(row[i], kc0 >> 1);
+                    next[i] = word(row[i], (kc0 >> 1) + 1);
+                }
+                for (int kc = kc0 & ~1; kc < kc1; kc += 2) {
                     ok = mbar_wait(bar(RAW_EMPTY) + 8u * d, ph ^ 1u, abort_flag);
                     if (!ok) break;
                     const uint32_t dst = sbase + raw0 + d * raw_bytes + (uint32_t)r * 16u;
                     const int n = nblk - kc * 8;   // bytes past the row's end belong to the next row
 #pragma unroll
-                    for (int i = 0; i < kMaxGroups; i++) {
-                        const uint32_t sh = ((uint32_t)(uintptr_t)row[i] + kc * 8) * 8u;   // funnel shifts take it modulo 32
-                        uint32_t v[4];
+                    for (int i = 0; i < kGroups; i++) {
+                        if (i >= g.groups) break;
+                        const uint32_t at = (uint32_t)(uintptr_t)row[i];
+                        uint32_t v[8] = {cur[i].x, cur[i].y, cur[i].z, cur[i].w, next[i].x, next[i].y, next[i].z, next[i].w};
+#pragma unroll
+                        for (int j = 0; j < 6; j++) v[j] = at & 8u ? v[j + 2] : v[j];
+#pragma unroll
+                        for (int j = 0; j < 5; j++) v[j] = at & 4u ? v[j + 1] : v[j];
 #pragma unroll
                         for (int j = 0; j < 4; j++) {
-                            v[j] = __funnelshift_r(w[i][j], w[i][j + 1], sh);
+                            v[j] = __funnelshift_r(v[j], v[j + 1], at * 8u);   // takes it modulo 32
                             if (n < 4 * j + 4) v[j] = n > 4 * j ? v[j] & ((1u << (8 * (n - 4 * j))) - 1u) : 0u;
                         }
+                        cur[i] = next[i];
+                        next[i] = word(row[i], (kc >> 1) + 2);
                         if (place[i])
                             asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(dst + (i ? kGroupBytes + (i - 1) * group_step : 0u)), "r"(v[0]), "r"(v[1]),
                                          "r"(v[2]), "r"(v[3])
