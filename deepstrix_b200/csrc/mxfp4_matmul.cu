@@ -30,6 +30,7 @@
 
 #include <algorithm>
 #include <atomic>
+#include <mutex>
 
 #include "head.cuh"
 #include "prefill.cuh"
@@ -666,7 +667,7 @@ mxfp4_matmul_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_con
 constexpr int kSmallMin = 77 * 1024, kSmallMax = 112 * 1024, kLargeMin = 160 * 1024, kLargeMax = 225 * 1024;
 
 struct Plan {
-    int tokens, fold, stages, slots, stage_bytes, scale_bufs, groups, tmem_cols, smem, per_sm, splits, tiles_w, tiles_m;
+    int tokens, fold, stages, slots, stage_bytes, scale_bufs, groups, tmem_cols, smem, per_sm, splits, tiles_w, tiles_m, at_once;
     bool pair;
 };
 
@@ -698,32 +699,43 @@ bool plan_block(int terms, int tokens, bool pair, Plan* p) {
     return p->stages * p->stage_bytes >= tokens * kWRows * 4;   // a partial tile fits into the ring
 }
 
-// Tokens a tile, pairs or single CTAs, and splits of the columns, from a model of the time in clocks.  A stage costs its MMAs and 150 clocks
-// of the issuing warp around them, or its copies at about 32 bytes a clock and SM from L2; a block about 3000 clocks before and after its
-// stages, a joined tile another 1500; and the operands come from HBM at about 23 bytes a clock and SM.
-bool make_plan(int64_t M, int64_t N, int K, int terms, int sms, bool pairs_run, Plan* best) {
+// What a device runs at once: clusters of 1, 2, 4 and 8 CTAs with an SM each (clusters do not reach across the groups that SMs come in, so there
+// are fewer than SMs suggest: 148, 74, 33, 15; on a partition of a device there may be none); of small blocks, at least twice as many.  Looked
+// up, and the opt-in to large shared memory made, once per device.
+struct Device {
+    int sms;
+    int clusters[4];   // [log2 of the size]
+};
+
+// Tokens a tile, pairs or single CTAs, and splits of the columns, from a model of the time in clocks.  A stage takes its MMAs on the tensor
+// core (N / 2 clocks each, 50 at least), or the issuing warp's 50 an MMA and what surrounds them (two blocks on an SM issue side by side), or
+// its copies at 80 bytes a clock and SM from L2; a round of tiles about 5500 clocks before and after its stages, a joined tile another 2500;
+// and the operands come from HBM at 26 bytes a clock and SM.  The constants were fitted to 600 tilings of 40 products, of 1 to 8192 tokens and 3
+// to 131072 rows of W: the model's choice is 0.5 % slower than the best of them on average, 16 % at worst (3176 x 3 x 3104).
+bool make_plan(int64_t M, int64_t N, int K, int terms, const Device& dev, Plan* best) {
     const int n_kc = (K + kStageK - 1) / kStageK;
     double best_t = 1e300;
-    for (int pair = 0; pair <= (pairs_run ? 1 : 0); pair++)
+    for (int pair = 0; pair <= 1; pair++)
         for (int tokens = 16; tokens <= kMaxN && tokens < M + 16; tokens += 16) {
             Plan p;
             if (!plan_block(terms, tokens, pair != 0, &p)) continue;
-            const int ctas = pair ? 2 : 1;
-            p.tiles_w = (int)((N + kWRows * ctas - 1) / (kWRows * ctas));
+            p.tiles_w = (int)((N + kWRows * (1 + pair) - 1) / (kWRows * (1 + pair)));
             p.tiles_m = (int)((M + tokens - 1) / tokens);
-            // an MMA: N / 2 clocks, 50 at least; what surrounds a stage's runs under the other block's where two share an SM
-            const double mma = 4.0 * (pair ? terms : 1) * std::max(50.0, tokens * p.fold / 2.0) + (p.per_sm == 2 ? 0.0 : 150.0);
-            const double stage = std::max(mma, p.stage_bytes / 32.0);
-            const double hbm = ((double)N + (double)terms * M) * K * 17 / 32 / (23.0 * sms);
-            for (int s = 1; s <= (pair ? 1 : 8) && s <= n_kc; s *= 2) {
-                const int64_t units = (int64_t)p.tiles_w * p.tiles_m * s, slots = (int64_t)sms / ctas;
-                if (s > 1 && units > slots * p.per_sm) break;
-                const double busiest = (double)((units + slots - 1) / slots);
-                const double t = std::max(busiest * ((n_kc + s - 1) / s) * stage, hbm) + 3000.0 * ((units + slots * p.per_sm - 1) / (slots * p.per_sm)) +
-                                 (s > 1 ? 1500.0 + 20.0 * tokens : 0.0) + 30.0 * tokens;
+            const int64_t tiles = (int64_t)p.tiles_w * p.tiles_m;
+            const double mmas = 4.0 * (pair ? terms : 1), tensor = mmas * std::max(50.0, tokens * p.fold / 2.0);
+            const double issue = pair ? 50.0 * mmas + 250.0 : p.per_sm == 1 ? 50.0 * mmas + 300.0 : (50.0 * mmas + 700.0) / 2;
+            const double stage = std::max({tensor, issue, p.stage_bytes / 80.0});
+            const double hbm = ((double)N + (double)terms * M) * K * 17 / 32 / (26.0 * dev.sms);
+            for (int l = 0; l <= (pair ? 0 : 3) && 1 << l <= n_kc; l++) {
+                p.at_once = p.per_sm * dev.clusters[l + pair];   // tiles
+                if (p.at_once == 0 || (l > 0 && tiles > p.at_once)) break;
+                const int64_t rounds = (tiles + p.at_once - 1) / p.at_once;
+                const int64_t busiest = (tiles * p.per_sm + p.at_once - 1) / p.at_once;   // tiles an SM
+                const double t = std::max((double)busiest * ((n_kc + (1 << l) - 1) >> l) * stage, hbm) + 5500.0 * rounds + (l > 0 ? 2500.0 + 2.0 * tokens : 0.0) +
+                                 45.0 * tokens;
                 if (t < best_t) {
                     best_t = t;
-                    p.splits = s;
+                    p.splits = 1 << l;
                     *best = p;
                 }
             }
@@ -732,11 +744,11 @@ bool make_plan(int64_t M, int64_t N, int K, int terms, int sms, bool pairs_run, 
 }
 
 template <int DT, int TERMS, bool PAIR>
-int launch(const Plan& p, const CUtensorMap (&maps)[4], const MatmulArgs& g, int sms, cudaStream_t stream) {
+int launch(const Plan& p, const CUtensorMap (&maps)[4], const MatmulArgs& g, cudaStream_t stream) {
     const int cluster = PAIR ? 2 : p.splits;
     const int64_t tiles = (int64_t)p.tiles_w * p.tiles_m;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)(cluster * (p.splits > 1 ? tiles : std::min<int64_t>(tiles, (int64_t)sms / cluster * p.per_sm))));
+    cfg.gridDim = dim3((unsigned)(cluster * std::min<int64_t>(tiles, p.at_once)));
     cfg.blockDim = dim3(kThreads);
     cfg.dynamicSmemBytes = (size_t)p.smem;
     cfg.stream = stream;
@@ -755,11 +767,11 @@ int launch(const Plan& p, const CUtensorMap (&maps)[4], const MatmulArgs& g, int
 }
 
 template <int DT>
-int launch_for(int terms, const Plan& p, const CUtensorMap (&maps)[4], const MatmulArgs& g, int sms, cudaStream_t stream) {
-    if (!p.pair) return launch<DT, 1, false>(p, maps, g, sms, stream);
-    if (terms == 1) return launch<DT, 1, true>(p, maps, g, sms, stream);
-    if (terms == 2) return launch<DT, 2, true>(p, maps, g, sms, stream);
-    return launch<DT, 3, true>(p, maps, g, sms, stream);
+int launch_for(int terms, const Plan& p, const CUtensorMap (&maps)[4], const MatmulArgs& g, cudaStream_t stream) {
+    if (!p.pair) return launch<DT, 1, false>(p, maps, g, stream);
+    if (terms == 1) return launch<DT, 1, true>(p, maps, g, stream);
+    if (terms == 2) return launch<DT, 2, true>(p, maps, g, stream);
+    return launch<DT, 3, true>(p, maps, g, stream);
 }
 
 template <int DT>
@@ -771,40 +783,46 @@ int allow_shared() {
     return DSX_OK;
 }
 
-// SM count of the current device and whether it runs CTA pairs (a partition of a device may not hold a cluster of two); looked up,
-// and the opt-in to large shared memory made, once per device.
-int configure(int* sms, bool* pairs_run) {
+template <bool PAIR>
+int max_clusters(int log2_size) {
+    cudaLaunchConfig_t lc = {};
+    lc.gridDim = dim3(8);
+    lc.blockDim = dim3(kThreads);
+    lc.dynamicSmemBytes = kLargeMax;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = 1u << log2_size;
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    lc.attrs = attr;
+    lc.numAttrs = 1;
+    int n = 0;
+    if (cudaOccupancyMaxActiveClusters(&n, mxfp4_matmul_kernel<DSX_F32, 1, PAIR>, &lc) != cudaSuccess) {
+        (void)cudaGetLastError();
+        return 0;
+    }
+    return n;
+}
+int configure(const Device** out) {
     constexpr int kMaxDevices = 64;
-    static std::atomic<int> known[kMaxDevices];   // SM count, its sign bit saying that pairs do not run
+    static Device devices[kMaxDevices];
+    static std::atomic<int> known[kMaxDevices];
+    static std::mutex mutex;
     int dev = 0;
     DSX_CUDA(cudaGetDevice(&dev));
     DSX_REQUIRE(dev >= 0 && dev < kMaxDevices, "mxfp4_matmul: device index %d out of range", dev);
-    int n = known[dev].load(std::memory_order_acquire);
-    if (n == 0) {
-        DSX_CUDA(cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev));
-        if (int rc = allow_shared<DSX_F32>()) return rc;
-        if (int rc = allow_shared<DSX_BF16>()) return rc;
-        if (int rc = allow_shared<DSX_F16>()) return rc;
-        cudaLaunchConfig_t lc = {};
-        lc.gridDim = dim3(2);
-        lc.blockDim = dim3(kThreads);
-        lc.dynamicSmemBytes = kLargeMax;
-        cudaLaunchAttribute attr[1];
-        attr[0].id = cudaLaunchAttributeClusterDimension;
-        attr[0].val.clusterDim.x = 2;
-        attr[0].val.clusterDim.y = 1;
-        attr[0].val.clusterDim.z = 1;
-        lc.attrs = attr;
-        lc.numAttrs = 1;
-        int clusters = 0;
-        if (cudaOccupancyMaxActiveClusters(&clusters, mxfp4_matmul_kernel<DSX_F32, 1, true>, &lc) != cudaSuccess || clusters < 1) {
-            (void)cudaGetLastError();
-            n = -n;
-        }
-        known[dev].store(n, std::memory_order_release);
-    }
-    *sms = n < 0 ? -n : n;
-    *pairs_run = n > 0;
+    *out = &devices[dev];
+    if (known[dev].load(std::memory_order_acquire)) return DSX_OK;
+    std::lock_guard<std::mutex> lock(mutex);
+    Device& d = devices[dev];
+    DSX_CUDA(cudaDeviceGetAttribute(&d.sms, cudaDevAttrMultiProcessorCount, dev));
+    if (int rc = allow_shared<DSX_F32>()) return rc;
+    if (int rc = allow_shared<DSX_BF16>()) return rc;
+    if (int rc = allow_shared<DSX_F16>()) return rc;
+    d.clusters[0] = d.sms;
+    for (int l = 1; l < 4; l++) d.clusters[l] = max_clusters<false>(l);
+    d.clusters[1] = std::min(d.clusters[1], max_clusters<true>(1));
+    known[dev].store(1, std::memory_order_release);
     return DSX_OK;
 }
 
@@ -827,11 +845,10 @@ int dsx_mxfp4_matmul(const void* a_codes, const void* a_scales, int n_terms, int
     DSX_REQUIRE(row_stride >= n || m == 1, "mxfp4_matmul: row stride %lld below the %lld columns of a row", (long long)row_stride, (long long)n);
     DSX_REQUIRE((((uintptr_t)a_codes | (uintptr_t)w_codes) & 15) == 0 && ((uintptr_t)out & (dtype_size(dtype) - 1)) == 0,
                 "mxfp4_matmul: codes must be 16-byte aligned, out aligned to its elements");
-    int sms = 0;
-    bool pairs_run = false;
-    if (int rc = configure(&sms, &pairs_run)) return rc;
+    const Device* dev = nullptr;
+    if (int rc = configure(&dev)) return rc;
     Plan p;
-    if (!make_plan(m, n, (int)k, n_terms, sms, pairs_run, &p)) return set_error(DSX_ERR_UNSUPPORTED, "mxfp4_matmul: no tile for %d terms", n_terms);
+    if (!make_plan(m, n, (int)k, n_terms, *dev, &p)) return set_error(DSX_ERR_UNSUPPORTED, "mxfp4_matmul: no tile for %d terms", n_terms);
     DSX_REQUIRE((int64_t)p.tiles_w * p.tiles_m < ((int64_t)1 << 30), "mxfp4_matmul: too many tiles");
     // codes and scales of both operands as (bytes, row) and (bytes, row, term); the maps of scales only where TMA can read them
     const bool scale_tma = k % 512 == 0 && (((uintptr_t)a_scales | (uintptr_t)w_scales) & 15) == 0;
@@ -868,9 +885,9 @@ int dsx_mxfp4_matmul(const void* a_codes, const void* a_scales, int n_terms, int
     g.scale_bufs = p.scale_bufs;
     g.pairs = dtype != DSX_F32 && n % 2 == 0 && (row_stride % 2 == 0 || m == 1) && ((uintptr_t)out & 3) == 0;
     const cudaStream_t s = (cudaStream_t)stream;
-    if (dtype == DSX_F32) return launch_for<DSX_F32>(n_terms, p, maps, g, sms, s);
-    if (dtype == DSX_BF16) return launch_for<DSX_BF16>(n_terms, p, maps, g, sms, s);
-    return launch_for<DSX_F16>(n_terms, p, maps, g, sms, s);
+    if (dtype == DSX_F32) return launch_for<DSX_F32>(n_terms, p, maps, g, s);
+    if (dtype == DSX_BF16) return launch_for<DSX_BF16>(n_terms, p, maps, g, s);
+    return launch_for<DSX_F16>(n_terms, p, maps, g, s);
 }
 
 int dsx_head_check(dsx_stream_t stream_, uint32_t* error_word) {
