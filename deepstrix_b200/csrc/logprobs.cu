@@ -528,9 +528,13 @@ int launch_for(const void* logits, int64_t t, int64_t v, int64_t row_stride, flo
     // of 32000 with 20 alternatives 98 against 72); also a row that a small block reads in one round
     const bool small = v <= 64 * kChunk || (t >= 8 * (int64_t)sms && v <= 16 * 64 * kChunk);
     // few rows: as many blocks a row as still give every thread two chunks, and no more than two blocks an SM in all (64 rows of 131072 f32
-    // 20.5 / 14.0 / 11.1 / 13.6 us with 1 / 2 / 4 / 8, 148 of bf16 13.0 / 12.2 / 14.3 / 17.6, one row of 32000 f32 7.0 / 6.6 / 5.8 / 5.4)
+    // 20.5 / 14.0 / 11.1 / 13.6 us with 1 / 2 / 4 / 8, 148 of bf16 13.0 / 12.2 / 14.3 / 17.6, one row of 32000 f32 7.0 / 6.6 / 5.8 / 5.4), or as many
+    // as are resident where every thread keeps 16 (300 rows of 131072 f32 40.9 / 30.0 / 34.2 us with 1 / 2 / 4, but 333 of 50021 f16 12.7 / 13.6)
     int splits = 1;
-    while (!small && splits < kMaxCluster && t * splits * 2 <= 2 * (int64_t)sms && v >= (int64_t)splits * 2 * 2 * 256 * kChunk) splits *= 2;
+    auto more = [&](int blocks_per_sm, int chunks) {
+        return splits < kMaxCluster && t * splits * 2 <= blocks_per_sm * (int64_t)sms && v >= (int64_t)splits * 2 * chunks * 256 * kChunk;
+    };
+    while (!small && (more(2, 2) || more(1280 / 256, 16))) splits *= 2;
     if (small) return launch<DT, 64>(logits, t, v, row_stride, scale, tokens, n_given, logprobs, entropy, n_alt, alts, alt_logprobs, splits, stream);
     return launch<DT, 256>(logits, t, v, row_stride, scale, tokens, n_given, logprobs, entropy, n_alt, alts, alt_logprobs, splits, stream);
 }
