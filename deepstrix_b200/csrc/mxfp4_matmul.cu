@@ -23,9 +23,9 @@
 // Every wait is bounded; on a timeout the block drains, frees its tensor memory and sets bit 1 of the error word.
 //
 // Bound and measured (launches back to back).  A few tokens: the weights' bytes; 8 x 131072 x 4096 of three terms takes 53 us, 5.4 TB/s, of which
-// about 7 us are start and end -- every further 37888 rows of W take 12.8 us, 6.45 TB/s.  One small matrix (1 x 1024 x 2048): 6.5 us, all of it
+// about 7 us are start and end -- every further 37888 rows of W take 12.8 us, 6.45 TB/s.  One small matrix (1 x 1024 x 2048): 6 us, all of it
 // latency.  Many tokens: the issuing warp's clocks and the power cap; 8192 x 8192 x 4096 takes 118 us with one term, 4.7 PFLOP/s (140 us after a
-// second of it at the capped clock), 291 with three, 5.7 PFLOP/s of MMAs executed; 777 x 5119 x 2336 of three terms, f16, 19.5 us.
+// second of it at the capped clock), 291 with three, 5.7 PFLOP/s of MMAs executed; 64 x 131072 x 4096 of three terms 61, 777 x 5119 x 2336 19.5.
 #include <cuda.h>
 
 #include <algorithm>
