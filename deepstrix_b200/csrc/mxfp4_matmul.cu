@@ -580,7 +580,7 @@ mxfp4_matmul_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_con
             }
             tc_fence_before();
             __syncwarp();
-            if (lane == 0) {
+            if (lane == 0 && tile + 2 * tile_step < g.tiles) {   // only where it is waited for: nothing may be on its way to a block that has ended
                 if (PAIR && half != 0) mbar_arrive_cluster(map_to_cta(bar(ACC_EMPTY) + 8u * b, 0u));
                 else mbar_arrive(bar(ACC_EMPTY) + 8u * b);
             }
@@ -622,8 +622,22 @@ mxfp4_matmul_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_con
     __syncwarp();
     tc_fence_before();
     __syncthreads();
+    if constexpr (PAIR) {
+        // Neither CTA's shared or tensor memory goes away while the other may still use it: nor while an arrival is on its way to it.  The last
+        // releases of stages and slots, which no role waited for, are waited for here (everything else on them has happened by now); after a
+        // timeout a fence has to do for arrivals that were left over.
+        if (threadIdx.x == 0 && !*abort_flag) {
+            const uint64_t own = tile0 < g.tiles ? (uint64_t)((g.tiles - tile0 + tile_step - 1) / tile_step) : 0;
+            const uint64_t staged = own * (uint64_t)(kc1 - kc0), slotted = own * (uint64_t)(((kc1 + 1) >> 1) - (kc0 >> 1));
+            for (uint64_t i = 0; i < (uint64_t)g.stages; i++)
+                mbar_wait(bar(EMPTY) + 8u * (uint32_t)((staged + i) % g.stages), (uint32_t)((staged + i) / g.stages + 1) & 1u, abort_flag);
+            for (uint64_t i = 0; i < (uint64_t)g.slots; i++)
+                mbar_wait(bar(SLOT_EMPTY) + 8u * (uint32_t)((slotted + i) % g.slots), (uint32_t)((slotted + i) / g.slots + 1) & 1u, abort_flag);
+        }
+        if (*abort_flag) __threadfence();
+        cluster_sync_relaxed();
+    }
     if (threadIdx.x == 0 && *abort_flag) atomicOr(&g_head_error, 1u);
-    if constexpr (PAIR) cluster_sync_relaxed();   // neither CTA's shared or tensor memory goes away while the other may still use it
     if (!PAIR && g.splits > 1) {
         cluster_sync_all();
         // CTA `rank` adds the tokens rank, rank + splits, ... of all partial tiles, in rank order
