@@ -290,7 +290,7 @@ mxfp4_matmul_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_con
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
     __shared__ __align__(8) uint64_t s_bars[2 * kMaxStages + 4 + 2 * kMaxScaleBufs + 2 * kMaxSlots];
-    __shared__ uint32_t s_misc[2];
+    __shared__ uint32_t s_misc[6];   // tensor memory, abort flag; a pair: where the rings of stages and slots have got to
     const uint32_t sbase = smem_u32(smem), bar0 = smem_u32(s_bars);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     // FULL[s]: the codes of the stage have landed (even CTA of a pair: in both); EMPTY[s]: the MMAs that read it have completed;
@@ -371,6 +371,10 @@ mxfp4_matmul_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_con
                     tma_load_3d(dst + kWBytes, &tmap_a, kc * kRowBytes, a0, 0, full);
                     if (++s == (uint32_t)g.stages) { s = 0; ph ^= 1u; }
                 }
+            }
+            if constexpr (PAIR) {
+                s_misc[2] = s;
+                s_misc[3] = ph;
             }
             if (!ok)   // gave up: let the copies in flight land before the block goes away
                 for (uint32_t i = 0; i < (uint32_t)g.stages; i++)
@@ -617,6 +621,10 @@ mxfp4_matmul_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_con
                 if (++d == (uint32_t)g.scale_bufs) { d = 0; dph ^= 1u; }
                 if (++v == (uint32_t)g.slots) { v = 0; vph ^= 1u; }
             }
+        if (PAIR && warp == 4 && lane == 0) {
+            s_misc[4] = v;
+            s_misc[5] = vph;
+        }
     }
 
     __syncwarp();
@@ -626,13 +634,10 @@ mxfp4_matmul_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_con
         // Neither CTA's shared or tensor memory goes away while the other may still use it: nor while an arrival is on its way to it.  The last
         // releases of stages and slots, which no role waited for, are waited for here (everything else on them has happened by now); after a
         // timeout a fence has to do for arrivals that were left over.
-        if (threadIdx.x == 0 && !*abort_flag) {
-            const uint64_t own = tile0 < g.tiles ? (uint64_t)((g.tiles - tile0 + tile_step - 1) / tile_step) : 0;
-            const uint64_t staged = own * (uint64_t)(kc1 - kc0), slotted = own * (uint64_t)(((kc1 + 1) >> 1) - (kc0 >> 1));
-            for (uint64_t i = 0; i < (uint64_t)g.stages; i++)
-                mbar_wait(bar(EMPTY) + 8u * (uint32_t)((staged + i) % g.stages), (uint32_t)((staged + i) / g.stages + 1) & 1u, abort_flag);
-            for (uint64_t i = 0; i < (uint64_t)g.slots; i++)
-                mbar_wait(bar(SLOT_EMPTY) + 8u * (uint32_t)((slotted + i) % g.slots), (uint32_t)((slotted + i) / g.slots + 1) & 1u, abort_flag);
+        if (warp == 0 && !*abort_flag) {   // a lane a barrier
+            const bool slot = lane >= 16;
+            const uint32_t n = (uint32_t)(slot ? g.slots : g.stages), i = (uint32_t)lane & 15u, next = s_misc[slot ? 4 : 2] + i;
+            if (i < n) mbar_wait(bar(slot ? SLOT_EMPTY : EMPTY) + 8u * (next < n ? next : next - n), s_misc[slot ? 5 : 3] ^ (next < n ? 1u : 0u), abort_flag);
         }
         if (*abort_flag) __threadfence();
         cluster_sync_relaxed();
