@@ -107,12 +107,13 @@ mxfp4_quantize_kernel(const void* __restrict__ x_, int64_t n_units, uint32_t uni
             if (t == 0) bad = amax >= 0x7F800000u;   // infinite or NaN (whose sign bit is clear behind max.NaN)
             const int e = min(max((int)(amax >> 23) - 2 + ((amax & 0x7FFFFFu) > 0x400000u ? 1 : 0), 1), 253);
             const float inv = __uint_as_float((uint32_t)(254 - e) << 23), scl = __uint_as_float((uint32_t)e << 23);
+            const uint64_t inv2 = pair(inv, inv), minus_scl2 = pair(-scl, -scl);
             uint32_t w[PER / 8];
 #pragma unroll
             for (int i = 0; i < PER / 8; i++) {
                 float sv[8];
 #pragma unroll
-                for (int j = 0; j < 8; j++) sv[j] = v[8 * i + j] * inv;
+                for (int j = 0; j < 8; j += 2) unpair(mul2(pair(v[8 * i + j], v[8 * i + j + 1]), inv2), sv[j], sv[j + 1]);
                 const uint32_t c = e2m1_encode8(sv);
                 w[i] = bad ? 0u : c;
                 if (t + 1 < TERMS) {
@@ -121,7 +122,8 @@ mxfp4_quantize_kernel(const void* __restrict__ x_, int64_t n_units, uint32_t uni
                     float d[8];
                     e2m1_values(c, d);
 #pragma unroll
-                    for (int j = 0; j < 8; j++) v[8 * i + j] = __fmaf_rn(-(d[j] + 0.0f), scl, v[8 * i + j]);   // exact: the residual
+                    for (int j = 0; j < 8; j += 2)   // exact: the residual
+                        unpair(fma2(add2(pair(d[j], d[j + 1]), pair(0.0f, 0.0f)), minus_scl2, pair(v[8 * i + j], v[8 * i + j + 1])), v[8 * i + j], v[8 * i + j + 1]);
                 }
             }
             uint32_t* to = codes + ((int64_t)t * n_units + g) * (PER / 8);
