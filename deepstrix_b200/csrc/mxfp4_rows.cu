@@ -10,7 +10,7 @@
 // scale byte is 255 (E8M0's NaN), its codes are 0, and its later terms are 0.
 //
 // Both directions are bound by HBM where there is one term (65536 x 2048 f32: 88.7 us to codes, 6.85 TB/s, 97 us back, 6.25; bf16 52 and 54 us),
-// by arithmetic for more (8192 x 4096 bf16: 13.6 and 12.9 us with one term, 35.8 and 28.7 with three), and by latency below a megabyte (2 us).
+// by arithmetic for more (8192 x 4096 bf16: 13.6 and 12.8 us with one term, 32.7 and 27.6 with three), and by latency below a megabyte (2 us).
 #include <algorithm>
 
 #include "head.cuh"
@@ -70,7 +70,7 @@ __device__ __forceinline__ float abs_max_nan(float a, float b) {
 // A lane holds PER consecutive values -- 8 f32 or 16 of 16 bits, 32 bytes -- so four or two neighbouring lanes make a block of 32: loads
 // are coalesced, the block's maximum is a shuffle or two away, and what a block costs beside its values is shared by as many as registers
 // allow.  Units of PER are numbered through all rows, so a short row wastes no lane; a block never straddles two quads or pairs.  48 KB
-// of loads are in flight an SM; the arithmetic (7 instructions a value and term, 25 a lane and term) is what bounds two and three terms.
+// of loads are in flight an SM; the arithmetic (6 instructions a value and term, scaling and residual in pairs, 25 a lane and term) is what bounds two and three terms.
 template <int DT> constexpr int kPer = DT == DSX_F32 ? 8 : 16;
 
 template <int DT, int TERMS, bool VEC>
@@ -168,7 +168,10 @@ mxfp4_dequantize_kernel(const uint8_t* __restrict__ codes, const uint8_t* __rest
                 float d[PER];
                 e2m1_values(w[i][t], d);
 #pragma unroll
-                for (int j = 0; j < PER; j++) v[j] = t == 0 ? d[j] * s : __fmaf_rn(d[j], s, v[j]);   // the product is exact
+                for (int j = 0; j < PER; j += 2) {   // the product is exact
+                    const uint64_t p = pair(d[j], d[j + 1]), s2 = pair(s, s);
+                    unpair(t == 0 ? mul2(p, s2) : fma2(p, s2, pair(v[j], v[j + 1])), v[j], v[j + 1]);
+                }
             }
             int64_t off = g * PER;
             if (!dense) {
