@@ -149,8 +149,7 @@ struct alignas(16) Shared {
     int n_readers;                          // threads whose maximum reaches the threshold,
     int reader[NT];                         // in any order
     int count;                              // candidates that reach it
-    int pending[kWarps];                    // second pass: candidates on the warps' lists,
-    uint64_t warp_list[kWarps][96];         // at most 31 left over and two of every lane
+    uint64_t warp_list[kWarps][96];         // second pass: a warp's candidates, at most 31 left over and two of every lane
     alignas(16) uint64_t list[kList + 2];
     alignas(16) uint64_t cluster_list[NT == 64 ? 2 : kMaxCluster * kMaxAlt];   // first block of a cluster: the bests of all blocks,
     float sums[kMaxCluster][3];                                 // and their sums
@@ -369,21 +368,23 @@ token_logprobs_kernel(const void* __restrict__ logits, int64_t V, int64_t row_st
             uint64_t* list = sh.warp_list[warp];
             uint64_t mine = 0ull;
             uint32_t kth = 0u, own = threshold;   // order of the list's n_alt-th; the lowest order that may still enter it
-            if (lane == 0) sh.pending[warp] = 0;
-            __syncwarp();
-            auto flush = [&](bool all) {   // merge candidates 32 at a time; the rest stays (or goes too, padded with nothing)
-                int pending = *(volatile int*)&sh.pending[warp];
-                if (!all && pending < 32) return;
-                while (pending >= 32 || (all && pending > 0)) {
+            int pending = 0;   // on the list; the same in every lane, advanced by ballots: no lane can see another count than its neighbours
+            auto append = [&](bool in, float v, uint32_t i) {
+                const uint32_t who = __ballot_sync(0xFFFFFFFFu, in);
+                if (in) list[pending + __popc(who & ((1u << lane) - 1u))] = key_of(v, i);
+                pending += __popc(who);
+            };
+            auto flush = [&](int keep) {   // merge candidates 32 at a time until at most `keep` are left (the last ones padded with nothing)
+                if (pending <= keep) return;
+                __syncwarp();   // the list is written
+                while (pending > keep) {
                     const int n = min(pending, 32);
                     const uint64_t k = lane < n ? list[pending - n + lane] : 0ull;
                     pending -= n;
                     mine = merge32(mine, sort32(k, lane), lane);
                 }
-                __syncwarp();
                 kth = (uint32_t)(__shfl_sync(0xFFFFFFFFu, mine, n_alt - 1) >> 32);
-                if (lane == 0) sh.pending[warp] = pending;
-                __syncwarp();
+                __syncwarp();   // and read, before it is written again
             };
             for (uint32_t ch = first; ch - lane < n_chunks; ch += step) {
                 uint32_t w[8];
@@ -399,20 +400,18 @@ token_logprobs_kernel(const void* __restrict__ logits, int64_t V, int64_t row_st
                         for (int i = 0; i < kChunk / 2; i++)
                             if (i == j && any) Ch::two(w, i, v0, v1);
                         const float bar = value_of(max(own, kth));   // within a round an equal logit may have the lower index
-                        if (v0 >= bar) list[atomicAdd(&sh.pending[warp], 1)] = key_of(v0, head + ch * (uint32_t)kChunk + 2 * j);
-                        if (v1 >= bar) list[atomicAdd(&sh.pending[warp], 1)] = key_of(v1, head + ch * (uint32_t)kChunk + 2 * j + 1);
-                        __syncwarp();
-                        flush(false);
+                        append(v0 >= bar, v0, head + ch * (uint32_t)kChunk + 2 * j);
+                        append(v1 >= bar, v1, head + ch * (uint32_t)kChunk + 2 * j + 1);
+                        flush(31);
                     }
                     own = max(own, kth + 1u);
                 }
             }
-            if (has_extra) {   // some of these come before all others: an equal logit may win
-                const float v = to_f32(x[extra_at]);
-                if (v >= kLowest) list[atomicAdd(&sh.pending[warp], 1)] = key_of(v, (uint32_t)extra_at);
+            {   // some of these come before all others: an equal logit may win
+                const float v = has_extra ? to_f32(x[extra_at]) : -INFINITY;
+                append(v >= kLowest, v, (uint32_t)extra_at);
             }
-            __syncwarp();
-            flush(true);
+            flush(0);
             __syncthreads();
             sh.list[threadIdx.x] = mine;   // 256 of them
             __syncthreads();

@@ -521,3 +521,28 @@ def test_same_bits_on_every_call_and_stream(torch_cuda, moe):
         for out in outs:
             for p, r in zip(out, want):
                 assert torch.equal(p, r)
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16", "float16"])
+@pytest.mark.parametrize("T,V", [(6, 701), (6, 9001), (6, 131077), (1200, 4099)])
+def test_logprobs_long_candidate_lists(torch_cuda, moe, T, V, dtype):
+    """Rows of which far more logits reach the threshold than a block lists, so that warps keep their best in a second pass: few survivors of a
+    mask by the type's lowest value, steps that rise and fall in plateaus of uneven width, few levels, candidates on some lanes only."""
+    torch = torch_cuda
+    rng = np.random.default_rng(V)
+    lowest = float(torch.finfo(_dtype(torch, dtype)).min)
+    i = np.arange(V)
+    wide = np.zeros((T, V + 1), np.float32)      # V + 1: rows start at different addresses modulo 16
+    x = wide[:, :V]
+    x[0] = lowest
+    x[0, rng.choice(V, 3, replace=False)] = [1.0, 2.0, 1.0]
+    x[1] = np.cumsum(rng.random(V) < 1 / 37) * 0.125 - 40      # rises, plateaus of 1 to a few hundred
+    x[2] = -x[1] - 80
+    x[3] = rng.integers(0, 3, V)
+    x[4] = np.where(i // 8 % 5 == 0, np.minimum(i, 4000) * 0.0078125, lowest)   # rises on one chunk of five or so, then level
+    x[5] = np.where(rng.random(V) < 0.3, 0.0, -0.0)
+    x[6:] = x[np.arange(T - 6) % 6]
+    dx = torch.from_numpy(wide).cuda().to(_dtype(torch, dtype))[:, :V]
+    tokens = rng.integers(0, V, (T, 1)).astype(np.int32)
+    for n_alt in (1, 20, 32):
+        _check_logprobs(torch, dx, tokens, n_alt)
