@@ -16,7 +16,7 @@
 // takes 160 us, as words of 4 bytes 178; with K of 4096 and TMA 121.  Loaders that moved every other buffer to tensor memory as well: 168).  Scale warps, one per lane quarter, move a
 // buffer to a slot of tensor memory at a time (ld.shared + tcgen05.st; the tensor core's own copy would queue behind its MMAs); where TMA
 // brings the scales the loader warps are a second set of them, and the sets take alternate buffers: one set alone needed 800 clocks a stage.
-// Warp roles: TMA of codes, MMA issue, TMA of scales, 4 scale warps, 4 epilogue warps, 4 loaders or scale warps; two accumulators, so that a
+// Warp roles: TMA of codes, MMA issue, TMA of scales, one idle, 4 scale warps, 4 epilogue warps, 4 loaders or scale warps; two accumulators, so that a
 // tile is read out under the next one's MMAs.
 // Few tiles: the columns are split over the CTAs of a cluster; each leaves its partial tile in shared memory and the cluster adds
 // them in rank order through distributed shared memory, so results do not depend on timing and need no workspace.
@@ -60,6 +60,10 @@ __device__ __forceinline__ void mbar_init(uint32_t bar, uint32_t count) {
 __device__ __forceinline__ void mbar_expect_tx(uint32_t bar, uint32_t bytes) {
     asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
 }
+// Takes `bytes` off what a barrier's phase still expects, as a copy of that size would.
+__device__ __forceinline__ void mbar_complete_tx(uint32_t bar, uint32_t bytes) {
+    asm volatile("mbarrier.complete_tx.relaxed.cta.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
+}
 __device__ __forceinline__ void mbar_arrive(uint32_t bar) { asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory"); }
 __device__ __forceinline__ bool mbar_try(uint32_t bar, uint32_t parity) {
     uint32_t ok;
@@ -76,30 +80,47 @@ __device__ __forceinline__ bool mbar_try(uint32_t bar, uint32_t parity) {
 __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatile uint32_t* abort_flag) {
     for (uint32_t i = 0; i < kSpinLimit; i++) {
         if (mbar_try(bar, parity)) return true;
-        if ((i & 255u) == 255u && *abort_flag) return false;
+        if ((i & 15u) == 15u && *abort_flag) return false;
     }
     *abort_flag = 1u;
     return false;
 }
 // The same for a warp that goes on as one.  Its lanes may see the phase complete at different polls, and what follows (tcgen05 loads and
 // stores, MMAs from uniform registers) wants them together: hence the __syncwarp, and no branch on the outcome -- when the wait runs out the
-// warp goes on, and what it then computes is reported as missing.
-__device__ __forceinline__ void mbar_wait_on(uint32_t bar, uint32_t parity, volatile uint32_t* abort_flag) {
-    uint32_t i = 0;
-    for (; i < kSpinLimit; i++) {
-        if (mbar_try(bar, parity)) break;
-        if ((i & 255u) == 255u && *abort_flag) break;
+// warp goes on to the tile's end, and what it then computes is reported as missing.  `leader` is cleared in a lane whose wait ran out.
+__device__ __forceinline__ void mbar_wait_on(uint32_t bar, uint32_t parity, volatile uint32_t* abort_flag, uint32_t& leader) {
+    for (uint32_t i = 0; !mbar_try(bar, parity); i++) {
+        if (i < kSpinLimit && ((i & 15u) != 15u || !*abort_flag)) continue;
+        *abort_flag = 1u;
+        leader = 0u;
+        break;
     }
-    if (i == kSpinLimit) *abort_flag = 1u;
     __syncwarp();
 }
+__device__ __forceinline__ void mbar_wait_on(uint32_t bar, uint32_t parity, volatile uint32_t* abort_flag) {
+    uint32_t unused = 0u;
+    mbar_wait_on(bar, parity, abort_flag, unused);
+}
+// Whether a role of the block has given up, the same for all lanes: asked once a tile.
+__device__ __forceinline__ bool gave_up(volatile uint32_t* abort_flag) { return __any_sync(0xFFFFFFFFu, *abort_flag != 0u); }
+// PAIR: `bar` is a barrier of either CTA of a pair (a shared::cluster address); the copy's bytes count there.
+template <bool PAIR = false>
 __device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap* map, int c0, int c1, uint32_t bar) {
-    asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(dst), "l"(map),
+    if constexpr (PAIR)
+        asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.cta_group::2 [%0], [%1, {%2, %3}], [%4];" ::"r"(dst), "l"(map),
+                     "r"(c0), "r"(c1), "r"(bar)
+                     : "memory");
+    else asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(dst), "l"(map),
                  "r"(c0), "r"(c1), "r"(bar)
                  : "memory");
 }
+template <bool PAIR = false>
 __device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map, int c0, int c1, int c2, uint32_t bar) {
-    asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst),
+    if constexpr (PAIR)
+        asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.cta_group::2 [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst),
+                     "l"(map), "r"(c0), "r"(c1), "r"(c2), "r"(bar)
+                     : "memory");
+    else asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst),
                  "l"(map), "r"(c0), "r"(c1), "r"(c2), "r"(bar)
                  : "memory");
 }
@@ -120,8 +141,19 @@ __device__ __forceinline__ void tc_commit(uint32_t leader, uint32_t bar) {
             "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(bar), "r"(leader)
             : "memory");
 }
-// Arrival on a barrier of the other CTA of a pair.  Relaxed: what it reports (tensor-memory accesses this warp has waited for) is finished
-// before it issues, and a release at cluster scope holds the thread for about a microsecond.
+// The same, on a barrier of this CTA only.
+template <bool PAIR>
+__device__ __forceinline__ void tc_commit_here(uint32_t leader, uint32_t bar) {
+    if constexpr (PAIR)
+        asm volatile(
+            "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %1, 0;\n\t"
+            "@q tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(bar), "r"(leader)
+            : "memory");
+    else tc_commit<false>(leader, bar);
+}
+// Arrival on a barrier of the other CTA of a pair, for tensor-memory accesses of this warp and nothing else: waited for (tcgen05.wait) and
+// fenced (fence::before_thread_sync) they are ordered by a relaxed arrival, as the instruction set's own hand-over of tensor memory between
+// threads is.  What lies in shared memory is not: see the stage barriers.  (A release at cluster scope holds the thread for about a microsecond.)
 __device__ __forceinline__ void mbar_arrive_cluster(uint32_t cluster_bar) {
     asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_bar) : "memory");
 }
@@ -204,6 +236,7 @@ __device__ __forceinline__ uint32_t map_to_cta(uint32_t saddr, uint32_t cta) {
     asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(saddr), "r"(cta));
     return r;
 }
+__device__ __forceinline__ void st_cluster(uint32_t addr, uint32_t v) { asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(addr), "r"(v) : "memory"); }
 __device__ __forceinline__ float4 ld_cluster_f32x4(uint32_t addr) {
     float4 v;
     asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
@@ -280,8 +313,9 @@ struct MatmulArgs {
 };
 
 // PAIR: clusters of two CTAs.  A pair takes 256 W rows, 128 each, and every MMA spans both; each CTA loads and holds half of the tile's A
-// rows (and the scales of all of them).  The even CTA issues; each CTA's loads count on its own barriers, the scale warps of both report to
-// the even one, commits arrive in both.  No load is broadcast.
+// rows (and the scales of all of them).  The even CTA issues; the codes of both CTAs count on the even one's stage barriers -- so that the copies
+// themselves make both halves visible to the MMAs, no thread passing the word on --, scales on their own CTA's, the scale warps of both report
+// to the even one, commits arrive in both.  No load is broadcast.
 template <int DT, int TERMS, bool PAIR>
 __global__ void __launch_bounds__(kThreads, PAIR ? 1 : 2)
 mxfp4_matmul_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_ws,
@@ -289,20 +323,22 @@ mxfp4_matmul_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_con
     using T = typename Elem<DT>::T;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
-    __shared__ __align__(8) uint64_t s_bars[2 * kMaxStages + 4 + 2 * kMaxScaleBufs + 2 * kMaxSlots];
-    __shared__ uint32_t s_misc[6];   // tensor memory, abort flag; a pair: where the rings of stages and slots have got to
+    __shared__ __align__(8) uint64_t s_bars[2 * kMaxStages + 4 + 2 * kMaxScaleBufs + 2 * kMaxSlots + 1];
+    // tensor memory, abort flag; a pair: where the rings of stages (and how many loads that were) and slots have got to; the odd CTA's stages
+    __shared__ uint32_t s_misc[10];
     const uint32_t sbase = smem_u32(smem), bar0 = smem_u32(s_bars);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    // FULL[s]: the codes of the stage have landed (even CTA of a pair: in both); EMPTY[s]: the MMAs that read it have completed;
+    // FULL[s]: the codes of the stage have landed (even CTA of a pair: in both; odd one: not used); EMPTY[s]: the MMAs that read it have completed;
     // ACC_FULL / ACC_EMPTY[b]: accumulator b is complete / read out; RAW_FULL / RAW_EMPTY[d]: two stages' scales have landed / are in tensor
     // memory; SLOT_FULL / SLOT_EMPTY[v]: and lie in slot v (a pair: of both CTAs) / the MMAs that used them have completed.
     constexpr int FULL = 0, EMPTY = FULL + kMaxStages, ACC_FULL = EMPTY + kMaxStages, ACC_EMPTY = ACC_FULL + 2, RAW_FULL = ACC_EMPTY + 2,
-                  RAW_EMPTY = RAW_FULL + kMaxScaleBufs, SLOT_FULL = RAW_EMPTY + kMaxScaleBufs, SLOT_EMPTY = SLOT_FULL + kMaxSlots;
+                  RAW_EMPTY = RAW_FULL + kMaxScaleBufs, SLOT_FULL = RAW_EMPTY + kMaxScaleBufs, SLOT_EMPTY = SLOT_FULL + kMaxSlots,
+                  DRAIN = SLOT_EMPTY + kMaxSlots;   // DRAIN: the MMAs issued before this block gave up have completed
     auto bar = [&](int i) { return bar0 + 8u * (uint32_t)i; };
     volatile uint32_t* abort_flag = s_misc + 1;
     if (threadIdx.x == 0) {
         for (int i = 0; i < kMaxStages; i++) {
-            mbar_init(bar(FULL + i), PAIR && cluster_ctarank() == 0 ? 2 : 1);   // + the odd CTA's report
+            mbar_init(bar(FULL + i), 1);
             mbar_init(bar(EMPTY + i), 1);
         }
         for (int b = 0; b < 2; b++) {
@@ -317,6 +353,7 @@ mxfp4_matmul_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_con
             mbar_init(bar(SLOT_FULL + v), PAIR ? 8 : 4);
             mbar_init(bar(SLOT_EMPTY + v), 1);
         }
+        mbar_init(bar(DRAIN), 1);
         *abort_flag = 0u;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         asm volatile("prefetch.tensormap [%0];" ::"l"(&tmap_w) : "memory");
@@ -358,25 +395,29 @@ mxfp4_matmul_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_con
     if (warp == 0) {
         // -------------------------------------------------------------- producer
         if (lane == 0) {
-            uint32_t s = 0, ph = 0;
+            uint32_t s = 0, ph = 0, n_loads = 0;
             bool ok = true;
+            const uint32_t full0 = PAIR ? map_to_cta(bar(FULL), 0u) : bar(FULL);
             for (int tile = tile0; tile < g.tiles && ok; tile += tile_step) {
                 const int w0 = (tile % g.tiles_w) * kTileW + half * kWRows, a0 = (tile / g.tiles_w) * tokens + half * held;
                 for (int kc = kc0; kc < kc1; kc++) {
                     ok = mbar_wait(bar(EMPTY) + 8u * s, ph ^ 1u, abort_flag);
                     if (!ok) break;
-                    const uint32_t dst = sbase + s * (uint32_t)g.stage_bytes, full = bar(FULL) + 8u * s;
-                    mbar_expect_tx(full, kWBytes + b_bytes);
-                    tma_load_2d(dst, &tmap_w, kc * kRowBytes, w0, full);
-                    tma_load_3d(dst + kWBytes, &tmap_a, kc * kRowBytes, a0, 0, full);
+                    const uint32_t dst = sbase + s * (uint32_t)g.stage_bytes, full = full0 + 8u * s;
+                    // The even CTA of a pair announces both halves.  (The odd one's may land first: the barrier's phase cannot end before the
+                    // announcement, and the odd CTA's next load of the stage waits for the MMAs of that phase.)
+                    if (half == 0) mbar_expect_tx(bar(FULL) + 8u * s, (PAIR ? 2u : 1u) * (kWBytes + b_bytes));
+                    tma_load_2d<PAIR>(dst, &tmap_w, kc * kRowBytes, w0, full);
+                    tma_load_3d<PAIR>(dst + kWBytes, &tmap_a, kc * kRowBytes, a0, 0, full);
+                    n_loads++;
                     if (++s == (uint32_t)g.stages) { s = 0; ph ^= 1u; }
                 }
             }
             if constexpr (PAIR) {
                 s_misc[2] = s;
                 s_misc[3] = ph;
-            }
-            if (!ok)   // gave up: let the copies in flight land before the block goes away
+                s_misc[6] = n_loads;
+            } else if (!ok)   // gave up: let the copies in flight land before the block goes away
                 for (uint32_t i = 0; i < (uint32_t)g.stages; i++)
                     for (uint32_t n = 0; n < kSpinLimit / 64 && !mbar_try(bar(FULL) + 8u * i, i < s ? ph : ph ^ 1u); n++) {}
         }
@@ -386,7 +427,7 @@ mxfp4_matmul_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_con
         // inside a branch of one lane each of them had to be carried there first -- 230 clocks an MMA, whatever its size, against 50.  This
         // warp bounds large products: a pair's stage takes it 580 clocks (four MMAs 200, a satisfied wait 80 each, a commit 35) with MMAs of
         // N = 208, which run 424, as of N = 16, with and without the copies and the scales.  Two warps that took turns were no faster.
-        const uint32_t leader = lane == 0 ? 1u : 0u;
+        uint32_t leader = lane == 0 ? 1u : 0u;   // cleared for good when a wait runs out: no MMA and no commit from there on
         uint32_t s = 0, ph = 0, t = 0, v = 0, vph = 0;
         const uint64_t d0 = operand_desc(sbase);
         const uint32_t hi = (uint32_t)(d0 >> 32), lo0 = (uint32_t)d0;
@@ -396,9 +437,10 @@ mxfp4_matmul_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_con
         const uint32_t quarter = nb == 2 ? 8u : 4u;   // columns of a quarter of A's scales
         const uint32_t idesc0 = mxf4_idesc(kTileW, BN, 0u), idesc2 = mxf4_idesc(kTileW, BN, 2u);
         for (int tile = tile0; tile < g.tiles && half == 0; tile += tile_step, t++) {
+            if (gave_up(abort_flag)) break;
             const uint32_t b = t & 1u, acc = tm + b * (uint32_t)BN;
             uint32_t started = 0u;
-            mbar_wait_on(bar(ACC_EMPTY) + 8u * b, ((t >> 1) & 1u) ^ 1u, abort_flag);
+            mbar_wait_on(bar(ACC_EMPTY) + 8u * b, ((t >> 1) & 1u) ^ 1u, abort_flag, leader);
             tc_fence_after();
             // the MMAs of one stage, the slot's first or second half
             auto stage = [&](uint32_t at, int kc, int h) {
@@ -423,12 +465,12 @@ mxfp4_matmul_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_con
                 started = 1u;
             };
             for (int kc = kc0; kc < kc1;) {   // a slot of scales at a time: its waits first, then the MMAs of both stages
-                mbar_wait_on(bar(SLOT_FULL) + 8u * v, vph, abort_flag);
-                mbar_wait_on(bar(FULL) + 8u * s, ph, abort_flag);
+                mbar_wait_on(bar(SLOT_FULL) + 8u * v, vph, abort_flag, leader);
+                mbar_wait_on(bar(FULL) + 8u * s, ph, abort_flag, leader);
                 const uint32_t s0 = s;
                 if (++s == (uint32_t)g.stages) { s = 0; ph ^= 1u; }
                 if ((kc & 1) == 0 && kc + 1 < kc1) {
-                    mbar_wait_on(bar(FULL) + 8u * s, ph, abort_flag);
+                    mbar_wait_on(bar(FULL) + 8u * s, ph, abort_flag, leader);
                     tc_fence_after();
                     stage(s0, kc, 0);
                     tc_commit<PAIR>(leader, bar(EMPTY) + 8u * s0);
@@ -447,8 +489,10 @@ mxfp4_matmul_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_con
             }
             tc_commit<PAIR>(leader, bar(ACC_FULL) + 8u * b);
         }
-        if (*abort_flag && t > 0)   // somebody gave up: let the MMAs in flight finish before tensor memory goes away
-            for (uint32_t n = 0; n < kSpinLimit / 64 && !mbar_try(bar(ACC_FULL) + 8u * ((t - 1u) & 1u), ((t - 1u) >> 1) & 1u); n++) {}
+        if (half == 0 && gave_up(abort_flag)) {   // let the MMAs in flight finish before tensor memory and operands go away
+            tc_commit_here<PAIR>(lane == 0 ? 1u : 0u, bar(DRAIN));
+            for (uint32_t n = 0; n < kSpinLimit / 64 && !mbar_try(bar(DRAIN), 0u); n++) {}
+        }
         __syncwarp();
     } else if (warp == 2) {
         // --------------------------------------------------------- TMA of scales
@@ -472,18 +516,7 @@ mxfp4_matmul_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_con
                     for (uint32_t n = 0; n < kSpinLimit / 64 && !mbar_try(bar(RAW_FULL) + 8u * i, i < d ? ph : ph ^ 1u); n++) {}
         }
     } else if (warp == 3) {
-        // ------------------------------ odd CTA of a pair: its landed stages reported to the even one
-        if (PAIR && half != 0 && lane == 0) {
-            uint32_t s = 0, ph = 0;
-            bool ok = true;
-            for (int tile = tile0; tile < g.tiles && ok; tile += tile_step)
-                for (int kc = kc0; kc < kc1; kc++) {
-                    ok = mbar_wait(bar(FULL) + 8u * s, ph, abort_flag);
-                    if (!ok) break;
-                    mbar_arrive_cluster(map_to_cta(bar(FULL) + 8u * s, 0u));
-                    if (++s == (uint32_t)g.stages) { s = 0; ph ^= 1u; }
-                }
-        }
+        // idle: roles that use whole warp groups start on their boundaries
     } else if (warp >= kLoadWarp0 && !g.scale_tma) {
         // --------------------------------------------------------- scale loaders
         {
@@ -553,7 +586,7 @@ mxfp4_matmul_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_con
         // -------------------------------------------------------------- epilogue
         const uint32_t q = (uint32_t)(warp & 3);
         uint32_t t = 0;
-        for (int tile = tile0; tile < g.tiles; tile += tile_step, t++) {
+        for (int tile = tile0; tile < g.tiles && !gave_up(abort_flag); tile += tile_step, t++) {
             const int64_t n = (int64_t)(tile % g.tiles_w) * kTileW + half * kWRows + q * 32 + lane, m0 = (int64_t)(tile / g.tiles_w) * tokens;
             const uint32_t b = t & 1u, acc = tmem + b * (uint32_t)BN + ((q * 32u) << 16);
             mbar_wait_on(bar(ACC_FULL) + 8u * b, (t >> 1) & 1u, abort_flag);
@@ -595,7 +628,7 @@ mxfp4_matmul_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_con
         const uint32_t q = (uint32_t)(warp & 3);
         const uint32_t set = warp >= kLoadWarp0 ? 1u : 0u, sets = g.scale_tma ? 2u : 1u;
         uint32_t u = 0, d = 0, dph = 0, v = 0, vph = 0;   // buffers so far; ring positions
-        for (int tile = tile0; tile < g.tiles; tile += tile_step)
+        for (int tile = tile0; tile < g.tiles && !gave_up(abort_flag); tile += tile_step)
             for (int kc = kc0; kc < kc1; kc = (kc | 1) + 1, u++) {
                 if (sets == 1u || (u & 1u) == set) {
                     mbar_wait_on(bar(RAW_FULL) + 8u * d, dph, abort_flag);
@@ -632,15 +665,43 @@ mxfp4_matmul_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_con
     __syncthreads();
     if constexpr (PAIR) {
         // Neither CTA's shared or tensor memory goes away while the other may still use it: nor while an arrival is on its way to it.  The last
-        // releases of stages and slots, which no role waited for, are waited for here (everything else on them has happened by now); after a
-        // timeout a fence has to do for arrivals that were left over.
-        if (warp == 0 && !*abort_flag) {   // a lane a barrier
+        // releases of stages and slots, which no role waited for, are waited for here (everything else on them has happened by now).
+        const uint32_t other = (uint32_t)half ^ 1u;
+        if (warp == 0 && !gave_up(abort_flag)) {   // a lane a barrier
             const bool slot = lane >= 16;
             const uint32_t n = (uint32_t)(slot ? g.slots : g.stages), i = (uint32_t)lane & 15u, next = s_misc[slot ? 4 : 2] + i;
             if (i < n) mbar_wait(bar(slot ? SLOT_EMPTY : EMPTY) + 8u * (next < n ? next : next - n), s_misc[slot ? 5 : 3] ^ (next < n ? 1u : 0u), abort_flag);
         }
-        if (*abort_flag) __threadfence();
+        if (warp == 0) {
+            __syncwarp();
+            if (gave_up(abort_flag) && lane == 0) {   // the other CTA hears of it
+                st_cluster(map_to_cta(smem_u32(s_misc + 1), other), 1u);
+                __threadfence();
+            }
+        }
         cluster_sync_relaxed();
+        if (*abort_flag) {   // from here on the same in both
+            // Copies may be in flight, on the even CTA's barriers.  It gets to know how far the odd one came, and makes up for what a stage that
+            // only one of them has asked for still lacks, so that the stage's phase ends when the copies that were made have landed.  (Neither
+            // can be further ahead than the ring is long: nothing was released by the MMA warp since its first wait ran out.)
+            if (threadIdx.x == 0 && half != 0) {
+                for (uint32_t i = 0; i < 2; i++) st_cluster(map_to_cta(smem_u32(s_misc + 7 + i), 0u), s_misc[2 + i]);
+                st_cluster(map_to_cta(smem_u32(s_misc + 9), 0u), s_misc[6]);
+            }
+            cluster_sync_all();
+            if (threadIdx.x == 0 && half == 0) {
+                const int ahead = (int)(s_misc[6] - s_misc[9]);   // loads this CTA asked for and the odd one did not
+                uint32_t s = s_misc[ahead >= 0 ? 2 : 7], ph = s_misc[ahead >= 0 ? 3 : 8];
+                for (int i = 1; i <= g.stages; i++) {   // back from the last load
+                    if (s == 0) { s = (uint32_t)g.stages; ph ^= 1u; }
+                    const uint32_t full = bar(FULL) + 8u * --s;
+                    if (i <= ahead) mbar_complete_tx(full, kWBytes + b_bytes);
+                    else if (i <= -ahead) mbar_expect_tx(full, kWBytes + b_bytes);
+                    for (uint32_t n = 0; n < kSpinLimit / 64 && !mbar_try(full, ph); n++) {}
+                }
+            }
+            cluster_sync_all();
+        }
     }
     if (threadIdx.x == 0 && *abort_flag) atomicOr(&g_head_error, 1u);
     if (!PAIR && g.splits > 1) {

@@ -546,3 +546,26 @@ def test_logprobs_long_candidate_lists(torch_cuda, moe, T, V, dtype):
     tokens = rng.integers(0, V, (T, 1)).astype(np.int32)
     for n_alt in (1, 20, 32):
         _check_logprobs(torch, dx, tokens, n_alt)
+
+
+@pytest.mark.parametrize("m,n,k,terms", [(4100, 4100, 1024, 1), (4100, 4100, 1536, 2), (4100, 4100, 1024, 3), (2100, 5003, 1056, 1), (2050, 2100, 1536, 3)])
+def test_matmul_pairs_of_ctas_exact_sums(torch_cuda, moe, m, n, k, terms):
+    """Products large enough for pairs of CTAs, several tiles a pair, scales by TMA and by loaders; exact for the same reason as above.  Twice
+    on two streams at once: each CTA of a pair reads what the other one's copies brought."""
+    torch = torch_cuda
+    from deepstrix_b200 import head
+    rng = np.random.default_rng(m + n + k + terms)
+    a, av = _rows(torch, rng, m, k, terms, 126, 129)
+    w, wv = _rows(torch, rng, n, k, 1, 126, 129)
+    want = torch.from_numpy(av.sum(0)).cuda() @ torch.from_numpy(wv[0]).cuda().T      # f64: exact
+    assert float(want.abs().max()) * 16 < 2 ** 22
+    want = want.float()
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream() for _ in range(2)], []
+    for i in range(4):
+        with torch.cuda.stream(streams[i % 2]):
+            got.append(head.Mxfp4Matmul.launch(a, w, torch.float32))
+    torch.cuda.synchronize()
+    for g in got:
+        assert torch.equal(g, want)
+    assert torch.equal(head.Mxfp4Matmul.launch(a, w, torch.bfloat16), want.to(torch.bfloat16))
