@@ -51,7 +51,8 @@ constexpr int kMaxScaleBufs = 4;     // two or four: see plan_block
 constexpr int kMaxSlots = 4;         // of scales in tensor memory, two stages each
 constexpr int kMaxStages = 8;
 constexpr int kMaxN = 208;           // of an MMA: two accumulators and two scale slots fill tensor memory
-constexpr uint32_t kSpinLimit = 1u << 22;
+constexpr uint32_t kPolls = 1u << 22;     // of a wait
+constexpr uint32_t kDrainPolls = 1u << 16;   // for what is in flight when a block has given up
 
 __device__ __forceinline__ uint32_t smem_u32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
 __device__ __forceinline__ void mbar_init(uint32_t bar, uint32_t count) {
@@ -76,30 +77,35 @@ __device__ __forceinline__ bool mbar_try(uint32_t bar, uint32_t parity) {
         : "memory");
     return ok != 0;
 }
+// How long a wait lasts, and where a role that has given up says so to the others of its block.
+struct Patience {
+    volatile uint32_t* abort_flag;
+    uint32_t polls;
+};
 // Bounded wait that also gives up when another role of the block has.
-__device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatile uint32_t* abort_flag) {
-    for (uint32_t i = 0; i < kSpinLimit; i++) {
+__device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, const Patience& p) {
+    for (uint32_t i = 0; i < p.polls; i++) {
         if (mbar_try(bar, parity)) return true;
-        if ((i & 15u) == 15u && *abort_flag) return false;
+        if ((i & 15u) == 15u && *p.abort_flag) return false;
     }
-    *abort_flag = 1u;
+    *p.abort_flag = 1u;
     return false;
 }
 // The same for a warp that goes on as one.  Its lanes may see the phase complete at different polls, and what follows (tcgen05 loads and
 // stores, MMAs from uniform registers) wants them together: hence the __syncwarp, and no branch on the outcome -- when the wait runs out the
 // warp goes on to the tile's end, and what it then computes is reported as missing.  `leader` is cleared in a lane whose wait ran out.
-__device__ __forceinline__ void mbar_wait_on(uint32_t bar, uint32_t parity, volatile uint32_t* abort_flag, uint32_t& leader) {
+__device__ __forceinline__ void mbar_wait_on(uint32_t bar, uint32_t parity, const Patience& p, uint32_t& leader) {
     for (uint32_t i = 0; !mbar_try(bar, parity); i++) {
-        if (i < kSpinLimit && ((i & 15u) != 15u || !*abort_flag)) continue;
-        *abort_flag = 1u;
+        if (i < p.polls && ((i & 15u) != 15u || !*p.abort_flag)) continue;
+        *p.abort_flag = 1u;
         leader = 0u;
         break;
     }
     __syncwarp();
 }
-__device__ __forceinline__ void mbar_wait_on(uint32_t bar, uint32_t parity, volatile uint32_t* abort_flag) {
+__device__ __forceinline__ void mbar_wait_on(uint32_t bar, uint32_t parity, const Patience& p) {
     uint32_t unused = 0u;
-    mbar_wait_on(bar, parity, abort_flag, unused);
+    mbar_wait_on(bar, parity, p, unused);
 }
 // Whether a role of the block has given up, the same for all lanes: asked once a tile.
 __device__ __forceinline__ bool gave_up(volatile uint32_t* abort_flag) { return __any_sync(0xFFFFFFFFu, *abort_flag != 0u); }
@@ -310,6 +316,7 @@ struct MatmulArgs {
     int tiles_w, tiles;      // tile t: W tile t % tiles_w, token tile t / tiles_w
     int scale_tma;           // rows of scales are 16-byte aligned: TMA brings them
     int pairs;               // results are 16-bit and pairs of columns 4-byte aligned in every row
+    uint32_t polls;          // of a wait
 };
 
 // PAIR: clusters of two CTAs.  A pair takes 256 W rows, 128 each, and every MMA spans both; each CTA loads and holds half of the tile's A
@@ -336,6 +343,7 @@ mxfp4_matmul_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_con
                   DRAIN = SLOT_EMPTY + kMaxSlots;   // DRAIN: the MMAs issued before this block gave up have completed
     auto bar = [&](int i) { return bar0 + 8u * (uint32_t)i; };
     volatile uint32_t* abort_flag = s_misc + 1;
+    const Patience patience{abort_flag, g.polls};
     if (threadIdx.x == 0) {
         for (int i = 0; i < kMaxStages; i++) {
             mbar_init(bar(FULL + i), 1);
@@ -401,7 +409,7 @@ mxfp4_matmul_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_con
             for (int tile = tile0; tile < g.tiles && ok; tile += tile_step) {
                 const int w0 = (tile % g.tiles_w) * kTileW + half * kWRows, a0 = (tile / g.tiles_w) * tokens + half * held;
                 for (int kc = kc0; kc < kc1; kc++) {
-                    ok = mbar_wait(bar(EMPTY) + 8u * s, ph ^ 1u, abort_flag);
+                    ok = mbar_wait(bar(EMPTY) + 8u * s, ph ^ 1u, patience);
                     if (!ok) break;
                     const uint32_t dst = sbase + s * (uint32_t)g.stage_bytes, full = full0 + 8u * s;
                     // The even CTA of a pair announces both halves.  (The odd one's may land first: the barrier's phase cannot end before the
@@ -419,7 +427,7 @@ mxfp4_matmul_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_con
                 s_misc[6] = n_loads;
             } else if (!ok)   // gave up: let the copies in flight land before the block goes away
                 for (uint32_t i = 0; i < (uint32_t)g.stages; i++)
-                    for (uint32_t n = 0; n < kSpinLimit / 64 && !mbar_try(bar(FULL) + 8u * i, i < s ? ph : ph ^ 1u); n++) {}
+                    for (uint32_t n = 0; n < kDrainPolls && !mbar_try(bar(FULL) + 8u * i, i < s ? ph : ph ^ 1u); n++) {}
         }
     } else if (warp == 1) {
         // ------------------------------------------------------------- MMA issue
@@ -440,7 +448,7 @@ mxfp4_matmul_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_con
             if (gave_up(abort_flag)) break;
             const uint32_t b = t & 1u, acc = tm + b * (uint32_t)BN;
             uint32_t started = 0u;
-            mbar_wait_on(bar(ACC_EMPTY) + 8u * b, ((t >> 1) & 1u) ^ 1u, abort_flag, leader);
+            mbar_wait_on(bar(ACC_EMPTY) + 8u * b, ((t >> 1) & 1u) ^ 1u, patience, leader);
             tc_fence_after();
             // the MMAs of one stage, the slot's first or second half
             auto stage = [&](uint32_t at, int kc, int h) {
@@ -465,12 +473,12 @@ mxfp4_matmul_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_con
                 started = 1u;
             };
             for (int kc = kc0; kc < kc1;) {   // a slot of scales at a time: its waits first, then the MMAs of both stages
-                mbar_wait_on(bar(SLOT_FULL) + 8u * v, vph, abort_flag, leader);
-                mbar_wait_on(bar(FULL) + 8u * s, ph, abort_flag, leader);
+                mbar_wait_on(bar(SLOT_FULL) + 8u * v, vph, patience, leader);
+                mbar_wait_on(bar(FULL) + 8u * s, ph, patience, leader);
                 const uint32_t s0 = s;
                 if (++s == (uint32_t)g.stages) { s = 0; ph ^= 1u; }
                 if ((kc & 1) == 0 && kc + 1 < kc1) {
-                    mbar_wait_on(bar(FULL) + 8u * s, ph, abort_flag, leader);
+                    mbar_wait_on(bar(FULL) + 8u * s, ph, patience, leader);
                     tc_fence_after();
                     stage(s0, kc, 0);
                     tc_commit<PAIR>(leader, bar(EMPTY) + 8u * s0);
@@ -491,7 +499,7 @@ mxfp4_matmul_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_con
         }
         if (half == 0 && gave_up(abort_flag)) {   // let the MMAs in flight finish before tensor memory and operands go away
             tc_commit_here<PAIR>(lane == 0 ? 1u : 0u, bar(DRAIN));
-            for (uint32_t n = 0; n < kSpinLimit / 64 && !mbar_try(bar(DRAIN), 0u); n++) {}
+            for (uint32_t n = 0; n < kDrainPolls && !mbar_try(bar(DRAIN), 0u); n++) {}
         }
         __syncwarp();
     } else if (warp == 2) {
@@ -502,7 +510,7 @@ mxfp4_matmul_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_con
             for (int tile = tile0; tile < g.tiles && ok; tile += tile_step) {
                 const int w0 = (tile % g.tiles_w) * kTileW + half * kWRows, a0 = (tile / g.tiles_w) * tokens;
                 for (int kc = kc0 & ~1; kc < kc1; kc += 2) {
-                    ok = mbar_wait(bar(RAW_EMPTY) + 8u * d, ph ^ 1u, abort_flag);
+                    ok = mbar_wait(bar(RAW_EMPTY) + 8u * d, ph ^ 1u, patience);
                     if (!ok) break;
                     const uint32_t dst = sbase + raw0 + d * raw_bytes, full = bar(RAW_FULL) + 8u * d;
                     mbar_expect_tx(full, kGroupBytes + (uint32_t)(TERMS * BN * 16));
@@ -513,7 +521,7 @@ mxfp4_matmul_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_con
             }
             if (!ok)
                 for (uint32_t i = 0; i < (uint32_t)g.scale_bufs; i++)
-                    for (uint32_t n = 0; n < kSpinLimit / 64 && !mbar_try(bar(RAW_FULL) + 8u * i, i < d ? ph : ph ^ 1u); n++) {}
+                    for (uint32_t n = 0; n < kDrainPolls && !mbar_try(bar(RAW_FULL) + 8u * i, i < d ? ph : ph ^ 1u); n++) {}
         }
     } else if (warp == 3) {
         // idle: roles that use whole warp groups start on their boundaries
@@ -552,7 +560,7 @@ mxfp4_matmul_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_con
                     next[i] = word(row[i], (kc0 >> 1) + 1);
                 }
                 for (int kc = kc0 & ~1; kc < kc1; kc += 2) {
-                    ok = mbar_wait(bar(RAW_EMPTY) + 8u * d, ph ^ 1u, abort_flag);
+                    ok = mbar_wait(bar(RAW_EMPTY) + 8u * d, ph ^ 1u, patience);
                     if (!ok) break;
                     const uint32_t dst = sbase + raw0 + d * raw_bytes + (uint32_t)r * 16u;
                     const int n = nblk - kc * 8;   // bytes past the row's end belong to the next row
@@ -589,7 +597,7 @@ mxfp4_matmul_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_con
         for (int tile = tile0; tile < g.tiles && !gave_up(abort_flag); tile += tile_step, t++) {
             const int64_t n = (int64_t)(tile % g.tiles_w) * kTileW + half * kWRows + q * 32 + lane, m0 = (int64_t)(tile / g.tiles_w) * tokens;
             const uint32_t b = t & 1u, acc = tmem + b * (uint32_t)BN + ((q * 32u) << 16);
-            mbar_wait_on(bar(ACC_FULL) + 8u * b, (t >> 1) & 1u, abort_flag);
+            mbar_wait_on(bar(ACC_FULL) + 8u * b, (t >> 1) & 1u, patience);
             tc_fence_after();
             const int rows = (int)min((int64_t)tokens, g.M - m0);     // tokens that exist
             T* o = reinterpret_cast<T*>(g.out) + m0 * g.row_stride + n;
@@ -631,8 +639,8 @@ mxfp4_matmul_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_con
         for (int tile = tile0; tile < g.tiles && !gave_up(abort_flag); tile += tile_step)
             for (int kc = kc0; kc < kc1; kc = (kc | 1) + 1, u++) {
                 if (sets == 1u || (u & 1u) == set) {
-                    mbar_wait_on(bar(RAW_FULL) + 8u * d, dph, abort_flag);
-                    mbar_wait_on(bar(SLOT_EMPTY) + 8u * v, vph ^ 1u, abort_flag);
+                    mbar_wait_on(bar(RAW_FULL) + 8u * d, dph, patience);
+                    mbar_wait_on(bar(SLOT_EMPTY) + 8u * v, vph ^ 1u, patience);
                     tc_fence_after();
                     const uint8_t* src = smem + raw0 + d * raw_bytes + lane * 16;
                     const uint32_t dst = slot0 + v * slot_cols + ((q * 32u) << 16);
@@ -670,7 +678,7 @@ mxfp4_matmul_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_con
         if (warp == 0 && !gave_up(abort_flag)) {   // a lane a barrier
             const bool slot = lane >= 16;
             const uint32_t n = (uint32_t)(slot ? g.slots : g.stages), i = (uint32_t)lane & 15u, next = s_misc[slot ? 4 : 2] + i;
-            if (i < n) mbar_wait(bar(slot ? SLOT_EMPTY : EMPTY) + 8u * (next < n ? next : next - n), s_misc[slot ? 5 : 3] ^ (next < n ? 1u : 0u), abort_flag);
+            if (i < n) mbar_wait(bar(slot ? SLOT_EMPTY : EMPTY) + 8u * (next < n ? next : next - n), s_misc[slot ? 5 : 3] ^ (next < n ? 1u : 0u), patience);
         }
         if (warp == 0) {
             __syncwarp();
@@ -697,7 +705,7 @@ mxfp4_matmul_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_con
                     const uint32_t full = bar(FULL) + 8u * --s;
                     if (i <= ahead) mbar_complete_tx(full, kWBytes + b_bytes);
                     else if (i <= -ahead) mbar_expect_tx(full, kWBytes + b_bytes);
-                    for (uint32_t n = 0; n < kSpinLimit / 64 && !mbar_try(full, ph); n++) {}
+                    for (uint32_t n = 0; n < kDrainPolls && !mbar_try(full, ph); n++) {}
                 }
             }
             cluster_sync_all();
@@ -787,17 +795,25 @@ struct Device {
     int clusters[4];   // [log2 of the size]
 };
 
+// A tiling set by dsx_mxfp4_matmul_pin: -1 and 0 leave a part to the model.
+struct Pin {
+    int8_t pair = -1;
+    uint8_t tokens = 0, splits = 0, unused = 0;
+};
+std::atomic<Pin> g_pin{Pin{}};
+
 // Tokens a tile, pairs or single CTAs, and splits of the columns, from a model of the time in clocks.  A stage takes its MMAs on the tensor
 // core (N / 2 clocks each, 50 at least), or the issuing warp's 50 an MMA and what surrounds them (two blocks on an SM issue side by side), or
 // its copies at 80 bytes a clock and SM from L2; a round of tiles about 5500 clocks before and after its stages, a joined tile another 2500;
 // and the operands come from HBM at 26 bytes a clock and SM.  The constants were fitted to 600 tilings of 40 products, of 1 to 8192 tokens and 3
 // to 131072 rows of W: the model's choice is 0.5 % slower than the best of them on average, 16 % at worst (3176 x 3 x 3104).
-bool make_plan(int64_t M, int64_t N, int K, int terms, const Device& dev, Plan* best) {
+bool make_plan(int64_t M, int64_t N, int K, int terms, const Device& dev, const Pin& pin, Plan* best) {
     const int n_kc = (K + kStageK - 1) / kStageK;
     double best_t = 1e300;
     for (int pair = 0; pair <= 1; pair++)
-        for (int tokens = 16; tokens <= kMaxN && tokens < M + 16; tokens += 16) {
+        for (int tokens = 16; tokens <= kMaxN && (tokens < M + 16 || tokens == pin.tokens); tokens += 16) {
             Plan p;
+            if ((pin.pair >= 0 && pair != pin.pair) || (pin.tokens > 0 && tokens != pin.tokens)) continue;
             if (!plan_block(terms, tokens, pair != 0, &p)) continue;
             p.tiles_w = (int)((N + kWRows * (1 + pair) - 1) / (kWRows * (1 + pair)));
             p.tiles_m = (int)((M + tokens - 1) / tokens);
@@ -807,6 +823,7 @@ bool make_plan(int64_t M, int64_t N, int K, int terms, const Device& dev, Plan* 
             const double stage = std::max({tensor, issue, p.stage_bytes / 80.0});
             const double hbm = ((double)N + (double)terms * M) * K * 17 / 32 / (26.0 * dev.sms);
             for (int l = 0; l <= (pair ? 0 : 3) && 1 << l <= n_kc; l++) {
+                if (pin.splits > 0 && 1 << l != pin.splits) continue;
                 p.at_once = p.per_sm * dev.clusters[l + pair];   // tiles
                 if (p.at_once == 0 || (l > 0 && tiles > p.at_once)) break;
                 const int64_t rounds = (tiles + p.at_once - 1) / p.at_once;
@@ -911,25 +928,58 @@ int configure(const Device** out) {
 
 using namespace dsx;
 
+namespace {
+// Sizes that make_plan takes.  2^24 columns: the longest a wait lasts (a tile's MMAs, 20 ms) stays far inside its limit.
+int check_sizes(int n_terms, int64_t m, int64_t n, int64_t k) {
+    DSX_REQUIRE(m >= 0 && n >= 0 && k >= 32 && k % 32 == 0 && m < ((int64_t)1 << 22) && n < ((int64_t)1 << 31) && k <= ((int64_t)1 << 24),
+                "mxfp4_matmul: %lld x %lld x %lld (k a multiple of 32, at most 2^24; m below 2^22)", (long long)m, (long long)n, (long long)k);
+    DSX_REQUIRE(n_terms >= 1 && n_terms <= 3, "mxfp4_matmul: %d terms (1 to 3)", n_terms);
+    return DSX_OK;
+}
+int choose_plan(int n_terms, int64_t m, int64_t n, int64_t k, Plan* p) {
+    const Device* dev = nullptr;
+    if (int rc = configure(&dev)) return rc;
+    if (!make_plan(m, n, (int)k, n_terms, *dev, g_pin.load(std::memory_order_relaxed), p))
+        return set_error(DSX_ERR_UNSUPPORTED, "mxfp4_matmul: no tiling for %d terms (or not the pinned one)", n_terms);
+    DSX_REQUIRE((int64_t)p->tiles_w * p->tiles_m < ((int64_t)1 << 30), "mxfp4_matmul: too many tiles");
+    return DSX_OK;
+}
+}  // namespace
+
 extern "C" {
+
+int dsx_mxfp4_matmul_tiling(int n_terms, int64_t m, int64_t n, int64_t k, int32_t* tiling) {
+    if (int rc = check_sizes(n_terms, m, n, k)) return rc;
+    DSX_REQUIRE(m > 0 && n > 0 && tiling, "mxfp4_matmul_tiling: nothing to multiply, or a null argument");
+    Plan p;
+    if (int rc = choose_plan(n_terms, m, n, k, &p)) return rc;
+    const int32_t values[8] = {p.pair, p.tokens, p.splits, p.tiles_w * p.tiles_m, p.at_once, p.stages, p.scale_bufs, p.slots};
+    std::copy(values, values + 8, tiling);
+    return DSX_OK;
+}
+
+int dsx_mxfp4_matmul_pin(int pair, int tokens, int splits) {
+    DSX_REQUIRE(pair >= -1 && pair <= 1 && tokens >= 0 && tokens <= kMaxN && tokens % 16 == 0 && splits >= 0 && splits <= 8 && (splits & (splits - 1)) == 0,
+                "mxfp4_matmul_pin: pair %d (-1 to 1), %d tokens (a multiple of 16, at most 208), %d splits (0, 1, 2, 4, 8)", pair, tokens, splits);
+    Pin pin;
+    pin.pair = (int8_t)pair;
+    pin.tokens = (uint8_t)tokens;
+    pin.splits = (uint8_t)splits;
+    g_pin.store(pin, std::memory_order_relaxed);
+    return DSX_OK;
+}
 
 int dsx_mxfp4_matmul(const void* a_codes, const void* a_scales, int n_terms, int64_t m, const void* w_codes, const void* w_scales, int64_t n,
                      int64_t k, void* out, int dtype, int64_t row_stride, dsx_stream_t stream) {
     DSX_REQUIRE(dtype_ok(dtype), "mxfp4_matmul: unknown element type %d", dtype);
-    // 2^24 columns: the longest a wait lasts (a tile's MMAs, 20 ms) stays far inside its limit
-    DSX_REQUIRE(m >= 0 && n >= 0 && k >= 32 && k % 32 == 0 && m < ((int64_t)1 << 22) && n < ((int64_t)1 << 31) && k <= ((int64_t)1 << 24),
-                "mxfp4_matmul: %lld x %lld x %lld (k a multiple of 32, at most 2^24; m below 2^22)", (long long)m, (long long)n, (long long)k);
-    DSX_REQUIRE(n_terms >= 1 && n_terms <= 3, "mxfp4_matmul: %d terms (1 to 3)", n_terms);
+    if (int rc = check_sizes(n_terms, m, n, k)) return rc;
     if (m == 0 || n == 0) return DSX_OK;
     DSX_REQUIRE(a_codes && a_scales && w_codes && w_scales && out, "mxfp4_matmul: null argument");
     DSX_REQUIRE(row_stride >= n || m == 1, "mxfp4_matmul: row stride %lld below the %lld columns of a row", (long long)row_stride, (long long)n);
     DSX_REQUIRE((((uintptr_t)a_codes | (uintptr_t)w_codes) & 15) == 0 && ((uintptr_t)out & (dtype_size(dtype) - 1)) == 0,
                 "mxfp4_matmul: codes must be 16-byte aligned, out aligned to its elements");
-    const Device* dev = nullptr;
-    if (int rc = configure(&dev)) return rc;
     Plan p;
-    if (!make_plan(m, n, (int)k, n_terms, *dev, &p)) return set_error(DSX_ERR_UNSUPPORTED, "mxfp4_matmul: no tile for %d terms", n_terms);
-    DSX_REQUIRE((int64_t)p.tiles_w * p.tiles_m < ((int64_t)1 << 30), "mxfp4_matmul: too many tiles");
+    if (int rc = choose_plan(n_terms, m, n, k, &p)) return rc;
     // codes and scales of both operands as (bytes, row) and (bytes, row, term); the maps of scales only where TMA can read them
     const bool scale_tma = k % 512 == 0 && (((uintptr_t)a_scales | (uintptr_t)w_scales) & 15) == 0;
     CUtensorMap maps[4];
@@ -963,6 +1013,7 @@ int dsx_mxfp4_matmul(const void* a_codes, const void* a_scales, int n_terms, int
     g.tiles_w = p.tiles_w; g.tiles = p.tiles_w * p.tiles_m;
     g.scale_tma = scale_tma;
     g.scale_bufs = p.scale_bufs;
+    g.polls = kPolls;
     g.pairs = dtype != DSX_F32 && n % 2 == 0 && (row_stride % 2 == 0 || m == 1) && ((uintptr_t)out & 3) == 0;
     const cudaStream_t s = (cudaStream_t)stream;
     if (dtype == DSX_F32) return launch_for<DSX_F32>(n_terms, p, maps, g, s);

@@ -26,6 +26,8 @@ _SIGNATURES = {
     "dsx_mxfp4_dequantize": [_P, _P, _L, _L, _I, _P, _I, _L, _P],
     "dsx_mxfp4_matmul": [_P, _P, _I, _L, _P, _P, _L, _L, _P, _I, _L, _P],
     "dsx_token_logprobs": [_P, _I, _L, _L, _L, _F, _P, _I, _P, _P, _I, _P, _P, _P],
+    "dsx_mxfp4_matmul_tiling": [_I, _L, _L, _L, C.POINTER(C.c_int32)],
+    "dsx_mxfp4_matmul_pin": [_I, _I, _I],
     "dsx_head_check": [_P, C.POINTER(C.c_uint32)],
 }
 _functions = {}
@@ -151,6 +153,18 @@ class Mxfp4Matmul:
         _call("dsx_mxfp4_matmul", a.codes_at, a.scales_at, a.n_terms, a.rows, w.codes_at, w.scales_at, w.rows, a.k, out.data_ptr(), DTYPES[dtype],
               _row_stride(out), _here(a._buffer, w._buffer, out))
         return out
+
+    @staticmethod
+    def tiling(n_terms: int, m: int, n: int, k: int) -> dict:
+        """How a product of these sizes is cut up on the current device (for tests and tuning)."""
+        values = (C.c_int32 * 8)()
+        _call("dsx_mxfp4_matmul_tiling", n_terms, m, n, k, values)
+        return dict(zip(("pair", "tokens", "splits", "tiles", "at_once", "stages", "scale_bufs", "slots"), values))
+
+    @staticmethod
+    def pin(pair: int = -1, tokens: int = 0, splits: int = 0):
+        """Fixes parts of the tiling for this process's products until the next call (no arguments: all chosen again)."""
+        _call("dsx_mxfp4_matmul_pin", pair, tokens, splits)
 
 
 def check() -> int:

@@ -532,6 +532,14 @@ DSX_API int dsx_mxfp4_dequantize(const void* codes, const void* scales, int64_t 
 DSX_API int dsx_mxfp4_matmul(const void* a_codes, const void* a_scales, int n_terms, int64_t m, const void* w_codes,
                              const void* w_scales, int64_t n, int64_t k, void* out, int dtype, int64_t row_stride,
                              dsx_stream_t stream);
+/* For tests and tuning; whole process, from the next product on (a captured one keeps what it was captured with).
+ * tiling: what dsx_mxfp4_matmul does with a product of these sizes on the current device: [0] 1 for tiles of pairs of CTAs (256 rows
+ *   of w, else 128), [1] tokens of a tile, [2] CTAs that split its columns, [3] tiles, [4] tiles at once, [5] stages of the ring of
+ *   codes, [6] buffers of scales, [7] slots of scales in tensor memory.  Eight values.
+ * pin: fixes pair (0, 1; -1: chosen per call), tokens (a multiple of 16; 0: chosen) and splits (1, 2, 4, 8; 0: chosen).  A product that the
+ *   pinned tiling cannot do returns DSX_ERR_UNSUPPORTED. */
+DSX_API int dsx_mxfp4_matmul_tiling(int n_terms, int64_t m, int64_t n, int64_t k, int32_t* tiling);
+DSX_API int dsx_mxfp4_matmul_pin(int pair, int tokens, int splits);
 /* Reads (and clears) the device-side error word of the product on the current device; synchronises the stream.  Non-zero (bit 1: a
  * bounded wait inside dsx_mxfp4_matmul ran out, results of that call are missing) returns DSX_ERR_DEVICE. */
 DSX_API int dsx_head_check(dsx_stream_t stream, uint32_t* error_word);

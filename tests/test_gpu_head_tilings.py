@@ -1,0 +1,142 @@
+"""Every form of the MXFP4 product, pinned, so that what is tested does not depend on which one the model of its time chooses: pairs of CTAs
+and single ones, one to three terms, scales by TMA and by loaders, rings that wrap over several tiles, columns split over clusters."""
+import itertools
+
+import pytest
+
+pytestmark = pytest.mark.gpu
+
+E2M1 = [0, .5, 1, 1.5, 2, 3, 4, 6, -0., -.5, -1, -1.5, -2, -3, -4, -6]
+
+
+@pytest.fixture(autouse=True)
+def _unpinned_and_clean(torch_cuda, moe):
+    from deepstrix_b200 import head
+    yield
+    head.Mxfp4Matmul.pin()
+    assert head.check() == 0
+
+
+def _rows(torch, g, terms, rows, k, shift=0):
+    """Random MXFP4 rows with scales of 2^-1 .. 2^1 (sums of products are exact in f32, see test_matmul_exact_sums), their f64 values summed over
+    the terms; the scale bytes start `shift` bytes off a 16-byte boundary."""
+    from deepstrix_b200 import head
+    codes = torch.randint(0, 256, (terms, rows, k // 2), generator=g, device="cuda", dtype=torch.uint8)
+    buf = torch.randint(126, 129, (terms * rows * (k // 32) + shift,), generator=g, device="cuda", dtype=torch.uint8)
+    scales = buf[shift:].view(terms, rows, k // 32)
+    table = torch.tensor(E2M1, dtype=torch.float64, device="cuda")
+    total = torch.zeros((rows, k), dtype=torch.float64, device="cuda")
+    for t in range(terms):
+        v = torch.stack([table[(codes[t] & 15).long()], table[(codes[t] >> 4).long()]], -1).view(rows, k // 32, 32)
+        total += (v * torch.exp2(scales[t].double() - 127)[..., None]).view(rows, k)
+    return head.Mxfp4Rows(codes, scales), total
+
+
+def _check_product(torch, a, av, w, wv, dtype):
+    """Exact, in place in a wider buffer, nothing else written, the same bits again; then with one NaN scale on either side."""
+    from deepstrix_b200 import head
+    m, n = av.shape[0], wv.shape[0]
+    exact = av @ wv.T
+    assert float(exact.abs().max()) * 16 < 2 ** 22
+    want = exact.float().to(dtype)
+    wide = torch.full((m + 9, n + 6), 7.0, dtype=dtype, device="cuda")
+    head.Mxfp4Matmul.launch(a, w, dtype, out=wide[:m, :n])
+    assert torch.equal(wide[:m, :n], want) and bool((wide[m:] == 7).all()) and bool((wide[:m, n:] == 7).all())
+    assert torch.equal(head.Mxfp4Matmul.launch(a, w, dtype), want)
+    term, row, col = a.n_terms - 1, m - 2, n // 2
+    kept = a.scales[term, row, -1].item(), w.scales[0, col, 0].item()
+    a.scales[term, row, -1], w.scales[0, col, 0] = 255, 255
+    got = head.Mxfp4Matmul.launch(a, w, dtype)
+    a.scales[term, row, -1], w.scales[0, col, 0] = kept
+    assert bool(got[row].isnan().all()) and bool(got[:, col].isnan().all())
+    rest = torch.ones((m, n), dtype=torch.bool, device="cuda")
+    rest[row], rest[:, col] = False, False
+    assert torch.equal(got[rest], want[rest])
+
+
+PAIRS = [(1, t) for t in (16, 48, 112, 128, 144, 208)] + [(2, t) for t in (16, 80, 128)] + [(3, t) for t in (16, 96, 112, 128)]
+SINGLES = [(1, t) for t in (16, 32, 80, 112, 128, 160, 208)] + [(2, t) for t in (16, 64, 96)] + [(3, t) for t in (16, 32, 48, 64)]
+FORMS = [(1,) + f for f in PAIRS] + [(0,) + f for f in SINGLES]
+
+
+@pytest.mark.parametrize("pair,terms,tokens", FORMS)
+def test_pinned_tiles(torch_cuda, moe, pair, terms, tokens):
+    """Four tiles and more for some CTAs (rings of stages, buffers and slots wrap over tiles), ragged at both ends.  K: two and five steps of
+    scales by TMA, an odd and an even number of stages by loaders, one short stage, scales at odd addresses."""
+    torch = torch_cuda
+    from deepstrix_b200 import head
+    g = torch.Generator(device="cuda").manual_seed(tokens * 8 + terms * 2 + pair)
+    head.Mxfp4Matmul.pin(pair, tokens, 1)
+    m, rows_w = 4 * tokens - 5, 256 if pair else 128
+    at_once = head.Mxfp4Matmul.tiling(terms, m, 4096, 1024)["at_once"]
+    n_tiles = -(-(3 * at_once + 2) // 4)
+    for k, odd, shift, dtype in ((1024, 0, 0, torch.float32), (2560, 1, 0, torch.bfloat16), (1056, 0, 0, torch.bfloat16), (1312, 1, 3, torch.float32),
+                                 (160, 0, 0, torch.float16)):
+        n = n_tiles * rows_w - 2 - odd
+        t = head.Mxfp4Matmul.tiling(terms, m, n, k)
+        assert (t["pair"], t["tokens"], t["splits"]) == (pair, tokens, 1) and t["tiles"] > 3 * t["at_once"]
+        a, av = _rows(torch, g, terms, m, k, shift)
+        w, wv = _rows(torch, g, 1, n, k, shift)
+        _check_product(torch, a, av, w, wv, dtype)
+
+
+@pytest.mark.parametrize("terms,tokens", SINGLES)
+@pytest.mark.parametrize("splits", [2, 4, 8])
+def test_pinned_splits(torch_cuda, moe, terms, tokens, splits):
+    """Columns of a tile shared by a cluster: even and uneven shares, shares that begin inside a buffer of scales."""
+    torch = torch_cuda
+    from deepstrix_b200 import head
+    g = torch.Generator(device="cuda").manual_seed(tokens * 8 + terms * 2 + splits)
+    head.Mxfp4Matmul.pin(0, tokens, splits)
+    for m, n, k, dtype in ((2 * tokens - 3, 301, 256 * splits, torch.float32), (tokens, 130, 4608, torch.bfloat16), (tokens + 1, 257, 2336, torch.float32)):
+        assert head.Mxfp4Matmul.tiling(terms, m, n, k)["splits"] == splits
+        a, av = _rows(torch, g, terms, m, k)
+        w, wv = _rows(torch, g, 1, n, k)
+        _check_product(torch, a, av, w, wv, dtype)
+
+
+def test_forms_cover_the_rings(torch_cuda, moe):
+    """The pinned forms include what differs in their synchronisation: two and four buffers of scales, two, three and four slots."""
+    from deepstrix_b200 import head
+    seen = set()
+    for pair, terms, tokens in FORMS:
+        head.Mxfp4Matmul.pin(pair, tokens, 1)
+        t = head.Mxfp4Matmul.tiling(terms, 1000, 4096, 1024)
+        seen.add((pair, t["scale_bufs"], t["slots"]))
+    assert {(1, 4, 2), (1, 2, 4), (1, 4, 4), (0, 2, 2), (0, 2, 3), (0, 2, 4), (0, 4, 4)} <= seen, seen
+
+
+def test_pinned_forms_agree_and_a_pin_is_taken_back(torch_cuda, moe):
+    """Forms of the same product give the same exact sums; what cannot be done as pinned is refused and writes nothing."""
+    torch = torch_cuda
+    from deepstrix_b200 import head
+    g = torch.Generator(device="cuda").manual_seed(1)
+    a, av = _rows(torch, g, 3, 300, 1536)
+    w, wv = _rows(torch, g, 1, 700, 1536)
+    chosen = head.Mxfp4Matmul.tiling(3, 300, 700, 1536)
+    want = (av @ wv.T).float()
+    for pair, tokens in itertools.product((0, 1), (16, 48, 64, 96, 128)):
+        head.Mxfp4Matmul.pin(pair, tokens)
+        if pair or tokens * 3 <= 208:
+            assert torch.equal(head.Mxfp4Matmul.launch(a, w, torch.float32), want)
+            continue
+        out = torch.full((300, 700), 7.0, device="cuda")
+        with pytest.raises(moe.DsxError, match="pinned"):
+            head.Mxfp4Matmul.launch(a, w, torch.float32, out=out)
+        assert bool((out == 7).all())
+    head.Mxfp4Matmul.pin()
+    assert head.Mxfp4Matmul.tiling(3, 300, 700, 1536) == chosen
+
+
+def test_chosen_forms(torch_cuda, moe):
+    """What the model chooses on a whole B200 where the difference is large: clusters for one small matrix, single CTAs for a few tokens on a large one,
+    pairs for prompts."""
+    torch = torch_cuda
+    from deepstrix_b200 import head
+    if torch.cuda.get_device_properties(0).multi_processor_count < 140:
+        pytest.skip("a partition of a device")
+    tiling = head.Mxfp4Matmul.tiling
+    assert tiling(3, 1, 1024, 2048)["splits"] > 1 and tiling(3, 1, 1024, 2048)["pair"] == 0
+    assert (tiling(3, 8, 131072, 4096)["pair"], tiling(3, 8, 131072, 4096)["splits"]) == (0, 1)
+    for terms in (1, 2, 3):
+        assert tiling(terms, 8192, 8192, 4096)["pair"] == 1

@@ -100,3 +100,16 @@ def test_python_checks(moe):
         head.Mxfp4Quantize.launch(torch.zeros((64, 4)).T)                              # columns not contiguous
     with pytest.raises(AssertionError):
         head.Mxfp4Matmul.launch(head.Mxfp4Rows(u8(5, 32), u8(5, 2)), head.Mxfp4Rows(u8(2, 5, 32), u8(2, 5, 2)))   # a weight of two terms
+
+
+def test_tiling_and_pin_refusals(moe):
+    lib = moe.lib()
+    out = (C.c_int32 * 8)()
+
+    def tiling(terms=1, m=4, n=8, k=64, to=out):
+        return _refused(moe, "dsx_mxfp4_matmul_tiling", terms, L(m), L(n), L(k), to)
+    assert "multiple of 32" in tiling(k=48) and "multiple of 32" in tiling(m=-1) and "terms" in tiling(terms=4)
+    assert "null" in tiling(to=None) and "nothing" in tiling(m=0) and "nothing" in tiling(n=0)
+    for pin in ((-2, 0, 0), (2, 0, 0), (0, -16, 0), (0, 8, 0), (0, 224, 0), (0, 0, -1), (0, 0, 3), (0, 0, 16)):
+        assert "pin" in _refused(moe, "dsx_mxfp4_matmul_pin", *pin)
+    assert lib.dsx_mxfp4_matmul_pin(1, 208, 1) == 0 and lib.dsx_mxfp4_matmul_pin(-1, 0, 0) == 0
