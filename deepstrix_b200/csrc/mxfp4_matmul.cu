@@ -20,7 +20,10 @@
 // tile is read out under the next one's MMAs.
 // Few tiles: the columns are split over the CTAs of a cluster; each leaves its partial tile in shared memory and the cluster adds
 // them in rank order through distributed shared memory, so results do not depend on timing and need no workspace.
-// Every wait is bounded; on a timeout the block drains, frees its tensor memory and sets bit 1 of the error word.
+// Every wait on a barrier in shared memory is bounded; when one runs out the block lets what it has in flight finish (bounded too), frees its
+// tensor memory and sets bit 1 of the error word.  Not bounded, because they end by themselves: the wait for the kernel before this one, the barriers of
+// a cluster (every role of every block comes to them) and the wait for tensor memory, which kernels of this library give back without
+// waiting for another block, or hold alone on their SM (see the two sizes of block below).
 //
 // Bound and measured (launches back to back).  A few tokens: the weights' bytes; 8 x 131072 x 4096 of three terms takes 53 us, 5.4 TB/s, of which
 // about 7 us are start and end -- every further 37888 rows of W take 12.8 us, 6.45 TB/s.  One small matrix (1 x 1024 x 2048): 6 us, all of it
@@ -51,7 +54,7 @@ constexpr int kMaxScaleBufs = 4;     // two or four: see plan_block
 constexpr int kMaxSlots = 4;         // of scales in tensor memory, two stages each
 constexpr int kMaxStages = 8;
 constexpr int kMaxN = 208;           // of an MMA: two accumulators and two scale slots fill tensor memory
-constexpr uint32_t kPolls = 1u << 22;     // of a wait
+constexpr uint32_t kPolls = 1u << 22;     // of a wait, unless dsx_mxfp4_matmul_set_polls says otherwise; a poll that fails takes 2 to 4 us
 constexpr uint32_t kDrainPolls = 1u << 16;   // for what is in flight when a block has given up
 
 __device__ __forceinline__ uint32_t smem_u32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
@@ -801,6 +804,7 @@ struct Pin {
     uint8_t tokens = 0, splits = 0, unused = 0;
 };
 std::atomic<Pin> g_pin{Pin{}};
+std::atomic<uint32_t> g_polls{kPolls};
 
 // Tokens a tile, pairs or single CTAs, and splits of the columns, from a model of the time in clocks.  A stage takes its MMAs on the tensor
 // core (N / 2 clocks each, 50 at least), or the issuing warp's 50 an MMA and what surrounds them (two blocks on an SM issue side by side), or
@@ -929,7 +933,7 @@ int configure(const Device** out) {
 using namespace dsx;
 
 namespace {
-// Sizes that make_plan takes.  2^24 columns: the longest a wait lasts (a tile's MMAs, 20 ms) stays far inside its limit.
+// Sizes that make_plan takes.  2^24 columns: the longest a wait lasts (a tile's MMAs, 20 ms) stays far inside its limit (about ten seconds).
 int check_sizes(int n_terms, int64_t m, int64_t n, int64_t k) {
     DSX_REQUIRE(m >= 0 && n >= 0 && k >= 32 && k % 32 == 0 && m < ((int64_t)1 << 22) && n < ((int64_t)1 << 31) && k <= ((int64_t)1 << 24),
                 "mxfp4_matmul: %lld x %lld x %lld (k a multiple of 32, at most 2^24; m below 2^22)", (long long)m, (long long)n, (long long)k);
@@ -966,6 +970,11 @@ int dsx_mxfp4_matmul_pin(int pair, int tokens, int splits) {
     pin.tokens = (uint8_t)tokens;
     pin.splits = (uint8_t)splits;
     g_pin.store(pin, std::memory_order_relaxed);
+    return DSX_OK;
+}
+
+int dsx_mxfp4_matmul_set_polls(uint32_t polls) {
+    g_polls.store(polls ? polls : kPolls, std::memory_order_relaxed);
     return DSX_OK;
 }
 
@@ -1013,7 +1022,7 @@ int dsx_mxfp4_matmul(const void* a_codes, const void* a_scales, int n_terms, int
     g.tiles_w = p.tiles_w; g.tiles = p.tiles_w * p.tiles_m;
     g.scale_tma = scale_tma;
     g.scale_bufs = p.scale_bufs;
-    g.polls = kPolls;
+    g.polls = g_polls.load(std::memory_order_relaxed);
     g.pairs = dtype != DSX_F32 && n % 2 == 0 && (row_stride % 2 == 0 || m == 1) && ((uintptr_t)out & 3) == 0;
     const cudaStream_t s = (cudaStream_t)stream;
     if (dtype == DSX_F32) return launch_for<DSX_F32>(n_terms, p, maps, g, s);

@@ -28,6 +28,7 @@ _SIGNATURES = {
     "dsx_token_logprobs": [_P, _I, _L, _L, _L, _F, _P, _I, _P, _P, _I, _P, _P, _P],
     "dsx_mxfp4_matmul_tiling": [_I, _L, _L, _L, C.POINTER(C.c_int32)],
     "dsx_mxfp4_matmul_pin": [_I, _I, _I],
+    "dsx_mxfp4_matmul_set_polls": [C.c_uint32],
     "dsx_head_check": [_P, C.POINTER(C.c_uint32)],
 }
 _functions = {}
@@ -165,6 +166,11 @@ class Mxfp4Matmul:
     def pin(pair: int = -1, tokens: int = 0, splits: int = 0):
         """Fixes parts of the tiling for this process's products until the next call (no arguments: all chosen again)."""
         _call("dsx_mxfp4_matmul_pin", pair, tokens, splits)
+
+    @staticmethod
+    def set_polls(polls: int = 0):
+        """How often a wait inside the product is tried before it gives up (0: the default)."""
+        _call("dsx_mxfp4_matmul_set_polls", polls)
 
 
 def check() -> int:

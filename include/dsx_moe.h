@@ -537,11 +537,16 @@ DSX_API int dsx_mxfp4_matmul(const void* a_codes, const void* a_scales, int n_te
  *   of w, else 128), [1] tokens of a tile, [2] CTAs that split its columns, [3] tiles, [4] tiles at once, [5] stages of the ring of
  *   codes, [6] buffers of scales, [7] slots of scales in tensor memory.  Eight values.
  * pin: fixes pair (0, 1; -1: chosen per call), tokens (a multiple of 16; 0: chosen) and splits (1, 2, 4, 8; 0: chosen).  A product that the
- *   pinned tiling cannot do returns DSX_ERR_UNSUPPORTED. */
+ *   pinned tiling cannot do returns DSX_ERR_UNSUPPORTED.
+ * set_polls: how often a wait inside the product is tried, 2 to 4 us each, before it gives up (0: the default, 2^22), like
+ *   dsx_ep_set_barrier_polls. */
 DSX_API int dsx_mxfp4_matmul_tiling(int n_terms, int64_t m, int64_t n, int64_t k, int32_t* tiling);
 DSX_API int dsx_mxfp4_matmul_pin(int pair, int tokens, int splits);
+DSX_API int dsx_mxfp4_matmul_set_polls(uint32_t polls);
 /* Reads (and clears) the device-side error word of the product on the current device; synchronises the stream.  Non-zero (bit 1: a
- * bounded wait inside dsx_mxfp4_matmul ran out, results of that call are missing) returns DSX_ERR_DEVICE. */
+ * bounded wait inside dsx_mxfp4_matmul ran out; what that call wrote to its out is undefined, the next call is as good as any) returns
+ * DSX_ERR_DEVICE.  One word a device, whatever the stream: it speaks of every product since the last check that has come to its end
+ * (those of `stream` for certain), and a non-zero word is reported to one caller only. */
 DSX_API int dsx_head_check(dsx_stream_t stream, uint32_t* error_word);
 /* Per row of v logits, with z = logit * inv_temperature:
  *   logprobs     f32 [t, n_given]  z[token] - logsumexp(z) of the given tokens; a token outside [0, v) gives -inf

@@ -1,5 +1,6 @@
 """Every form of the MXFP4 product, pinned, so that what is tested does not depend on which one the model of its time chooses: pairs of CTAs
 and single ones, one to three terms, scales by TMA and by loaders, rings that wrap over several tiles, columns split over clusters."""
+import ctypes as C
 import itertools
 
 import pytest
@@ -14,6 +15,7 @@ def _unpinned_and_clean(torch_cuda, moe):
     from deepstrix_b200 import head
     yield
     head.Mxfp4Matmul.pin()
+    head.Mxfp4Matmul.set_polls()
     assert head.check() == 0
 
 
@@ -140,3 +142,35 @@ def test_chosen_forms(torch_cuda, moe):
     assert (tiling(3, 8, 131072, 4096)["pair"], tiling(3, 8, 131072, 4096)["splits"]) == (0, 1)
     for terms in (1, 2, 3):
         assert tiling(terms, 8192, 8192, 4096)["pair"] == 1
+
+
+@pytest.mark.parametrize("pin,terms,m,n,k", [((0, 16, 2), 3, 30, 300, 65536), ((0, 16, 1), 1, 100, 40000, 16384), ((0, 208, 1), 1, 500, 3000, 16416),
+                                             ((1, 128, 1), 3, 1000, 20000, 16384), ((1, 208, 1), 1, 1000, 20000, 16416), ((1, 16, 1), 2, 100, 20000, 16384)])
+def test_a_wait_that_runs_out_is_reported(torch_cuda, moe, pin, terms, m, n, k):
+    """With waits of one poll (a few us, where a tile takes 20 and more) the product gives up, says so once, and returns: the call after it is right."""
+    torch = torch_cuda
+    from deepstrix_b200 import head
+    g = torch.Generator(device="cuda").manual_seed(k + terms)
+
+    def rows(t, r):
+        return head.Mxfp4Rows(torch.randint(0, 256, (t, r, k // 2), generator=g, device="cuda", dtype=torch.uint8),
+                              torch.randint(120, 125, (t, r, k // 32), generator=g, device="cuda", dtype=torch.uint8))
+    a, w = rows(terms, m), rows(1, n)
+    head.Mxfp4Matmul.pin(*pin)
+    want = head.Mxfp4Matmul.launch(a, w, torch.float32)
+    assert head.check() == 0
+    wide = torch.full((m + 3, n + 5), 7.0, device="cuda")
+    for polls in (1, 2):
+        head.Mxfp4Matmul.set_polls(polls)
+        head.Mxfp4Matmul.launch(a, w, torch.float32, out=wide[:m, :n])
+        head.Mxfp4Matmul.launch(a, w, torch.float32, out=wide[:m, :n])
+        head.Mxfp4Matmul.set_polls()
+        got = head.Mxfp4Matmul.launch(a, w, torch.float32)
+        assert head.check() == 1 and head.check() == 0
+        assert torch.equal(got, want)
+        assert bool((wide[m:] == 7).all()) and bool((wide[:, n:] == 7).all())
+    word = C.c_uint32()
+    head.Mxfp4Matmul.set_polls(1)
+    head.Mxfp4Matmul.launch(a, w, torch.float32)
+    head.Mxfp4Matmul.set_polls()
+    assert moe.lib().dsx_head_check(moe._stream(), C.byref(word)) == -3 and word.value == 1
