@@ -915,6 +915,7 @@ int configure(const Device** out) {
     *out = &devices[dev];
     if (known[dev].load(std::memory_order_acquire)) return DSX_OK;
     std::lock_guard<std::mutex> lock(mutex);
+    if (known[dev].load(std::memory_order_relaxed)) return DSX_OK;   // by a thread that held the lock before: others may be reading it
     Device& d = devices[dev];
     DSX_CUDA(cudaDeviceGetAttribute(&d.sms, cudaDevAttrMultiProcessorCount, dev));
     if (int rc = allow_shared<DSX_F32>()) return rc;

@@ -23,6 +23,8 @@
 // clamp + SwiGLU + routing weight (gate/up) and store mid (f16) or the per-pick
 // partial rows (f32).  Every wait is bounded; on a timeout the block raises an
 // abort flag, all roles drain, TMEM is freed and the layer's error word is set.
+#include <atomic>
+
 #include "prefill.cuh"
 
 namespace dsx {
@@ -633,13 +635,15 @@ typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t,
 // cuTensorMapEncodeTiled through the runtime's driver entry point (the library links no libcuda).
 int tmap_encode(CUtensorMap* map, CUtensorMapDataType type, int rank, const void* base, const cuuint64_t* dims, const cuuint64_t* strides,
                 const cuuint32_t* box, CUtensorMapSwizzle swizzle) {
-    static EncodeTiledFn fn = nullptr;
+    static std::atomic<EncodeTiledFn> known{nullptr};   // several threads may come here first
+    EncodeTiledFn fn = known.load(std::memory_order_relaxed);
     if (!fn) {
         void* p = nullptr;
         cudaDriverEntryPointQueryResult qres;
         DSX_CUDA(cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &qres));
         if (qres != cudaDriverEntryPointSuccess || !p) return set_error(DSX_ERR_UNSUPPORTED, "driver has no cuTensorMapEncodeTiled");
         fn = (EncodeTiledFn)p;
+        known.store(fn, std::memory_order_relaxed);
     }
     const cuuint32_t estr[5] = {1, 1, 1, 1, 1};
     const CUresult r = fn(map, type, (cuuint32_t)rank, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle,

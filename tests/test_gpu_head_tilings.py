@@ -2,6 +2,9 @@
 and single ones, one to three terms, scales by TMA and by loaders, rings that wrap over several tiles, columns split over clusters."""
 import ctypes as C
 import itertools
+import os
+import subprocess
+import sys
 
 import pytest
 
@@ -174,3 +177,39 @@ def test_a_wait_that_runs_out_is_reported(torch_cuda, moe, pin, terms, m, n, k):
     head.Mxfp4Matmul.launch(a, w, torch.float32)
     head.Mxfp4Matmul.set_polls()
     assert moe.lib().dsx_head_check(moe._stream(), C.byref(word)) == -3 and word.value == 1
+
+
+FIRST_CALLS = """
+import sys, threading
+sys.path.insert(0, sys.argv[1])
+import torch
+from deepstrix_b200 import head
+def rows(t, r, k):
+    return head.Mxfp4Rows(torch.randint(0, 256, (t, r, k // 2), device="cuda", dtype=torch.uint8),
+                          torch.randint(126, 129, (t, r, k // 32), device="cuda", dtype=torch.uint8))
+sizes = [(1, 300, 2048, 3), (40, 700, 544, 2), (2000, 3000, 1024, 3), (300, 300, 1024, 1)] * 4
+work = [(rows(t, m, k), rows(1, n, k)) for m, n, k, t in sizes]
+torch.cuda.synchronize()
+got, start = [None] * len(work), threading.Barrier(len(work))
+def call(i):
+    with torch.cuda.stream(torch.cuda.Stream()):
+        start.wait()
+        got[i] = [head.Mxfp4Matmul.launch(*work[i], torch.float32) for _ in range(3)]
+threads = [threading.Thread(target=call, args=(i,)) for i in range(len(work))]
+[t.start() for t in threads]
+[t.join() for t in threads]
+torch.cuda.synchronize()
+for (a, w), results in zip(work, got):
+    want = head.Mxfp4Matmul.launch(a, w, torch.float32)
+    assert all(torch.equal(r, want) for r in results)
+assert head.check() == 0
+print("same")
+"""
+
+
+def test_first_calls_of_a_process_from_many_threads(torch_cuda, moe):
+    """What the product looks up once a device is looked up by sixteen threads at once: each gets the results that a single thread does."""
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    for _ in range(2):
+        out = subprocess.run([sys.executable, "-c", FIRST_CALLS, root], capture_output=True, text=True, timeout=300)
+        assert out.returncode == 0 and out.stdout.strip() == "same", out.stderr[-2000:]
