@@ -131,15 +131,28 @@ __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatil
     *abort_flag = 1u;
     return false;
 }
+// PAIR: `bar` is a barrier of either CTA of a pair (a shared::cluster address); the copy's bytes count there.
+template <bool PAIR>
 __device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map, int c0, int c1, int c2, uint32_t bar) {
-    asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst),
-                 "l"(map), "r"(c0), "r"(c1), "r"(c2), "r"(bar)
-                 : "memory");
+    if constexpr (PAIR)
+        asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.cta_group::2 [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst),
+                     "l"(map), "r"(c0), "r"(c1), "r"(c2), "r"(bar)
+                     : "memory");
+    else
+        asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst),
+                     "l"(map), "r"(c0), "r"(c1), "r"(c2), "r"(bar)
+                     : "memory");
 }
+template <bool PAIR>
 __device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map, int c0, int c1, int c2, int c3, uint32_t bar) {
-    asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(dst),
-                 "l"(map), "r"(c0), "r"(c1), "r"(c2), "r"(c3), "r"(bar)
-                 : "memory");
+    if constexpr (PAIR)
+        asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.cta_group::2 [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(dst),
+                     "l"(map), "r"(c0), "r"(c1), "r"(c2), "r"(c3), "r"(bar)
+                     : "memory");
+    else
+        asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(dst),
+                     "l"(map), "r"(c0), "r"(c1), "r"(c2), "r"(c3), "r"(bar)
+                     : "memory");
 }
 __device__ __forceinline__ void tma_prefetch_4d(const CUtensorMap* map, int c0, int c1, int c2, int c3) {
     asm volatile("cp.async.bulk.prefetch.tensor.4d.L2.global.tile [%0, {%1, %2, %3, %4}];" ::"l"(map), "r"(c0), "r"(c1), "r"(c2), "r"(c3)
@@ -200,10 +213,10 @@ __device__ __forceinline__ uint32_t map_to_cta(uint32_t saddr, uint32_t cta) {  
     asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(saddr), "r"(cta));
     return r;
 }
-// Arrival on a barrier of the other CTA of a pair.  Relaxed on purpose: what the arrival reports (tensor-memory stores
-// this warp has waited for, TMA bytes whose barrier it has seen complete) is finished before the instruction issues, and
-// the default .release form at cluster scope held the issuing thread for about a microsecond per arrival, which bounded
-// a whole pipeline stage when one thread forwarded an arrival per stage.
+// Arrival on a barrier of the other CTA of a pair, for tensor-memory accesses of this warp and nothing else: waited for
+// (tcgen05.wait) and fenced (fence::before_thread_sync) they are ordered by a relaxed arrival, as the instruction set's own hand-over
+// of tensor memory between threads is; the .release form at cluster scope held the issuing thread for about a microsecond.  What
+// lies in shared memory, and what another warp did, is not ordered by it: the codes of both CTAs therefore count on the even CTA's barriers.
 __device__ __forceinline__ void mbar_arrive_cluster(uint32_t cluster_bar) {
     asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_bar) : "memory");
 }
@@ -280,9 +293,9 @@ mx_gemm_kernel(const __grid_constant__ CUtensorMap tmap_b32, const __grid_consta
     const uint32_t sbase = smem_u32(smem);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t bar0 = sbase + kSmemBar;
-    // FULL[s]: the stage's codes and scales have landed in this CTA (TMA bytes); SC_FULL[s]: the scale warps have moved the
-    // stage's scales into tensor memory (a pair: those of both CTAs, all counted in the even CTA, so it also says that the
-    // odd CTA's operands have landed); EMPTY[s]: the MMAs reading stage s have completed (one tcgen05.commit per issuing
+    // FULL[s]: the stage's codes and scales have landed (TMA bytes; a pair: the codes of both CTAs count in the even one, scales in their
+    // own); SC_FULL[s]: the scale warps have moved the stage's scales into tensor memory (a pair: those of both CTAs, all
+    // counted in the even CTA); EMPTY[s]: the MMAs reading stage s have completed (one tcgen05.commit per issuing
     // warp); ACC_FULL[b] / ACC_EMPTY[b]: the accumulators of buffer b are complete / drained.  Buffer 1 exists only when every
     // segment is short (at most kShortRows rows; single CTAs): a tile's two accumulators then take 2 x 96 of the 384
     // accumulator columns, tiles alternate between the two halves, and a tile's read-out runs under the next tile's MMAs.
@@ -306,7 +319,7 @@ mx_gemm_kernel(const __grid_constant__ CUtensorMap tmap_b32, const __grid_consta
         }
         for (int b = 0; b < 2; b++) {
             mbar_init(bar(ACC_FULL + b), kMmaWarps);
-            mbar_init(bar(ACC_EMPTY + b), (TWO && rank == 0) ? kEpiWarps + 1 : kEpiWarps);   // + one forwarded arrival for the odd CTA's twelve
+            mbar_init(bar(ACC_EMPTY + b), TWO ? 2 * kEpiWarps : kEpiWarps);   // a pair: the warps of both CTAs, in the even one
         }
         *abort_flag = 0u;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -386,10 +399,12 @@ mx_gemm_kernel(const __grid_constant__ CUtensorMap tmap_b32, const __grid_consta
                     ok = mbar_wait(bar(EMPTY + s), ((cnt / kStages) & 1u) ^ 1u, abort_flag);
                     if (!ok) break;
                     const uint32_t a_dst = sbase + kSmemA + s * kABytes;
-                    const uint32_t full = bar(FULL + s);   // every CTA's loads count on its own barrier
-                    mbar_expect_tx(full, tile_tx + sf_tx);
-                    tma_load_4d(a_dst, m_w, kc * kRowBytes, w_row(mb), 0, slot, full);
-                    tma_load_3d(sbase + kSmemB + s * kBBytes, m_b, kc * kRowBytes, b_row0, 0, full);
+                    // The even CTA of a pair announces the codes of both.  (The odd one's may land first: the barrier's phase cannot end
+                    // before the announcement, and the odd CTA's next load of the stage waits for the MMAs of that phase.)
+                    const uint32_t full = bar(FULL + s), codes = TWO ? map_to_cta(full, 0u) : full;
+                    mbar_expect_tx(full, !TWO ? tile_tx + sf_tx : (rank == 0 ? 2u * tile_tx + sf_tx : sf_tx));
+                    tma_load_4d<TWO>(a_dst, m_w, kc * kRowBytes, w_row(mb), 0, slot, codes);
+                    tma_load_3d<TWO>(sbase + kSmemB + s * kBBytes, m_b, kc * kRowBytes, b_row0, 0, codes);
                     bulk_load(sbase + kSmemSfa + s * kSfaBytes, sfa + (int64_t)kc * 4 * kSfChunk, kSfaBytes, full);
                     bulk_load(sbase + kSmemSfb + s * kSfbBytes, sfb + (int64_t)kc * kSfbBytes, kSfbBytes, full);
                     cnt++;
@@ -403,15 +418,7 @@ mx_gemm_kernel(const __grid_constant__ CUtensorMap tmap_b32, const __grid_consta
         // accumulator's weight scales and its own copy of the activation scales to tensor memory, so its MMAs depend only
         // on its own copies.
         if (TWO && rank != 0) {
-            // odd CTA of a pair: nothing to issue.  One thread forwards "all twelve epilogue warps here have read tile t's
-            // accumulators" to the even CTA.
-            if (warp == 2 && lane == 0) {
-                uint32_t t = 0;
-                for (int tile = unit0; tile < n_tiles; tile += unit_step, t++) {
-                    if (!mbar_wait(bar(ACC_EMPTY), t & 1u, abort_flag)) break;
-                    mbar_arrive_cluster(map_to_cta(bar(ACC_EMPTY), 0u));
-                }
-            }
+            // odd CTA of a pair: nothing to issue
         } else if (lane == 0) {
             const int mw = warp - 1;
             constexpr int kAPW = kAccs / kMmaWarps;   // accumulators per issuing warp
@@ -589,7 +596,9 @@ mx_gemm_kernel(const __grid_constant__ CUtensorMap tmap_b32, const __grid_consta
             }
             tc_fence_before();
             __syncwarp();
-            if (lane == 0) mbar_arrive(bar(ACC_EMPTY) + 8u * buf);   // (odd CTA of a pair: its own barrier; warp 2 forwards the completed phase)
+            if (lane == 0) {
+                if (TWO && rank != 0) mbar_arrive_cluster(map_to_cta(bar(ACC_EMPTY), 0u)); else mbar_arrive(bar(ACC_EMPTY) + 8u * buf);
+            }
             if (b2) {
                 emit(c0 + 32, v0, v1);
                 if (b3) emit(c0 + 48, u0, u1);
