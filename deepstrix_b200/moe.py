@@ -282,12 +282,14 @@ class RoutedExpertWeights:
 
     def load_float(self, which: int, w: torch.Tensor, slot: int = -1):
         """Quantise matrix `which` of `slot` (w [rows, K] f32 / bf16 / f16 on the GPU; -1: all slots, w [n_slots, rows, K])
-        to MXFP4 and load it (one term of :class:`deepstrix_b200.head.Mxfp4Quantize`; values must be finite)."""
+        to MXFP4 and load it (one term of :class:`deepstrix_b200.head.Mxfp4Quantize`).  Values must be finite: looked at
+        before anything is loaded, which waits for the stream (a stream that is being captured cannot wait, and is not looked at)."""
         from .head import Mxfp4Quantize
         assert self.fmt == FMT_MXFP4, "load_float quantises to MXFP4 stores"
         shape = (self.hidden, self.ffn) if which == MAT_DOWN else (self.ffn, self.hidden)
         assert tuple(w.shape) == (shape if slot >= 0 else (self.n_slots,) + shape)
         q = Mxfp4Quantize.launch(w if slot >= 0 else w.reshape(-1, shape[1]))
+        assert torch.cuda.is_current_stream_capturing() or not bool((q.scales == 255).any()), "a weight is infinite or NaN"
         self.load(which, SRC_MXFP4_HF, q.codes, q.scales, slot)
 
     def unpack(self, slot: int, which: int):

@@ -569,3 +569,25 @@ def test_matmul_pairs_of_ctas_exact_sums(torch_cuda, moe, m, n, k, terms):
     for g in got:
         assert torch.equal(g, want)
     assert torch.equal(head.Mxfp4Matmul.launch(a, w, torch.bfloat16), want.to(torch.bfloat16))
+
+
+@pytest.mark.parametrize("value", [math.nan, math.inf, -math.inf])
+def test_expert_store_refuses_weights_that_are_not_finite(torch_cuda, moe, value):
+    """load_float with one bad weight is refused and leaves the store as it was; its neighbours in the type's range are taken."""
+    torch = torch_cuda
+    from deepstrix_b200.config import FMT_MXFP4
+    st = moe.RoutedExpertWeights(FMT_MXFP4, 2, 512, 256)
+    w = torch.randn((2, 256, 512), generator=torch.Generator(device="cuda").manual_seed(0), device="cuda")
+    w[0, 3, 3] = torch.finfo(torch.float32).max
+    st.load_float(moe.MAT_GATE, w)
+    before = [t.clone() for slot in range(2) for t in st.unpack(slot, moe.MAT_GATE)]
+    for dtype in (torch.float32, torch.bfloat16, torch.float16):
+        bad = torch.randn((2, 256, 512), device="cuda").to(dtype)
+        bad[1, 255, 511] = value
+        with pytest.raises(AssertionError, match="infinite or NaN"):
+            st.load_float(moe.MAT_GATE, bad)
+        with pytest.raises(AssertionError, match="infinite or NaN"):
+            st.load_float(moe.MAT_GATE, bad[1], slot=1)
+    after = [t for slot in range(2) for t in st.unpack(slot, moe.MAT_GATE)]
+    assert all(torch.equal(a, b) for a, b in zip(before, after))
+    st.close()
