@@ -71,7 +71,7 @@ def _row_stride(t: torch.Tensor) -> int:
 class Mxfp4Rows:
     """Rows as sums of MXFP4 terms: uint8 ``codes`` [terms, rows, K / 2] (element 2i in the low nibble) and E8M0 ``scales``
     [terms, rows, K / 32]; two-dimensional tensors are one term (a stored matrix)."""
-    __slots__ = ("n_terms", "rows", "k", "codes_at", "scales_at", "_buffer", "_codes", "_scales")
+    __slots__ = ("n_terms", "rows", "k", "_buffer", "_codes", "_scales", "_checked")
 
     def __init__(self, codes: torch.Tensor, scales: torch.Tensor):
         assert codes.dtype == torch.uint8 and scales.dtype == torch.uint8 and codes.is_contiguous() and scales.is_contiguous()
@@ -79,8 +79,8 @@ class Mxfp4Rows:
         assert len(shape) in (2, 3) and shape[:-1] == scales.shape[:-1] and shape[-1] == 16 * scales.shape[-1], "codes [.., K / 2] and scales [.., K / 32]"
         assert codes.device == scales.device
         self.n_terms, self.rows, self.k = shape[0] if len(shape) == 3 else 1, shape[-2], 2 * shape[-1]
-        self._buffer, self._codes, self._scales = codes, codes, scales
-        self.codes_at, self.scales_at = codes.data_ptr(), scales.data_ptr()
+        self._buffer, self._codes, self._scales = None, codes, scales
+        self._checked = codes.data_ptr(), scales.data_ptr()
 
     @classmethod
     def _empty(cls, n_terms: int, rows: int, k: int, device) -> "Mxfp4Rows":
@@ -90,13 +90,34 @@ class Mxfp4Rows:
         n = n_terms * rows * k
         q.n_terms, q.rows, q.k, q._codes, q._scales = n_terms, rows, k, None, None
         q._buffer = torch.empty(n // 2 + n // 32, dtype=torch.uint8, device=device)
-        q.codes_at = q._buffer.data_ptr()
-        q.scales_at = q.codes_at + n // 2
         return q
+
+    def _at(self) -> tuple[int, int]:
+        """Where codes and scales lie now: given tensors are asked at every call, since their owner may have put other memory under them."""
+        if self._buffer is not None:
+            at = self._buffer.data_ptr()
+            return at, at + self.n_terms * self.rows * self.k // 2
+        at = self._codes.data_ptr(), self._scales.data_ptr()
+        if at != self._checked:   # other memory: it has to be of the same form
+            now = Mxfp4Rows(self._codes, self._scales)
+            assert (now.n_terms, now.rows, now.k) == (self.n_terms, self.rows, self.k), "codes and scales have changed shape"
+            self._checked = at
+        return at
+
+    @property
+    def codes_at(self) -> int:
+        return self._at()[0]
+
+    @property
+    def scales_at(self) -> int:
+        return self._at()[1]
+
+    def _tensors(self):
+        return (self._buffer,) if self._buffer is not None else (self._codes, self._scales)
 
     @property
     def device(self) -> torch.device:
-        return self._buffer.device
+        return self._tensors()[0].device
 
     @property
     def codes(self) -> torch.Tensor:
@@ -124,7 +145,7 @@ class Mxfp4Quantize:
         stream = _here(x)
         rows, k = x.shape
         q = Mxfp4Rows._empty(n_terms, rows, k, x.device)
-        _call("dsx_mxfp4_quantize", x.data_ptr(), DTYPES[x.dtype], rows, k, stride, n_terms, q.codes_at, q.scales_at, stream)
+        _call("dsx_mxfp4_quantize", x.data_ptr(), DTYPES[x.dtype], rows, k, stride, n_terms, *q._at(), stream)
         return q
 
 
@@ -136,8 +157,7 @@ class Mxfp4Dequantize:
         if out is None:
             out = torch.empty(q.rows, q.k, dtype=dtype, device=q.device)
         assert out.shape == (q.rows, q.k) and out.dtype == dtype and dtype in DTYPES
-        _call("dsx_mxfp4_dequantize", q.codes_at, q.scales_at, q.rows, q.k, q.n_terms, out.data_ptr(), DTYPES[dtype], _row_stride(out),
-              _here(q._buffer, out))
+        _call("dsx_mxfp4_dequantize", *q._at(), q.rows, q.k, q.n_terms, out.data_ptr(), DTYPES[dtype], _row_stride(out), _here(*q._tensors(), out))
         return out
 
 
@@ -151,8 +171,8 @@ class Mxfp4Matmul:
         if out is None:
             out = torch.empty(a.rows, w.rows, dtype=dtype, device=a.device)
         assert out.shape == (a.rows, w.rows) and out.dtype == dtype and dtype in DTYPES
-        _call("dsx_mxfp4_matmul", a.codes_at, a.scales_at, a.n_terms, a.rows, w.codes_at, w.scales_at, w.rows, a.k, out.data_ptr(), DTYPES[dtype],
-              _row_stride(out), _here(a._buffer, w._buffer, out))
+        _call("dsx_mxfp4_matmul", *a._at(), a.n_terms, a.rows, *w._at(), w.rows, a.k, out.data_ptr(), DTYPES[dtype], _row_stride(out),
+              _here(*a._tensors(), *w._tensors(), out))
         return out
 
     @staticmethod

@@ -113,3 +113,22 @@ def test_tiling_and_pin_refusals(moe):
     for pin in ((-2, 0, 0), (2, 0, 0), (0, -16, 0), (0, 8, 0), (0, 224, 0), (0, 0, -1), (0, 0, 3), (0, 0, 16)):
         assert "pin" in _refused(moe, "dsx_mxfp4_matmul_pin", *pin)
     assert lib.dsx_mxfp4_matmul_pin(1, 208, 1) == 0 and lib.dsx_mxfp4_matmul_pin(-1, 0, 0) == 0
+
+
+def test_rows_follow_their_tensors(moe):
+    """The memory of a given tensor may be exchanged under it (weights loaded anew): the next call takes what lies there then."""
+    u8 = lambda *s: torch.zeros(s, dtype=torch.uint8)  # noqa: E731
+    codes, scales = u8(5, 32), u8(5, 2)
+    q = head.Mxfp4Rows(codes, scales)
+    assert (q.codes_at, q.scales_at) == (codes.data_ptr(), scales.data_ptr())
+    codes.data, new_scales = u8(5, 32) + 1, u8(5, 2)
+    scales.set_(new_scales)
+    assert (q.codes_at, q.scales_at) == (codes.data_ptr(), new_scales.data_ptr()) and q.codes[0, 0] == 1
+    codes.data = u8(6, 32)
+    with pytest.raises(AssertionError):
+        q.codes_at
+    scales.data = u8(6, 2)
+    with pytest.raises(AssertionError, match="changed shape"):
+        q.codes_at
+    codes.data, scales.data = u8(5, 32), u8(5, 2)
+    assert q.codes_at == codes.data_ptr()
