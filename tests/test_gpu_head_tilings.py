@@ -213,3 +213,43 @@ def test_first_calls_of_a_process_from_many_threads(torch_cuda, moe):
     for _ in range(2):
         out = subprocess.run([sys.executable, "-c", FIRST_CALLS, root], capture_output=True, text=True, timeout=300)
         assert out.returncode == 0 and out.stdout.strip() == "same", out.stderr[-2000:]
+
+
+@pytest.mark.parametrize("fmt", ["mxfp4", "q8_0"])
+@pytest.mark.parametrize("T", [300, 2500])
+def test_product_beside_the_layer(torch_cuda, moe, fmt, T):
+    """Products of every kind of block on one stream, the layer's tensor-core kernels on another: they share SMs and tensor memory, and both
+    write the bits that they write alone."""
+    import numpy as np
+
+    from deepstrix_b200 import head, synth
+    from deepstrix_b200.config import FMT_MXFP4, FMT_Q8_0, MoeConfig, RouterConfig
+    torch = torch_cuda
+    cfg = MoeConfig(hidden=1024, ffn=512, shared_ffn=512, fmt=FMT_MXFP4 if fmt == "mxfp4" else FMT_Q8_0,
+                    router=RouterConfig(n_expert=32, n_used=4, n_group=1, topk_group=1, score_fn=1, route_scale=2.5))
+    layer = moe.build_layer_from_host(cfg, synth.make_layer(cfg, 5), max_tokens=T)
+    x = torch.from_numpy(synth.make_tokens(cfg, 5, T).view(np.int16)).cuda().view(torch.bfloat16)
+    g = torch.Generator(device="cuda").manual_seed(T)
+    work = [(pin, _rows(torch, g, terms, m, k)[0], _rows(torch, g, 1, n, k)[0])
+            for pin, terms, m, n, k in (((0, 16, 1), 3, 16, 40000, 1024), ((0, 16, 8), 3, 1, 1024, 2048), ((1, 208, 1), 1, 900, 9000, 1024),
+                                        ((0, 208, 1), 1, 400, 9000, 1056), ((1, 128, 1), 3, 500, 5000, 1056))]
+
+    def products(times):
+        results = []
+        for pin, a, w in work * times:
+            head.Mxfp4Matmul.pin(*pin)
+            results.append(head.Mxfp4Matmul.launch(a, w, torch.float32))
+        head.Mxfp4Matmul.pin()
+        return results
+    want_layer, want = layer.forward(x), products(1)
+    torch.cuda.synchronize()
+    one, two = torch.cuda.Stream(), torch.cuda.Stream()
+    for _ in range(6):
+        with torch.cuda.stream(one):
+            got = products(3)
+        with torch.cuda.stream(two):
+            got_layer = [layer.forward(x) for _ in range(4)]
+        torch.cuda.synchronize()
+        assert all(torch.equal(r, want[i % len(want)]) for i, r in enumerate(got))
+        assert all(torch.equal(r.view(torch.int16), want_layer.view(torch.int16)) for r in got_layer)
+    assert layer.check() == 0
