@@ -51,8 +51,7 @@ def _here(*tensors) -> int:
     """All on the current device, whose current stream (returned) the kernels run on."""
     device = torch.cuda.current_device() if tensors[0].is_cuda else None
     for t in tensors:
-        assert t.is_cuda, "tensors must be on the GPU"
-        assert t.get_device() == device, f"tensor on {t.device}, current device is cuda:{device}"
+        assert t.get_device() == device, f"tensor on {t.device}, not on the current GPU"   # the CPU's is -1
     return torch._C._cuda_getCurrentRawStream(device)
 
 
@@ -71,16 +70,16 @@ def _row_stride(t: torch.Tensor) -> int:
 class Mxfp4Rows:
     """Rows as sums of MXFP4 terms: uint8 ``codes`` [terms, rows, K / 2] (element 2i in the low nibble) and E8M0 ``scales``
     [terms, rows, K / 32]; two-dimensional tensors are one term (a stored matrix)."""
-    __slots__ = ("n_terms", "rows", "k", "_buffer", "_codes", "_scales", "_checked")
+    __slots__ = ("n_terms", "rows", "k", "codes_at", "scales_at", "_buffer", "_codes", "_scales", "_given")
 
     def __init__(self, codes: torch.Tensor, scales: torch.Tensor):
         assert codes.dtype == torch.uint8 and scales.dtype == torch.uint8 and codes.is_contiguous() and scales.is_contiguous()
         shape = codes.shape
         assert len(shape) in (2, 3) and shape[:-1] == scales.shape[:-1] and shape[-1] == 16 * scales.shape[-1], "codes [.., K / 2] and scales [.., K / 32]"
-        assert codes.device == scales.device
+        assert codes.get_device() == scales.get_device()
         self.n_terms, self.rows, self.k = shape[0] if len(shape) == 3 else 1, shape[-2], 2 * shape[-1]
-        self._buffer, self._codes, self._scales = None, codes, scales
-        self._checked = codes.data_ptr(), scales.data_ptr()
+        self._buffer, self._codes, self._scales, self._given = codes, codes, scales, True
+        self.codes_at, self.scales_at = codes.data_ptr(), scales.data_ptr()
 
     @classmethod
     def _empty(cls, n_terms: int, rows: int, k: int, device) -> "Mxfp4Rows":
@@ -88,36 +87,23 @@ class Mxfp4Rows:
         assert n_terms >= 1 and k % 32 == 0, f"{n_terms} terms of rows of {k} columns (a multiple of 32)"
         q = cls.__new__(cls)
         n = n_terms * rows * k
-        q.n_terms, q.rows, q.k, q._codes, q._scales = n_terms, rows, k, None, None
+        q.n_terms, q.rows, q.k, q._codes, q._scales, q._given = n_terms, rows, k, None, None, False
         q._buffer = torch.empty(n // 2 + n // 32, dtype=torch.uint8, device=device)
+        q.codes_at = q._buffer.data_ptr()
+        q.scales_at = q.codes_at + n // 2
         return q
 
-    def _at(self) -> tuple[int, int]:
-        """Where codes and scales lie now: given tensors are asked at every call, since their owner may have put other memory under them."""
-        if self._buffer is not None:
-            at = self._buffer.data_ptr()
-            return at, at + self.n_terms * self.rows * self.k // 2
-        at = self._codes.data_ptr(), self._scales.data_ptr()
-        if at != self._checked:   # other memory: it has to be of the same form
-            now = Mxfp4Rows(self._codes, self._scales)
+    def _follow(self):
+        """Given tensors are asked where they lie at every call: their owner may have put other memory, of the same form, under them."""
+        codes, scales = self._codes, self._scales
+        if codes.data_ptr() != self.codes_at or scales.data_ptr() != self.scales_at:
+            now = Mxfp4Rows(codes, scales)
             assert (now.n_terms, now.rows, now.k) == (self.n_terms, self.rows, self.k), "codes and scales have changed shape"
-            self._checked = at
-        return at
-
-    @property
-    def codes_at(self) -> int:
-        return self._at()[0]
-
-    @property
-    def scales_at(self) -> int:
-        return self._at()[1]
-
-    def _tensors(self):
-        return (self._buffer,) if self._buffer is not None else (self._codes, self._scales)
+            self.codes_at, self.scales_at = now.codes_at, now.scales_at
 
     @property
     def device(self) -> torch.device:
-        return self._tensors()[0].device
+        return self._buffer.device
 
     @property
     def codes(self) -> torch.Tensor:
@@ -145,7 +131,7 @@ class Mxfp4Quantize:
         stream = _here(x)
         rows, k = x.shape
         q = Mxfp4Rows._empty(n_terms, rows, k, x.device)
-        _call("dsx_mxfp4_quantize", x.data_ptr(), DTYPES[x.dtype], rows, k, stride, n_terms, *q._at(), stream)
+        _call("dsx_mxfp4_quantize", x.data_ptr(), DTYPES[x.dtype], rows, k, stride, n_terms, q.codes_at, q.scales_at, stream)
         return q
 
 
@@ -157,7 +143,10 @@ class Mxfp4Dequantize:
         if out is None:
             out = torch.empty(q.rows, q.k, dtype=dtype, device=q.device)
         assert out.shape == (q.rows, q.k) and out.dtype == dtype and dtype in DTYPES
-        _call("dsx_mxfp4_dequantize", *q._at(), q.rows, q.k, q.n_terms, out.data_ptr(), DTYPES[dtype], _row_stride(out), _here(*q._tensors(), out))
+        if q._given:
+            q._follow()
+        _call("dsx_mxfp4_dequantize", q.codes_at, q.scales_at, q.rows, q.k, q.n_terms, out.data_ptr(), DTYPES[dtype], _row_stride(out),
+              _here(q._buffer, out))
         return out
 
 
@@ -171,8 +160,12 @@ class Mxfp4Matmul:
         if out is None:
             out = torch.empty(a.rows, w.rows, dtype=dtype, device=a.device)
         assert out.shape == (a.rows, w.rows) and out.dtype == dtype and dtype in DTYPES
-        _call("dsx_mxfp4_matmul", *a._at(), a.n_terms, a.rows, *w._at(), w.rows, a.k, out.data_ptr(), DTYPES[dtype], _row_stride(out),
-              _here(*a._tensors(), *w._tensors(), out))
+        if a._given:
+            a._follow()
+        if w._given:
+            w._follow()
+        _call("dsx_mxfp4_matmul", a.codes_at, a.scales_at, a.n_terms, a.rows, w.codes_at, w.scales_at, w.rows, a.k, out.data_ptr(), DTYPES[dtype],
+              _row_stride(out), _here(a._buffer, w._buffer, out))
         return out
 
     @staticmethod

@@ -115,20 +115,30 @@ def test_tiling_and_pin_refusals(moe):
     assert lib.dsx_mxfp4_matmul_pin(1, 208, 1) == 0 and lib.dsx_mxfp4_matmul_pin(-1, 0, 0) == 0
 
 
-def test_rows_follow_their_tensors(moe):
-    """The memory of a given tensor may be exchanged under it (weights loaded anew): the next call takes what lies there then."""
+def test_rows_follow_their_tensors(moe, monkeypatch):
+    """The memory of a given tensor may be exchanged under it (weights loaded anew): the next call takes what lies there then, if it has
+    the same form."""
     u8 = lambda *s: torch.zeros(s, dtype=torch.uint8)  # noqa: E731
-    codes, scales = u8(5, 32), u8(5, 2)
+    calls = []
+    monkeypatch.setattr(head, "_call", lambda name, *args: calls.append(args))
+    monkeypatch.setattr(head, "_here", lambda *tensors: 0)
+    codes, scales, other = u8(5, 32), u8(5, 2), head.Mxfp4Rows(u8(3, 32), u8(3, 2))
     q = head.Mxfp4Rows(codes, scales)
-    assert (q.codes_at, q.scales_at) == (codes.data_ptr(), scales.data_ptr())
+
+    def addresses():
+        head.Mxfp4Dequantize.launch(q)
+        head.Mxfp4Matmul.launch(q, other)
+        head.Mxfp4Matmul.launch(other, q)
+        return {calls[-3][:2], calls[-2][:2], calls[-1][4:6]}
+    assert addresses() == {(codes.data_ptr(), scales.data_ptr())}
     codes.data, new_scales = u8(5, 32) + 1, u8(5, 2)
     scales.set_(new_scales)
-    assert (q.codes_at, q.scales_at) == (codes.data_ptr(), new_scales.data_ptr()) and q.codes[0, 0] == 1
+    assert addresses() == {(codes.data_ptr(), new_scales.data_ptr())} and q.codes[0, 0] == 1
     codes.data = u8(6, 32)
     with pytest.raises(AssertionError):
-        q.codes_at
+        addresses()
     scales.data = u8(6, 2)
     with pytest.raises(AssertionError, match="changed shape"):
-        q.codes_at
+        addresses()
     codes.data, scales.data = u8(5, 32), u8(5, 2)
-    assert q.codes_at == codes.data_ptr()
+    assert addresses() == {(codes.data_ptr(), scales.data_ptr())}
