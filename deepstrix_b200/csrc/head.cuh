@@ -86,8 +86,10 @@ __device__ __forceinline__ float e8m0_value(uint32_t e) {
 }
 // The codes in nibble k of either half of x as two f16 values: the two exponent bits and the mantissa bit of a code sit where an f16 has its
 // lowest exponent bits and its highest mantissa bit (code 1 is an f16 subnormal there, as it is E2M1's own), so what is left is a factor of 2^14.
-// Four integer instructions a pair.  (The hardware's decoder, cvt.rn.f16x2.e2m1x2, is two instructions shorter, but gave zeros or wrong
-// values inside two kernels of this library although it is right in isolation: CUDA 12.9, sm_100a.)
+// Four integer instructions a pair.  (The hardware's decoder, cvt.rn.f16x2.e2m1x2, is two instructions shorter.  Twice it gave other values than
+// the codes stand for in a kernel although it is right in isolation (CUDA 12.9, sm_100a): zeros in a build of the dequantiser to f32, wrong residuals in
+// the layer's quantiser of activations.  The cause is not known.  The library uses it in the decode kernels, the f16-operand kernels
+// and, behind an exclusive-or, that quantiser, whose results the tests hold against the CPU's; the encoder's codes (mxfp4_rows.cu) are compared bit for bit.)
 template <int K>
 __device__ __forceinline__ float2 e2m1_pair(uint32_t x) {
     const uint32_t mag = K == 0 ? x << 9 : (K == 1 ? x << 5 : (K == 2 ? x << 1 : x >> 3));

@@ -11,13 +11,16 @@
 // The alternatives cost the loop nothing: afterwards the n_alt-th largest of the maxima of 32 or 64 groups of threads is a value that
 // at least n_alt logits reach, and hardly more do, so only the threads whose maximum reaches it have their chunks read again (from L2) for
 // the few logits that do; those are ranked by counting.  Where more than the list holds reach it -- a row of equal logits, say, or one masked with the
-// lowest value -- a second pass keeps the best 32 of every warp in registers, sorting candidates 32 at a time.
+// lowest value -- a second pass keeps the best 32 of every warp in registers, sorting candidates 32 at a time.  That comes on top: every
+// logit that reaches the threshold has been counted by then, a shared atomic each.  64 rows of 131072 f32 that hold the lowest value but for three
+// logits take 45.5 us with twenty alternatives where random rows take 10.5 (and rows masked by -inf 9.5), 512 such rows 240 and 57.
 // A row belongs to one block, or, when there are few rows, to the blocks of a cluster that join their sums and lists through
 // distributed shared memory: one launch, no workspace, and the order of every addition is fixed.
 //
 // Bound: HBM; bf16 and f16 rows at the full rate are 11.6 elements a clock and SM, of which the exponentials can take 16.  2048 rows of 131072
-// f32 take 172 us, 6.25 TB/s; 4096 of bf16 177 without alternatives and 191 with five (the part behind the loop of one block in five at a
-// time); 64 rows of f32 with twenty 11 us, one row of 32000 5.8, latency.  A ring of asynchronous copies that ran on into the next row was
+// f32 take 160 us without and 173 with five alternatives, 6.7 and 6.2 TB/s (167 and 180 after a second of it); 4096 of bf16 174 and 187
+// (the part behind the loop of one block in five at a time), 200 and 212 once the power cap holds the clock, 5.1 TB/s; 64 rows of f32 with twenty
+// 16 us from HBM and 10.5 from L2, one row of 32000 6, latency.  A ring of asynchronous copies that ran on into the next row was
 // slower (227 us when the loop took 199: its instructions, not the loads in flight, were what the loop lacked), and so were chunks requested 2 to 6
 // ahead for a few rows (0.1 to 1.3 us more), and keeping the chunk of every thread's maximum so that it need not be read again (loop 5 to 10 % longer).
 #include "head.cuh"
@@ -32,7 +35,7 @@ constexpr float kLowest = -3.402823466e38f;
 constexpr uint32_t kFloor = 0x00800000u;   // order_of(kLowest): nothing finite is below it
 constexpr float kLn2 = 0.6931471805599453f, kLog2e = 1.4426950408889634f;
 
-// 2^x; the instruction is off by at most 2 ulp, and 0 for x below -150
+// 2^x; the instruction is off by at most 2 ulp, and 0 for x below -126 (subnormal results are flushed)
 __device__ __forceinline__ float exp2_fast(float x) {
     float r;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
@@ -174,7 +177,8 @@ __device__ __forceinline__ void rank_list(const uint64_t* list, int n, int n_alt
 }
 
 // NT threads a block: 256, or 64 for many short rows, whose time is the part behind the loop.  48 registers a thread (1280 threads an SM, 40 KB
-// of logits in flight): 4096 rows of 131072 bf16 take 191 us, 2048 of f32 172; with 64 registers (1024 threads) 198 and 191.
+// of logits in flight) against 64 (1024 threads): 4096 rows of 131072 bf16 191 us against 198, 2048 of f32 172 against 191.  The f16 kernels
+// spill 20 and 32 bytes at 48 registers, the others nothing.
 template <int DT, int NT>
 __global__ void __launch_bounds__(NT, 1280 / NT)
 token_logprobs_kernel(const void* __restrict__ logits, int64_t V, int64_t row_stride, float scale, const int32_t* __restrict__ tokens, int n_given,
@@ -364,7 +368,7 @@ token_logprobs_kernel(const void* __restrict__ logits, int64_t V, int64_t row_st
             rank_list<NT>(sh.list, sh.count, n_alt, sh.best);
         } else {
             // too many: a second pass over the part, in which a warp keeps its best 32 (one a lane) and lists only what may enter them.
-            // Its chunks come in ascending order, so an equal logit behind a full list is out: rows of equal logits cost one compare each.
+            // Its chunks come in ascending order, so an equal logit behind a full list is out: in this pass, equal logits cost one compare each.
             uint64_t* list = sh.warp_list[warp];
             uint64_t mine = 0ull;
             uint32_t kth = 0u, own = threshold;   // order of the list's n_alt-th; the lowest order that may still enter it
@@ -505,7 +509,8 @@ int launch_for(const void* logits, int64_t t, int64_t v, int64_t row_stride, flo
     const bool small = v <= 64 * kChunk || (t >= 8 * (int64_t)sms && v <= 16 * 64 * kChunk);
     // few rows: as many blocks a row as still give every thread two chunks, and no more than two blocks an SM in all (64 rows of 131072 f32
     // 20.5 / 14.0 / 11.1 / 13.6 us with 1 / 2 / 4 / 8, 148 of bf16 13.0 / 12.2 / 14.3 / 17.6, one row of 32000 f32 7.0 / 6.6 / 5.8 / 5.4), or as many
-    // as are resident where every thread keeps 16 (300 rows of 131072 f32 40.9 / 30.0 / 34.2 us with 1 / 2 / 4, but 333 of 50021 f16 12.7 / 13.6)
+    // as are resident where every thread keeps 16 (300 rows of 131072 f32 40.9 / 30.0 / 34.2 us with 1 / 2 / 4, but 333 of 50021 f16 12.7 / 13.6; 250 of
+    // 131072 bf16 pay for the rule, 18.5 with two and 17.7 with one)
     int splits = 1;
     auto more = [&](int blocks_per_sm, int chunks) {
         return splits < kMaxCluster && t * splits * 2 <= blocks_per_sm * (int64_t)sms && v >= (int64_t)splits * 2 * chunks * 256 * kChunk;

@@ -13,7 +13,7 @@
 // Scales are read as stored (row-major bytes; nothing is laid out beforehand), 16 bytes of every row -- 512 columns, two stages -- at a time
 // into a ring of their own: by TMA where rows of scales are 16-byte aligned (K a multiple of 512), else by four loader warps, a row of
 // every 128-row group a thread, as the aligned 16-byte words that hold them, requested a step ahead and shifted into place (8192 x 8192 x 4128
-// takes 160 us, as words of 4 bytes 178; with K of 4096 and TMA 121.  Loaders that moved every other buffer to tensor memory as well: 168).  Scale warps, one per lane quarter, move a
+// takes 165 us, as words of 4 bytes 178; with K of 4096 and TMA 118.  Loaders that moved every other buffer to tensor memory as well: 168).  Scale warps, one per lane quarter, move a
 // buffer to a slot of tensor memory at a time (ld.shared + tcgen05.st; the tensor core's own copy would queue behind its MMAs); where TMA
 // brings the scales the loader warps are a second set of them, and the sets take alternate buffers: one set alone needed 800 clocks a stage.
 // Warp roles: TMA of codes, MMA issue, TMA of scales, one idle, 4 scale warps, 4 epilogue warps, 4 loaders or scale warps; two accumulators, so that a
@@ -25,10 +25,11 @@
 // a cluster (every role of every block comes to them) and the wait for tensor memory, which kernels of this library give back without
 // waiting for another block, or hold alone on their SM (see the two sizes of block below).
 //
-// Bound and measured (launches back to back).  A few tokens: the weights' bytes; 8 x 131072 x 4096 of three terms takes 53 us, 5.4 TB/s, of which
-// about 7 us are start and end -- every further 37888 rows of W take 12.8 us, 6.45 TB/s.  One small matrix (1 x 1024 x 2048): 6 us, all of it
-// latency.  Many tokens: the issuing warp's clocks and the power cap; 8192 x 8192 x 4096 takes 118 us with one term, 4.7 PFLOP/s (140 us after a
-// second of it at the capped clock), 291 with three, 5.7 PFLOP/s of MMAs executed; 64 x 131072 x 4096 of three terms 61, 777 x 5119 x 2336 19.5.
+// Bound and measured (launches back to back, operands that rotate; a burst, and in brackets after a second of it, at the clock of the power cap).
+// A few tokens: the weights' bytes; 8 x 131072 x 4096 of three terms takes 54 us (55), 5.3 TB/s, of which about 7 us are start and end -- every
+// further 37888 rows of W take 12.8 us, 6.45 TB/s.  One small matrix (1 x 1024 x 2048): 6 us, all of it latency.  Many tokens: the issuing
+// warp's clocks and the power cap; 8192 x 8192 x 4096 takes 119 us (139) with one term, 4.6 PFLOP/s (4.0), 289 (333) with three, 5.7 PFLOP/s (4.9)
+// of MMAs executed; 64 x 131072 x 4096 of three terms 62 (74), 777 x 5119 x 2336 20.
 #include <cuda.h>
 
 #include <algorithm>

@@ -9,8 +9,11 @@
 // is exact in f32, so the bytes can be restated on a CPU.  A block with a NaN or an infinity is NaN as a whole: its first
 // scale byte is 255 (E8M0's NaN), its codes are 0, and its later terms are 0.
 //
-// Both directions are bound by HBM where there is one term (65536 x 2048 f32: 88.7 us to codes, 6.85 TB/s, 97 us back, 6.25; bf16 52 and 54 us),
-// by arithmetic for more (8192 x 4096 bf16: 13.6 and 12.8 us with one term, 32.7 and 27.6 with three), and by latency below a megabyte (2 us).
+// Both directions are bound by HBM where there is one term (65536 x 2048 f32: 89 us to codes, 6.8 TB/s, 98 us back, 6.2; bf16 53 and 55 us), and
+// by latency below a megabyte (2 us).  More terms: 8192 x 4096 bf16 15 and 15 us with one, 33 and 28 with three, where the bytes want 18.4.
+// Counters of 32768 x 4096 bf16 with three (124 and 104 us, bytes 74): the quantiser issues in 71 % of the clocks (integer pipe 69 %, the
+// largest stalls waits for that pipe and for loads) with 37 warps an SM, 40 registers a thread allowing 12 blocks of the 16 its grid
+// has an SM, so that the last quarter of them runs by itself; the dequantiser issues in 82 % (integer pipe 77 %) with 26 warps (72 registers).
 #include <algorithm>
 
 #include "head.cuh"
@@ -70,7 +73,7 @@ __device__ __forceinline__ float abs_max_nan(float a, float b) {
 // A lane holds PER consecutive values -- 8 f32 or 16 of 16 bits, 32 bytes -- so four or two neighbouring lanes make a block of 32: loads
 // are coalesced, the block's maximum is a shuffle or two away, and what a block costs beside its values is shared by as many as registers
 // allow.  Units of PER are numbered through all rows, so a short row wastes no lane; a block never straddles two quads or pairs.  48 KB
-// of loads are in flight an SM; the arithmetic (6 instructions a value and term, scaling and residual in pairs, 25 a lane and term) is what bounds two and three terms.
+// of loads are in flight an SM.
 template <int DT> constexpr int kPer = DT == DSX_F32 ? 8 : 16;
 
 template <int DT, int TERMS, bool VEC>
@@ -190,7 +193,7 @@ mxfp4_dequantize_kernel(const uint8_t* __restrict__ codes, const uint8_t* __rest
     }
 }
 
-constexpr int kPerSm = 2048 / kThreads;   // blocks an SM holds
+constexpr int kPerSm = 2048 / kThreads;   // blocks of a grid an SM; what is resident at once is less where a thread has more than 32 registers (down to 7)
 
 template <typename K, typename... A>
 int launch_rows(K kernel, int64_t blocks, cudaStream_t s, A... args) {
@@ -218,8 +221,8 @@ int launch_dequantize_terms(cudaStream_t s, const uint8_t* codes, const uint8_t*
     const uint32_t per_row = (uint32_t)(k / kOut<DT>);
     int sms = 0;
     if (int rc = head_sm_count(&sms)) return rc;
-    // four items a lane once there are more than one for every lane of a full grid, and more blocks than run at once (65536 x 2048 to bf16: 65 us,
-    // 70 us in a grid of what runs at once; two items 68, one 81)
+    // four items a lane once there are more than one for every lane of sixteen blocks an SM, and more blocks than that (65536 x 2048 to bf16 in an
+    // earlier build: 65 us, 70 us in a grid of sixteen an SM; two items 68, one 81)
     const int64_t lanes = (int64_t)sms * kPerSm * kThreads;
     if (n <= lanes) return launch_rows(mxfp4_dequantize_kernel<DT, TERMS, VEC, 1>, (n + kThreads - 1) / kThreads, s, codes, scales, n, per_row, out, stride);
     const int64_t blocks = std::min<int64_t>((n + 4 * kThreads - 1) / (4 * kThreads), 4 * sms * kPerSm);

@@ -711,9 +711,9 @@ __device__ __forceinline__ void mx_terms_of_block(float (&v)[32], uint32_t opaqu
 #pragma unroll
                     for (int j = 0; j < 8; j++) d[j] = e2m1_value(w[g] >> (4 * j));
                 } else {
-                    // the decoder must not see that its input comes straight from the encoder above: with the two chained,
-                    // the compiled code produced wrong residuals (CUDA 12.9, sm_100a); an exclusive-or with a kernel
-                    // argument that is always zero separates them
+                    // with the decoder chained straight to the encoder above, residuals were wrong (CUDA 12.9, sm_100a); with an
+                    // exclusive-or with a kernel argument that is always zero between them they are right.  Why is not known: the
+                    // decoder has also been seen to go wrong where nothing was chained (see e2m1_pair in head.cuh).
                     e2m1_unpack8(w[g] ^ opaque_zero, d);
                 }
 #pragma unroll

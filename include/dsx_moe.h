@@ -516,7 +516,9 @@ DSX_API int dsx_ep_check(dsx_ep_comm* comm, dsx_stream_t stream, uint32_t* error
 enum dsx_dtype { DSX_F32 = 0, DSX_BF16 = 1, DSX_F16 = 2 };
 
 /* MXFP4 rows of K columns (K a multiple of 32), HF layout: codes [n_terms, rows, K/2] (element 2i in the low nibble; 16-byte
- * aligned) and scales [n_terms, rows, K/32] (E8M0: 2^(e-127), 255 = NaN).  A row is the SUM of its terms.
+ * aligned) and scales [n_terms, rows, K/32] (E8M0: 2^(e-127), 255 = NaN).  A row is the SUM of its terms.  Scales may lie at any
+ * address; the product reads the aligned 16-byte words that hold them as a whole where K is no multiple of 512 or they are not 16-byte
+ * aligned, that is up to 15 bytes before and behind an array, and does nothing with those.
  *
  * quantize: term 0 holds x, each further term what the earlier ones leave over, per block of 32 with the scale
  * 2^ceil(log2(max|.| / 6)) (byte kept in 1..253) and codes rounded to nearest, ties to even.  Relative error of a row of normal
