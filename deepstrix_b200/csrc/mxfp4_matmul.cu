@@ -13,7 +13,8 @@
 // Scales are read as stored (row-major bytes; nothing is laid out beforehand), 16 bytes of every row -- 512 columns, two stages -- at a time
 // into a ring of their own: by TMA where rows of scales are 16-byte aligned (K a multiple of 512), else by four loader warps, a row of
 // every 128-row group a thread, as the aligned 16-byte words that hold them, requested a step ahead and shifted into place (8192 x 8192 x 4128
-// takes 165 us, as words of 4 bytes 178; with K of 4096 and TMA 118.  Loaders that moved every other buffer to tensor memory as well: 168).  Scale warps, one per lane quarter, move a
+// takes 165 us, with K of 4096 and TMA 118; when it took 160, words of 4 bytes took 178 and loaders that moved every other buffer to
+// tensor memory as well 168).  Scale warps, one per lane quarter, move a
 // buffer to a slot of tensor memory at a time (ld.shared + tcgen05.st; the tensor core's own copy would queue behind its MMAs); where TMA
 // brings the scales the loader warps are a second set of them, and the sets take alternate buffers: one set alone needed 800 clocks a stage.
 // Warp roles: TMA of codes, MMA issue, TMA of scales, one idle, 4 scale warps, 4 epilogue warps, 4 loaders or scale warps; two accumulators, so that a
