@@ -21,8 +21,9 @@
 // tile is read out under the next one's MMAs.
 // Few tiles: the columns are split over the CTAs of a cluster; each leaves its partial tile in shared memory and the cluster adds
 // them in rank order through distributed shared memory, so results do not depend on timing and need no workspace.
-// Every wait on a barrier in shared memory is bounded; when one runs out the block lets what it has in flight finish (bounded too), frees its
-// tensor memory and sets bit 1 of the error word.  Not bounded, because they end by themselves: the wait for the kernel before this one, the barriers of
+// Every wait on a barrier in shared memory is bounded; when one runs out the block lets what it has in flight finish (bounded too: MMAs and copies
+// are waited for by the roles that issue them, always, since another role may give up after they have ended), frees its tensor memory and sets bit 1
+// of the error word.  Not bounded, because they end by themselves: the wait for the kernel before this one, the barriers of
 // a cluster (every role of every block comes to them) and the wait for tensor memory, which kernels of this library give back without
 // waiting for another block, or hold alone on their SM (see the two sizes of block below).
 //
@@ -57,7 +58,7 @@ constexpr int kMaxSlots = 4;         // of scales in tensor memory, two stages e
 constexpr int kMaxStages = 8;
 constexpr int kMaxN = 208;           // of an MMA: two accumulators and two scale slots fill tensor memory
 constexpr uint32_t kPolls = 1u << 22;     // of a wait, unless dsx_mxfp4_matmul_set_polls says otherwise; a poll that fails takes 2 to 4 us
-constexpr uint32_t kDrainPolls = 1u << 16;   // for what is in flight when a block has given up
+constexpr uint32_t kDrainPolls = 1u << 16;   // for what is in flight when a role has nothing more to do
 
 __device__ __forceinline__ uint32_t smem_u32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
 __device__ __forceinline__ void mbar_init(uint32_t bar, uint32_t count) {
@@ -345,7 +346,7 @@ mxfp4_matmul_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_con
     // memory; SLOT_FULL / SLOT_EMPTY[v]: and lie in slot v (a pair: of both CTAs) / the MMAs that used them have completed.
     constexpr int FULL = 0, EMPTY = FULL + kMaxStages, ACC_FULL = EMPTY + kMaxStages, ACC_EMPTY = ACC_FULL + 2, RAW_FULL = ACC_EMPTY + 2,
                   RAW_EMPTY = RAW_FULL + kMaxScaleBufs, SLOT_FULL = RAW_EMPTY + kMaxScaleBufs, SLOT_EMPTY = SLOT_FULL + kMaxSlots,
-                  DRAIN = SLOT_EMPTY + kMaxSlots;   // DRAIN: the MMAs issued before this block gave up have completed
+                  DRAIN = SLOT_EMPTY + kMaxSlots;   // DRAIN: all MMAs have completed
     auto bar = [&](int i) { return bar0 + 8u * (uint32_t)i; };
     volatile uint32_t* abort_flag = s_misc + 1;
     const Patience patience{abort_flag, g.polls};
@@ -430,7 +431,7 @@ mxfp4_matmul_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_con
                 s_misc[2] = s;
                 s_misc[3] = ph;
                 s_misc[6] = n_loads;
-            } else if (!ok)   // gave up: let the copies in flight land before the block goes away
+            } else   // all copies have landed before this role ends, whoever gives up and when (a pair: see the end)
                 for (uint32_t i = 0; i < (uint32_t)g.stages; i++)
                     for (uint32_t n = 0; n < kDrainPolls && !mbar_try(bar(FULL) + 8u * i, i < s ? ph : ph ^ 1u); n++) {}
         }
@@ -502,7 +503,7 @@ mxfp4_matmul_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_con
             }
             tc_commit<PAIR>(leader, bar(ACC_FULL) + 8u * b);
         }
-        if (half == 0 && gave_up(abort_flag)) {   // let the MMAs in flight finish before tensor memory and operands go away
+        if (half == 0) {   // all MMAs have finished before this role ends, whoever gives up and when
             tc_commit_here<PAIR>(lane == 0 ? 1u : 0u, bar(DRAIN));
             for (uint32_t n = 0; n < kDrainPolls && !mbar_try(bar(DRAIN), 0u); n++) {}
         }
@@ -524,9 +525,8 @@ mxfp4_matmul_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_con
                     if (++d == (uint32_t)g.scale_bufs) { d = 0; ph ^= 1u; }
                 }
             }
-            if (!ok)
-                for (uint32_t i = 0; i < (uint32_t)g.scale_bufs; i++)
-                    for (uint32_t n = 0; n < kDrainPolls && !mbar_try(bar(RAW_FULL) + 8u * i, i < d ? ph : ph ^ 1u); n++) {}
+            for (uint32_t i = 0; i < (uint32_t)g.scale_bufs; i++)
+                for (uint32_t n = 0; n < kDrainPolls && !mbar_try(bar(RAW_FULL) + 8u * i, i < d ? ph : ph ^ 1u); n++) {}
         }
     } else if (warp == 3) {
         // idle: roles that use whole warp groups start on their boundaries
